@@ -31,6 +31,9 @@ MEM_AUTO, MEM_HOST, MEM_DEVICE = 0, 1, 2
 FLAG_ASYNC = 1
 FLAG_PAIR_ON, FLAG_PAIR_OFF = 2, 4
 NOALLOC_SCRATCH_BYTES = 8 << 20
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+MAX_GROUPS, MAX_TOP_K, MAX_RANK = 1024, 32, 256
 
 # Every symbol include/cpu_ops_b200.h declares.
 EXPORTED_SYMBOLS = (
@@ -49,6 +52,10 @@ EXPORTED_SYMBOLS = (
     "cpuops_b200_last_plan",
     "cpuops_b200_prepare_b",
     "cpuops_b200_release_b",
+    "cpuops_b200_route",
+    "cpuops_b200_group_rows",
+    "cpuops_b200_gemm_grouped",
+    "cpuops_b200_adapters",
     "cpuops_b200_last_error",
     "cpuops_b200_abi_version",
     "cpuops_b200_device_count",
@@ -85,6 +92,38 @@ class GemmDesc(C.Structure):
         ("memory_space", C.c_int32), ("stream", C.c_void_p), ("flags", C.c_uint32),
         ("device", C.c_int32), ("tile_n", C.c_int32),
     ]
+
+
+def _fields(kind, names):
+    return [(name, kind) for name in names.split()]
+
+
+_PLACE = [("stream", C.c_void_p), ("flags", C.c_uint32), ("device", C.c_int32), ("memory_space", C.c_int32)]
+
+
+class RouteDesc(C.Structure):
+    _fields_ = ([("struct_size", C.c_uint32)] +
+                _fields(C.c_int32, "tokens experts top_k scoring n_groups top_groups group_best renormalize") +
+                [("scale", C.c_float)] + _fields(C.c_int32, "logits_type ld_logits") +
+                _fields(C.c_void_p, "logits bias ids weights offsets order") + _PLACE)
+
+
+class GroupRowsDesc(C.Structure):
+    _fields_ = ([("struct_size", C.c_uint32)] + _fields(C.c_int32, "rows groups") +
+                _fields(C.c_void_p, "ids offsets order") + _PLACE)
+
+
+class GemmGroupedDesc(C.Structure):
+    _fields_ = ([("struct_size", C.c_uint32)] +
+                _fields(C.c_int32, "a_format b_format rows n k groups gated a_rows pairs_per_a_row pairs_per_d_row "
+                                   "b_group_rows lda ldb ld_scales_a ld_scales_b ldd") +
+                _fields(C.c_void_p, "a b a_scales b_scales offsets order ids row_weights d") + _PLACE)
+
+
+class AdaptersDesc(C.Structure):
+    _fields_ = ([("struct_size", C.c_uint32)] +
+                _fields(C.c_int32, "m n k rank adapters x_type w_type ldx lda ldb ldc ldd") +
+                _fields(C.c_int64, "a_stride b_stride") + _fields(C.c_void_p, "x a b ids scales c d") + _PLACE)
 
 
 _lib = None
@@ -129,6 +168,11 @@ def load() -> C.CDLL:
     lib.cpuops_b200_prepare_b.argtypes = [C.c_void_p, C.POINTER(C.c_void_p)]
     lib.cpuops_b200_release_b.restype = C.c_int
     lib.cpuops_b200_release_b.argtypes = [C.c_void_p]
+    for name, desc in (("route", RouteDesc), ("group_rows", GroupRowsDesc), ("gemm_grouped", GemmGroupedDesc),
+                       ("adapters", AdaptersDesc)):
+        entry = getattr(lib, "cpuops_b200_" + name)
+        entry.restype = C.c_int
+        entry.argtypes = [C.POINTER(desc)]
     lib.cpuops_b200_last_plan.restype = C.c_int
     lib.cpuops_b200_last_plan.argtypes = [C.POINTER(Plan)]
     lib.cpuops_b200_last_error.restype = C.c_char_p

@@ -1797,3 +1797,5 @@ CPUOPS_B200_API int cpuops_b200_gemm_i8_noalloc(const cpuops_b200_gemm_desc* d) 
 }
 
 }  // extern "C"
+
+#include "row_chosen_api.h"

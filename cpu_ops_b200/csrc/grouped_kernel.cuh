@@ -1,0 +1,607 @@
+// The experts' products: for every pair q of group g in a row plan, D[q] = A[row of q] * B_g^T on MX
+// operands (OCP MX fp8 / fp4, one E8M0 scale per 32 k-elements), f32 sums, optionally
+// silu(gate) * up of two such products and a weight per pair.
+//
+// Kernel view, as in the small-m kernel (decode_kernel.cuh): the weights W (B_g, 128-row tiles)
+// sit on the MMA M side, the pairs' rows X on the N side.  A work item is one tile of W times up
+// to BN pairs of its group, over all of k.  Which groups have pairs, and how many, is known on
+// the device only: every CTA reads the plan's offsets at its start, makes the prefix sum of the
+// groups' item counts in shared memory, and takes items blockIdx.x, + gridDim.x, ...  Items of one
+// group are neighbours, those of one W tile next to each other, so what runs at the same time
+// shares W and X in L2 and W leaves HBM once.
+//
+//   * The N of an item is what its pairs need (a group's pairs are cut evenly, in steps of 16):
+//     groups of any size waste less than 16 columns of tensor-core time per tile.
+//   * X rows are gathered by TMA (tile::gather4, four rows by their numbers per instruction), one
+//     lane of a warp for every four rows; their scales by the scale-writer warps, which read them by
+//     row anyway.  No gathered or padded copy of A is ever made.
+//   * Gated: a tile holds 64 gate rows and their 64 up rows, 16 and 16 in each warp's lane quarter, so
+//     that the two accumulators of an output meet in one warp (lane l and l + 16): one exchange
+//     between lanes, and D is written once, at its final size.
+//   * A thread holds one W row (a column of D), so the lanes of a warp write 128 (gated 64)
+//     contiguous bytes of one row of D at a time: rows go wherever the plan says, with no
+//     staging.
+//
+// Roles (352 threads): warp 0 TMA producer of W, warp 1 MMA issuer (owns tensor memory), warps 2-5
+// scale writers, warps 6-9 epilogue (one TMEM lane quarter each), warp 10 gathers X.
+// Every wait is bounded, as in the other kernels.
+#pragma once
+
+#include "decode_kernel.cuh"
+#include "route_kernel.cuh"
+
+namespace b200 {
+
+constexpr int kGroupedThreads = 352;
+constexpr int kGroupedMaxStages = 8;
+constexpr int kGroupedMaxBN = 192;   // two accumulators and four slots of scales fit tensor memory
+constexpr int kGroupedFetchAhead = 3;
+
+struct GroupedParams {
+  const uint8_t* sw;          // W's scales, row-major
+  const uint8_t* sx;          // X's
+  const int32_t* offsets;     // the plan
+  const int32_t* order;
+  const float* row_weights;   // or null
+  float* d;
+  int64_t ldd;
+  int64_t ld_sw, ld_sx;
+  int32_t rows, groups;       // pairs; groups of the plan
+  int32_t n;                  // columns of D
+  int32_t b_group_rows;       // rows of W from one group to the next
+  int32_t a_rows, pairs_per_a_row;
+  int32_t tiles;              // W tiles of a group
+  int32_t k_blocks, kblocks32;
+  int32_t BN, stages;
+  int32_t w_tile_bytes;       // what the loads of a W tile credit to the barrier
+  int32_t align_w, align_x;   // scale rows start on multiples of 16, 4 or 1 bytes
+  uint32_t idesc;             // without N
+  uint32_t wait_budget_us;
+  int32_t* error;
+};
+
+__host__ __device__ inline int grouped_stage_bytes(int BN) { return kTileM * 128 + BN * 128; }
+__host__ __device__ inline int grouped_atoms(int BN, int ka) { return ka * (1 + (BN > 128 ? 2 : 1)); }
+__host__ __device__ inline int grouped_staging_bytes(int BN) { return kGroupedFetchAhead * (kTileM + BN) * 16; }
+__host__ __device__ inline int grouped_table_bytes(int groups) { return (2 * (groups + 1) * 4 + 15) / 16 * 16; }
+constexpr int kGroupedBarrierBytes = 256;
+__host__ __device__ inline int grouped_smem_bytes(int BN, int stages, int ka, int groups) {
+  return 1024 + stages * (grouped_stage_bytes(BN) + grouped_atoms(BN, ka) * 512) + grouped_staging_bytes(BN) +
+         grouped_table_bytes(groups) + kGroupedBarrierBytes;
+}
+
+// One item: a tile of a group's W times pairs order[p0 .. p0 + count).
+struct GroupedItem {
+  int group, tile, p0, count;
+};
+
+// Item `it` from the prefix sums (first[g] = items of the groups before g) and the groups' starts.
+__device__ __forceinline__ GroupedItem grouped_item(const int32_t* first, const int32_t* start, int groups, int tiles,
+                                                    int BN, int it) {
+  int lo = 0, hi = groups;  // first[lo] <= it < first[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first[mid] <= it) lo = mid; else hi = mid;
+  }
+  const int pairs = start[lo + 1] - start[lo];
+  const int cuts = (pairs + BN - 1) / BN;
+  const int width = ((pairs + cuts - 1) / cuts + 15) & ~15;  // <= BN, a multiple of 16
+  const int local = it - first[lo];
+  GroupedItem item;
+  item.group = lo;
+  item.tile = local / cuts;
+  const int cut = local - item.tile * cuts;
+  item.p0 = start[lo] + cut * width;
+  item.count = min(width, pairs - cut * width);  // (at least 1: all cuts but one hold width <= BN each)
+  return item;
+}
+
+// Four rows of a 128-byte wide box, by their numbers (tile::gather4).
+__device__ __forceinline__ void tma_gather4(uint32_t smem_dst, const CUtensorMap* tm, uint32_t bar, int32_t x,
+                                            int32_t r0, int32_t r1, int32_t r2, int32_t r3) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+      :
+      : "r"(smem_dst), "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3)
+      : "memory");
+}
+
+// 16 bytes of a scale row into this thread's own staging slot: `valid` of them exist, the others
+// become zero.  Rows that start on 16- or 4-byte boundaries are copied asynchronously.
+__device__ __forceinline__ void fetch_scales(uint32_t dst, const uint8_t* src, int valid, int align) {
+  if (align == 16) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid) : "memory");
+  } else if (align == 4) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int left = min(4, max(0, valid - 4 * j));
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + 4 * j), "l"(src + (left > 0 ? 4 * j : 0)),
+                   "r"(left)
+                   : "memory");
+    }
+  } else {
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (j < valid) w[j >> 2] |= static_cast<uint32_t>(src[j]) << (8 * (j & 3));
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                 : "memory");
+  }
+}
+
+// kGated: silu(gate) * up.  KIND: kKindMxf8 (also fp4 weights under fp8 rows) or kKindMxf4.
+template <int KIND, bool kGated>
+__global__ void __launch_bounds__(kGroupedThreads, 1)
+    grouped_mx_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+                      const GroupedParams p) {
+  constexpr int kSfBytes = KIND == kKindMxf4 ? 8 : 4;  // scale bytes per row and k-block
+  constexpr int kKa = kSfBytes / 4;                    // atoms along k per operand
+  constexpr int kUnitsPerChunk = 16 / kSfBytes;        // k-blocks served by one 16-byte fetch of a scale row
+  constexpr int kTileCols = kGated ? 64 : 128;         // columns of D per tile
+  constexpr unsigned kAll = 0xffffffffu;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t pad = ((raw_addr + 1023u) & ~1023u) - raw_addr;
+  uint8_t* smem = smem_raw + pad;
+  const uint32_t smem_base = raw_addr + pad;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int stages = p.stages, BN = p.BN;
+  const int x_halves = BN > 128 ? 2 : 1;
+  const uint32_t stage_bytes = static_cast<uint32_t>(grouped_stage_bytes(BN));
+  const uint32_t atoms = static_cast<uint32_t>(grouped_atoms(BN, kKa));
+  const uint32_t atom_bytes = atoms * 512u;
+  const uint32_t atom_base = smem_base + stages * stage_bytes;
+  const uint32_t staging_base = atom_base + stages * atom_bytes;
+  const uint32_t table_off = staging_base + static_cast<uint32_t>(grouped_staging_bytes(BN)) - smem_base;
+  int32_t* first = reinterpret_cast<int32_t*>(smem + table_off);  // [groups + 1]
+  int32_t* start = first + p.groups + 1;                          // [groups + 1]
+  const uint32_t bar_base = smem_base + table_off + static_cast<uint32_t>(grouped_table_bytes(p.groups));
+  auto full_bar = [&](int s) { return bar_base + 8u * s; };
+  auto empty_bar = [&](int s) { return bar_base + 8u * (kGroupedMaxStages + s); };
+  auto acc_full_bar = [&](int b) { return bar_base + 8u * (2 * kGroupedMaxStages + b); };
+  auto acc_empty_bar = [&](int b) { return bar_base + 8u * (2 * kGroupedMaxStages + 2 + b); };
+  const uint32_t drain_bar = bar_base + 8u * (2 * kGroupedMaxStages + 4);
+  constexpr int kBarriers = 2 * kGroupedMaxStages + 5;
+  static_assert(8 * kBarriers + 8 <= kGroupedBarrierBytes, "barrier region too small");
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (bar_base - smem_base) + 8 * kBarriers);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const uint64_t budget_ns = static_cast<uint64_t>(p.wait_budget_us) * 1000ull;
+
+  if (warp == 2) {
+    if (lane < kBarriers) {
+      // full: the two producers' arrive.expect_tx and one arrival per scale-writer warp; empty,
+      // accumulator full, drain: one tcgen05.commit; accumulator empty: the epilogue warps
+      uint32_t count = 1u;
+      if (lane < kGroupedMaxStages) count = 6u;
+      if (lane == 2 * kGroupedMaxStages + 2 || lane == 2 * kGroupedMaxStages + 3) count = 4u;
+      mbar_init(bar_base + 8u * static_cast<uint32_t>(lane), count);
+    }
+    if (lane == 0) *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), 512u);
+    tmem_relinquish();
+  }
+  if (warp == 0 && lane == 0) {
+    prefetch_tensormap(&tmW);
+    prefetch_tensormap(&tmX);
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // Whatever the array holds, the starts become an ascending sequence within 0 .. rows: no item
+  // reaches outside `order`, and there are no more items than the launcher allowed for.
+  for (int g = threadIdx.x; g <= p.groups; g += kGroupedThreads) start[g] = min(max(p.offsets[g], 0), p.rows);
+  __syncthreads();
+  if (warp == 2) {
+    int sum = 0, high = start[0];  // items and highest start so far
+    for (int g0 = 0; g0 < p.groups; g0 += 32) {
+      const int g = g0 + lane;
+      int end = g < p.groups ? start[g + 1] : 0;
+      if (lane == 0) end = max(end, high);
+#pragma unroll
+      for (int s = 1; s < 32; s <<= 1) {
+        const int up = __shfl_up_sync(kAll, end, s);
+        if (lane >= s) end = max(end, up);
+      }
+      int begin = __shfl_up_sync(kAll, end, 1);
+      if (lane == 0) begin = high;
+      const int own = (end - begin + BN - 1) / BN * p.tiles;
+      int v = own;
+#pragma unroll
+      for (int s = 1; s < 32; s <<= 1) {
+        const int up = __shfl_up_sync(kAll, v, s);
+        if (lane >= s) v += up;
+      }
+      if (g < p.groups) {
+        first[g] = sum + v - own;
+        start[g + 1] = end;
+      }
+      sum += __shfl_sync(kAll, v, 31);
+      high = __shfl_sync(kAll, end, 31);
+    }
+    if (lane == 0) first[p.groups] = sum;
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  const int n_items = first[p.groups];
+  const int step = static_cast<int>(gridDim.x);
+  auto item_at = [&](int it) { return grouped_item(first, start, p.groups, p.tiles, BN, it); };
+  // The pair at place p0 + r of an item's run, or -1.
+  auto pair_at = [&](const GroupedItem& item, int r) {
+    if (r >= item.count) return -1;
+    const int q = p.order[item.p0 + r];
+    return q >= 0 && q < p.rows ? q : -1;
+  };
+  auto a_row_of = [&](int q) { return q < 0 ? -1 : min(q / p.pairs_per_a_row, p.a_rows - 1); };
+  auto columns_of = [&](const GroupedItem& item) { return max(16, (item.count + 15) & ~15); };
+
+  if (warp == 0) {
+    // ------------------------------ W producer ------------------------------
+    const uint32_t el = elect_one() ? 1u : 0u;
+    int s = 0;
+    uint32_t ph = 0;
+    bool alive = true;
+    for (int it = blockIdx.x; it < n_items && alive; it += step) {
+      const GroupedItem item = item_at(it);
+      const int base = item.group * p.b_group_rows;
+      for (int kb = 0; kb < p.k_blocks; ++kb) {
+        if (!__all_sync(kAll, mbar_wait_bounded(empty_bar(s), ph ^ 1u, abort_flag, budget_ns))) {
+          if (el) {
+            leave_error(p.error, kErrProducerWait);
+            *abort_flag = 1;
+          }
+          alive = false;
+          break;
+        }
+        mbar_expect_tx_p(full_bar(s), static_cast<uint32_t>(p.w_tile_bytes), el);
+        const uint32_t dst = smem_base + s * stage_bytes;
+        if constexpr (kGated) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int row = base + item.tile * 64 + 16 * q;
+            tma_load_2d_g<false>(dst + (32 * q) * 128, &tmW, full_bar(s), kb * 128, row, el);
+            tma_load_2d_g<false>(dst + (32 * q + 16) * 128, &tmW, full_bar(s), kb * 128, row + p.n, el);
+          }
+        } else {
+          tma_load_2d_g<false>(dst, &tmW, full_bar(s), kb * 128, base + item.tile * kTileM, el);
+        }
+        if (++s == stages) { s = 0; ph ^= 1u; }
+      }
+    }
+    if (*abort_flag != 0 && el) {
+      // give the copies already issued time to land before the CTA exits
+      const uint64_t t_end = global_timer_ns() + 200000;
+      while (global_timer_ns() < t_end) __nanosleep(1000);
+    }
+    __syncwarp();
+  } else if (warp == 10) {
+    // ------------------------------ X gather ------------------------------
+    // Lane l gathers rows 4 l .. 4 l + 3 of the item's X, and those 128 further on.  Rows that do not
+    // exist inside a group of four are read as the group's first one; groups without any row
+    // are left as they are (their columns are computed and never read).
+    int s = 0;
+    uint32_t ph = 0;
+    bool alive = true;
+    for (int it = blockIdx.x; it < n_items && alive; it += step) {
+      const GroupedItem item = item_at(it);
+      int row[2][4];
+      bool mine[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r0 = 128 * h + 4 * lane;
+        mine[h] = r0 < item.count;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) row[h][j] = a_row_of(pair_at(item, r0 + j));
+        if (row[h][0] < 0) row[h][0] = 0;
+#pragma unroll
+        for (int j = 1; j < 4; ++j)
+          if (row[h][j] < 0) row[h][j] = row[h][0];
+      }
+      const uint32_t bytes = static_cast<uint32_t>(max(0, (item.count + 3) >> 2)) * 512u;
+      for (int kb = 0; kb < p.k_blocks; ++kb) {
+        if (!__all_sync(kAll, mbar_wait_bounded(empty_bar(s), ph ^ 1u, abort_flag, budget_ns))) {
+          if (lane == 0) {
+            leave_error(p.error, kErrProducerWait);
+            *abort_flag = 1;
+          }
+          alive = false;
+          break;
+        }
+        if (lane == 0) mbar_expect_tx(full_bar(s), bytes);
+        __syncwarp();
+        const uint32_t dst = smem_base + s * stage_bytes + kTileM * 128 + static_cast<uint32_t>(lane) * 512u;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (mine[h])
+            tma_gather4(dst + h * 128u * 128u, &tmX, full_bar(s), kb * 128, row[h][0], row[h][1], row[h][2], row[h][3]);
+        if (++s == stages) { s = 0; ph ^= 1u; }
+      }
+    }
+    if (*abort_flag != 0) {
+      const uint64_t t_end = global_timer_ns() + 200000;
+      while (global_timer_ns() < t_end) __nanosleep(1000);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------- MMA issuer -------------------------------
+    const uint32_t el = elect_one() ? 1u : 0u;
+    const uint64_t op_hi64 = make_smem_desc_hi(16, 1024, 2);  // K-major, 128-byte swizzle
+    const uint32_t op_hi = static_cast<uint32_t>(op_hi64 >> 32);
+    const uint32_t a_lo0 = static_cast<uint32_t>(op_hi64) | (smem_base >> 4);
+    const uint32_t b_lo0 = static_cast<uint32_t>(op_hi64) | ((smem_base + kTileM * 128) >> 4);
+    const uint64_t sf_hi64 = make_smem_desc_hi(0, 128, 0);
+    const uint32_t sf_hi = static_cast<uint32_t>(sf_hi64 >> 32);
+    const uint32_t sf_lo0 = static_cast<uint32_t>(sf_hi64) | (atom_base >> 4);
+    const uint32_t sf_t0 = tmem_base + 2u * static_cast<uint32_t>(BN);
+    const uint32_t sf_cols = 4u * atoms;
+    const uint32_t sfb_half = 4u * static_cast<uint32_t>(x_halves);
+    int s = 0, buf = 0, sf_q = 0;
+    uint32_t ph = 0, acc_ph = 0;
+    bool ok = true;
+    for (int it = blockIdx.x; it < n_items && ok; it += step) {
+      const GroupedItem item = item_at(it);
+      const uint32_t idesc = p.idesc | (static_cast<uint32_t>(columns_of(item)) >> 3) << 17;
+      if (!__all_sync(kAll, mbar_wait_bounded(acc_empty_bar(buf), acc_ph ^ 1u, abort_flag, budget_ns))) {
+        if (el) {
+          leave_error(p.error, kErrMmaWaitAcc);
+          *abort_flag = 1;
+        }
+        break;
+      }
+      tc_fence_after_sync();
+      const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(buf * BN);
+      uint32_t accumulate = 0;
+      for (int kb = 0; kb < p.k_blocks; ++kb) {
+        if (!__all_sync(kAll, mbar_wait_bounded(full_bar(s), ph, abort_flag, budget_ns))) {
+          if (el) {
+            leave_error(p.error, kErrMmaWaitFull);
+            *abort_flag = 1;
+          }
+          ok = false;
+          break;
+        }
+        tc_fence_after_sync();
+        const uint32_t a_lo = a_lo0 + s * (stage_bytes >> 4), b_lo = b_lo0 + s * (stage_bytes >> 4);
+        const uint32_t sfa_t = sf_t0 + static_cast<uint32_t>(sf_q) * sf_cols, sfb_t = sfa_t + 4u * kKa;
+        {
+          uint32_t src = sf_lo0 + s * (atom_bytes >> 4), dst = sfa_t;
+          for (uint32_t a = 0; a < atoms; ++a, src += 32, dst += 4) tmem_cp_atom_g<false>(dst, src, sf_hi, el);
+        }
+        if constexpr (KIND == kKindMxf8) {
+          mma_mxf8f6f4_g<false>(d_tmem, a_lo, op_hi, b_lo, op_hi, idesc, sfa_t, sfb_t, accumulate, el);
+          mma_mxf8f6f4_g<false>(d_tmem, a_lo + 2, op_hi, b_lo + 2, op_hi, idesc_with_sf_ids(idesc, 1, 1), sfa_t, sfb_t, 1u, el);
+          mma_mxf8f6f4_g<false>(d_tmem, a_lo + 4, op_hi, b_lo + 4, op_hi, idesc_with_sf_ids(idesc, 2, 2), sfa_t, sfb_t, 1u, el);
+          mma_mxf8f6f4_g<false>(d_tmem, a_lo + 6, op_hi, b_lo + 6, op_hi, idesc_with_sf_ids(idesc, 3, 3), sfa_t, sfb_t, 1u, el);
+        } else {
+          const uint32_t id2 = idesc_with_sf_ids(idesc, 2, 2);
+          mma_mxf4_g<false>(d_tmem, a_lo, op_hi, b_lo, op_hi, idesc, sfa_t, sfb_t, accumulate, el);
+          mma_mxf4_g<false>(d_tmem, a_lo + 2, op_hi, b_lo + 2, op_hi, id2, sfa_t, sfb_t, 1u, el);
+          mma_mxf4_g<false>(d_tmem, a_lo + 4, op_hi, b_lo + 4, op_hi, idesc, sfa_t + 4u, sfb_t + sfb_half, 1u, el);
+          mma_mxf4_g<false>(d_tmem, a_lo + 6, op_hi, b_lo + 6, op_hi, id2, sfa_t + 4u, sfb_t + sfb_half, 1u, el);
+        }
+        accumulate = 1u;
+        tc_commit_g<false>(empty_bar(s), el);  // frees the stage once these MMAs and copies have read it
+        if (++sf_q == kDecodeSfSlots) sf_q = 0;
+        if (++s == stages) { s = 0; ph ^= 1u; }
+      }
+      if (!ok) break;
+      tc_commit_g<false>(acc_full_bar(buf), el);
+      if (++buf == 2) { buf = 0; acc_ph ^= 1u; }
+    }
+    // nothing may still be executing when tensor memory is released
+    tc_commit_g<false>(drain_bar, el);
+    int dummy = 0;
+    if (!__all_sync(kAll, mbar_wait_bounded(drain_bar, 0, &dummy, budget_ns)) && el) {
+      leave_error(p.error, kErrDrainWait);
+      *abort_flag = 1;
+    }
+    __syncwarp();
+  } else if (warp < 6) {
+    // ------------------------------ scale writers ------------------------------
+    // Thread r (0..127) owns row r of the W tile and rows r and r + 128 of X.  As in the small-m
+    // kernel it fetches its rows' scale bytes 16 at a time, a few fetches ahead, and turns them
+    // into the atoms of the k-blocks that share the fetch.
+    const int r = (warp - 2) * 32 + lane;
+    const uint32_t slot_off = static_cast<uint32_t>((r & 31) * 16 + (r >> 5) * 4);
+    const uint32_t stage_w = staging_base + static_cast<uint32_t>(r) * 16u;
+    const uint32_t kStagingSlot = static_cast<uint32_t>(kTileM + BN) * 16u;
+    // The k-blocks of a fetch are handed over together (one proxy fence) where the ring holds two
+    // such chunks, one by one in a shorter ring, which a chunk would fill.
+    const bool flush_each = stages < 2 * kUnitsPerChunk;
+    // (BN need not reach 128 or 256: threads beyond it have no slot)
+    const bool slot0 = r < BN, slot1 = r + 128 < BN;
+    int f_it = blockIdx.x, f_kb = 0;
+    const uint8_t *f_w = nullptr, *f_x0 = nullptr, *f_x1 = nullptr;  // rows of the item being fetched, or null
+    auto enter = [&]() {  // the item at the fetch cursor
+      f_w = f_x0 = f_x1 = nullptr;
+      if (f_it >= n_items) return;
+      const GroupedItem item = item_at(f_it);
+      int col, row;
+      if constexpr (kGated) {
+        col = item.tile * 64 + (r >> 5) * 16 + (r & 15);
+        row = col + ((r & 16) ? p.n : 0);
+      } else {
+        col = row = item.tile * kTileM + r;
+      }
+      if (col < p.n) f_w = p.sw + (static_cast<int64_t>(item.group) * p.b_group_rows + row) * p.ld_sw;
+      const int a0 = a_row_of(pair_at(item, r));
+      if (a0 >= 0) f_x0 = p.sx + a0 * p.ld_sx;
+      if (slot1) {
+        const int a1 = a_row_of(pair_at(item, r + 128));
+        if (a1 >= 0) f_x1 = p.sx + a1 * p.ld_sx;
+      }
+    };
+    auto fetch = [&](int slot) {
+      if (f_it < n_items) {
+        const int col = (f_kb * kSfBytes) & ~15;
+        const int valid = min(16, p.kblocks32 - col);
+        const uint32_t dst = stage_w + slot * kStagingSlot;
+        fetch_scales(dst, f_w != nullptr ? f_w + col : p.sw, f_w != nullptr ? valid : 0, p.align_w);
+        if (slot0) fetch_scales(dst + kTileM * 16u, f_x0 != nullptr ? f_x0 + col : p.sx, f_x0 != nullptr ? valid : 0, p.align_x);
+        if (slot1)
+          fetch_scales(dst + kTileM * 32u, f_x1 != nullptr ? f_x1 + col : p.sx, f_x1 != nullptr ? valid : 0, p.align_x);
+        f_kb = (f_kb | (kUnitsPerChunk - 1)) + 1;
+        if (f_kb >= p.k_blocks) {
+          f_kb = 0;
+          f_it += step;
+          enter();
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");  // always: the group count stays in step
+    };
+    enter();
+    for (int j = 0; j < kGroupedFetchAhead; ++j) fetch(j);
+    int s = 0, kb = 0, c_slot = 0;
+    uint32_t ph = 0;
+    bool alive = true;
+    for (int it = blockIdx.x; it < n_items && alive;) {
+      const int in_chunk = min(kUnitsPerChunk - (kb & (kUnitsPerChunk - 1)), p.k_blocks - kb);
+      asm volatile("cp.async.wait_group %0;" ::"n"(kGroupedFetchAhead - 1) : "memory");
+      uint4 cw, cx0 = make_uint4(0, 0, 0, 0), cx1 = make_uint4(0, 0, 0, 0);
+      const uint32_t from = stage_w + c_slot * kStagingSlot;
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(cw.x), "=r"(cw.y), "=r"(cw.z), "=r"(cw.w) : "r"(from));
+      if (slot0)
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(cx0.x), "=r"(cx0.y), "=r"(cx0.z), "=r"(cx0.w)
+                     : "r"(from + kTileM * 16u));
+      if (slot1)
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(cx1.x), "=r"(cx1.y), "=r"(cx1.z), "=r"(cx1.w)
+                     : "r"(from + kTileM * 32u));
+      int s2 = s;
+      uint32_t ph2 = ph;
+      for (int u = 0; u < in_chunk; ++u) {
+        // the stage's previous atoms have been copied to tensor memory (its MMAs are done)
+        if (!__all_sync(kAll, mbar_wait_bounded(empty_bar(s2), ph2 ^ 1u, abort_flag, budget_ns))) {
+          if (lane == 0) {
+            leave_error(p.error, kErrProducerWait);
+            *abort_flag = 1;
+          }
+          alive = false;
+          break;
+        }
+        const int sub = ((kb + u) & (kUnitsPerChunk - 1)) * kKa;
+        const uint32_t aw = atom_base + s2 * atom_bytes + slot_off, ax = aw + kKa * 512u;
+#pragma unroll
+        for (int a = 0; a < kKa; ++a) {
+          asm volatile("st.shared.u32 [%0], %1;" ::"r"(aw + 512u * a), "r"(pick_word(cw, sub + a)) : "memory");
+          asm volatile("st.shared.u32 [%0], %1;" ::"r"(ax + 512u * (a * x_halves)), "r"(pick_word(cx0, sub + a)) : "memory");
+          if (x_halves == 2)
+            asm volatile("st.shared.u32 [%0], %1;" ::"r"(ax + 512u * (a * 2 + 1)), "r"(pick_word(cx1, sub + a)) : "memory");
+        }
+        if (flush_each) {
+          fence_proxy_async_shared_cta();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(full_bar(s2));
+        }
+        if (++s2 == stages) { s2 = 0; ph2 ^= 1u; }
+      }
+      if (!alive) break;
+      if (!flush_each) {
+        fence_proxy_async_shared_cta();  // these writes -> visible to tcgen05.cp (one fence per chunk)
+        __syncwarp();
+      }
+      if (!flush_each && lane == 0) {
+        int s3 = s;
+        for (int u = 0; u < in_chunk; ++u) {
+          mbar_arrive(full_bar(s3));
+          if (++s3 == stages) s3 = 0;
+        }
+      }
+      fetch(c_slot);
+      if (++c_slot == kGroupedFetchAhead) c_slot = 0;
+      s = s2;
+      ph = ph2;
+      kb += in_chunk;
+      if (kb == p.k_blocks) {
+        kb = 0;
+        it += step;
+      }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+  } else {
+    // -------------------------------- epilogue --------------------------------
+    const int quarter = warp & 3;  // the TMEM lane quarter this warp can read
+    int buf = 0;
+    uint32_t acc_ph = 0;
+    for (int it = blockIdx.x; it < n_items; it += step) {
+      const GroupedItem item = item_at(it);
+      const bool got = mbar_wait_bounded(acc_full_bar(buf), acc_ph, abort_flag, budget_ns);
+      if (!__all_sync(kAll, got)) {
+        if (lane == 0) {
+          leave_error(p.error, kErrEpilogueWait);
+          *abort_flag = 1;
+        }
+        break;
+      }
+      tc_fence_after_sync();
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(buf * BN);
+      const int col = item.tile * kTileCols + (kGated ? quarter * 16 + (lane & 15) : quarter * 32 + lane);
+      const bool in = col < p.n;
+      for (int c = 0; c < item.count; c += 32) {
+        uint32_t acc[32];
+        tmem_ld_32x32(taddr + static_cast<uint32_t>(c), acc);
+        const int q_mine = pair_at(item, c + lane);
+        const float w_mine = p.row_weights != nullptr && q_mine >= 0 ? p.row_weights[q_mine] : 1.0f;
+        tmem_ld_wait();
+        if constexpr (kGated) {
+          // lanes 0-15 hold the gate, 16-31 the up product: the lower lanes finish the even columns,
+          // the upper ones the odd
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const uint32_t give = lane < 16 ? acc[j + 1] : acc[j];
+            const float other = __uint_as_float(__shfl_xor_sync(kAll, give, 16));
+            const float kept = __uint_as_float(lane < 16 ? acc[j] : acc[j + 1]);
+            const float y = silu_f32(lane < 16 ? kept : other) * (lane < 16 ? other : kept);
+            const int from = j + (lane >> 4);
+            const int q = __shfl_sync(kAll, q_mine, from);
+            const float w = __shfl_sync(kAll, w_mine, from);
+            if (in && q >= 0) p.d[q * p.ldd + col] = p.row_weights != nullptr ? y * w : y;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const int q = __shfl_sync(kAll, q_mine, j);
+            const float w = __shfl_sync(kAll, w_mine, j);
+            const float y = __uint_as_float(acc[j]);
+            if (in && q >= 0) p.d[q * p.ldd + col] = p.row_weights != nullptr ? y * w : y;
+          }
+        }
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty_bar(buf));
+      if (++buf == 2) { buf = 0; acc_ph ^= 1u; }
+    }
+  }
+
+  tc_fence_before_sync();
+  __syncwarp();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem_base, 512u);
+}
+
+// D[t] = the sum of row t's `per` pairs, ascending; pairs in no group add nothing.
+__global__ void __launch_bounds__(256) sum_pairs_kernel(const float* pairs, const int32_t* ids, int groups, int per,
+                                                        int64_t rows, int n, float* d, int64_t ldd) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (int64_t t = blockIdx.y; t < rows; t += gridDim.y) {
+    for (int col = blockIdx.x * 256 + threadIdx.x; col < n; col += gridDim.x * 256) {
+      float sum = 0.0f;
+      for (int s = 0; s < per; ++s) {
+        const int64_t q = t * per + s;
+        const int id = ids[q];
+        if (id >= 0 && id < groups) sum += pairs[q * n + col];
+      }
+      d[t * ldd + col] = sum;
+    }
+  }
+}
+
+}  // namespace b200

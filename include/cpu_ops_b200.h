@@ -264,6 +264,151 @@ CPUOPS_B200_API int cpuops_b200_profile_collect(double* total_ms, int32_t* launc
 CPUOPS_B200_API int cpuops_b200_prepare_b(const cpuops_b200_gemm_desc* d, void** handle);
 CPUOPS_B200_API int cpuops_b200_release_b(void* handle);
 
+/* ---- projections whose weights are chosen per row -------------------------------------------
+ * No counterpart in the reference: the products of a layer of experts, the routing that picks
+ * them, and low-rank adapters beside a shared projection.  Unlike cpuops_b200_gemm these take
+ * device memory only (a pointer to host memory, or to another device's, is refused with
+ * CPUOPS_B200_STATUS_INVALID_ARGUMENTS), since what they compute depends on index arrays that the
+ * host never reads.  `stream`, `flags` (CPUOPS_B200_FLAG_ASYNC), `device` and `memory_space` mean
+ * what they mean in cpuops_b200_gemm_desc (MEM_DEVICE skips the check of the pointers), locking
+ * and stream capture are the same too.  Calls whose comment says so use the stream's workspace:
+ * graphs captured from one stream share it, so replay such graphs one after another, not side by
+ * side.  Results are bit-identical from run to run.  Outputs must not overlap inputs or one
+ * another, except where a comment allows it. */
+
+/* Element types of rows that are not quantised. */
+enum { CPUOPS_B200_TYPE_F32 = 0, CPUOPS_B200_TYPE_F16 = 1, CPUOPS_B200_TYPE_BF16 = 2 };
+
+/* How logits become scores. */
+enum { CPUOPS_B200_SCORE_SOFTMAX = 0, CPUOPS_B200_SCORE_SIGMOID = 1 };
+
+#define CPUOPS_B200_MAX_GROUPS 1024 /* experts of a route call, groups of a plan */
+#define CPUOPS_B200_MAX_TOP_K 32
+
+/* A row plan sorts "pairs" (a row and one of the groups it goes to, numbered row by row: pair
+ * q = row * pairs_per_row + slot) by group: offsets[g] .. offsets[g + 1] are the places in
+ * `order` of the pairs of group g, in ascending order.  Pairs whose id lies outside [0, groups)
+ * belong to no group; as many entries at the end of `order` are -1. */
+
+/* Routing: for every token
+ *     score[e]  = softmax(logits)[e]  or  1 / (1 + exp(-logits[e]))
+ *     choice[e] = score[e] + bias[e]
+ * With n_groups > 1 the experts are cut into n_groups runs of equal length; a run counts as the
+ * sum of its `group_best` (1 or 2) best choices, and only the top_groups best runs stay (of
+ * equal ones the first).  ids are the top_k experts of those by choice, the best first (of equal
+ * ones the first); weights their scores (without bias), divided by their sum if `renormalize`
+ * (a sum of zero gives zeros), times `scale`.
+ * An expert whose logit or bias is NaN or -inf is out, also of the softmax's sum; where fewer than top_k
+ * are left, the remaining ids are -1 and their weights 0.  A logit of +inf counts as the largest
+ * number there is (several share the softmax).
+ * Choices are made in double precision: which experts a token gets does not hang on rounding.
+ * offsets (experts + 1) and order (tokens * top_k): the plan of ids; both NULL: none is made.
+ * Uses the stream's workspace when a plan of more than 4096 pairs is made. */
+typedef struct cpuops_b200_route_desc {
+  uint32_t struct_size; /* sizeof(cpuops_b200_route_desc), checked */
+  int32_t tokens, experts, top_k;
+  int32_t scoring;      /* CPUOPS_B200_SCORE_*                     */
+  int32_t n_groups, top_groups, group_best;
+  int32_t renormalize;
+  float scale;
+  int32_t logits_type;  /* CPUOPS_B200_TYPE_*                      */
+  int32_t ld_logits;    /* elements from one token to the next     */
+  const void* logits;
+  const float* bias;    /* one per expert, or NULL                 */
+  int32_t* ids;         /* tokens x top_k, contiguous              */
+  float* weights;       /* the same                                */
+  int32_t* offsets;
+  int32_t* order;
+  void* stream;
+  uint32_t flags;
+  int32_t device;
+  int32_t memory_space;
+} cpuops_b200_route_desc;
+CPUOPS_B200_API int cpuops_b200_route(const cpuops_b200_route_desc* desc);
+
+/* The plan of `rows` ids (the second half of cpuops_b200_route, for ids from elsewhere). */
+typedef struct cpuops_b200_group_rows_desc {
+  uint32_t struct_size;
+  int32_t rows, groups;
+  const int32_t* ids;   /* rows       */
+  int32_t* offsets;     /* groups + 1 */
+  int32_t* order;       /* rows       */
+  void* stream;
+  uint32_t flags;
+  int32_t device;
+  int32_t memory_space;
+} cpuops_b200_group_rows_desc;
+CPUOPS_B200_API int cpuops_b200_group_rows(const cpuops_b200_group_rows_desc* desc);
+
+/* The experts' products, on MX operands (the formats, scales and leading dimensions of
+ * cpuops_b200_gemm_desc).  For every pair q of group g in the plan
+ *     acc[j] = sum_k A[q / pairs_per_a_row][k] * B_g[j][k]                 (f32 sums)
+ *     y[j]   = acc[j],  or  silu(acc[j]) * acc[n + j]  with `gated`
+ *     y[j]  *= row_weights[q]                                              (if given)
+ *     D[q]   = y       if pairs_per_d_row == 1 (rows of pairs in no group are left as they were)
+ *     D[t]   = the sum of y over t's pairs_per_d_row pairs, ascending, otherwise (pairs in no group
+ *              add nothing; a row without any is zero).  `ids` are then the ids the plan was
+ *              made from, and the call uses the stream's workspace (rows * n floats).
+ * B_g is n (gated: 2n, the gate's rows first) rows of k, the first of them row g * b_group_rows
+ * of B.  A and B: 16-byte aligned, rows a multiple of 16 bytes apart, an even k for e2m1.  A
+ * and B may both be 8-bit formats, both e2m1, or e2m1 weights under 8-bit rows (then B 32-byte
+ * aligned, its rows a multiple of 32 bytes apart, k a multiple of 128).  The scale arrays may lie
+ * anywhere; 16-byte aligned rows of them are read fastest. */
+typedef struct cpuops_b200_gemm_grouped_desc {
+  uint32_t struct_size;
+  int32_t a_format, b_format; /* CPUOPS_B200_FMT_E4M3, _E5M2, _E2M1           */
+  int32_t rows;               /* pairs of the plan (length of order)         */
+  int32_t n, k, groups;
+  int32_t gated;
+  int32_t a_rows;             /* rows of A                                   */
+  int32_t pairs_per_a_row, pairs_per_d_row;
+  int32_t b_group_rows;       /* rows of B from one group to the next        */
+  int32_t lda, ldb, ld_scales_a, ld_scales_b;
+  int32_t ldd;
+  const void* a;
+  const void* b;
+  const void* a_scales;
+  const void* b_scales;
+  const int32_t* offsets;     /* groups + 1                                  */
+  const int32_t* order;       /* rows                                        */
+  const int32_t* ids;         /* rows; pairs_per_d_row > 1 only              */
+  const float* row_weights;   /* rows, or NULL                               */
+  float* d;                   /* rows / pairs_per_d_row rows of n, row-major */
+  void* stream;
+  uint32_t flags;
+  int32_t device;
+  int32_t memory_space;
+} cpuops_b200_gemm_grouped_desc;
+CPUOPS_B200_API int cpuops_b200_gemm_grouped(const cpuops_b200_gemm_grouped_desc* desc);
+
+/* Low-rank adapters of many requests beside a shared projection (whose result is C):
+ *     D[t] = C[t] + scales[g] * (X[t] A_g^T) B_g^T     with g = ids[t]
+ * and D[t] = C[t] where ids[t] lies outside [0, adapters).  A_g is `rank` rows of k (rows lda,
+ * adapters a_stride elements apart), B_g n rows of `rank` (ldb, b_stride).  An adapter of a smaller
+ * rank is padded with zeros.  X may be f32 with A and B f16 or bf16, or all three the same
+ * 16-bit type; C, D and every sum are f32.  D may be C.  16-byte aligned rows of X, A and B are read
+ * fastest.  Uses the stream's workspace from a few hundred rows on. */
+typedef struct cpuops_b200_adapters_desc {
+  uint32_t struct_size;
+  int32_t m, n, k, rank, adapters;
+  int32_t x_type, w_type;   /* CPUOPS_B200_TYPE_*                   */
+  int32_t ldx, lda, ldb, ldc, ldd;
+  int64_t a_stride, b_stride;
+  const void* x;
+  const void* a;
+  const void* b;
+  const int32_t* ids;       /* m                                    */
+  const float* scales;      /* one per adapter, or NULL (all 1)     */
+  const float* c;
+  float* d;
+  void* stream;
+  uint32_t flags;
+  int32_t device;
+  int32_t memory_space;
+} cpuops_b200_adapters_desc;
+#define CPUOPS_B200_MAX_RANK 256
+CPUOPS_B200_API int cpuops_b200_adapters(const cpuops_b200_adapters_desc* desc);
+
 /* What the calling thread's last cpuops_b200_gemm call that reached a tensor-core kernel
  * launched (diagnostics for tests and benchmarks): */
 typedef struct cpuops_b200_plan {
