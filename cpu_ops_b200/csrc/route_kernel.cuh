@@ -219,10 +219,18 @@ __global__ void __launch_bounds__(kPlanThreads) count_ids_kernel(const int32_t* 
 // Shared memory: 32 x (groups + 1) counters of the warps, then one start per bin.
 __host__ __device__ inline int plan_smem_bytes(int groups) { return (groups + 1) * (32 * 2 + 4); }
 
-// `counts`: from count_ids_kernel, or null with a single block.
+// A group's pairs cut into tiles of up to kPlanTileRows, for kernels that work tile by tile.
+constexpr int kPlanTileRows = 64;
+__host__ __device__ inline int64_t plan_max_tiles(int64_t rows, int groups) {
+  return rows / kPlanTileRows + (rows < groups + 1 ? rows : groups + 1);
+}
+
+// `counts`: from count_ids_kernel, or null with a single block.  `offsets` may be null.  With `tiles`
+// (plan_max_tiles entries) the pairs in no group are kept, as a group behind the last, and the tiles of
+// all groups are listed: {group, first place in order, pairs, 0}, then empty ones.
 __global__ void __launch_bounds__(kPlanThreads) group_rows_kernel(const int32_t* ids, int64_t rows, int groups,
                                                                   const int32_t* counts, int32_t* offsets,
-                                                                  int32_t* order) {
+                                                                  int32_t* order, int4* tiles) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   extern __shared__ int32_t plan_smem[];
@@ -306,16 +314,50 @@ __global__ void __launch_bounds__(kPlanThreads) group_rows_kernel(const int32_t*
     const int g = static_cast<int>(threadIdx.x) * kPerThread + j;
     if (g < bins) {
       start[g] = at + before[j];
-      if (blockIdx.x == 0) offsets[g] = at;  // (offsets[groups]: where the pairs in no group begin)
+      // (offsets[groups]: where the pairs in no group begin)
+      if (blockIdx.x == 0 && offsets != nullptr) offsets[g] = at;
       at += total[j];
     }
   }
   __syncthreads();
+  if (tiles != nullptr && blockIdx.x == 0) {
+    // the same scan over the bins' tiles
+    int own = 0;
+#pragma unroll
+    for (int j = 0; j < kPerThread; ++j) own += (total[j] + kPlanTileRows - 1) / kPlanTileRows;
+    int v = own;
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+      const int up = __shfl_up_sync(kAll, v, s);
+      if (lane >= s) v += up;
+    }
+    if (lane == 31) warp_sums[warp] = v;
+    __syncthreads();
+    if (warp == 0) {
+      int w = warp_sums[lane];
+#pragma unroll
+      for (int s = 1; s < 32; s <<= 1) {
+        const int up = __shfl_up_sync(kAll, w, s);
+        if (lane >= s) w += up;
+      }
+      warp_sums[lane] = w;
+    }
+    __syncthreads();
+    int slot = v - own + (warp > 0 ? warp_sums[warp - 1] : 0);
+#pragma unroll
+    for (int j = 0; j < kPerThread; ++j) {
+      const int g = static_cast<int>(threadIdx.x) * kPerThread + j;
+      for (int done = 0; done < total[j]; done += kPlanTileRows)
+        tiles[slot++] = make_int4(g, start[g] + done, min(kPlanTileRows, total[j] - done), 0);
+    }
+    const int listed = warp_sums[31], most = static_cast<int>(plan_max_tiles(rows, groups));
+    for (int s = listed + static_cast<int>(threadIdx.x); s < most; s += kPlanThreads) tiles[s] = make_int4(0, 0, 0, 0);
+  }
 #pragma unroll
   for (int i = 0; i < kPlanRounds; ++i) {
     if (bin[i] >= 0)
       order[start[bin[i]] + seen[warp * bins + bin[i]] + rank[i]] =
-          bin[i] < groups ? static_cast<int32_t>(q0 + i * 32 + lane) : -1;
+          bin[i] < groups || tiles != nullptr ? static_cast<int32_t>(q0 + i * 32 + lane) : -1;
   }
 }
 

@@ -104,6 +104,23 @@ GroupedKernel grouped_kernel(int kind, bool gated) {
   return gated ? grouped_mx_kernel<kKindMxf8, true> : grouped_mx_kernel<kKindMxf8, false>;
 }
 
+// The kernels for many rows: ranks in chunks of 16 or 64.
+using AdapterTileKernel = void (*)(AdapterTileParams);
+template <typename X, typename W>
+AdapterTileKernel adapter_down_for(bool narrow, int* smem) {
+  *smem = narrow ? down_smem_bytes<X, 16>() : down_smem_bytes<X, 64>();
+  return narrow ? adapter_down_kernel<X, W, 16> : adapter_down_kernel<X, W, 64>;
+}
+AdapterTileKernel adapter_down(int x_type, int w_type, bool narrow, int* smem) {
+  if (x_type == CPUOPS_B200_TYPE_F16) return adapter_down_for<__half, __half>(narrow, smem);
+  if (x_type == CPUOPS_B200_TYPE_BF16) return adapter_down_for<__nv_bfloat16, __nv_bfloat16>(narrow, smem);
+  return w_type == CPUOPS_B200_TYPE_F16 ? adapter_down_for<float, __half>(narrow, smem)
+                                        : adapter_down_for<float, __nv_bfloat16>(narrow, smem);
+}
+AdapterTileKernel adapter_up(int w_type) {
+  return w_type == CPUOPS_B200_TYPE_F16 ? adapter_up_kernel<__half> : adapter_up_kernel<__nv_bfloat16>;
+}
+
 // Kernel attributes, once per device (under its lock): the most dynamic shared memory each may take.
 int row_kernels_ready(DeviceState& st) {
   static bool ready[64] = {};
@@ -114,6 +131,14 @@ int row_kernels_ready(DeviceState& st) {
   CUDA_TRY(cudaFuncSetAttribute(group_rows_kernel, kMost, plan_smem_bytes(kMaxGroups)));
   for (int kind : {kKindMxf8, kKindMxf4})
     for (bool gated : {false, true}) CUDA_TRY(cudaFuncSetAttribute(grouped_kernel(kind, gated), kMost, st.smem_optin));
+  for (int x_type : {kTypeF32, kTypeF16, kTypeBf16})
+    for (int w_type : {kTypeF16, kTypeBf16})
+      for (bool narrow : {false, true}) {
+        int smem = 0;
+        AdapterTileKernel down = adapter_down(x_type, w_type, narrow, &smem);
+        CUDA_TRY(cudaFuncSetAttribute(down, kMost, smem));
+      }
+  for (int w_type : {kTypeF16, kTypeBf16}) CUDA_TRY(cudaFuncSetAttribute(adapter_up(w_type), kMost, up_smem_bytes(kMaxRank)));
   ready[st.device] = true;
   return 0;
 }
@@ -127,13 +152,13 @@ size_t plan_workspace(int64_t rows, int groups) {
 
 // `counts`: plan_workspace() bytes.
 int launch_plan(const int32_t* ids, int64_t rows, int groups, int32_t* offsets, int32_t* order,
-                int32_t* counts, cudaStream_t stream) {
+                int32_t* counts, int4* tiles, cudaStream_t stream) {
   const unsigned blocks = static_cast<unsigned>(std::max<int64_t>(1, (rows + kPlanPairs - 1) / kPlanPairs));
   if (blocks > 1) {
     if (int rc = launch_after(count_ids_kernel, dim3(blocks), kPlanThreads, 0, stream, ids, rows, groups, counts)) return rc;
   }
   return launch_after(group_rows_kernel, dim3(blocks), kPlanThreads, static_cast<size_t>(plan_smem_bytes(groups)), stream, ids, rows, groups,
-                      static_cast<const int32_t*>(blocks > 1 ? counts : nullptr), offsets, order);
+                      static_cast<const int32_t*>(blocks > 1 ? counts : nullptr), offsets, order, tiles);
 }
 
 int group_rows_call(const cpuops_b200_group_rows_desc* d) {
@@ -152,7 +177,7 @@ int group_rows_call(const cpuops_b200_group_rows_desc* d) {
     if (int rc = ensure_workspace(*call.st, call.stream, need, &ws)) return rc;
   }
   if (int rc = launch_plan(d->ids, d->rows, d->groups, d->offsets, d->order, reinterpret_cast<int32_t*>(ws),
-                           call.stream))
+                           nullptr, call.stream))
     return rc;
   return call.finish();
 }
@@ -218,7 +243,7 @@ int route_call(const cpuops_b200_route_desc* d) {
   }
   if (d->offsets) {
     if (int rc = launch_plan(d->ids, pairs, d->experts, d->offsets, d->order, reinterpret_cast<int32_t*>(ws),
-                             call.stream))
+                             nullptr, call.stream))
       return rc;
   }
   return call.finish();
@@ -361,6 +386,45 @@ AdapterKernel adapter_rows(int x_type, int w_type) {
   return w_type == CPUOPS_B200_TYPE_F16 ? adapter_rows_kernel<float, __half> : adapter_rows_kernel<float, __nv_bfloat16>;
 }
 
+// Rows sorted by adapter, then both products tile by tile.
+int adapters_by_tiles(RowCall& call, const AdapterParams& p, int x_type, int w_type) {
+  AdapterTileParams t;
+  t.a = p;
+  t.rank_pad = (p.rank + 7) / 8 * 8;
+  const int64_t tiles = plan_max_tiles(p.m, p.adapters);
+  const bool narrow = p.rank <= 16;
+  const int chunks = narrow ? 1 : (p.rank + 63) / 64;
+  // parts of k: four CTAs for every SM, at least four stages each
+  const int64_t rows_tiles = std::max<int64_t>(1, p.m / kPlanTileRows);
+  int parts = static_cast<int>(std::min<int64_t>((4 * call.st->sms() + rows_tiles * chunks - 1) / (rows_tiles * chunks), 16));
+  parts = std::max(1, std::min(parts, (p.k + 4 * kDownDepth - 1) / (4 * kDownDepth)));
+  t.depth = ((p.k + parts - 1) / parts + kDownDepth - 1) / kDownDepth * kDownDepth;
+  t.splits = (p.k + t.depth - 1) / t.depth;
+  Plan plan;
+  const size_t off_counts = plan.take(plan_workspace(p.m, p.adapters));
+  const size_t off_order = plan.take(static_cast<size_t>(p.m) * sizeof(int32_t));
+  const size_t off_tiles = plan.take(static_cast<size_t>(tiles) * sizeof(int4));
+  const size_t off_u = plan.take(static_cast<size_t>(t.splits) * p.m * t.rank_pad * sizeof(float));
+  uint8_t* ws = nullptr;
+  if (int rc = ensure_workspace(*call.st, call.stream, plan.total, &ws)) return rc;
+  int32_t* order = reinterpret_cast<int32_t*>(ws + off_order);
+  int4* table = reinterpret_cast<int4*>(ws + off_tiles);
+  t.order = order;
+  t.tiles = table;
+  t.u = reinterpret_cast<float*>(ws + off_u);
+  if (int rc = launch_plan(p.ids, p.m, p.adapters, nullptr, order, reinterpret_cast<int32_t*>(ws + off_counts), table,
+                           call.stream))
+    return rc;
+  int smem = 0;
+  AdapterTileKernel down = adapter_down(x_type, w_type, narrow, &smem);
+  if (int rc = launch_after(down, dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(t.splits), static_cast<unsigned>(chunks)),
+                            128, static_cast<size_t>(smem), call.stream, t))
+    return rc;
+  return launch_after(adapter_up(w_type), dim3(static_cast<unsigned>((p.n + kAdapterTileCols - 1) / kAdapterTileCols),
+                                               static_cast<unsigned>(tiles)),
+                      256, static_cast<size_t>(up_smem_bytes(t.rank_pad)), call.stream, t);
+}
+
 int adapters_call(const cpuops_b200_adapters_desc* d) {
   if (int rc = check_desc(d)) return rc;
   if (!type_ok(d->x_type) || !type_ok(d->w_type)) {
@@ -414,6 +478,11 @@ int adapters_call(const cpuops_b200_adapters_desc* d) {
   };
   p.wide_k = on16(d->x, d->ldx, 0, x_size) && on16(d->a, d->lda, d->a_stride, 2) ? 1 : 0;
   p.wide_r = on16(d->b, d->ldb, d->b_stride, 2) ? 1 : 0;
+  // Few rows: each reads its adapter by itself (from L2, where rows share one).
+  if (p.adapters > 0 && p.adapters <= kMaxGroups && p.m >= 256 && plan_max_tiles(p.m, p.adapters) <= 65535) {
+    if (int rc = adapters_by_tiles(call, p, d->x_type, d->w_type)) return rc;
+    return call.finish();
+  }
   if (static_cast<int64_t>(d->m) * kAdapterCluster > INT32_MAX) return refuse("adapters: too many rows");
   if (int rc = launch_after(adapter_rows(d->x_type, d->w_type), dim3(static_cast<unsigned>(d->m) * kAdapterCluster),
                             kAdapterThreads, 0, call.stream, p))
