@@ -13,9 +13,9 @@
 // what the memory traffic takes, 2 rank operations per byte of x, C or D):
 //   down: u = x A^T for a tile and a part of k, f32 partial sums to the workspace.  16-bit x and A
 //         are multiplied as they are.
-//   up:   D = C + scale * (the parts' sum, ascending) B^T for a tile and 128 columns.
-// A factor in f32 (x where it is f32, and always u, which is not rounded to 16 bits) is cut into two
-// tf32 numbers, 22 bits together; 16-bit factors are tf32 numbers as they are.
+//   up:   D = C + scale * (the parts' sum, ascending) B^T for a tile and some columns.
+// A factor in f32 is not rounded to 16 bits: x (where it is f32) is cut into two tf32 numbers, 22 bits
+// together (16-bit factors are tf32 numbers as they are), u into two or three of B's type.
 #pragma once
 
 #include <type_traits>
@@ -39,7 +39,7 @@ struct AdapterParams {
   float* d;
   int64_t ldx, lda, ldb, a_stride, b_stride, ldc, ldd;
   int32_t m, n, k, rank, adapters;
-  int32_t wide_k, wide_r;  // 1: rows of x and A (of B) start on 16-byte boundaries
+  int32_t align_k, align_r, align_c, align_d;  // what rows of x and A (of B, C, D) start on: 16, 8, 4 or 2 bytes
 };
 
 template <typename T>
@@ -99,8 +99,8 @@ __global__ void __launch_bounds__(kAdapterThreads) __cluster_dims__(kAdapterClus
       float sum = 0.0f;
       for (int i = k0 + lane * 8; i < k1; i += 256) {
         float xv[8], av[8];
-        load8<X>(x, i, k1, p.wide_k, xv);
-        load8<W>(aj, i, k1, p.wide_k, av);
+        load8<X>(x, i, k1, p.align_k == 16, xv);
+        load8<W>(aj, i, k1, p.align_k == 16, av);
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum = __fmaf_rn(xv[e], av[e], sum);
       }
@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kAdapterThreads) __cluster_dims__(kAdapterClus
       const W* bj = b + col * p.ldb;
       for (int i = 0; i < p.rank; i += 8) {
         float bv[8];
-        load8<W>(bj, i, p.rank, p.wide_r, bv);
+        load8<W>(bj, i, p.rank, p.align_r == 16, bv);
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           if (i + e < p.rank) sum = __fmaf_rn(u[i + e], bv[e], sum);
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kAdapterThreads) __cluster_dims__(kAdapterClus
 
 // ---- many rows ---------------------------------------------------------------------------------
 
-constexpr int kAdapterTileCols = 128;  // columns of D per CTA of the up kernel
+constexpr int kUpCols = 64;            // columns of D per step of the up kernel
 constexpr int kDownStages = 4;
 constexpr int kDownDepth = 64;         // elements of k per stage
 
@@ -187,12 +187,13 @@ __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
                : "r"(addr)
                : "memory");
 }
-// v = hi + lo, both tf32 (11 bits each; what is left is below 2^-22 of v).  Of an infinity or NaN hi keeps it.
+// v = hi + lo, both tf32 (11 bits each; what is left is below 2^-22 of v).  hi is cut, lo rounded, by
+// masks: the conversion instruction has a sixteenth of their rate and bound the up kernel (127 us of
+// 8192 rows, rank 64, n 4096).  Of an infinity or NaN hi keeps it.
 __device__ __forceinline__ void split_tf32(float v, uint32_t& hi, uint32_t& lo) {
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(v));
+  hi = __float_as_uint(v) & 0xffffe000u;
   const float rest = v - __uint_as_float(hi);
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(rest));
-  if (!(fabsf(rest) < INFINITY)) lo = 0u;
+  lo = fabsf(rest) < INFINITY ? (__float_as_uint(rest) + 0x1000u) & 0xffffe000u : 0u;
 }
 // Two 16-bit numbers of a word as f32 bits.
 template <typename W>
@@ -208,15 +209,31 @@ __device__ __forceinline__ void widen(uint32_t pair, uint32_t& first, uint32_t& 
 }
 
 // One 16-byte piece of a row into shared memory: elements i .. of `row`, `left` of which exist (the
-// others become zero).  wide: the piece is 16-byte aligned in global memory (asynchronous copy).
+// others become zero).  `align`: the boundary that pieces start on in global memory; from four bytes
+// on the copies are asynchronous (synchronous ones of a D of 777 x 1999, eight-byte aligned, took
+// 15.6 us where these take 12.6).
+template <int kBytes>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, int bytes) {
+  if constexpr (kBytes == 16) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+  } else {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(bytes), "n"(kBytes) : "memory");
+  }
+}
 template <typename T>
-__device__ __forceinline__ void fill_piece(uint32_t dst, const T* row, int i, int left, bool wide) {
+__device__ __forceinline__ void fill_piece(uint32_t dst, const T* row, int i, int left, int align) {
   constexpr int kPer = 16 / static_cast<int>(sizeof(T));
   const int valid = min(max(left, 0), kPer);
-  if (wide) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(valid > 0 ? row + i : row),
-                 "r"(valid * static_cast<int>(sizeof(T)))
-                 : "memory");
+  const int bytes = valid * static_cast<int>(sizeof(T));
+  const char* from = reinterpret_cast<const char*>(valid > 0 ? row + i : row);
+  if (align == 16) {
+    copy_async<16>(dst, from, bytes);
+  } else if (align == 8) {
+#pragma unroll
+    for (int j = 0; j < 16; j += 8) copy_async<8>(dst + j, from + (bytes > j ? j : 0), min(8, max(0, bytes - j)));
+  } else if (align == 4) {
+#pragma unroll
+    for (int j = 0; j < 16; j += 4) copy_async<4>(dst + j, from + (bytes > j ? j : 0), min(4, max(0, bytes - j)));
   } else {
     __align__(16) T v[kPer];
 #pragma unroll
@@ -231,8 +248,9 @@ struct AdapterTileParams {
   const int4* tiles;      // {adapter, first place, rows, -}
   const int32_t* order;   // rows sorted by adapter
   float* u;               // [splits][m][rank_pad]
-  int32_t rank_pad;       // a multiple of 8
+  int32_t rank_pad;       // a multiple of 16
   int32_t splits, depth;  // parts of k and their length (a multiple of kDownDepth)
+  int32_t up_cols;        // columns of D per CTA of the up kernel (a multiple of kUpCols)
 };
 
 template <typename X>
@@ -241,8 +259,9 @@ template <typename X, int kRanks>
 __host__ __device__ constexpr int down_smem_bytes() { return kDownStages * (down_x_bytes<X>() + kRanks * kDownDepth * 2); }
 
 // Ranks blockIdx.z * kRanks .. of u for tile blockIdx.x and part blockIdx.y of k.  128 threads, a warp for
-// every 16 rows.
-template <typename X, typename W, int kRanks>
+// every 16 rows.  kWide: rows of x and A start on 16-byte boundaries (the other kinds of copy in the
+// same loop cost 2 us of 28).
+template <typename X, typename W, int kRanks, bool kWide>
 __global__ void __launch_bounds__(128) adapter_down_kernel(const AdapterTileParams t) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -250,6 +269,7 @@ __global__ void __launch_bounds__(128) adapter_down_kernel(const AdapterTilePara
   const AdapterParams& p = t.a;
   const int4 tile = t.tiles[blockIdx.x];
   if (tile.z == 0 || tile.x >= p.adapters) return;
+  const int align = kWide ? 16 : p.align_k;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank0 = static_cast<int>(blockIdx.z) * kRanks;
   const int k0 = static_cast<int>(blockIdx.y) * t.depth, k1 = min(k0 + t.depth, p.k);
@@ -278,14 +298,14 @@ __global__ void __launch_bounds__(128) adapter_down_kernel(const AdapterTilePara
       const int piece = tid + 128 * i, r = piece / kXPieces, c = piece % kXPieces;
       const int at = k + c * (16 / static_cast<int>(sizeof(X)));
       fill_piece<X>(xs + r * (kXPieces * 16) + ((c ^ (r & 7)) << 4), xrow[i] ? xrow[i] : static_cast<const X*>(p.x), at,
-                    xrow[i] ? k1 - at : 0, p.wide_k);
+                    xrow[i] ? k1 - at : 0, align);
     }
 #pragma unroll
     for (int i = 0; i < kATurns; ++i) {
       const int piece = tid + 128 * i, j = piece >> 3, c = piece & 7;
       const int at = k + c * 8;
       fill_piece<W>(as + j * 128 + ((c ^ (j & 7)) << 4), arow[i] ? arow[i] : static_cast<const W*>(p.a), at,
-                    arow[i] ? k1 - at : 0, p.wide_k);
+                    arow[i] ? k1 - at : 0, align);
     }
   };
   const int steps = (k1 - k0 + kDownDepth - 1) / kDownDepth;
@@ -366,16 +386,54 @@ __global__ void __launch_bounds__(128) adapter_down_kernel(const AdapterTilePara
   }
 }
 
-// Shared memory of the up kernel: u (rows rank_pad + 4 floats apart), then B's 128 rows (rank_pad + 8
-// elements apart): a warp's fragment reads meet every bank once.
-__host__ __device__ inline int up_smem_bytes(int rank_pad) {
-  return kPlanTileRows * (rank_pad + 4) * 4 + kAdapterTileCols * (rank_pad + 8) * 2;
+// u in the up kernel, as 16-bit numbers that the tensor cores multiply with B as it is: three bf16 terms
+// (24 bits), or two f16 terms (22 bits) of a row scaled by a power of two that brings its largest
+// element to [2^14, 2^15) (f16's range would be too small for the row as it is; what is lost below its
+// smallest number is 2^-40 of the largest).
+template <typename W>
+struct UpTerms;
+template <>
+struct UpTerms<__nv_bfloat16> {
+  static constexpr int kCount = 3;
+};
+template <>
+struct UpTerms<__half> {
+  static constexpr int kCount = 2;
+};
+// The next term of v, which is left with the rest.
+__device__ __forceinline__ __nv_bfloat16 take_term(float& v, __nv_bfloat16) {
+  const __nv_bfloat16 h = __float2bfloat16(v);
+  v -= __bfloat162float(h);
+  if (!(fabsf(v) < INFINITY)) v = 0.0f;  // (of an infinity or NaN the first term keeps it)
+  return h;
+}
+__device__ __forceinline__ __half take_term(float& v, __half) {
+  const __half h = __float2half(v);
+  v -= __half2float(h);
+  if (!(fabsf(v) < INFINITY)) v = 0.0f;
+  return h;
 }
 
-// D = C + u B^T for tile blockIdx.y and columns blockIdx.x * 128 ..; 256 threads, a warp for 16 rows x 64
-// columns.  Rows without an adapter make up tiles of their own, of which D is C.
-template <typename W>
-__global__ void __launch_bounds__(256) adapter_up_kernel(const AdapterTileParams t) {
+// Steps in the ring: three, two where u's terms leave no room for three.
+__host__ __device__ inline int up_stages(int rank_pad) { return rank_pad <= 128 ? 3 : 2; }
+constexpr int kUpCWords = kUpCols + 8;  // words from one row of C to the next in shared memory (8 modulo 32)
+// Shared memory of the up kernel: u's terms, 64 rows each; per stage 64 rows of B and 64 rows of C; the
+// rows' scales.  Rows of u and B are rank_pad + 8 elements of 16 bits apart: ldmatrix, and the
+// reads of C by fragment, meet every bank once.
+__host__ __device__ inline int up_stage_bytes(int rank_pad) { return kUpCols * (rank_pad + 8) * 2 + kPlanTileRows * kUpCWords * 4; }
+__host__ __device__ inline int up_smem_bytes(int rank_pad, int terms) {
+  return terms * kPlanTileRows * (rank_pad + 8) * 2 + up_stages(rank_pad) * up_stage_bytes(rank_pad) + kPlanTileRows * 4;
+}
+
+// D = C + u B^T for tile blockIdx.y and t.up_cols columns from blockIdx.x * t.up_cols on, 64 at a time;
+// 256 threads, a warp for 16 rows x 32 columns of a step.  The time is that of the traffic, C in and D
+// out, so B and C come through a ring in shared memory, a step or two ahead.  (C one step ahead in
+// registers, with three CTAs per SM: 8192 rows, rank 64, n 4096 97 us.)
+// Rows without an adapter make up tiles of their own, of which D is C.
+// kWhole: 16-byte aligned rows of B, C and D, whole steps of 64 columns and ranks in eights, so nothing
+// needs a check: a step is 400 instructions of a warp with them, 200 without (85 / 70 us of the above).
+template <typename W, int kUpStages, bool kWhole>
+__global__ void __launch_bounds__(256, 2) adapter_up_kernel(const AdapterTileParams t) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   extern __shared__ __align__(128) uint8_t up_smem[];
@@ -386,108 +444,192 @@ __global__ void __launch_bounds__(256) adapter_up_kernel(const AdapterTileParams
   if (!has && p.c == p.d) return;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, i = lane & 3;
-  const int row0 = (warp >> 1) * 16, col0 = static_cast<int>(blockIdx.x) * kAdapterTileCols + (warp & 1) * 64;
+  const int row0 = (warp >> 1) * 16, half = (warp & 1) * 32;
+  const int first = static_cast<int>(blockIdx.x) * t.up_cols, last = min(first + t.up_cols, p.n);
 
-  // C first: its loads are in flight during all that follows.  A thread has rows g and g + 8 of its 16
-  // and columns 2 i, 2 i + 1 of every eight.
-  const bool pairs = (p.ldc & 1) == 0 && (p.ldd & 1) == 0 && (reinterpret_cast<uintptr_t>(p.c) & 7) == 0 &&
-                     (reinterpret_cast<uintptr_t>(p.d) & 7) == 0;
-  int64_t row[2];
+  // The rows whose C this thread copies in and whose D it copies out, four columns of 64 each (rows that
+  // do not exist are read as the tile's last).
+  const bool wide_d = kWhole || p.align_d == 16;
+  const float* c_from[4];
+  float* d_to[4];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int r = row0 + g + 8 * h;
-    row[h] = r < tile.z ? t.order[tile.y + r] : -1;
+  for (int j = 0; j < 4; ++j) {
+    const int64_t row = t.order[tile.y + min((tid >> 4) + 16 * j, tile.z - 1)];
+    c_from[j] = p.c + row * p.ldc + first + (tid & 15) * 4;
+    d_to[j] = p.d + row * p.ldd + first + (tid & 15) * 4;
   }
-  float2 c[8][2];
+  constexpr int kTerms = UpTerms<W>::kCount;
+  const int ld = t.rank_pad + 8, pieces = t.rank_pad / 8;
+  W* us = reinterpret_cast<W*>(up_smem);
+  const uint32_t us0 = smem_u32(up_smem), ring0 = us0 + kTerms * kPlanTileRows * ld * 2;
+  const uint32_t stage_bytes = static_cast<uint32_t>(up_stage_bytes(t.rank_pad)), c_off = static_cast<uint32_t>(kUpCols * ld * 2);
+  float* row_scale = reinterpret_cast<float*>(up_smem + kTerms * kPlanTileRows * ld * 2 + kUpStages * stage_bytes);
+  // B: four threads to a row
+  const W* b_from = static_cast<const W*>(p.b) + (has ? tile.x * p.b_stride : 0) + (first + (tid >> 2)) * p.ldb;
+  const uint32_t c_to = c_off + ((tid >> 4) * kUpCWords + (tid & 15) * 4) * 4, b_to = (tid >> 2) * ld * 2;
+  // (called for one step after another: the pointers move on)
+  auto fill = [&](int col0, int stage) {
+    const uint32_t to = ring0 + stage * stage_bytes;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int col = col0 + j * 8 + 2 * i;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      c[j][h] = make_float2(0.0f, 0.0f);
-      if (row[h] >= 0) {
-        const float* src = p.c + row[h] * p.ldc + col;
-        if (pairs && col + 1 < p.n) {
-          c[j][h] = *reinterpret_cast<const float2*>(src);
-        } else {
-          if (col < p.n) c[j][h].x = src[0];
-          if (col + 1 < p.n) c[j][h].y = src[1];
-        }
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t dst = to + c_to + 16 * j * kUpCWords * 4;
+      if constexpr (kWhole) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(c_from[j]) : "memory");
+      } else {
+        fill_piece<float>(dst, c_from[j], 0, p.n - col0 - (tid & 15) * 4, p.align_c);
       }
+      c_from[j] += kUpCols;
     }
-  }
-  float acc[8][4];
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[j][e] = 0.0f;
-  if (has) {
-    float* us = reinterpret_cast<float*>(up_smem);
-    const int u_ld = t.rank_pad + 4, b_ld = t.rank_pad + 8;
-    const uint32_t bs = smem_u32(up_smem) + kPlanTileRows * u_ld * 4;
-    const W* b = static_cast<const W*>(p.b) + tile.x * p.b_stride;
-    const int pieces = t.rank_pad / 8;
-    for (int q = tid; q < kAdapterTileCols * pieces; q += 256) {
-      const int n = q / pieces, piece = q - n * pieces;
-      const int col = static_cast<int>(blockIdx.x) * kAdapterTileCols + n;
-      const bool in = col < p.n;
-      fill_piece<W>(bs + (n * b_ld + piece * 8) * 2, in ? b + col * p.ldb : b, piece * 8, in ? p.rank - piece * 8 : 0, p.wide_r);
+    if (has) {
+      if constexpr (kWhole) {
+        for (int piece = tid & 3; piece < pieces; piece += 4)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + b_to + piece * 16),
+                       "l"(b_from + (piece * 8 < p.rank ? piece * 8 : 0)), "r"(piece * 8 < p.rank ? 16 : 0)
+                       : "memory");
+      } else {
+        const bool in = col0 + (tid >> 2) < p.n;
+        for (int piece = tid & 3; piece < pieces; piece += 4)
+          fill_piece<W>(to + b_to + piece * 16, in ? b_from : static_cast<const W*>(p.b), piece * 8,
+                        in ? p.rank - piece * 8 : 0, p.align_r);
+      }
+      b_from += kUpCols * p.ldb;
     }
+  };
+#pragma unroll
+  for (int s = 0; s < kUpStages - 1; ++s) {
+    if (first + s * kUpCols < last) fill(first + s * kUpCols, s);
     cp_async_commit();
+  }
+  if (has) {
     const float scale = p.scales != nullptr ? p.scales[tile.x] : 1.0f;
-    for (int q = tid; q < kPlanTileRows * (t.rank_pad / 4); q += 256) {
-      const int r = q / (t.rank_pad / 4), e = (q - r * (t.rank_pad / 4)) * 4;
+    const int r = tid >> 2;  // four threads to a row
+    // elements e .. e + 3 of this thread's row: the parts of k in ascending order, four of them on their
+    // way at a time (one after another they took a third of a CTA's time)
+    auto sum_at = [&](int e) {
       float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (r < tile.z) {
         const float* from = t.u + static_cast<int64_t>(tile.y + r) * t.rank_pad + e;
-        for (int s = 0; s < t.splits; ++s) {
-          const float4 v = *reinterpret_cast<const float4*>(from + static_cast<int64_t>(s) * p.m * t.rank_pad);
-          sum.x += v.x;
-          sum.y += v.y;
-          sum.z += v.z;
-          sum.w += v.w;
+        const int64_t step = static_cast<int64_t>(p.m) * t.rank_pad;
+        for (int s0 = 0; s0 < t.splits; s0 += 4) {
+          float4 v[4];
+#pragma unroll
+          for (int s = 0; s < 4; ++s)
+            v[s] = s0 + s < t.splits ? *reinterpret_cast<const float4*>(from + (s0 + s) * step) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            if (s0 + s >= t.splits) break;
+            sum.x += v[s].x;
+            sum.y += v[s].y;
+            sum.z += v[s].z;
+            sum.w += v[s].w;
+          }
         }
       }
-      *reinterpret_cast<float4*>(us + r * u_ld + e) = make_float4(sum.x * scale, sum.y * scale, sum.z * scale, sum.w * scale);
+      return make_float4(sum.x * scale, sum.y * scale, sum.z * scale, sum.w * scale);
+    };
+    float grow = 1.0f;
+    if constexpr (std::is_same<W, __half>::value) {
+      float top = 0.0f;
+      for (int e = (tid & 3) * 4; e < t.rank_pad; e += 16) {
+        const float4 v = sum_at(e);
+        top = fmaxf(fmaxf(fmaxf(top, fabsf(v.x)), fmaxf(fabsf(v.y), fabsf(v.z))), fabsf(v.w));
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // top's exponent field, kept where both powers of two are normal numbers (127 for an infinity)
+      const int field = static_cast<int>(__float_as_uint(top) >> 23);
+      const int at = field == 255 ? 141 : max(field, 15);
+      grow = __uint_as_float(static_cast<uint32_t>(268 - at) << 23);             // 2^(141 - at)
+      if ((tid & 3) == 0) row_scale[r] = __uint_as_float(static_cast<uint32_t>(at - 14) << 23);  // 2^(at - 141)
     }
-    cp_async_wait<0>();
-    __syncthreads();
-    const int nb = (warp & 1) * 64;
-    for (int kk = 0; kk < pieces; ++kk) {
-      uint32_t hi[4], lo[4];
+#pragma unroll 4
+    for (int e = (tid & 3) * 4; e < t.rank_pad; e += 16) {
+      const float4 sum = sum_at(e);
+      float v[4] = {sum.x * grow, sum.y * grow, sum.z * grow, sum.w * grow};
+#pragma unroll
+      for (int term = 0; term < kTerms; ++term) {
+        __align__(8) W w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = take_term(v[j], W());
+        *reinterpret_cast<uint2*>(us + (term * kPlanTileRows + r) * ld + e) = *reinterpret_cast<const uint2*>(w);
+      }
+    }
+  }
+  const uint32_t a_at = us0 + ((row0 + (lane & 15)) * ld + (lane >> 4) * 8) * 2;
+  const uint32_t b_at = ((half + (lane & 7) + ((lane >> 4) << 3)) * ld + ((lane >> 3) & 1) * 8) * 2;
+  const uint32_t c_at = c_off + ((row0 + g) * kUpCWords + half + 2 * i) * 4;
+  int stage = 0;
+  for (int col0 = first; col0 < last; col0 += kUpCols) {
+    cp_async_wait<kUpStages - 2>();
+    __syncthreads();  // this step's B and C (and u) are in place; everyone is done with the stage filled next
+    if (const int ahead = col0 + (kUpStages - 1) * kUpCols; ahead < last)
+      fill(ahead, stage == 0 ? kUpStages - 1 : stage - 1);
+    cp_async_commit();
+    const uint32_t at = ring0 + stage * stage_bytes;
+    float acc[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[j][e] = 0.0f;
+    if (has) {
+      for (int kk = 0; kk < pieces / 2; ++kk) {
+        uint32_t b[2][4];  // 16 elements of k x 32 columns
+        ldmatrix_x4(b[0], at + b_at + kk * 32);
+        ldmatrix_x4(b[1], at + b_at + 16 * ld * 2 + kk * 32);
+#pragma unroll
+        for (int term = kTerms - 1; term >= 0; --term) {
+          uint32_t a[4];
+          ldmatrix_x4(a, a_at + term * kPlanTileRows * ld * 2 + kk * 32);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) mma_f16(acc[j], a, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1], W());
+        }
+      }
+      if constexpr (std::is_same<W, __half>::value) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[j][e] *= row_scale[row0 + g + 8 * (e >> 1)];
+      }
+    }
+    // D takes C's place in the stage (a row without an adapter is C itself: no zero is added to it) ...
+    if (has) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float2 v = *reinterpret_cast<const float2*>(us + (row0 + g + 8 * h) * u_ld + kk * 8 + 2 * i);
-        split_tf32(v.x, hi[h], lo[h]);
-        split_tf32(v.y, hi[h + 2], lo[h + 2]);
-      }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        uint32_t pair, b0, b1;
-        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(pair) : "r"(bs + ((nb + j * 8 + g) * b_ld + kk * 8 + 2 * i) * 2));
-        widen<W>(pair, b0, b1);
-        mma_tf32(acc[j], lo, b0, b1);
-        mma_tf32(acc[j], hi, b0, b1);
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t place = at + c_at + (8 * h * kUpCWords + j * 8) * 4;
+          float2 y;
+          asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(y.x), "=f"(y.y) : "r"(place));
+          y.x += acc[j][2 * h];
+          y.y += acc[j][2 * h + 1];
+          asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(place), "f"(y.x), "f"(y.y) : "memory");
+        }
       }
     }
-  }
+    __syncthreads();
+    // ... and leaves it row by row, 256 bytes at a time
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int col = col0 + j * 8 + 2 * i;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (row[h] < 0) continue;
-      float* dst = p.d + row[h] * p.ldd + col;
-      // (a row without an adapter is C itself: no zero is added to it)
-      const float2 y = has ? make_float2(c[j][h].x + acc[j][2 * h], c[j][h].y + acc[j][2 * h + 1]) : c[j][h];
-      if (pairs && col + 1 < p.n) {
-        *reinterpret_cast<float2*>(dst) = y;
-      } else {
-        if (col < p.n) dst[0] = y.x;
-        if (col + 1 < p.n) dst[1] = y.y;
+    for (int j = 0; j < 4; ++j) {
+      float4 y;
+      asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(y.x), "=f"(y.y), "=f"(y.z), "=f"(y.w)
+                   : "r"(at + c_to + 16 * j * kUpCWords * 4));
+      if ((tid >> 4) + 16 * j < tile.z) {
+        const int left = kWhole ? 4 : p.n - col0 - (tid & 15) * 4;  // columns from here on
+        if (wide_d && left >= 4) {
+          *reinterpret_cast<float4*>(d_to[j]) = y;
+        } else {
+          if (left > 0) d_to[j][0] = y.x;
+          if (left > 1) d_to[j][1] = y.y;
+          if (left > 2) d_to[j][2] = y.z;
+          if (left > 3) d_to[j][3] = y.w;
+        }
       }
+      d_to[j] += kUpCols;
     }
+    if (++stage == kUpStages) stage = 0;
   }
+  cp_async_wait<0>();
 }
 
 }  // namespace b200

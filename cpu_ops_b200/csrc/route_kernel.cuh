@@ -216,8 +216,8 @@ __global__ void __launch_bounds__(kPlanThreads) count_ids_kernel(const int32_t* 
     counts[static_cast<int64_t>(blockIdx.x) * (groups + 1) + g] = bins[g];
 }
 
-// Shared memory: 32 x (groups + 1) counters of the warps, then one start per bin.
-__host__ __device__ inline int plan_smem_bytes(int groups) { return (groups + 1) * (32 * 2 + 4); }
+// Shared memory: per bin its start, all blocks' pairs, those of the blocks before, the warps' counters.
+__host__ __device__ inline int plan_smem_bytes(int groups) { return (groups + 1) * (3 * 4 + 32 * 2); }
 
 // A group's pairs cut into tiles of up to kPlanTileRows, for kernels that work tile by tile.
 constexpr int kPlanTileRows = 64;
@@ -236,7 +236,8 @@ __global__ void __launch_bounds__(kPlanThreads) group_rows_kernel(const int32_t*
   extern __shared__ int32_t plan_smem[];
   const int bins = groups + 1;
   int32_t* start = plan_smem;                                     // [bins]
-  uint16_t* seen = reinterpret_cast<uint16_t*>(plan_smem + bins);  // [32][bins]
+  int32_t* all = plan_smem + bins;                                // [2][bins]
+  uint16_t* seen = reinterpret_cast<uint16_t*>(plan_smem + 3 * bins);  // [32][bins]
   __shared__ int32_t warp_sums[32];
   constexpr unsigned kAll = 0xffffffffu;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -261,8 +262,21 @@ __global__ void __launch_bounds__(kPlanThreads) group_rows_kernel(const int32_t*
     __syncwarp();
   }
   __syncthreads();
-  // Per bin (thread g, or the threads in turn): the warps' counts become the warps' starts within
-  // the block; all blocks' pairs and those of the blocks before this one.
+  // All blocks' pairs per bin, and those of the blocks before this one.
+  if (counts != nullptr) {
+    for (int g = threadIdx.x; g < 2 * bins; g += kPlanThreads) all[g] = 0;
+    __syncthreads();
+    const int n = static_cast<int>(gridDim.x) * bins;
+    for (int i = threadIdx.x; i < n; i += kPlanThreads) {
+      const int b = i / bins, g = i - b * bins, c = counts[i];
+      if (c != 0) {
+        atomicAdd(&all[g], c);
+        if (b < static_cast<int>(blockIdx.x)) atomicAdd(&all[bins + g], c);
+      }
+    }
+    __syncthreads();
+  }
+  // Per bin the warps' counts become the warps' starts within the block.
   constexpr int kPerThread = (kMaxGroups + 1 + kPlanThreads - 1) / kPlanThreads;
   int total[kPerThread], before[kPerThread];
   int sum = 0;  // of this thread's bins: kPerThread neighbouring ones
@@ -271,21 +285,17 @@ __global__ void __launch_bounds__(kPlanThreads) group_rows_kernel(const int32_t*
     const int g = static_cast<int>(threadIdx.x) * kPerThread + j;
     total[j] = before[j] = 0;
     if (g < bins) {
+      int c[32];
+#pragma unroll
+      for (int w = 0; w < 32; ++w) c[w] = seen[w * bins + g];
       int in_block = 0;
+#pragma unroll
       for (int w = 0; w < 32; ++w) {
-        const int c = seen[w * bins + g];
         seen[w * bins + g] = static_cast<uint16_t>(in_block);
-        in_block += c;
+        in_block += c[w];
       }
-      total[j] = in_block;
-      if (counts != nullptr) {
-        total[j] = 0;
-        for (int b = 0; b < static_cast<int>(gridDim.x); ++b) {
-          const int c = counts[static_cast<int64_t>(b) * bins + g];
-          if (b < static_cast<int>(blockIdx.x)) before[j] += c;
-          total[j] += c;
-        }
-      }
+      total[j] = counts != nullptr ? all[g] : in_block;
+      before[j] = counts != nullptr ? all[bins + g] : 0;
       sum += total[j];
     }
   }

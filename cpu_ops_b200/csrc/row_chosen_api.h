@@ -107,18 +107,27 @@ GroupedKernel grouped_kernel(int kind, bool gated) {
 // The kernels for many rows: ranks in chunks of 16 or 64.
 using AdapterTileKernel = void (*)(AdapterTileParams);
 template <typename X, typename W>
-AdapterTileKernel adapter_down_for(bool narrow, int* smem) {
+AdapterTileKernel adapter_down_for(bool narrow, bool wide, int* smem) {
   *smem = narrow ? down_smem_bytes<X, 16>() : down_smem_bytes<X, 64>();
-  return narrow ? adapter_down_kernel<X, W, 16> : adapter_down_kernel<X, W, 64>;
+  if (narrow) return wide ? adapter_down_kernel<X, W, 16, true> : adapter_down_kernel<X, W, 16, false>;
+  return wide ? adapter_down_kernel<X, W, 64, true> : adapter_down_kernel<X, W, 64, false>;
 }
-AdapterTileKernel adapter_down(int x_type, int w_type, bool narrow, int* smem) {
-  if (x_type == CPUOPS_B200_TYPE_F16) return adapter_down_for<__half, __half>(narrow, smem);
-  if (x_type == CPUOPS_B200_TYPE_BF16) return adapter_down_for<__nv_bfloat16, __nv_bfloat16>(narrow, smem);
-  return w_type == CPUOPS_B200_TYPE_F16 ? adapter_down_for<float, __half>(narrow, smem)
-                                        : adapter_down_for<float, __nv_bfloat16>(narrow, smem);
+AdapterTileKernel adapter_down(int x_type, int w_type, bool narrow, bool wide, int* smem) {
+  if (x_type == CPUOPS_B200_TYPE_F16) return adapter_down_for<__half, __half>(narrow, wide, smem);
+  if (x_type == CPUOPS_B200_TYPE_BF16) return adapter_down_for<__nv_bfloat16, __nv_bfloat16>(narrow, wide, smem);
+  return w_type == CPUOPS_B200_TYPE_F16 ? adapter_down_for<float, __half>(narrow, wide, smem)
+                                        : adapter_down_for<float, __nv_bfloat16>(narrow, wide, smem);
 }
-AdapterTileKernel adapter_up(int w_type) {
-  return w_type == CPUOPS_B200_TYPE_F16 ? adapter_up_kernel<__half> : adapter_up_kernel<__nv_bfloat16>;
+int adapter_up_smem(int w_type, int rank_pad) {
+  return up_smem_bytes(rank_pad, w_type == CPUOPS_B200_TYPE_F16 ? UpTerms<__half>::kCount : UpTerms<__nv_bfloat16>::kCount);
+}
+template <typename W>
+AdapterTileKernel adapter_up_for(int rank_pad, bool whole) {
+  if (up_stages(rank_pad) == 3) return whole ? adapter_up_kernel<W, 3, true> : adapter_up_kernel<W, 3, false>;
+  return whole ? adapter_up_kernel<W, 2, true> : adapter_up_kernel<W, 2, false>;
+}
+AdapterTileKernel adapter_up(int w_type, int rank_pad, bool whole) {
+  return w_type == CPUOPS_B200_TYPE_F16 ? adapter_up_for<__half>(rank_pad, whole) : adapter_up_for<__nv_bfloat16>(rank_pad, whole);
 }
 
 // Kernel attributes, once per device (under its lock): the most dynamic shared memory each may take.
@@ -133,12 +142,16 @@ int row_kernels_ready(DeviceState& st) {
     for (bool gated : {false, true}) CUDA_TRY(cudaFuncSetAttribute(grouped_kernel(kind, gated), kMost, st.smem_optin));
   for (int x_type : {kTypeF32, kTypeF16, kTypeBf16})
     for (int w_type : {kTypeF16, kTypeBf16})
-      for (bool narrow : {false, true}) {
-        int smem = 0;
-        AdapterTileKernel down = adapter_down(x_type, w_type, narrow, &smem);
-        CUDA_TRY(cudaFuncSetAttribute(down, kMost, smem));
-      }
-  for (int w_type : {kTypeF16, kTypeBf16}) CUDA_TRY(cudaFuncSetAttribute(adapter_up(w_type), kMost, up_smem_bytes(kMaxRank)));
+      for (bool narrow : {false, true})
+        for (bool wide : {false, true}) {
+          int smem = 0;
+          AdapterTileKernel down = adapter_down(x_type, w_type, narrow, wide, &smem);
+          CUDA_TRY(cudaFuncSetAttribute(down, kMost, smem));
+        }
+  for (int w_type : {kTypeF16, kTypeBf16})
+    for (int rank : {128, kMaxRank})
+      for (bool whole : {false, true})
+        CUDA_TRY(cudaFuncSetAttribute(adapter_up(w_type, rank, whole), kMost, adapter_up_smem(w_type, rank)));
   ready[st.device] = true;
   return 0;
 }
@@ -390,16 +403,30 @@ AdapterKernel adapter_rows(int x_type, int w_type) {
 int adapters_by_tiles(RowCall& call, const AdapterParams& p, int x_type, int w_type) {
   AdapterTileParams t;
   t.a = p;
-  t.rank_pad = (p.rank + 7) / 8 * 8;
+  t.rank_pad = (p.rank + 15) / 16 * 16;
   const int64_t tiles = plan_max_tiles(p.m, p.adapters);
   const bool narrow = p.rank <= 16;
   const int chunks = narrow ? 1 : (p.rank + 63) / 64;
-  // parts of k: four CTAs for every SM, at least four stages each
-  const int64_t rows_tiles = std::max<int64_t>(1, p.m / kPlanTileRows);
-  int parts = static_cast<int>(std::min<int64_t>((4 * call.st->sms() + rows_tiles * chunks - 1) / (rows_tiles * chunks), 16));
+  // parts of k: as many as fit the SMs at once with three CTAs each, at least four stages to a part
+  int parts = static_cast<int>(std::min<int64_t>(3 * call.st->sms() / (tiles * chunks), 16));
   parts = std::max(1, std::min(parts, (p.k + 4 * kDownDepth - 1) / (4 * kDownDepth)));
   t.depth = ((p.k + parts - 1) / parts + kDownDepth - 1) / kDownDepth * kDownDepth;
   t.splits = (p.k + t.depth - 1) / t.depth;
+  // Columns per CTA of the up kernel, two CTAs of which share an SM: of the counts that fill up to four
+  // rounds of them, the one that leaves the fewest idle in the last round (of equal ones the least, since
+  // every CTA reads u anew): 8192 rows, rank 64, n 4096: 2 CTAs per tile 70 us, 7 took 78.
+  const int64_t steps = (p.n + kUpCols - 1) / kUpCols, slots = 2 * call.st->sms();
+  int64_t ctas = 1;
+  double best = 0.0;
+  for (int64_t c = 1; c <= steps && (c == 1 || c * tiles <= 4 * slots); ++c) {
+    const int64_t per = (steps + c - 1) / c, rounds = (tiles * c + slots - 1) / slots;
+    const double busy = static_cast<double>(tiles * steps) / static_cast<double>(rounds * slots * per);
+    if (busy > best + 0.02) {
+      best = busy;
+      ctas = c;
+    }
+  }
+  t.up_cols = static_cast<int>((steps + ctas - 1) / ctas) * kUpCols;
   Plan plan;
   const size_t off_counts = plan.take(plan_workspace(p.m, p.adapters));
   const size_t off_order = plan.take(static_cast<size_t>(p.m) * sizeof(int32_t));
@@ -416,13 +443,14 @@ int adapters_by_tiles(RowCall& call, const AdapterParams& p, int x_type, int w_t
                            call.stream))
     return rc;
   int smem = 0;
-  AdapterTileKernel down = adapter_down(x_type, w_type, narrow, &smem);
+  AdapterTileKernel down = adapter_down(x_type, w_type, narrow, p.align_k == 16, &smem);
   if (int rc = launch_after(down, dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(t.splits), static_cast<unsigned>(chunks)),
                             128, static_cast<size_t>(smem), call.stream, t))
     return rc;
-  return launch_after(adapter_up(w_type), dim3(static_cast<unsigned>((p.n + kAdapterTileCols - 1) / kAdapterTileCols),
+  const bool whole = p.align_r == 16 && p.align_c == 16 && p.align_d == 16 && p.n % kUpCols == 0 && p.rank % 8 == 0;
+  return launch_after(adapter_up(w_type, t.rank_pad, whole), dim3(static_cast<unsigned>((p.n + t.up_cols - 1) / t.up_cols),
                                                static_cast<unsigned>(tiles)),
-                      256, static_cast<size_t>(up_smem_bytes(t.rank_pad)), call.stream, t);
+                      256, static_cast<size_t>(adapter_up_smem(w_type, t.rank_pad)), call.stream, t);
 }
 
 int adapters_call(const cpuops_b200_adapters_desc* d) {
@@ -473,11 +501,14 @@ int adapters_call(const cpuops_b200_adapters_desc* d) {
   p.rank = d->rank;
   p.adapters = any ? d->adapters : 0;
   const int x_size = d->x_type == CPUOPS_B200_TYPE_F32 ? 4 : 2;
-  auto on16 = [](const void* ptr, int64_t ld, int64_t stride, int size) {
-    return reinterpret_cast<uintptr_t>(ptr) % 16 == 0 && ld * size % 16 == 0 && stride * size % 16 == 0;
+  auto align = [](const void* ptr, int64_t ld, int64_t stride, int size) {
+    const uint64_t bits = reinterpret_cast<uintptr_t>(ptr) | static_cast<uint64_t>(ld * size) | static_cast<uint64_t>(stride * size);
+    return bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : 2;
   };
-  p.wide_k = on16(d->x, d->ldx, 0, x_size) && on16(d->a, d->lda, d->a_stride, 2) ? 1 : 0;
-  p.wide_r = on16(d->b, d->ldb, d->b_stride, 2) ? 1 : 0;
+  p.align_k = std::min(align(d->x, d->ldx, 0, x_size), align(d->a, d->lda, d->a_stride, 2));
+  p.align_r = align(d->b, d->ldb, d->b_stride, 2);
+  p.align_c = align(d->c, d->ldc, 0, 4);
+  p.align_d = align(d->d, d->ldd, 0, 4);
   // Few rows: each reads its adapter by itself (from L2, where rows share one).
   if (p.adapters > 0 && p.adapters <= kMaxGroups && p.m >= 256 && plan_max_tiles(p.m, p.adapters) <= 65535) {
     if (int rc = adapters_by_tiles(call, p, d->x_type, d->w_type)) return rc;
