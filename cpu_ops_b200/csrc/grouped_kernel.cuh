@@ -14,7 +14,10 @@
 //     groups of any size waste less than 16 columns of tensor-core time per tile.
 //   * X rows are gathered by TMA (tile::gather4, four rows by their numbers per instruction), one
 //     lane of a warp for every four rows; their scales by the scale-writer warps, which read them by
-//     row anyway.  No gathered or padded copy of A is ever made.
+//     row anyway.  A gather costs the TMA unit about 38 cycles whatever its rows, which W's own time hides
+//     while items have few pairs.  With many, gather_rows_kernel copies the rows in plan order once,
+//     and X comes in boxes of 16 rows (2048 rows x 4 of 32 experts, 4096 x 4096 e4m3: 650 us
+//     gathered, TBD copied, the copy's 10 included).
 //   * Gated: a tile holds 64 gate rows and their 64 up rows, 16 and 16 in each warp's lane quarter, so
 //     that the two accumulators of an output meet in one warp (lane l and l + 16): one exchange
 //     between lanes, and D is written once, at its final size.
@@ -55,6 +58,7 @@ struct GroupedParams {
   int32_t BN, stages;
   int32_t w_tile_bytes;       // what the loads of a W tile credit to the barrier
   int32_t align_w, align_x;   // scale rows start on multiples of 16, 4 or 1 bytes
+  int32_t sorted;             // 1: X (and sx) hold a row per pair, in plan order
   uint32_t idesc;             // without N
   uint32_t wait_budget_us;
   int32_t* error;
@@ -237,7 +241,12 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
     const int q = p.order[item.p0 + r];
     return q >= 0 && q < p.rows ? q : -1;
   };
-  auto a_row_of = [&](int q) { return q < 0 ? -1 : min(q / p.pairs_per_a_row, p.a_rows - 1); };
+  // The row of X behind the pair at place p0 + r of an item's run, or -1.
+  auto x_row = [&](const GroupedItem& item, int r) {
+    if (p.sorted) return r < item.count ? item.p0 + r : -1;
+    const int q = pair_at(item, r);
+    return q < 0 ? -1 : min(q / p.pairs_per_a_row, p.a_rows - 1);
+  };
   auto columns_of = [&](const GroupedItem& item) { return max(16, (item.count + 15) & ~15); };
 
   if (warp == 0) {
@@ -281,6 +290,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
     __syncwarp();
   } else if (warp == 10) {
     // ------------------------------ X gather ------------------------------
+    // Rows in plan order: lane l loads rows 16 l .. 16 l + 15.  Otherwise:
     // Lane l gathers rows 4 l .. 4 l + 3 of the item's X, and those 128 further on.  Rows that do not
     // exist inside a group of four are read as the group's first one; groups without any row
     // are left as they are (their columns are computed and never read).
@@ -291,18 +301,20 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
       const GroupedItem item = item_at(it);
       int row[2][4];
       bool mine[2];
+      const bool box = p.sorted && 16 * lane < item.count;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int r0 = 128 * h + 4 * lane;
-        mine[h] = r0 < item.count;
+        mine[h] = !p.sorted && r0 < item.count;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) row[h][j] = a_row_of(pair_at(item, r0 + j));
+        for (int j = 0; j < 4; ++j) row[h][j] = p.sorted ? -1 : x_row(item, r0 + j);
         if (row[h][0] < 0) row[h][0] = 0;
 #pragma unroll
         for (int j = 1; j < 4; ++j)
           if (row[h][j] < 0) row[h][j] = row[h][0];
       }
-      const uint32_t bytes = static_cast<uint32_t>(max(0, (item.count + 3) >> 2)) * 512u;
+      const uint32_t bytes = p.sorted ? static_cast<uint32_t>((item.count + 15) >> 4) * 2048u
+                                      : static_cast<uint32_t>((item.count + 3) >> 2) * 512u;
       for (int kb = 0; kb < p.k_blocks; ++kb) {
         if (!__all_sync(kAll, mbar_wait_bounded(empty_bar(s), ph ^ 1u, abort_flag, budget_ns))) {
           if (lane == 0) {
@@ -314,7 +326,9 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
         }
         if (lane == 0) mbar_expect_tx(full_bar(s), bytes);
         __syncwarp();
-        const uint32_t dst = smem_base + s * stage_bytes + kTileM * 128 + static_cast<uint32_t>(lane) * 512u;
+        const uint32_t x_base = smem_base + s * stage_bytes + kTileM * 128;
+        if (box) tma_load_2d(x_base + static_cast<uint32_t>(lane) * 2048u, &tmX, full_bar(s), kb * 128, item.p0 + 16 * lane);
+        const uint32_t dst = x_base + static_cast<uint32_t>(lane) * 512u;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
           if (mine[h])
@@ -429,10 +443,10 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
         col = row = item.tile * kTileM + r;
       }
       if (col < p.n) f_w = p.sw + (static_cast<int64_t>(item.group) * p.b_group_rows + row) * p.ld_sw;
-      const int a0 = a_row_of(pair_at(item, r));
+      const int a0 = x_row(item, r);
       if (a0 >= 0) f_x0 = p.sx + a0 * p.ld_sx;
       if (slot1) {
-        const int a1 = a_row_of(pair_at(item, r + 128));
+        const int a1 = x_row(item, r + 128);
         if (a1 >= 0) f_x1 = p.sx + a1 * p.ld_sx;
       }
     };
@@ -584,6 +598,37 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
   __syncwarp();
   __syncthreads();
   if (warp == 1) tmem_dealloc(tmem_base, 512u);
+}
+
+// Rows of A (elements, then scales) in plan order: row p of `x` and `sx` belongs to pair order[p].  A block
+// for every place in turn; places without a pair are left as they are.
+__global__ void __launch_bounds__(256) gather_rows_kernel(const uint8_t* a, int64_t a_pitch, const uint8_t* sa,
+                                                          int64_t sa_pitch, const int32_t* order, int rows, int a_rows,
+                                                          int pairs_per_a_row, int row_bytes, int scale_bytes, uint8_t* x,
+                                                          int64_t x_pitch, uint8_t* sx, int64_t sx_pitch) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (int place = blockIdx.x * 8 + static_cast<int>(threadIdx.x >> 5); place < rows; place += static_cast<int>(gridDim.x) * 8) {
+    const int lane = threadIdx.x & 31;
+    const int q = order[place];
+    if (q < 0 || q >= rows) continue;
+    const int64_t row = min(q / pairs_per_a_row, a_rows - 1);
+    const uint8_t* from = a + row * a_pitch;
+    uint8_t* to = x + place * x_pitch;
+    int i = lane * 16;
+    for (; i + 1552 <= row_bytes; i += 2048) {  // four pieces on their way at a time
+      uint4 v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint4*>(from + i + 512 * j);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(to + i + 512 * j) = v[j];
+    }
+    for (; i + 16 <= row_bytes; i += 512) *reinterpret_cast<uint4*>(to + i) = *reinterpret_cast<const uint4*>(from + i);
+    for (int j = (row_bytes & ~15) + lane; j < row_bytes; j += 32) to[j] = from[j];
+    const uint8_t* sfrom = sa + row * sa_pitch;
+    uint8_t* sto = sx + place * sx_pitch;
+    for (int j = lane; j < scale_bytes; j += 32) sto[j] = sfrom[j];
+  }
 }
 
 // D[t] = the sum of row t's `per` pairs, ascending; pairs in no group add nothing.

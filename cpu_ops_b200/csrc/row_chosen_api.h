@@ -351,11 +351,29 @@ int gemm_grouped_call(const cpuops_b200_gemm_grouped_desc* d) {
   p.wait_budget_us = g_wait_budget_us.load();
   p.error = st.error_dev;
 
+  // Rows copied in plan order, where groups have more pairs than gathering hides behind W's loads.
+  p.sorted = groups > 0 && rows / groups >= 48 ? 1 : 0;
+  const int row_bytes = fp4_a ? k / 2 : k;
+  const int64_t x_pitch = align_up(row_bytes, 16), sx_pitch = align_up(blocks32, 16);
+  Plan plan;
+  const size_t off_x = plan.take(p.sorted ? static_cast<size_t>(rows) * x_pitch : 0);
+  const size_t off_sx = plan.take(p.sorted ? static_cast<size_t>(rows) * sx_pitch : 0);
+  const size_t off_sum = plan.take(summed ? static_cast<size_t>(rows) * n * sizeof(float) : 0);
   uint8_t* ws = nullptr;
-  if (summed) {
-    if (int rc = ensure_workspace(st, call.stream, static_cast<size_t>(rows) * n * sizeof(float), &ws)) return rc;
+  if (plan.total > 0) {
+    if (int rc = ensure_workspace(st, call.stream, plan.total, &ws)) return rc;
   }
-  p.d = summed ? reinterpret_cast<float*>(ws) : d->d;
+  if (p.sorted) {
+    p.sx = ws + off_sx;
+    p.ld_sx = sx_pitch;
+    p.align_x = 16;
+    const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((static_cast<int64_t>(rows) + 7) / 8, 8 * st.sm_count));
+    if (int rc = launch_after(gather_rows_kernel, dim3(blocks), 256, 0, call.stream, static_cast<const uint8_t*>(d->a), a_pitch,
+                              static_cast<const uint8_t*>(d->a_scales), static_cast<int64_t>(d->ld_scales_a), d->order, rows,
+                              d->a_rows, d->pairs_per_a_row, row_bytes, blocks32, ws + off_x, x_pitch, ws + off_sx, sx_pitch))
+      return rc;
+  }
+  p.d = summed ? reinterpret_cast<float*>(ws + off_sum) : d->d;
   p.ldd = summed ? n : d->ldd;
 
   const int64_t most_items = (static_cast<int64_t>(std::min(groups, rows)) + rows / p.BN) * tiles;
@@ -368,7 +386,11 @@ int gemm_grouped_call(const cpuops_b200_gemm_grouped_desc* d) {
     } else {
       if (int rc = make_tensor_map(&tmW, d->b, fp4_b ? k / 2 : k, b_rows, b_pitch, box)) return rc;
     }
-    if (int rc = make_tensor_map(&tmX, d->a, fp4_a ? k / 2 : k, d->a_rows, a_pitch, 1)) return rc;
+    if (p.sorted) {
+      if (int rc = make_tensor_map(&tmX, ws + off_x, row_bytes, rows, x_pitch, 16)) return rc;
+    } else {
+      if (int rc = make_tensor_map(&tmX, d->a, row_bytes, d->a_rows, a_pitch, 1)) return rc;
+    }
     const int ka = kind == kKindMxf4 ? 2 : 1;
     const int fixed = grouped_smem_bytes(p.BN, 0, ka, groups);
     p.stages = std::min(kGroupedMaxStages,
