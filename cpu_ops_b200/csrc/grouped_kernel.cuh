@@ -26,7 +26,7 @@
 //     staging.
 //
 // Roles (352 threads): warp 0 TMA producer of W, warp 1 MMA issuer (owns tensor memory), warps 2-5
-// scale writers, warps 6-9 epilogue (one TMEM lane quarter each), warp 10 gathers X.
+// scale writers, warps 6-9 (kTwo: 11-14 too) epilogue (one TMEM lane quarter each), warp 10 loads X.
 // Every wait is bounded, as in the other kernels.
 #pragma once
 
@@ -35,10 +35,11 @@
 
 namespace b200 {
 
-constexpr int kGroupedThreads = 352;
+constexpr int kGroupedThreads = 352;      // kTwo: 128 more, four epilogue warps
+__host__ __device__ constexpr int grouped_threads(bool two) { return two ? kGroupedThreads + 128 : kGroupedThreads; }
 constexpr int kGroupedMaxStages = 8;
 constexpr int kGroupedMaxBN = 192;   // two accumulators and four slots of scales fit tensor memory
-constexpr int kGroupedFetchAhead = 3;
+__host__ __device__ constexpr int grouped_fetch_ahead(bool two) { return two ? 2 : 3; }  // scale fetches in flight
 
 struct GroupedParams {
   const uint8_t* sw;          // W's scales, row-major
@@ -64,13 +65,20 @@ struct GroupedParams {
   int32_t* error;
 };
 
-__host__ __device__ inline int grouped_stage_bytes(int BN) { return kTileM * 128 + BN * 128; }
-__host__ __device__ inline int grouped_atoms(int BN, int ka) { return ka * (1 + (BN > 128 ? 2 : 1)); }
-__host__ __device__ inline int grouped_staging_bytes(int BN) { return kGroupedFetchAhead * (kTileM + BN) * 16; }
+// W tiles of a CTA: one, or (kTwo) two that share X.
+__host__ __device__ inline int grouped_stage_bytes(int BN, bool two) { return (two ? 2 : 1) * kTileM * 128 + BN * 128; }
+__host__ __device__ inline int grouped_atoms(int BN, int ka, bool two) { return ka * ((two ? 2 : 1) + (BN > 128 ? 2 : 1)); }
+__host__ __device__ inline int grouped_staging_bytes(int BN, bool two) {
+  return grouped_fetch_ahead(two) * ((two ? 2 : 1) * kTileM + BN) * 16;
+}
+// Tensor memory: accumulators of BN columns (two sets of them, where they fit), four slots of scales.
+__host__ __device__ inline int grouped_acc_sets(int BN, int ka, bool two) {
+  return 2 * (two ? 2 : 1) * BN + kDecodeSfSlots * 4 * grouped_atoms(BN, ka, two) <= 512 ? 2 : 1;
+}
 __host__ __device__ inline int grouped_table_bytes(int groups) { return (2 * (groups + 1) * 4 + 15) / 16 * 16; }
 constexpr int kGroupedBarrierBytes = 256;
-__host__ __device__ inline int grouped_smem_bytes(int BN, int stages, int ka, int groups) {
-  return 1024 + stages * (grouped_stage_bytes(BN) + grouped_atoms(BN, ka) * 512) + grouped_staging_bytes(BN) +
+__host__ __device__ inline int grouped_smem_bytes(int BN, int stages, int ka, int groups, bool two) {
+  return 1024 + stages * (grouped_stage_bytes(BN, two) + grouped_atoms(BN, ka, two) * 512) + grouped_staging_bytes(BN, two) +
          grouped_table_bytes(groups) + kGroupedBarrierBytes;
 }
 
@@ -135,14 +143,21 @@ __device__ __forceinline__ void fetch_scales(uint32_t dst, const uint8_t* src, i
 }
 
 // kGated: silu(gate) * up.  KIND: kKindMxf8 (also fp4 weights under fp8 rows) or kKindMxf4.
-template <int KIND, bool kGated>
-__global__ void __launch_bounds__(kGroupedThreads, 1)
+// kTwo: two W tiles share a stage's X (gated: the gate's and the up projection's 128 rows).  A stage's
+// loads take some 2000 cycles from the moment it is free, so the ring has to hold that much work:
+// with one tile five stages of 144 pairs hold 1440 cycles of it, with two four stages hold 2300, and every
+// role has twice the time for a k-block.  (275 -> TBD us, 2048 rows x 4 of 32 experts, 4096 x 4096 e4m3.)
+template <int KIND, bool kGated, bool kTwo>
+__global__ void __launch_bounds__(grouped_threads(kTwo), 1)
     grouped_mx_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                       const GroupedParams p) {
   constexpr int kSfBytes = KIND == kKindMxf4 ? 8 : 4;  // scale bytes per row and k-block
   constexpr int kKa = kSfBytes / 4;                    // atoms along k per operand
   constexpr int kUnitsPerChunk = 16 / kSfBytes;        // k-blocks served by one 16-byte fetch of a scale row
-  constexpr int kTileCols = kGated ? 64 : 128;         // columns of D per tile
+  constexpr int kTiles = kTwo ? 2 : 1;
+  constexpr int kTileCols = 128 * kTiles / (kGated ? 2 : 1);  // columns of D per item
+  constexpr int kThreads = grouped_threads(kTwo), kFetchAhead = grouped_fetch_ahead(kTwo);
+  constexpr uint32_t kWBytes = kTiles * kTileM * 128;
   constexpr unsigned kAll = 0xffffffffu;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
@@ -154,12 +169,12 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int stages = p.stages, BN = p.BN;
   const int x_halves = BN > 128 ? 2 : 1;
-  const uint32_t stage_bytes = static_cast<uint32_t>(grouped_stage_bytes(BN));
-  const uint32_t atoms = static_cast<uint32_t>(grouped_atoms(BN, kKa));
+  const uint32_t stage_bytes = static_cast<uint32_t>(grouped_stage_bytes(BN, kTwo));
+  const uint32_t atoms = static_cast<uint32_t>(grouped_atoms(BN, kKa, kTwo));
   const uint32_t atom_bytes = atoms * 512u;
   const uint32_t atom_base = smem_base + stages * stage_bytes;
   const uint32_t staging_base = atom_base + stages * atom_bytes;
-  const uint32_t table_off = staging_base + static_cast<uint32_t>(grouped_staging_bytes(BN)) - smem_base;
+  const uint32_t table_off = staging_base + static_cast<uint32_t>(grouped_staging_bytes(BN, kTwo)) - smem_base;
   int32_t* first = reinterpret_cast<int32_t*>(smem + table_off);  // [groups + 1]
   int32_t* start = first + p.groups + 1;                          // [groups + 1]
   const uint32_t bar_base = smem_base + table_off + static_cast<uint32_t>(grouped_table_bytes(p.groups));
@@ -173,6 +188,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (bar_base - smem_base) + 8 * kBarriers);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const uint64_t budget_ns = static_cast<uint64_t>(p.wait_budget_us) * 1000ull;
+  const int acc_sets = grouped_acc_sets(BN, kKa, kTwo), acc_cols = kTiles * BN;
 
   if (warp == 2) {
     if (lane < kBarriers) {
@@ -180,7 +196,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
       // accumulator full, drain: one tcgen05.commit; accumulator empty: the epilogue warps
       uint32_t count = 1u;
       if (lane < kGroupedMaxStages) count = 6u;
-      if (lane == 2 * kGroupedMaxStages + 2 || lane == 2 * kGroupedMaxStages + 3) count = 4u;
+      if (lane == 2 * kGroupedMaxStages + 2 || lane == 2 * kGroupedMaxStages + 3) count = 4u * kTiles;
       mbar_init(bar_base + 8u * static_cast<uint32_t>(lane), count);
     }
     if (lane == 0) *abort_flag = 0;
@@ -197,7 +213,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   // Whatever the array holds, the starts become an ascending sequence within 0 .. rows: no item
   // reaches outside `order`, and there are no more items than the launcher allowed for.
-  for (int g = threadIdx.x; g <= p.groups; g += kGroupedThreads) start[g] = min(max(p.offsets[g], 0), p.rows);
+  for (int g = threadIdx.x; g <= p.groups; g += kThreads) start[g] = min(max(p.offsets[g], 0), p.rows);
   __syncthreads();
   if (warp == 2) {
     int sum = 0, high = start[0];  // items and highest start so far
@@ -269,7 +285,11 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
         }
         mbar_expect_tx_p(full_bar(s), static_cast<uint32_t>(p.w_tile_bytes), el);
         const uint32_t dst = smem_base + s * stage_bytes;
-        if constexpr (kGated) {
+        if constexpr (kTwo) {
+          const int row = base + item.tile * (kGated ? kTileM : 2 * kTileM);
+          tma_load_2d_g<false>(dst, &tmW, full_bar(s), kb * 128, row, el);
+          tma_load_2d_g<false>(dst + kTileM * 128, &tmW, full_bar(s), kb * 128, row + (kGated ? p.n : kTileM), el);
+        } else if constexpr (kGated) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const int row = base + item.tile * 64 + 16 * q;
@@ -326,7 +346,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
         }
         if (lane == 0) mbar_expect_tx(full_bar(s), bytes);
         __syncwarp();
-        const uint32_t x_base = smem_base + s * stage_bytes + kTileM * 128;
+        const uint32_t x_base = smem_base + s * stage_bytes + kWBytes;
         if (box) tma_load_2d(x_base + static_cast<uint32_t>(lane) * 2048u, &tmX, full_bar(s), kb * 128, item.p0 + 16 * lane);
         const uint32_t dst = x_base + static_cast<uint32_t>(lane) * 512u;
 #pragma unroll
@@ -347,11 +367,11 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
     const uint64_t op_hi64 = make_smem_desc_hi(16, 1024, 2);  // K-major, 128-byte swizzle
     const uint32_t op_hi = static_cast<uint32_t>(op_hi64 >> 32);
     const uint32_t a_lo0 = static_cast<uint32_t>(op_hi64) | (smem_base >> 4);
-    const uint32_t b_lo0 = static_cast<uint32_t>(op_hi64) | ((smem_base + kTileM * 128) >> 4);
+    const uint32_t b_lo0 = static_cast<uint32_t>(op_hi64) | ((smem_base + kWBytes) >> 4);
     const uint64_t sf_hi64 = make_smem_desc_hi(0, 128, 0);
     const uint32_t sf_hi = static_cast<uint32_t>(sf_hi64 >> 32);
     const uint32_t sf_lo0 = static_cast<uint32_t>(sf_hi64) | (atom_base >> 4);
-    const uint32_t sf_t0 = tmem_base + 2u * static_cast<uint32_t>(BN);
+    const uint32_t sf_t0 = tmem_base + static_cast<uint32_t>(acc_sets * acc_cols);
     const uint32_t sf_cols = 4u * atoms;
     const uint32_t sfb_half = 4u * static_cast<uint32_t>(x_halves);
     int s = 0, buf = 0, sf_q = 0;
@@ -368,7 +388,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
         break;
       }
       tc_fence_after_sync();
-      const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(buf * BN);
+      const uint32_t d_tmem0 = tmem_base + static_cast<uint32_t>(buf * acc_cols);
       uint32_t accumulate = 0;
       for (int kb = 0; kb < p.k_blocks; ++kb) {
         if (!__all_sync(kAll, mbar_wait_bounded(full_bar(s), ph, abort_flag, budget_ns))) {
@@ -380,23 +400,28 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
           break;
         }
         tc_fence_after_sync();
-        const uint32_t a_lo = a_lo0 + s * (stage_bytes >> 4), b_lo = b_lo0 + s * (stage_bytes >> 4);
-        const uint32_t sfa_t = sf_t0 + static_cast<uint32_t>(sf_q) * sf_cols, sfb_t = sfa_t + 4u * kKa;
+        const uint32_t b_lo = b_lo0 + s * (stage_bytes >> 4);
+        const uint32_t sf_t = sf_t0 + static_cast<uint32_t>(sf_q) * sf_cols, sfb_t = sf_t + 4u * kKa * kTiles;
         {
-          uint32_t src = sf_lo0 + s * (atom_bytes >> 4), dst = sfa_t;
+          uint32_t src = sf_lo0 + s * (atom_bytes >> 4), dst = sf_t;
           for (uint32_t a = 0; a < atoms; ++a, src += 32, dst += 4) tmem_cp_atom_g<false>(dst, src, sf_hi, el);
         }
-        if constexpr (KIND == kKindMxf8) {
-          mma_mxf8f6f4_g<false>(d_tmem, a_lo, op_hi, b_lo, op_hi, idesc, sfa_t, sfb_t, accumulate, el);
-          mma_mxf8f6f4_g<false>(d_tmem, a_lo + 2, op_hi, b_lo + 2, op_hi, idesc_with_sf_ids(idesc, 1, 1), sfa_t, sfb_t, 1u, el);
-          mma_mxf8f6f4_g<false>(d_tmem, a_lo + 4, op_hi, b_lo + 4, op_hi, idesc_with_sf_ids(idesc, 2, 2), sfa_t, sfb_t, 1u, el);
-          mma_mxf8f6f4_g<false>(d_tmem, a_lo + 6, op_hi, b_lo + 6, op_hi, idesc_with_sf_ids(idesc, 3, 3), sfa_t, sfb_t, 1u, el);
-        } else {
-          const uint32_t id2 = idesc_with_sf_ids(idesc, 2, 2);
-          mma_mxf4_g<false>(d_tmem, a_lo, op_hi, b_lo, op_hi, idesc, sfa_t, sfb_t, accumulate, el);
-          mma_mxf4_g<false>(d_tmem, a_lo + 2, op_hi, b_lo + 2, op_hi, id2, sfa_t, sfb_t, 1u, el);
-          mma_mxf4_g<false>(d_tmem, a_lo + 4, op_hi, b_lo + 4, op_hi, idesc, sfa_t + 4u, sfb_t + sfb_half, 1u, el);
-          mma_mxf4_g<false>(d_tmem, a_lo + 6, op_hi, b_lo + 6, op_hi, id2, sfa_t + 4u, sfb_t + sfb_half, 1u, el);
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+          const uint32_t a_lo = a_lo0 + s * (stage_bytes >> 4) + t * (kTileM * 128 / 16);
+          const uint32_t d_tmem = d_tmem0 + static_cast<uint32_t>(t * BN), sfa_t = sf_t + 4u * kKa * t;
+          if constexpr (KIND == kKindMxf8) {
+            mma_mxf8f6f4_g<false>(d_tmem, a_lo, op_hi, b_lo, op_hi, idesc, sfa_t, sfb_t, accumulate, el);
+            mma_mxf8f6f4_g<false>(d_tmem, a_lo + 2, op_hi, b_lo + 2, op_hi, idesc_with_sf_ids(idesc, 1, 1), sfa_t, sfb_t, 1u, el);
+            mma_mxf8f6f4_g<false>(d_tmem, a_lo + 4, op_hi, b_lo + 4, op_hi, idesc_with_sf_ids(idesc, 2, 2), sfa_t, sfb_t, 1u, el);
+            mma_mxf8f6f4_g<false>(d_tmem, a_lo + 6, op_hi, b_lo + 6, op_hi, idesc_with_sf_ids(idesc, 3, 3), sfa_t, sfb_t, 1u, el);
+          } else {
+            const uint32_t id2 = idesc_with_sf_ids(idesc, 2, 2);
+            mma_mxf4_g<false>(d_tmem, a_lo, op_hi, b_lo, op_hi, idesc, sfa_t, sfb_t, accumulate, el);
+            mma_mxf4_g<false>(d_tmem, a_lo + 2, op_hi, b_lo + 2, op_hi, id2, sfa_t, sfb_t, 1u, el);
+            mma_mxf4_g<false>(d_tmem, a_lo + 4, op_hi, b_lo + 4, op_hi, idesc, sfa_t + 4u, sfb_t + sfb_half, 1u, el);
+            mma_mxf4_g<false>(d_tmem, a_lo + 6, op_hi, b_lo + 6, op_hi, id2, sfa_t + 4u, sfb_t + sfb_half, 1u, el);
+          }
         }
         accumulate = 1u;
         tc_commit_g<false>(empty_bar(s), el);  // frees the stage once these MMAs and copies have read it
@@ -405,7 +430,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
       }
       if (!ok) break;
       tc_commit_g<false>(acc_full_bar(buf), el);
-      if (++buf == 2) { buf = 0; acc_ph ^= 1u; }
+      if (++buf == acc_sets) { buf = 0; acc_ph ^= 1u; }
     }
     // nothing may still be executing when tensor memory is released
     tc_commit_g<false>(drain_bar, el);
@@ -423,26 +448,34 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
     const int r = (warp - 2) * 32 + lane;
     const uint32_t slot_off = static_cast<uint32_t>((r & 31) * 16 + (r >> 5) * 4);
     const uint32_t stage_w = staging_base + static_cast<uint32_t>(r) * 16u;
-    const uint32_t kStagingSlot = static_cast<uint32_t>(kTileM + BN) * 16u;
+    const uint32_t kStagingSlot = static_cast<uint32_t>(kTiles * kTileM + BN) * 16u, x_slot = kTiles * kTileM * 16u;
     // The k-blocks of a fetch are handed over together (one proxy fence) where the ring holds two
     // such chunks, one by one in a shorter ring, which a chunk would fill.
     const bool flush_each = stages < 2 * kUnitsPerChunk;
     // (BN need not reach 128 or 256: threads beyond it have no slot)
     const bool slot0 = r < BN, slot1 = r + 128 < BN;
     int f_it = blockIdx.x, f_kb = 0;
-    const uint8_t *f_w = nullptr, *f_x0 = nullptr, *f_x1 = nullptr;  // rows of the item being fetched, or null
+    const uint8_t *f_w[kTiles], *f_x0 = nullptr, *f_x1 = nullptr;  // rows of the item being fetched, or null
     auto enter = [&]() {  // the item at the fetch cursor
-      f_w = f_x0 = f_x1 = nullptr;
+      f_x0 = f_x1 = nullptr;
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) f_w[t] = nullptr;
       if (f_it >= n_items) return;
       const GroupedItem item = item_at(f_it);
-      int col, row;
-      if constexpr (kGated) {
-        col = item.tile * 64 + (r >> 5) * 16 + (r & 15);
-        row = col + ((r & 16) ? p.n : 0);
-      } else {
-        col = row = item.tile * kTileM + r;
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) {
+        int col, row;
+        if constexpr (kTwo) {
+          col = item.tile * kTileCols + (kGated ? 0 : t * kTileM) + r;
+          row = col + (kGated && t == 1 ? p.n : 0);
+        } else if constexpr (kGated) {
+          col = item.tile * kTileCols + (r >> 5) * 16 + (r & 15);
+          row = col + ((r & 16) ? p.n : 0);
+        } else {
+          col = row = item.tile * kTileCols + r;
+        }
+        if (col < p.n) f_w[t] = p.sw + (static_cast<int64_t>(item.group) * p.b_group_rows + row) * p.ld_sw;
       }
-      if (col < p.n) f_w = p.sw + (static_cast<int64_t>(item.group) * p.b_group_rows + row) * p.ld_sw;
       const int a0 = x_row(item, r);
       if (a0 >= 0) f_x0 = p.sx + a0 * p.ld_sx;
       if (slot1) {
@@ -455,10 +488,12 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
         const int col = (f_kb * kSfBytes) & ~15;
         const int valid = min(16, p.kblocks32 - col);
         const uint32_t dst = stage_w + slot * kStagingSlot;
-        fetch_scales(dst, f_w != nullptr ? f_w + col : p.sw, f_w != nullptr ? valid : 0, p.align_w);
-        if (slot0) fetch_scales(dst + kTileM * 16u, f_x0 != nullptr ? f_x0 + col : p.sx, f_x0 != nullptr ? valid : 0, p.align_x);
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+          fetch_scales(dst + t * kTileM * 16u, f_w[t] != nullptr ? f_w[t] + col : p.sw, f_w[t] != nullptr ? valid : 0, p.align_w);
+        if (slot0) fetch_scales(dst + x_slot, f_x0 != nullptr ? f_x0 + col : p.sx, f_x0 != nullptr ? valid : 0, p.align_x);
         if (slot1)
-          fetch_scales(dst + kTileM * 32u, f_x1 != nullptr ? f_x1 + col : p.sx, f_x1 != nullptr ? valid : 0, p.align_x);
+          fetch_scales(dst + x_slot + kTileM * 16u, f_x1 != nullptr ? f_x1 + col : p.sx, f_x1 != nullptr ? valid : 0, p.align_x);
         f_kb = (f_kb | (kUnitsPerChunk - 1)) + 1;
         if (f_kb >= p.k_blocks) {
           f_kb = 0;
@@ -469,24 +504,28 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
       asm volatile("cp.async.commit_group;" ::: "memory");  // always: the group count stays in step
     };
     enter();
-    for (int j = 0; j < kGroupedFetchAhead; ++j) fetch(j);
+    for (int j = 0; j < kFetchAhead; ++j) fetch(j);
     int s = 0, kb = 0, c_slot = 0;
     uint32_t ph = 0;
     bool alive = true;
     for (int it = blockIdx.x; it < n_items && alive;) {
       const int in_chunk = min(kUnitsPerChunk - (kb & (kUnitsPerChunk - 1)), p.k_blocks - kb);
-      asm volatile("cp.async.wait_group %0;" ::"n"(kGroupedFetchAhead - 1) : "memory");
-      uint4 cw, cx0 = make_uint4(0, 0, 0, 0), cx1 = make_uint4(0, 0, 0, 0);
+      asm volatile("cp.async.wait_group %0;" ::"n"(kFetchAhead - 1) : "memory");
+      uint4 cw[kTiles], cx0 = make_uint4(0, 0, 0, 0), cx1 = make_uint4(0, 0, 0, 0);
       const uint32_t from = stage_w + c_slot * kStagingSlot;
-      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(cw.x), "=r"(cw.y), "=r"(cw.z), "=r"(cw.w) : "r"(from));
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(cw[t].x), "=r"(cw[t].y), "=r"(cw[t].z), "=r"(cw[t].w)
+                     : "r"(from + t * kTileM * 16u));
       if (slot0)
         asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                      : "=r"(cx0.x), "=r"(cx0.y), "=r"(cx0.z), "=r"(cx0.w)
-                     : "r"(from + kTileM * 16u));
+                     : "r"(from + x_slot));
       if (slot1)
         asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                      : "=r"(cx1.x), "=r"(cx1.y), "=r"(cx1.z), "=r"(cx1.w)
-                     : "r"(from + kTileM * 32u));
+                     : "r"(from + x_slot + kTileM * 16u));
       int s2 = s;
       uint32_t ph2 = ph;
       for (int u = 0; u < in_chunk; ++u) {
@@ -500,10 +539,12 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
           break;
         }
         const int sub = ((kb + u) & (kUnitsPerChunk - 1)) * kKa;
-        const uint32_t aw = atom_base + s2 * atom_bytes + slot_off, ax = aw + kKa * 512u;
+        const uint32_t aw = atom_base + s2 * atom_bytes + slot_off, ax = aw + kTiles * kKa * 512u;
 #pragma unroll
         for (int a = 0; a < kKa; ++a) {
-          asm volatile("st.shared.u32 [%0], %1;" ::"r"(aw + 512u * a), "r"(pick_word(cw, sub + a)) : "memory");
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t)
+            asm volatile("st.shared.u32 [%0], %1;" ::"r"(aw + 512u * (t * kKa + a)), "r"(pick_word(cw[t], sub + a)) : "memory");
           asm volatile("st.shared.u32 [%0], %1;" ::"r"(ax + 512u * (a * x_halves)), "r"(pick_word(cx0, sub + a)) : "memory");
           if (x_halves == 2)
             asm volatile("st.shared.u32 [%0], %1;" ::"r"(ax + 512u * (a * 2 + 1)), "r"(pick_word(cx1, sub + a)) : "memory");
@@ -528,7 +569,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
         }
       }
       fetch(c_slot);
-      if (++c_slot == kGroupedFetchAhead) c_slot = 0;
+      if (++c_slot == kFetchAhead) c_slot = 0;
       s = s2;
       ph = ph2;
       kb += in_chunk;
@@ -540,7 +581,9 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
     asm volatile("cp.async.wait_group 0;" ::: "memory");
   } else {
     // -------------------------------- epilogue --------------------------------
+    // kTwo: two warps to a lane quarter.  Gated they take 32 columns in turn, else a W tile each.
     const int quarter = warp & 3;  // the TMEM lane quarter this warp can read
+    const int half = warp >= 11 ? 1 : 0;
     int buf = 0;
     uint32_t acc_ph = 0;
     for (int it = blockIdx.x; it < n_items; it += step) {
@@ -554,16 +597,28 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
         break;
       }
       tc_fence_after_sync();
-      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(buf * BN);
-      const int col = item.tile * kTileCols + (kGated ? quarter * 16 + (lane & 15) : quarter * 32 + lane);
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
+                             static_cast<uint32_t>(buf * acc_cols + (kTwo && !kGated ? half * BN : 0));
+      int col = item.tile * kTileCols;
+      if constexpr (kTwo) col += (kGated ? 0 : half * kTileM) + quarter * 32 + lane;
+      else col += kGated ? quarter * 16 + (lane & 15) : quarter * 32 + lane;
       const bool in = col < p.n;
-      for (int c = 0; c < item.count; c += 32) {
+      for (int c = kTwo && kGated ? 32 * half : 0; c < item.count; c += kTwo && kGated ? 64 : 32) {
         uint32_t acc[32];
         tmem_ld_32x32(taddr + static_cast<uint32_t>(c), acc);
         const int q_mine = pair_at(item, c + lane);
         const float w_mine = p.row_weights != nullptr && q_mine >= 0 ? p.row_weights[q_mine] : 1.0f;
-        tmem_ld_wait();
-        if constexpr (kGated) {
+        if constexpr (kGated && kTwo) {
+          uint32_t up[32];
+          tmem_ld_32x32(taddr + static_cast<uint32_t>(BN + c), up);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            acc[j] = __float_as_uint(silu_f32(__uint_as_float(acc[j])) * __uint_as_float(up[j]));
+        } else {
+          tmem_ld_wait();
+        }
+        if constexpr (kGated && !kTwo) {
           // lanes 0-15 hold the gate, 16-31 the up product: the lower lanes finish the even columns,
           // the upper ones the odd
 #pragma unroll
@@ -590,7 +645,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(acc_empty_bar(buf));
-      if (++buf == 2) { buf = 0; acc_ph ^= 1u; }
+      if (++buf == acc_sets) { buf = 0; acc_ph ^= 1u; }
     }
   }
 

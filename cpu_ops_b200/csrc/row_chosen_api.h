@@ -99,10 +99,21 @@ size_t route_smem_bytes(int experts, int n_groups) {
 }
 
 using GroupedKernel = void (*)(CUtensorMap, CUtensorMap, GroupedParams);
-GroupedKernel grouped_kernel(int kind, bool gated) {
-  if (kind == kKindMxf4) return gated ? grouped_mx_kernel<kKindMxf4, true> : grouped_mx_kernel<kKindMxf4, false>;
-  return gated ? grouped_mx_kernel<kKindMxf8, true> : grouped_mx_kernel<kKindMxf8, false>;
+template <int KIND>
+GroupedKernel grouped_kernel_for(bool gated, bool two) {
+  if (two) return gated ? grouped_mx_kernel<KIND, true, true> : grouped_mx_kernel<KIND, false, true>;
+  return gated ? grouped_mx_kernel<KIND, true, false> : grouped_mx_kernel<KIND, false, false>;
 }
+GroupedKernel grouped_kernel(int kind, bool gated, bool two) {
+  return kind == kKindMxf4 ? grouped_kernel_for<kKindMxf4>(gated, two) : grouped_kernel_for<kKindMxf8>(gated, two);
+}
+
+// Tiles of one launch of the experts' kernel.
+struct GroupedChoice {
+  bool two = false;     // two W tiles per CTA
+  bool sorted = false;  // rows of A copied in plan order first
+  int BN = 32, stages = 2, tile_cols = 128;
+};
 
 // The kernels for many rows: ranks in chunks of 16 or 64.
 using AdapterTileKernel = void (*)(AdapterTileParams);
@@ -139,7 +150,8 @@ int row_kernels_ready(DeviceState& st) {
     CUDA_TRY(cudaFuncSetAttribute(route_kernel_for(experts), kMost, static_cast<int>(route_smem_bytes(experts, experts))));
   CUDA_TRY(cudaFuncSetAttribute(group_rows_kernel, kMost, plan_smem_bytes(kMaxGroups)));
   for (int kind : {kKindMxf8, kKindMxf4})
-    for (bool gated : {false, true}) CUDA_TRY(cudaFuncSetAttribute(grouped_kernel(kind, gated), kMost, st.smem_optin));
+    for (bool gated : {false, true})
+      for (bool two : {false, true}) CUDA_TRY(cudaFuncSetAttribute(grouped_kernel(kind, gated, two), kMost, st.smem_optin));
   for (int x_type : {kTypeF32, kTypeF16, kTypeBf16})
     for (int w_type : {kTypeF16, kTypeBf16})
       for (bool narrow : {false, true})
@@ -264,6 +276,52 @@ int route_call(const cpuops_b200_route_desc* d) {
 
 // ---- the experts' products -----------------------------------------------------------------
 
+int grouped_stages(int smem_optin, int BN, int ka, int groups, bool two) {
+  return std::min(kGroupedMaxStages, (smem_optin - grouped_smem_bytes(BN, 0, ka, groups, two)) /
+                                         (grouped_stage_bytes(BN, two) + grouped_atoms(BN, ka, two) * 512));
+}
+
+// The host knows how many pairs there are, not how they spread: it plans for equal groups.
+//   * Few pairs per group (below 48): one W tile, room for twice the average, rows gathered.  Such calls are bound
+//     by reading W, and the width does not matter to that.
+//   * Many: the width and the tile count whose estimated time is least: rounds of items over the SMs
+//     x (k-blocks x cycles per k-block + a fixed part).  A k-block takes its MMAs' time (2 cycles per
+//     pair and W tile), or 2000 cycles over the stages where the ring is too short for that.
+GroupedChoice choose_grouped(const DeviceState& st, int rows, int n, int groups, int k_blocks, int ka, bool gated) {
+  GroupedChoice best;
+  const int average = rows / std::max(1, groups), sms = st.sms();
+  if (average < 48) {
+    best.BN = std::max(32, std::min(kGroupedMaxBN, (std::min(rows, 2 * average) + 31) / 32 * 32));
+    best.stages = grouped_stages(st.smem_optin, best.BN, ka, groups, false);
+    best.tile_cols = gated ? 64 : 128;
+    return best;
+  }
+  double least = 0.0;
+  for (bool two : {true, false}) {
+    for (int BN = 64; BN <= kGroupedMaxBN; BN += 16) {
+      GroupedChoice c;
+      c.two = two;
+      c.sorted = true;
+      c.BN = BN;
+      c.tile_cols = (gated ? 64 : 128) * (two ? 2 : 1);
+      c.stages = grouped_stages(st.smem_optin, BN, ka, groups, two);
+      if (c.stages < 2) continue;
+      const int wide = average + average / 8;  // (groups differ: cuts for a somewhat larger one)
+      const int cuts = (wide + BN - 1) / BN, width = ((average + cuts - 1) / cuts + 15) / 16 * 16;
+      const int64_t items = static_cast<int64_t>(groups) * cuts * ((n + c.tile_cols - 1) / c.tile_cols);
+      const double rounds = static_cast<double>((items + sms - 1) / sms);
+      const double block = std::max(2.0 * width * (two ? 2 : 1), 2000.0 / c.stages);
+      const double drain = grouped_acc_sets(BN, ka, two) == 2 ? 500.0 : 500.0 + 10.0 * width;
+      const double cycles = rounds * (k_blocks * block + drain);
+      if (least == 0.0 || cycles < least) {
+        least = cycles;
+        best = c;
+      }
+    }
+  }
+  return best;
+}
+
 int gemm_grouped_call(const cpuops_b200_gemm_grouped_desc* d) {
   if (int rc = check_desc(d)) return rc;
   auto ok_fmt = [](int f) { return f == CPUOPS_B200_FMT_E4M3 || f == CPUOPS_B200_FMT_E5M2 || f == CPUOPS_B200_FMT_E2M1; };
@@ -308,9 +366,6 @@ int gemm_grouped_call(const cpuops_b200_gemm_grouped_desc* d) {
     return refuse("gemm_grouped: A and B must be 16-byte aligned with rows a multiple of 16 bytes apart (e2m1 weights "
                   "under 8-bit rows: 32 bytes, and k a multiple of 128)");
   const int kind = fp4_a ? kKindMxf4 : kKindMxf8;
-  const int tile_cols = d->gated ? 64 : 128;
-  const int tiles = static_cast<int>((static_cast<int64_t>(n) + tile_cols - 1) / tile_cols);
-
   RowCall call;
   if (int rc = call.enter(*d)) return rc;
   DeviceState& st = *call.st;
@@ -333,16 +388,18 @@ int gemm_grouped_call(const cpuops_b200_gemm_grouped_desc* d) {
   p.b_group_rows = d->b_group_rows;
   p.a_rows = d->a_rows;
   p.pairs_per_a_row = d->pairs_per_a_row;
-  p.tiles = tiles;
+  const int ka = kind == kKindMxf4 ? 2 : 1;
   p.k_blocks = (k + (kind == kKindMxf4 ? 255 : 127)) / (kind == kKindMxf4 ? 256 : 128);
   p.kblocks32 = blocks32;
-  // twice the pairs that a group has on average, in steps of 32
-  p.BN = std::min(kGroupedMaxBN, (std::min(rows, 2 * (rows / std::max(1, groups))) + 31) / 32 * 32);
-  p.BN = std::max(p.BN, 32);
+  const GroupedChoice choice = choose_grouped(st, rows, n, groups, p.k_blocks, ka, d->gated != 0);
+  p.BN = choice.BN;
+  p.stages = choice.stages;
+  p.sorted = choice.sorted ? 1 : 0;
+  p.tiles = static_cast<int>((static_cast<int64_t>(n) + choice.tile_cols - 1) / choice.tile_cols);
   auto alignment = [&](const void* ptr, int64_t ld) { return on(ptr, ld, 16) ? 16 : on(ptr, ld, 4) ? 4 : 1; };
   p.align_w = alignment(d->b_scales, d->ld_scales_b);
   p.align_x = alignment(d->a_scales, d->ld_scales_a);
-  p.w_tile_bytes = kTileM * (mixed ? 64 : 128);
+  p.w_tile_bytes = (choice.two ? 2 : 1) * kTileM * (mixed ? 64 : 128);
   {
     auto code = [](int f) { return f == CPUOPS_B200_FMT_E5M2 ? 1u : f == CPUOPS_B200_FMT_E2M1 ? 5u : 0u; };
     p.idesc = kind == kKindMxf4 ? make_idesc_block_scaled(1u, 1u, kTileM, 0)
@@ -351,8 +408,6 @@ int gemm_grouped_call(const cpuops_b200_gemm_grouped_desc* d) {
   p.wait_budget_us = g_wait_budget_us.load();
   p.error = st.error_dev;
 
-  // Rows copied in plan order, where groups have more pairs than gathering hides behind W's loads.
-  p.sorted = groups > 0 && rows / groups >= 48 ? 1 : 0;
   const int row_bytes = fp4_a ? k / 2 : k;
   const int64_t x_pitch = align_up(row_bytes, 16), sx_pitch = align_up(blocks32, 16);
   Plan plan;
@@ -376,11 +431,11 @@ int gemm_grouped_call(const cpuops_b200_gemm_grouped_desc* d) {
   p.d = summed ? reinterpret_cast<float*>(ws + off_sum) : d->d;
   p.ldd = summed ? n : d->ldd;
 
-  const int64_t most_items = (static_cast<int64_t>(std::min(groups, rows)) + rows / p.BN) * tiles;
+  const int64_t most_items = (static_cast<int64_t>(std::min(groups, rows)) + rows / p.BN) * p.tiles;
   if (most_items > INT32_MAX) return refuse("gemm_grouped: the problem has more tiles than fit 31 bits");
   if (groups > 0) {
     CUtensorMap tmW, tmX;
-    const uint32_t box = d->gated ? 16 : 128;
+    const uint32_t box = d->gated && !choice.two ? 16 : 128;
     if (mixed) {
       if (int rc = make_tensor_map_fp4_padded(&tmW, d->b, k, b_rows, b_pitch, box)) return rc;
     } else {
@@ -391,15 +446,11 @@ int gemm_grouped_call(const cpuops_b200_gemm_grouped_desc* d) {
     } else {
       if (int rc = make_tensor_map(&tmX, d->a, row_bytes, d->a_rows, a_pitch, 1)) return rc;
     }
-    const int ka = kind == kKindMxf4 ? 2 : 1;
-    const int fixed = grouped_smem_bytes(p.BN, 0, ka, groups);
-    p.stages = std::min(kGroupedMaxStages,
-                        (st.smem_optin - fixed) / (grouped_stage_bytes(p.BN) + grouped_atoms(p.BN, ka) * 512));
     // (one CTA per SM: it takes all of tensor memory)
-    const int smem = std::max(grouped_smem_bytes(p.BN, p.stages, ka, groups), 120 * 1024);
-    GroupedKernel kernel = grouped_kernel(kind, d->gated != 0);
+    const int smem = std::max(grouped_smem_bytes(p.BN, p.stages, ka, groups, choice.two), 120 * 1024);
     const unsigned grid = static_cast<unsigned>(std::min<int64_t>(most_items, st.sms()));
-    if (int rc = launch_after(kernel, dim3(grid), kGroupedThreads, static_cast<size_t>(smem), call.stream, tmW, tmX, p))
+    if (int rc = launch_after(grouped_kernel(kind, d->gated != 0, choice.two), dim3(grid), grouped_threads(choice.two),
+                              static_cast<size_t>(smem), call.stream, tmW, tmX, p))
       return rc;
   }
   if (summed) {
