@@ -25,8 +25,11 @@
 //     contiguous bytes of one row of D at a time: rows go wherever the plan says, with no
 //     staging.
 //
-// Roles (352 threads): warp 0 TMA producer of W, warp 1 MMA issuer (owns tensor memory), warps 2-5
-// scale writers, warps 6-9 (kTwo: 11-14 too) epilogue (one TMEM lane quarter each), warp 10 loads X.
+// Roles (512 threads, kTwo 640): warp 0 TMA producer of W, warp 1 MMA issuer (owns tensor memory), warps
+// 2-9 scale writers (two sets of four in turn), warps 10-11 load X (in turn), warps 12-15 (kTwo: -19)
+// epilogue (one TMEM lane quarter each).  What a role does for a k-block is a chain of latencies of
+// some 600 cycles (wait, a few operations, fence, arrival), which with one warp or set was longer
+// than the k-block's loads took: hence the turns.
 // Every wait is bounded, as in the other kernels.
 #pragma once
 
@@ -35,11 +38,13 @@
 
 namespace b200 {
 
-constexpr int kGroupedThreads = 352;      // kTwo: 128 more, four epilogue warps
-__host__ __device__ constexpr int grouped_threads(bool two) { return two ? kGroupedThreads + 128 : kGroupedThreads; }
+// Warps: 0 loads W, 1 issues MMAs, 2-9 write scales, 10-11 load X, from 12 on the epilogue.
+constexpr int kGroupedEpilogueWarp = 12;
+__host__ __device__ constexpr int grouped_threads(bool two) { return 32 * (kGroupedEpilogueWarp + (two ? 8 : 4)); }
 constexpr int kGroupedMaxStages = 8;
 constexpr int kGroupedMaxBN = 192;   // two accumulators and four slots of scales fit tensor memory
-__host__ __device__ constexpr int grouped_fetch_ahead(bool two) { return two ? 2 : 3; }  // scale fetches in flight
+// 16-byte scale chunks that each of the two sets of scale writers has in flight
+__host__ __device__ constexpr int grouped_fetch_ahead(bool two) { return two ? 1 : 2; }
 
 struct GroupedParams {
   const uint8_t* sw;          // W's scales, row-major
@@ -69,7 +74,7 @@ struct GroupedParams {
 __host__ __device__ inline int grouped_stage_bytes(int BN, bool two) { return (two ? 2 : 1) * kTileM * 128 + BN * 128; }
 __host__ __device__ inline int grouped_atoms(int BN, int ka, bool two) { return ka * ((two ? 2 : 1) + (BN > 128 ? 2 : 1)); }
 __host__ __device__ inline int grouped_staging_bytes(int BN, bool two) {
-  return grouped_fetch_ahead(two) * ((two ? 2 : 1) * kTileM + BN) * 16;
+  return 2 * grouped_fetch_ahead(two) * ((two ? 2 : 1) * kTileM + BN) * 16;
 }
 // Tensor memory: accumulators of BN columns (two sets of them, where they fit), four slots of scales.
 __host__ __device__ inline int grouped_acc_sets(int BN, int ka, bool two) {
@@ -308,20 +313,21 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
       while (global_timer_ns() < t_end) __nanosleep(1000);
     }
     __syncwarp();
-  } else if (warp == 10) {
-    // ------------------------------ X gather ------------------------------
-    // Rows in plan order: lane l loads rows 16 l .. 16 l + 15.  Otherwise:
-    // Lane l gathers rows 4 l .. 4 l + 3 of the item's X, and those 128 further on.  Rows that do not
-    // exist inside a group of four are read as the group's first one; groups without any row
-    // are left as they are (their columns are computed and never read).
-    int s = 0;
+  } else if (warp == 10 || warp == 11) {
+    // ------------------------------ X ------------------------------
+    // Two warps, k-blocks in turn (as for the scale writers' runs, a ring of two stages or more keeps the
+    // parities apart).  Rows in plan order: one or two boxes of BN / 2 rows.  Otherwise lane l
+    // gathers rows 4 l .. 4 l + 3 of the item's X, and those 128 further on; rows that do not exist
+    // inside a group of four are read as the group's first one.  What is not loaded is left as it is
+    // (its columns are computed and never read).
+    const uint32_t el = elect_one() ? 1u : 0u;
+    int s = 0, turn = 0;
     uint32_t ph = 0;
     bool alive = true;
     for (int it = blockIdx.x; it < n_items && alive; it += step) {
       const GroupedItem item = item_at(it);
       int row[2][4];
       bool mine[2];
-      const bool box = p.sorted && 16 * lane < item.count;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int r0 = 128 * h + 4 * lane;
@@ -333,26 +339,34 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
         for (int j = 1; j < 4; ++j)
           if (row[h][j] < 0) row[h][j] = row[h][0];
       }
-      const uint32_t bytes = p.sorted ? static_cast<uint32_t>((item.count + 15) >> 4) * 2048u
+      const bool second = item.count > BN / 2;
+      const uint32_t bytes = p.sorted ? static_cast<uint32_t>(BN / 2 * 128 * (second ? 2 : 1))
                                       : static_cast<uint32_t>((item.count + 3) >> 2) * 512u;
       for (int kb = 0; kb < p.k_blocks; ++kb) {
-        if (!__all_sync(kAll, mbar_wait_bounded(empty_bar(s), ph ^ 1u, abort_flag, budget_ns))) {
-          if (lane == 0) {
-            leave_error(p.error, kErrProducerWait);
-            *abort_flag = 1;
+        if (turn == warp - 10) {
+          if (!__all_sync(kAll, mbar_wait_bounded(empty_bar(s), ph ^ 1u, abort_flag, budget_ns))) {
+            if (el) {
+              leave_error(p.error, kErrProducerWait);
+              *abort_flag = 1;
+            }
+            alive = false;
+            break;
           }
-          alive = false;
-          break;
-        }
-        if (lane == 0) mbar_expect_tx(full_bar(s), bytes);
-        __syncwarp();
-        const uint32_t x_base = smem_base + s * stage_bytes + kWBytes;
-        if (box) tma_load_2d(x_base + static_cast<uint32_t>(lane) * 2048u, &tmX, full_bar(s), kb * 128, item.p0 + 16 * lane);
-        const uint32_t dst = x_base + static_cast<uint32_t>(lane) * 512u;
+          mbar_expect_tx_p(full_bar(s), bytes, el);
+          const uint32_t x_base = smem_base + s * stage_bytes + kWBytes;
+          if (p.sorted) {
+            tma_load_2d_g<false>(x_base, &tmX, full_bar(s), kb * 128, item.p0, el);
+            tma_load_2d_g<false>(x_base + BN / 2 * 128, &tmX, full_bar(s), kb * 128, item.p0 + BN / 2, second ? el : 0u);
+          } else {
+            __syncwarp();  // (the bytes are announced before any can arrive)
+            const uint32_t dst = x_base + static_cast<uint32_t>(lane) * 512u;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          if (mine[h])
-            tma_gather4(dst + h * 128u * 128u, &tmX, full_bar(s), kb * 128, row[h][0], row[h][1], row[h][2], row[h][3]);
+            for (int h = 0; h < 2; ++h)
+              if (mine[h])
+                tma_gather4(dst + h * 128u * 128u, &tmX, full_bar(s), kb * 128, row[h][0], row[h][1], row[h][2], row[h][3]);
+          }
+        }
+        turn ^= 1;
         if (++s == stages) { s = 0; ph ^= 1u; }
       }
     }
@@ -440,18 +454,23 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
       *abort_flag = 1;
     }
     __syncwarp();
-  } else if (warp < 6) {
+  } else if (warp < 10) {
     // ------------------------------ scale writers ------------------------------
-    // Thread r (0..127) owns row r of the W tile and rows r and r + 128 of X.  As in the small-m
-    // kernel it fetches its rows' scale bytes 16 at a time, a few fetches ahead, and turns them
-    // into the atoms of the k-blocks that share the fetch.
-    const int r = (warp - 2) * 32 + lane;
+    // Two sets of four warps that take runs of kRun k-blocks in turn.  Thread r (0..127) of a set owns
+    // row r of each W tile and rows r and r + 128 of X.  As in the small-m kernel it fetches its rows'
+    // scale bytes 16 at a time, ahead, and turns them into the atoms of its k-blocks among those that
+    // share the fetch.
+    // A set waits for its own stages only, and a parity wait tells a phase from the one two before it only
+    // if that one is known to be over.  It is: the set has seen the stage of the k-block in front of
+    // the other's run free, hence (MMAs end in order) all k-blocks up to a ring's length before that
+    // one done; the phase in question is two ring lengths back, no later than that while a
+    // run is shorter than the ring.
+    constexpr int kRun = kUnitsPerChunk / 2;
+    const int set = (warp - 2) >> 2;
+    const int r = ((warp - 2) & 3) * 32 + lane;
     const uint32_t slot_off = static_cast<uint32_t>((r & 31) * 16 + (r >> 5) * 4);
-    const uint32_t stage_w = staging_base + static_cast<uint32_t>(r) * 16u;
     const uint32_t kStagingSlot = static_cast<uint32_t>(kTiles * kTileM + BN) * 16u, x_slot = kTiles * kTileM * 16u;
-    // The k-blocks of a fetch are handed over together (one proxy fence) where the ring holds two
-    // such chunks, one by one in a shorter ring, which a chunk would fill.
-    const bool flush_each = stages < 2 * kUnitsPerChunk;
+    const uint32_t stage_w = staging_base + static_cast<uint32_t>(r) * 16u + static_cast<uint32_t>(set * kFetchAhead) * kStagingSlot;
     // (BN need not reach 128 or 256: threads beyond it have no slot)
     const bool slot0 = r < BN, slot1 = r + 128 < BN;
     int f_it = blockIdx.x, f_kb = 0;
@@ -494,7 +513,7 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
         if (slot0) fetch_scales(dst + x_slot, f_x0 != nullptr ? f_x0 + col : p.sx, f_x0 != nullptr ? valid : 0, p.align_x);
         if (slot1)
           fetch_scales(dst + x_slot + kTileM * 16u, f_x1 != nullptr ? f_x1 + col : p.sx, f_x1 != nullptr ? valid : 0, p.align_x);
-        f_kb = (f_kb | (kUnitsPerChunk - 1)) + 1;
+        f_kb += kUnitsPerChunk;
         if (f_kb >= p.k_blocks) {
           f_kb = 0;
           f_it += step;
@@ -505,11 +524,11 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
     };
     enter();
     for (int j = 0; j < kFetchAhead; ++j) fetch(j);
-    int s = 0, kb = 0, c_slot = 0;
+    int s = 0, kb = 0, c_slot = 0, run = 0;  // run: k-blocks so far, modulo two runs
     uint32_t ph = 0;
     bool alive = true;
     for (int it = blockIdx.x; it < n_items && alive;) {
-      const int in_chunk = min(kUnitsPerChunk - (kb & (kUnitsPerChunk - 1)), p.k_blocks - kb);
+      const int in_chunk = min(kUnitsPerChunk, p.k_blocks - kb);
       asm volatile("cp.async.wait_group %0;" ::"n"(kFetchAhead - 1) : "memory");
       uint4 cw[kTiles], cx0 = make_uint4(0, 0, 0, 0), cx1 = make_uint4(0, 0, 0, 0);
       const uint32_t from = stage_w + c_slot * kStagingSlot;
@@ -526,52 +545,49 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
         asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                      : "=r"(cx1.x), "=r"(cx1.y), "=r"(cx1.z), "=r"(cx1.w)
                      : "r"(from + x_slot + kTileM * 16u));
-      int s2 = s;
-      uint32_t ph2 = ph;
+      int first_s = s, pending = 0;  // stages written and not yet handed over
       for (int u = 0; u < in_chunk; ++u) {
-        // the stage's previous atoms have been copied to tensor memory (its MMAs are done)
-        if (!__all_sync(kAll, mbar_wait_bounded(empty_bar(s2), ph2 ^ 1u, abort_flag, budget_ns))) {
-          if (lane == 0) {
-            leave_error(p.error, kErrProducerWait);
-            *abort_flag = 1;
+        if (run / kRun == set) {
+          // the stage's previous atoms have been copied to tensor memory (its MMAs are done)
+          if (!__all_sync(kAll, mbar_wait_bounded(empty_bar(s), ph ^ 1u, abort_flag, budget_ns))) {
+            if (lane == 0) {
+              leave_error(p.error, kErrProducerWait);
+              *abort_flag = 1;
+            }
+            alive = false;
+            break;
           }
-          alive = false;
-          break;
-        }
-        const int sub = ((kb + u) & (kUnitsPerChunk - 1)) * kKa;
-        const uint32_t aw = atom_base + s2 * atom_bytes + slot_off, ax = aw + kTiles * kKa * 512u;
+          const int sub = u * kKa;
+          const uint32_t aw = atom_base + s * atom_bytes + slot_off, ax = aw + kTiles * kKa * 512u;
 #pragma unroll
-        for (int a = 0; a < kKa; ++a) {
+          for (int a = 0; a < kKa; ++a) {
 #pragma unroll
-          for (int t = 0; t < kTiles; ++t)
-            asm volatile("st.shared.u32 [%0], %1;" ::"r"(aw + 512u * (t * kKa + a)), "r"(pick_word(cw[t], sub + a)) : "memory");
-          asm volatile("st.shared.u32 [%0], %1;" ::"r"(ax + 512u * (a * x_halves)), "r"(pick_word(cx0, sub + a)) : "memory");
-          if (x_halves == 2)
-            asm volatile("st.shared.u32 [%0], %1;" ::"r"(ax + 512u * (a * 2 + 1)), "r"(pick_word(cx1, sub + a)) : "memory");
+            for (int t = 0; t < kTiles; ++t)
+              asm volatile("st.shared.u32 [%0], %1;" ::"r"(aw + 512u * (t * kKa + a)), "r"(pick_word(cw[t], sub + a)) : "memory");
+            asm volatile("st.shared.u32 [%0], %1;" ::"r"(ax + 512u * (a * x_halves)), "r"(pick_word(cx0, sub + a)) : "memory");
+            if (x_halves == 2)
+              asm volatile("st.shared.u32 [%0], %1;" ::"r"(ax + 512u * (a * 2 + 1)), "r"(pick_word(cx1, sub + a)) : "memory");
+          }
+          if (pending++ == 0) first_s = s;
         }
-        if (flush_each) {
-          fence_proxy_async_shared_cta();
+        if (++run == 2 * kRun) run = 0;
+        if (++s == stages) { s = 0; ph ^= 1u; }
+        // a run (or chunk) has ended: hand its stages over (one proxy fence for all)
+        if (pending > 0 && (u + 1 == in_chunk || run / kRun != set)) {
+          fence_proxy_async_shared_cta();  // these writes -> visible to tcgen05.cp
           __syncwarp();
-          if (lane == 0) mbar_arrive(full_bar(s2));
+          if (lane == 0) {
+            for (int j = 0; j < pending; ++j) {
+              mbar_arrive(full_bar(first_s));
+              if (++first_s == stages) first_s = 0;
+            }
+          }
+          pending = 0;
         }
-        if (++s2 == stages) { s2 = 0; ph2 ^= 1u; }
       }
       if (!alive) break;
-      if (!flush_each) {
-        fence_proxy_async_shared_cta();  // these writes -> visible to tcgen05.cp (one fence per chunk)
-        __syncwarp();
-      }
-      if (!flush_each && lane == 0) {
-        int s3 = s;
-        for (int u = 0; u < in_chunk; ++u) {
-          mbar_arrive(full_bar(s3));
-          if (++s3 == stages) s3 = 0;
-        }
-      }
       fetch(c_slot);
       if (++c_slot == kFetchAhead) c_slot = 0;
-      s = s2;
-      ph = ph2;
       kb += in_chunk;
       if (kb == p.k_blocks) {
         kb = 0;
@@ -581,13 +597,21 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
     asm volatile("cp.async.wait_group 0;" ::: "memory");
   } else {
     // -------------------------------- epilogue --------------------------------
-    // kTwo: two warps to a lane quarter.  Gated they take 32 columns in turn, else a W tile each.
+    // 16 columns (pairs) at a time; their pairs and weights are fetched one step ahead, those of an
+    // item's first step before its accumulator is waited for.  kTwo: two warps to a lane quarter;
+    // gated they take the steps in turn, else a W tile each.
     const int quarter = warp & 3;  // the TMEM lane quarter this warp can read
-    const int half = warp >= 11 ? 1 : 0;
+    const int half = (warp - kGroupedEpilogueWarp) >> 2;
+    constexpr bool kTurns = kTwo && kGated;
+    constexpr int kStep = kTurns ? 32 : 16;
+    const bool weighted = p.row_weights != nullptr;
     int buf = 0;
     uint32_t acc_ph = 0;
     for (int it = blockIdx.x; it < n_items; it += step) {
       const GroupedItem item = item_at(it);
+      const int c0 = kTurns ? 16 * half : 0;
+      int q_next = pair_at(item, c0 + (lane & 15));
+      float w_next = weighted && q_next >= 0 ? p.row_weights[q_next] : 1.0f;
       const bool got = mbar_wait_bounded(acc_full_bar(buf), acc_ph, abort_flag, budget_ns);
       if (!__all_sync(kAll, got)) {
         if (lane == 0) {
@@ -602,45 +626,54 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
       int col = item.tile * kTileCols;
       if constexpr (kTwo) col += (kGated ? 0 : half * kTileM) + quarter * 32 + lane;
       else col += kGated ? quarter * 16 + (lane & 15) : quarter * 32 + lane;
+      float* const d_col = p.d + col;
       const bool in = col < p.n;
-      for (int c = kTwo && kGated ? 32 * half : 0; c < item.count; c += kTwo && kGated ? 64 : 32) {
-        uint32_t acc[32];
-        tmem_ld_32x32(taddr + static_cast<uint32_t>(c), acc);
-        const int q_mine = pair_at(item, c + lane);
-        const float w_mine = p.row_weights != nullptr && q_mine >= 0 ? p.row_weights[q_mine] : 1.0f;
-        if constexpr (kGated && kTwo) {
-          uint32_t up[32];
-          tmem_ld_32x32(taddr + static_cast<uint32_t>(BN + c), up);
+      for (int c = c0; c < item.count; c += kStep) {
+        const int q_mine = q_next;
+        const float w_mine = w_next;
+        q_next = pair_at(item, c + kStep + (lane & 15));
+        uint32_t acc[16];
+        tmem_ld_32x16(taddr + static_cast<uint32_t>(c), acc);
+        if constexpr (kTurns) {
+          uint32_t up[16];
+          tmem_ld_32x16(taddr + static_cast<uint32_t>(BN + c), up);
           tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
+          for (int j = 0; j < 16; ++j)
             acc[j] = __float_as_uint(silu_f32(__uint_as_float(acc[j])) * __uint_as_float(up[j]));
         } else {
           tmem_ld_wait();
         }
-        if constexpr (kGated && !kTwo) {
-          // lanes 0-15 hold the gate, 16-31 the up product: the lower lanes finish the even columns,
-          // the upper ones the odd
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            const uint32_t give = lane < 16 ? acc[j + 1] : acc[j];
-            const float other = __uint_as_float(__shfl_xor_sync(kAll, give, 16));
-            const float kept = __uint_as_float(lane < 16 ? acc[j] : acc[j + 1]);
-            const float y = silu_f32(lane < 16 ? kept : other) * (lane < 16 ? other : kept);
-            const int from = j + (lane >> 4);
-            const int q = __shfl_sync(kAll, q_mine, from);
-            const float w = __shfl_sync(kAll, w_mine, from);
-            if (in && q >= 0) p.d[q * p.ldd + col] = p.row_weights != nullptr ? y * w : y;
-          }
-        } else {
+        for (int j0 = 0; j0 < 16; j0 += 4) {
+          if (c + j0 >= item.count) break;
+          if constexpr (kGated && !kTwo) {
+            // lanes 0-15 hold the gate, 16-31 the up product: the lower lanes finish the even columns,
+            // the upper ones the odd
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const int q = __shfl_sync(kAll, q_mine, j);
-            const float w = __shfl_sync(kAll, w_mine, j);
-            const float y = __uint_as_float(acc[j]);
-            if (in && q >= 0) p.d[q * p.ldd + col] = p.row_weights != nullptr ? y * w : y;
+            for (int j = j0; j < j0 + 4; j += 2) {
+              const uint32_t give = lane < 16 ? acc[j + 1] : acc[j];
+              const float other = __uint_as_float(__shfl_xor_sync(kAll, give, 16));
+              const float kept = __uint_as_float(lane < 16 ? acc[j] : acc[j + 1]);
+              float y = silu_f32(lane < 16 ? kept : other) * (lane < 16 ? other : kept);
+              const int from = j + (lane >> 4);
+              const int q = __shfl_sync(kAll, q_mine, from);
+              const float w = __shfl_sync(kAll, w_mine, from);
+              if (weighted) y *= w;
+              if (in && q >= 0) d_col[q * p.ldd] = y;
+            }
+          } else {
+#pragma unroll
+            for (int j = j0; j < j0 + 4; ++j) {
+              const int q = __shfl_sync(kAll, q_mine, j);
+              const float w = __shfl_sync(kAll, w_mine, j);
+              float y = __uint_as_float(acc[j]);
+              if (weighted) y *= w;
+              if (in && q >= 0) d_col[q * p.ldd] = y;
+            }
           }
         }
+        w_next = weighted && q_next >= 0 ? p.row_weights[q_next] : 1.0f;
       }
       tc_fence_before_sync();
       __syncwarp();

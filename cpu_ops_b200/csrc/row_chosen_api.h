@@ -305,7 +305,7 @@ GroupedChoice choose_grouped(const DeviceState& st, int rows, int n, int groups,
       c.BN = BN;
       c.tile_cols = (gated ? 64 : 128) * (two ? 2 : 1);
       c.stages = grouped_stages(st.smem_optin, BN, ka, groups, two);
-      if (c.stages < 2) continue;
+      if (c.stages < 3) continue;  // (longer than a run of the scale writers)
       const int wide = average + average / 8;  // (groups differ: cuts for a somewhat larger one)
       const int cuts = (wide + BN - 1) / BN, width = ((average + cuts - 1) / cuts + 15) / 16 * 16;
       const int64_t items = static_cast<int64_t>(groups) * cuts * ((n + c.tile_cols - 1) / c.tile_cols);
@@ -442,7 +442,7 @@ int gemm_grouped_call(const cpuops_b200_gemm_grouped_desc* d) {
       if (int rc = make_tensor_map(&tmW, d->b, fp4_b ? k / 2 : k, b_rows, b_pitch, box)) return rc;
     }
     if (p.sorted) {
-      if (int rc = make_tensor_map(&tmX, ws + off_x, row_bytes, rows, x_pitch, 16)) return rc;
+      if (int rc = make_tensor_map(&tmX, ws + off_x, row_bytes, rows, x_pitch, static_cast<uint32_t>(p.BN / 2))) return rc;
     } else {
       if (int rc = make_tensor_map(&tmX, d->a, row_bytes, d->a_rows, a_pitch, 1)) return rc;
     }
