@@ -285,8 +285,11 @@ int grouped_stages(int smem_optin, int BN, int ka, int groups, bool two) {
 //   * Few pairs per group (below 48): one W tile, room for twice the average, rows gathered.  Such calls are bound
 //     by reading W, and the width does not matter to that.
 //   * Many: the width and the tile count whose estimated time is least: rounds of items over the SMs
-//     x (k-blocks x cycles per k-block + a fixed part).  A k-block takes its MMAs' time (2 cycles per
-//     pair and W tile), or 2000 cycles over the stages where the ring is too short for that.
+//     x (k-blocks x cycles per k-block + a fixed part).  A k-block takes its loads' time at 44 bytes a
+//     cycle, what an SM was seen to get out of L2 beside all others, or its MMAs' (2 cycles per pair
+//     and W tile); with one set of accumulators D's stores, 100 cycles per pair, are not hidden.
+//     (us, 8192 rows x 4096 x 4096 e4m3, one group: two tiles of 112 pairs 171, 144 214, 192 190; one
+//     tile of 112 271, 192 232.)
 GroupedChoice choose_grouped(const DeviceState& st, int rows, int n, int groups, int k_blocks, int ka, bool gated) {
   GroupedChoice best;
   const int average = rows / std::max(1, groups), sms = st.sms();
@@ -310,8 +313,8 @@ GroupedChoice choose_grouped(const DeviceState& st, int rows, int n, int groups,
       const int cuts = (wide + BN - 1) / BN, width = ((average + cuts - 1) / cuts + 15) / 16 * 16;
       const int64_t items = static_cast<int64_t>(groups) * cuts * ((n + c.tile_cols - 1) / c.tile_cols);
       const double rounds = static_cast<double>((items + sms - 1) / sms);
-      const double block = std::max(2.0 * width * (two ? 2 : 1), 2000.0 / c.stages);
-      const double drain = grouped_acc_sets(BN, ka, two) == 2 ? 500.0 : 500.0 + 10.0 * width;
+      const double block = std::max(2.0 * width * (two ? 2 : 1), (16384.0 * (two ? 2 : 1) + 128.0 * BN) / 44.0);
+      const double drain = grouped_acc_sets(BN, ka, two) == 2 ? 1000.0 : 1000.0 + 100.0 * width;
       const double cycles = rounds * (k_blocks * block + drain);
       if (least == 0.0 || cycles < least) {
         least = cycles;
