@@ -94,8 +94,11 @@ RouteKernel route_kernel_for(int experts) {
   return per_lane <= 1 ? route_kernel<1> : per_lane <= 2 ? route_kernel<2> : per_lane <= 4 ? route_kernel<4>
        : per_lane <= 8 ? route_kernel<8> : per_lane <= 16 ? route_kernel<16> : route_kernel<32>;
 }
-size_t route_smem_bytes(int experts, int n_groups) {
-  return n_groups > 1 ? static_cast<size_t>(kRouteWarps) * (experts + n_groups) * sizeof(double) : 0;
+using RouteFewKernel = void (*)(RouteParams, int32_t*, int32_t*);
+RouteFewKernel route_few_kernel_for(int experts) {
+  const int per_lane = (experts + 31) / 32;
+  return per_lane <= 1 ? route_few_kernel<1> : per_lane <= 2 ? route_few_kernel<2> : per_lane <= 4 ? route_few_kernel<4>
+       : per_lane <= 8 ? route_few_kernel<8> : per_lane <= 16 ? route_few_kernel<16> : route_few_kernel<32>;
 }
 
 using GroupedKernel = void (*)(CUtensorMap, CUtensorMap, GroupedParams);
@@ -146,8 +149,10 @@ int row_kernels_ready(DeviceState& st) {
   static bool ready[64] = {};
   if (ready[st.device]) return 0;
   constexpr auto kMost = cudaFuncAttributeMaxDynamicSharedMemorySize;
-  for (int experts = 32; experts <= kMaxGroups; experts *= 2)
+  for (int experts = 32; experts <= kMaxGroups; experts *= 2) {
     CUDA_TRY(cudaFuncSetAttribute(route_kernel_for(experts), kMost, static_cast<int>(route_smem_bytes(experts, experts))));
+    CUDA_TRY(cudaFuncSetAttribute(route_few_kernel_for(experts), kMost, static_cast<int>(route_few_smem_bytes(experts, experts))));
+  }
   CUDA_TRY(cudaFuncSetAttribute(group_rows_kernel, kMost, plan_smem_bytes(kMaxGroups)));
   for (int kind : {kKindMxf8, kKindMxf4})
     for (bool gated : {false, true})
@@ -261,6 +266,12 @@ int route_call(const cpuops_b200_route_desc* d) {
     p.group_best = d->group_best;
     p.renormalize = d->renormalize ? 1 : 0;
     p.scale = d->scale;
+    if (d->offsets && d->tokens <= kRouteFewTokens && pairs <= kRouteFewPairs) {
+      if (int rc = launch_after(route_few_kernel_for(d->experts), dim3(1), kRouteWarps * 32,
+                                route_few_smem_bytes(d->experts, d->n_groups), call.stream, p, d->offsets, d->order))
+        return rc;
+      return call.finish();
+    }
     const unsigned blocks = static_cast<unsigned>((d->tokens + kRouteWarps - 1) / kRouteWarps);
     if (int rc = launch_after(route_kernel_for(d->experts), dim3(blocks), kRouteWarps * 32,
                               route_smem_bytes(d->experts, d->n_groups), call.stream, p))

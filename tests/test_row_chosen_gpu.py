@@ -109,6 +109,31 @@ def test_route_masks_infinities_and_nan(gpu):
             check_route(dev(x), "f32", 5, bias=b, sigmoid=sigmoid, n_groups=3, top_groups=2, group_best=2)
 
 
+@pytest.mark.parametrize("sigmoid", [False, True])
+def test_route_choices_that_f32_cannot_settle(gpu, sigmoid):
+    """Scores a rounding of f32 apart, saturated ones, zeros of either sign, numbers below every digit."""
+    rng = W.rng_for(10, 5)
+    x = np.zeros((24, 64), np.float32)
+    base = rng.standard_normal(24).astype(np.float32)
+    for t in range(24):   # neighbours one or two steps of f32 apart, shuffled
+        steps = rng.permutation(64) % 13
+        v = np.full(64, base[t], np.float32)
+        for j in range(64):
+            for _ in range(int(steps[j])):
+                v[j] = np.nextafter(v[j], np.float32(np.inf))
+        x[t] = v
+    x[4] = rng.permutation(np.concatenate((np.float32([20, 25, 28, 30]).repeat(8), np.arange(45, 77)))).astype(np.float32)
+    x[5] = -x[4]
+    x[6] = np.where(np.arange(64) % 3 == 0, -0.0, 0.0)
+    x[7] = rng.permutation(64).astype(np.float32) * np.float32(1e-30)
+    x[8] = rng.permutation(64).astype(np.float32) * np.float32(-1000)
+    x[9] = rng.permutation(64).astype(np.float32) * np.float32(40)
+    bias = rng.permutation((np.float32(0.25) + np.arange(64) * np.float32(2.0 ** -24))).astype(np.float32)
+    for b in (None, bias):
+        for kw in ({}, {"n_groups": 8, "top_groups": 3, "group_best": 2}, {"n_groups": 64, "top_groups": 20}):
+            check_route(dev(x), "f32", 7, bias=b, sigmoid=sigmoid, **kw)
+
+
 def test_route_padded_rows_and_no_plan(gpu):
     rng = W.rng_for(8, 5)
     wide = dev(rng.standard_normal((19, 45)).astype(np.float32))
