@@ -50,6 +50,21 @@ __device__ __forceinline__ float route_logit(const RouteParams& p, int64_t row, 
   const float v = load_float(p.logits, p.type, row + e);
   return v == v ? fminf(v, 3.402823466e38f) + 0.0f : -INFINITY;
 }
+// A lane's logits (-inf behind the last expert).
+template <int kPerLane>
+__device__ __forceinline__ void route_logits(const RouteParams& p, int64_t row, float (&x)[kPerLane]) {
+  const int lane = threadIdx.x & 31;
+  auto all = [&](auto* base) {
+    const auto* from = base + row + lane;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) x[i] = lane + 32 * i < p.experts ? static_cast<float>(from[32 * i]) : -INFINITY;
+  };
+  if (p.type == kTypeF32) all(static_cast<const float*>(p.logits));
+  else if (p.type == kTypeF16) all(static_cast<const __half*>(p.logits));
+  else all(static_cast<const __nv_bfloat16*>(p.logits));
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i) x[i] = x[i] == x[i] ? fminf(x[i], 3.402823466e38f) + 0.0f : -INFINITY;
+}
 // e / per for e < 1024 (magic = ceil(2^20 / per)).
 __device__ __forceinline__ int group_of(int e, uint32_t magic) { return static_cast<int>((static_cast<uint32_t>(e) * magic) >> 20); }
 
@@ -160,93 +175,153 @@ __device__ __forceinline__ uint32_t order_key(float v) {
 }
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
-// The same choice from f32 scores, and whether these settle it.  Two neighbours in the order of choice
-// (the first one left out among them) have to be further apart than both scores' errors: `apart`.
+// Which groups stay, in the precision of T: bit g * share of the result, share lanes to a group (n_groups <=
+// 32).  `v`: a lane's choices (-inf: out); scratch: experts + n_groups numbers of this warp.  `near`: the
+// last group that stays and the first that does not are no further apart than `slack` times their size and
+// `least`.
+template <typename T, int kPerLane>
+__device__ __forceinline__ unsigned groups_kept(const RouteParams& p, const T (&v)[kPerLane], T* scratch, uint32_t magic,
+                                                int share, T slack, T least, bool& near) {
+  constexpr unsigned kAll = 0xffffffffu;
+  const int lane = threadIdx.x & 31;
+  const int per = p.experts / p.n_groups;
+  const T kOut = -INFINITY;
+  // per + 1 places to a group; the warp's lanes share the groups evenly
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i) {
+    const int e = lane + 32 * i;
+    if (e < p.experts) scratch[e + group_of(e, magic)] = v[i];
+  }
+  __syncwarp();
+  const int g = lane / share, part = lane & (share - 1);
+  const bool mine = g < p.n_groups;
+  T best = kOut, second = kOut;
+  if (mine)
+    for (int j = part; j < per; j += share) {
+      const T w = scratch[g * (per + 1) + j];
+      const T less = best < w ? best : w;
+      second = second < less ? less : second;
+      best = best < w ? w : best;
+    }
+  for (int s = 1; s < share; s <<= 1) {
+    const T b2 = __shfl_xor_sync(kAll, best, s), s2 = __shfl_xor_sync(kAll, second, s);
+    const T less = best < b2 ? best : b2, most = second < s2 ? s2 : second;
+    second = most < less ? less : most;
+    best = best < b2 ? b2 : best;
+  }
+  const T score = p.group_best == 2 && second != kOut ? best + second : best;
+  int ahead = 0;
+  bool close = false;
+  for (int j = 0; j < p.n_groups; ++j) {
+    const T other = __shfl_sync(kAll, score, j * share);
+    ahead += other > score || (other == score && j < g);
+    const T size = (other < 0 ? -other : other) + (score < 0 ? -score : score);
+    const T gap = other < score ? score - other : other - score;
+    close = close || (j != g && other != kOut && score != kOut && !(gap > slack * size + least));
+  }
+  near = __any_sync(kAll, mine && close);
+  return __ballot_sync(kAll, mine && ahead < p.top_groups && part == 0);
+}
+
+// Lane j's choice of expert `id` in double precision (softmax: `total` is the sum of exponentials).
+__device__ __forceinline__ double exact_choice(const RouteParams& p, int64_t row, int id, float top, double total) {
+  const double v = static_cast<double>(route_logit(p, row, id));
+  const double score = p.sigmoid ? 1.0 / (1.0 + exp(-v)) : exp(v - static_cast<double>(top)) / total;
+  return p.bias != nullptr ? score + static_cast<double>(p.bias[id]) : score;
+}
+__device__ __noinline__ double exact_total(const RouteParams& p, int64_t row, float top) {
+  double total = 0.0;
+  for (int e = threadIdx.x & 31; e < p.experts; e += 32) {
+    const float v = route_logit(p, row, e);
+    if (v != -INFINITY && (p.bias == nullptr || p.bias[e] > -INFINITY))
+      total += exp(static_cast<double>(v) - static_cast<double>(top));
+  }
+  for (int s = 16; s > 0; s >>= 1) total += __shfl_xor_sync(0xffffffffu, total, s);
+  return total;
+}
+// The groups that stay, in double precision.
+template <int kPerLane>
+__device__ __noinline__ unsigned groups_kept_exact(const RouteParams& p, int64_t row, double* scratch, uint32_t magic,
+                                                   int share, float top) {
+  const int lane = threadIdx.x & 31;
+  const double total = p.sigmoid ? 1.0 : exact_total(p, row, top);
+  double v[kPerLane];
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i) {
+    const int e = lane + 32 * i;
+    v[i] = -INFINITY;
+    if (e < p.experts && route_logit(p, row, e) != -INFINITY && (p.bias == nullptr || p.bias[e] > -INFINITY))
+      v[i] = exact_choice(p, row, e, top, total);
+  }
+  bool near;
+  return groups_kept<double, kPerLane>(p, v, scratch, magic, share, 0.0, 0.0, near);
+}
+
+// The choice from f32 scores, with doubles only where those do not settle it: experts are picked by their f32
+// choice until the next one is further below the last of the top_k than both scores' errors; where two
+// neighbours are no further apart than that, the picked ones are put in order in double precision.
+// False: more than 32 are that close (route_exact decides).
 // Without a bias the order is that of the logits themselves, which f32 holds exactly.
 template <int kPerLane>
-__device__ __forceinline__ int route_fast(const RouteParams& p, int64_t row, float* scratch, float& top, bool& settled) {
+__device__ __forceinline__ bool route_fast(const RouteParams& p, int64_t row, double* scratch, float& top, int& my_id) {
   constexpr unsigned kAll = 0xffffffffu;
   const int lane = threadIdx.x & 31;
   const bool by_logit = p.bias == nullptr && p.n_groups == 1;
   float x[kPerLane];
   uint32_t key[kPerLane];
   top = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < kPerLane; ++i) {
-    const int e = lane + 32 * i;
-    x[i] = e < p.experts ? route_logit(p, row, e) : -INFINITY;
-  }
+  my_id = -1;
+  route_logits<kPerLane>(p, row, x);
   float bias[kPerLane], largest_bias = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kPerLane; ++i) {
-    const int e = lane + 32 * i;
-    bias[i] = p.bias != nullptr && e < p.experts ? p.bias[e] : 0.0f;
-    if (!(bias[i] > -INFINITY)) x[i] = -INFINITY;
-    if (x[i] != -INFINITY) largest_bias = fmaxf(largest_bias, fabsf(bias[i]));
-    top = fmaxf(top, x[i]);
-  }
-  if (p.bias != nullptr) largest_bias = __uint_as_float(__reduce_max_sync(kAll, __float_as_uint(largest_bias)));
-  top = key_value(__reduce_max_sync(kAll, order_key(top)));
-  float inverse = 1.0f;
-  if (!by_logit) {
-    float total = 0.0f;
+  for (int i = 0; i < kPerLane; ++i) bias[i] = 0.0f;
+  if (p.bias != nullptr) {
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i)
+      if (lane + 32 * i < p.experts) bias[i] = p.bias[lane + 32 * i];
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) {
-      const float e = x[i] == -INFINITY ? 0.0f : p.sigmoid ? 1.0f / (1.0f + expf(-x[i])) : expf(x[i] - top);
-      total += e;
-      if (x[i] != -INFINITY) x[i] = e;
+      if (!(bias[i] > -INFINITY)) x[i] = -INFINITY;
+      if (x[i] != -INFINITY) largest_bias = fmaxf(largest_bias, fabsf(bias[i]));
+    }
+    largest_bias = __uint_as_float(__reduce_max_sync(kAll, __float_as_uint(largest_bias)));
+  }
+  if (!p.sigmoid) {
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) top = fmaxf(top, x[i]);
+    top = key_value(__reduce_max_sync(kAll, order_key(top)));
+  }
+  if (!by_logit) {
+    float total = 0.0f, inverse = 1.0f;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+      const float e = __expf(p.sigmoid ? -x[i] : x[i] - top);  // (of an expert that is out it is not used)
+      const float score = p.sigmoid ? __fdividef(1.0f, 1.0f + e) : e;
+      const bool in = x[i] != -INFINITY;
+      total += in ? score : 0.0f;
+      x[i] = in ? score : -INFINITY;
     }
     if (!p.sigmoid) {
       for (int s = 16; s > 0; s >>= 1) total += __shfl_xor_sync(kAll, total, s);
-      inverse = 1.0f / total;
+      inverse = __fdividef(1.0f, total);
     }
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i)
-      if (x[i] != -INFINITY) x[i] = x[i] * inverse + bias[i];
+    for (int i = 0; i < kPerLane; ++i) x[i] = x[i] != -INFINITY ? x[i] * inverse + bias[i] : -INFINITY;
   }
-  settled = true;
+  // How far two f32 choices of a summed size have to be apart.  Scores (at most 1, and at most the choice and the
+  // bias together) are within 5e-6 of themselves (an exponential's argument of up to 60 within 2^-24; below
+  // exp(-60) is `least`), sums within 1.2e-7; twice that for either.
+  const float least = 1e-25f + 4e-5f * fminf(largest_bias, 1.0f);
+  const float slack = 1.1e-5f;
   if (p.n_groups > 1) {
-    if (p.n_groups > 32) {  // (a group to a lane below)
-      settled = false;
-      return -1;
-    }
-    // per + 1 words to a group in shared memory; the warp's lanes share the groups evenly
-    const int per = p.experts / p.n_groups;
-    const uint32_t magic = ((1u << 20) + per - 1) / per;
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
-      const int e = lane + 32 * i;
-      if (e < p.experts) scratch[e + group_of(e, magic)] = x[i];
-    }
-    __syncwarp();
+    if (p.n_groups > 32) return false;  // (a group to a lane at least)
+    const uint32_t magic = ((1u << 20) + p.experts / p.n_groups - 1) / (p.experts / p.n_groups);
     int share = 1;  // lanes per group
     while (2 * share * p.n_groups <= 32) share *= 2;
-    const int g = lane / share, part = lane & (share - 1);
-    float best = -INFINITY, second = -INFINITY;
-    if (g < p.n_groups)
-      for (int j = part; j < per; j += share) {
-        const float v = scratch[g * (per + 1) + j];
-        second = fmaxf(second, fminf(best, v));
-        best = fmaxf(best, v);
-      }
-    for (int s = 1; s < share; s <<= 1) {
-      const float b2 = __shfl_xor_sync(kAll, best, s), s2 = __shfl_xor_sync(kAll, second, s);
-      second = fmaxf(fmaxf(second, s2), fminf(best, b2));
-      best = fmaxf(best, b2);
-    }
-    const float score = p.group_best == 2 && second != -INFINITY ? best + second : best;
-    int ahead = 0;
-    for (int j = 0; j < p.n_groups; ++j) {
-      const float other = __shfl_sync(kAll, score, j * share);
-      ahead += other > score || (other == score && j < g);
-    }
-    const bool mine = g < p.n_groups, stays = mine && ahead < p.top_groups;
-    // the last group that stays and the first that does not
-    const float low = -key_value(__reduce_max_sync(kAll, stays ? order_key(-score) : 0u));
-    const float high = key_value(__reduce_max_sync(kAll, mine && !stays ? order_key(score) : order_key(-INFINITY)));
-    if (p.top_groups < p.n_groups && !(low - high > 1e-6f * (2.0f + fabsf(low) + fabsf(high))) && high != -INFINITY) settled = false;
-    const unsigned kept = __ballot_sync(kAll, stays && part == 0);  // bit g * share
+    bool near;
+    unsigned kept = groups_kept<float, kPerLane>(p, x, reinterpret_cast<float*>(scratch), magic, share, slack, 2.0f * least, near);
+    if (near && p.top_groups < p.n_groups) kept = groups_kept_exact<kPerLane>(p, row, scratch, magic, share, top);
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) {
       const int e = lane + 32 * i;
@@ -256,49 +331,64 @@ __device__ __forceinline__ int route_fast(const RouteParams& p, int64_t row, flo
 #pragma unroll
   for (int i = 0; i < kPerLane; ++i) key[i] = order_key(x[i]);
   const uint32_t out = order_key(-INFINITY);
-  int my_id = -1;
-  float my_value = -INFINITY, after = -INFINITY;  // after: the first one left out
-  for (int j = 0; j <= p.top_k; ++j) {
+  float my_value = -INFINITY, last = -INFINITY;  // last: the choice of slot top_k - 1
+  bool apart = true;                             // every pick so far from the one before it
+  int picked = 0;
+  float before = INFINITY;
+  while (true) {
     uint32_t best = out;
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) best = max(best, key[i]);
     best = __reduce_max_sync(kAll, best);
     if (best == out) break;
+    const float value = key_value(best);
+    bool far;
+    if (by_logit) {
+      // equal logits are equal; others differ in double precision too, unless it has run out of digits:
+      // close to one another, or where scores end at 0 or 1
+      far = before == INFINITY || before == value || before - value > 1e-8f;
+      if (picked < p.top_k && !(p.sigmoid ? fabsf(value) < 15.0f : value - top > -600.0f)) return false;
+    } else {
+      far = picked == 0 || before - value > slack * (fabsf(before) + fabsf(value)) + least;
+    }
+    if (picked >= p.top_k) {  // left out, if it is far enough below the last one in
+      const bool enough = by_logit ? far : last - value > slack * (fabsf(last) + fabsf(value)) + least;
+      if (enough) break;
+      if (picked == 32) return false;
+    }
+    apart = apart && far;
     uint32_t at = kMaxGroups;
 #pragma unroll
     for (int i = kPerLane - 1; i >= 0; --i) at = key[i] == best ? lane + 32 * i : at;
     at = __reduce_min_sync(kAll, at);
-    if (j == p.top_k) {
-      after = key_value(best);
-      break;
-    }
-    if (lane == j) {
+    if (lane == picked) {
       my_id = static_cast<int>(at);
-      my_value = key_value(best);
+      my_value = value;
     }
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i)
       if (at == lane + 32 * i) key[i] = out;
+    before = value;
+    if (++picked == p.top_k) last = value;
   }
-  // lane j against slot j + 1 (the last one against the one left out)
-  float next = __shfl_down_sync(kAll, my_value, 1);
-  if (lane == p.top_k - 1) next = after;
-  bool apart = true;
-  if (my_id >= 0 && lane < p.top_k) {
-    if (by_logit) {
-      // equal logits are equal; others differ in double precision too, unless it has run out of digits
-      apart = my_value == next || next == -INFINITY || my_value - next > 1e-8f;
-      apart = apart && (p.sigmoid ? fabsf(my_value) < 15.0f : my_value - top > -600.0f);
-    } else {
-      // scores (at most 1, and at most the value and the bias together) are within 1e-6 of themselves,
-      // sums within 1.2e-7; twice that for either
-      const float size = fabsf(my_value) + fabsf(next);
-      const float scores = fminf(size + 2.0f * largest_bias, 2.0f);
-      apart = next == -INFINITY || my_value - next > 2e-6f * scores + 4e-7f * size + 1e-37f;
+  if (!apart) {
+    const double total = p.sigmoid ? 1.0 : exact_total(p, row, top);
+    const double mine = my_id >= 0 ? exact_choice(p, row, my_id, top, total) : 0.0;
+    int place = 0;
+    for (int j = 0; j < picked; ++j) {
+      const double other = __shfl_sync(kAll, mine, j);
+      const int other_id = __shfl_sync(kAll, my_id, j);
+      place += other > mine || (other == mine && other_id < my_id);
     }
+    int sorted = -1;
+    for (int j = 0; j < picked; ++j) {
+      const int id = __shfl_sync(kAll, my_id, j), at = __shfl_sync(kAll, place, j);
+      if (at == lane) sorted = id;
+    }
+    my_id = sorted;
   }
-  settled = settled && __all_sync(kAll, apart);
-  return my_id;
+  if (lane >= p.top_k) my_id = -1;
+  return true;
 }
 
 // Shared memory (the grouped case only): experts + n_groups doubles per warp.
@@ -308,21 +398,11 @@ __device__ __forceinline__ void route_token(const RouteParams& p, int token, dou
   const int lane = threadIdx.x & 31;
   const int64_t row = static_cast<int64_t>(token) * p.ld;
   float top;
-  bool settled;
-  int my_id = route_fast<kPerLane>(p, row, reinterpret_cast<float*>(scratch), top, settled);
-  if (!settled) my_id = route_exact<kPerLane>(p, row, scratch);
+  int my_id;
+  if (!route_fast<kPerLane>(p, row, scratch, top, my_id)) my_id = route_exact<kPerLane>(p, row, scratch);
 
   // Weights: the chosen experts' scores in double precision.
-  double total = 1.0;
-  if (!p.sigmoid && !p.renormalize) {
-    total = 0.0;
-    for (int e = lane; e < p.experts; e += 32) {
-      const float v = route_logit(p, row, e);
-      if (v != -INFINITY && (p.bias == nullptr || p.bias[e] > -INFINITY))
-        total += exp(static_cast<double>(v) - static_cast<double>(top));
-    }
-    for (int s = 16; s > 0; s >>= 1) total += __shfl_xor_sync(kAll, total, s);
-  }
+  const double total = !p.sigmoid && !p.renormalize ? exact_total(p, row, top) : 1.0;
   double score = 0.0;
   if (my_id >= 0) {
     const double v = static_cast<double>(route_logit(p, row, my_id));
@@ -386,9 +466,12 @@ __global__ void __launch_bounds__(kPlanThreads) count_ids_kernel(const int32_t* 
     counts[static_cast<int64_t>(blockIdx.x) * (groups + 1) + g] = bins[g];
 }
 
-// Shared memory: per bin its start, all blocks' pairs, those of the blocks before, the warps' counters.
+// Shared memory: per bin its start, all blocks' pairs, those of the blocks before, this block's; the warps'
+// counters of 16 bits, plan_row of them to a warp (an odd number of words: the warps' counters of a
+// bin lie in different banks).
+__host__ __device__ inline int plan_row(int groups) { return 2 * ((groups + 2) / 2 | 1); }
 __host__ __device__ inline int plan_smem_bytes(int groups, int threads = kPlanThreads) {
-  return (groups + 1) * (3 * 4 + threads / 32 * 2);
+  return (groups + 1) * 4 * 4 + threads / 32 * plan_row(groups) * 2;
 }
 
 // A group's pairs cut into tiles of up to kPlanTileRows, for kernels that work tile by tile.
@@ -407,11 +490,13 @@ __device__ __forceinline__ void plan_block(const int32_t* ids, int64_t rows, int
   const int bins = groups + 1;
   int32_t* start = plan_smem;                                     // [bins]
   int32_t* all = plan_smem + bins;                                // [2][bins]
-  uint16_t* seen = reinterpret_cast<uint16_t*>(plan_smem + 3 * bins);  // [kWarps][bins]
+  int32_t* own = plan_smem + 3 * bins;                            // [bins]
+  const int ld = plan_row(groups);
+  uint16_t* seen = reinterpret_cast<uint16_t*>(plan_smem + 4 * bins);  // [kWarps][ld]
   __shared__ int32_t warp_sums[kWarps];
   constexpr unsigned kAll = 0xffffffffu;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int i = threadIdx.x; i < kWarps * bins; i += kThreads) seen[i] = 0;
+  for (int i = threadIdx.x; i < kWarps * ld / 2; i += kThreads) reinterpret_cast<uint32_t*>(seen)[i] = 0u;
   __syncthreads();
   const int64_t q0 = static_cast<int64_t>(blockIdx.x) * (kThreads * kRounds) + warp * (32 * kRounds);
   int bin[kRounds], rank[kRounds];
@@ -420,15 +505,23 @@ __device__ __forceinline__ void plan_block(const int32_t* ids, int64_t rows, int
     const int64_t q = q0 + i * 32 + lane;
     bin[i] = q < rows ? plan_bin(ids, q, groups) : -1;
   }
+  const int bits = 33 - __clz(bins);  // (-1, behind the last pair, differs from all bins in the highest)
 #pragma unroll
   for (int i = 0; i < kRounds; ++i) {
-    const unsigned same = __match_any_sync(kAll, bin[i]);
+    // the lanes with the same bin, bit by bit (the instruction for it takes as long as there are
+    // different ones: 4096 pairs of 60 groups 10.2 us, 9.0 so)
+    unsigned same = kAll;
+    for (int bit = 0; bit < bits; ++bit) {
+      const bool one = (bin[i] >> bit & 1) != 0;
+      const unsigned ones = __ballot_sync(kAll, one);
+      same &= one ? ones : ~ones;
+    }
     const int below = __popc(same & ((1u << lane) - 1u));
     rank[i] = 0;
-    if (bin[i] >= 0) rank[i] = seen[warp * bins + bin[i]] + below;
+    if (bin[i] >= 0) rank[i] = seen[warp * ld + bin[i]] + below;
     __syncwarp();
     if (bin[i] >= 0 && below == 0)
-      seen[warp * bins + bin[i]] = static_cast<uint16_t>(seen[warp * bins + bin[i]] + __popc(same));
+      seen[warp * ld + bin[i]] = static_cast<uint16_t>(seen[warp * ld + bin[i]] + __popc(same));
     __syncwarp();
   }
   __syncthreads();
@@ -436,17 +529,37 @@ __device__ __forceinline__ void plan_block(const int32_t* ids, int64_t rows, int
   if (counts != nullptr) {
     for (int g = threadIdx.x; g < 2 * bins; g += kThreads) all[g] = 0;
     __syncthreads();
-    const int n = static_cast<int>(gridDim.x) * bins;
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      const int b = i / bins, g = i - b * bins, c = counts[i];
-      if (c != 0) {
-        atomicAdd(&all[g], c);
-        if (b < static_cast<int>(blockIdx.x)) atomicAdd(&all[bins + g], c);
+    for (int b = warp; b < static_cast<int>(gridDim.x); b += kWarps) {
+      const int32_t* from = counts + static_cast<int64_t>(b) * bins;
+      const bool earlier = b < static_cast<int>(blockIdx.x);
+      for (int g0 = lane; g0 < bins; g0 += 32 * 4) {
+        int c[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c[j] = g0 + 32 * j < bins ? from[g0 + 32 * j] : 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (c[j] != 0) {
+            atomicAdd(&all[g0 + 32 * j], c[j]);
+            if (earlier) atomicAdd(&all[bins + g0 + 32 * j], c[j]);
+          }
       }
     }
     __syncthreads();
   }
-  // Per bin the warps' counts become the warps' starts within the block.
+  // Per bin the warps' counts become the warps' starts within the block: a warp for every bin in turn, lane
+  // w for warp w.
+  for (int g = warp; g < bins; g += kWarps) {
+    const int c = lane < kWarps ? seen[lane * ld + g] : 0;
+    int v = c;
+#pragma unroll
+    for (int s = 1; s < kWarps; s <<= 1) {
+      const int up = __shfl_up_sync(kAll, v, s);
+      if (lane >= s) v += up;
+    }
+    if (lane < kWarps) seen[lane * ld + g] = static_cast<uint16_t>(v - c);
+    if (lane == kWarps - 1) own[g] = v;
+  }
+  __syncthreads();
   constexpr int kPerThread = (kMaxGroups + 1 + kThreads - 1) / kThreads;
   int total[kPerThread], before[kPerThread];
   int sum = 0;  // of this thread's bins: kPerThread neighbouring ones
@@ -455,16 +568,7 @@ __device__ __forceinline__ void plan_block(const int32_t* ids, int64_t rows, int
     const int g = static_cast<int>(threadIdx.x) * kPerThread + j;
     total[j] = before[j] = 0;
     if (g < bins) {
-      int c[kWarps];
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) c[w] = seen[w * bins + g];
-      int in_block = 0;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        seen[w * bins + g] = static_cast<uint16_t>(in_block);
-        in_block += c[w];
-      }
-      total[j] = counts != nullptr ? all[g] : in_block;
+      total[j] = counts != nullptr ? all[g] : own[g];
       before[j] = counts != nullptr ? all[bins + g] : 0;
       sum += total[j];
     }
@@ -502,10 +606,10 @@ __device__ __forceinline__ void plan_block(const int32_t* ids, int64_t rows, int
   __syncthreads();
   if (tiles != nullptr && blockIdx.x == 0) {
     // the same scan over the bins' tiles
-    int own = 0;
+    int mine = 0;
 #pragma unroll
-    for (int j = 0; j < kPerThread; ++j) own += (total[j] + kPlanTileRows - 1) / kPlanTileRows;
-    int v = own;
+    for (int j = 0; j < kPerThread; ++j) mine += (total[j] + kPlanTileRows - 1) / kPlanTileRows;
+    int v = mine;
 #pragma unroll
     for (int s = 1; s < 32; s <<= 1) {
       const int up = __shfl_up_sync(kAll, v, s);
@@ -523,7 +627,7 @@ __device__ __forceinline__ void plan_block(const int32_t* ids, int64_t rows, int
       if (lane < kWarps) warp_sums[lane] = w;
     }
     __syncthreads();
-    int slot = v - own + (warp > 0 ? warp_sums[warp - 1] : 0);
+    int slot = v - mine + (warp > 0 ? warp_sums[warp - 1] : 0);
 #pragma unroll
     for (int j = 0; j < kPerThread; ++j) {
       const int g = static_cast<int>(threadIdx.x) * kPerThread + j;
@@ -536,7 +640,7 @@ __device__ __forceinline__ void plan_block(const int32_t* ids, int64_t rows, int
 #pragma unroll
   for (int i = 0; i < kRounds; ++i) {
     if (bin[i] >= 0)
-      order[start[bin[i]] + seen[warp * bins + bin[i]] + rank[i]] =
+      order[start[bin[i]] + seen[warp * ld + bin[i]] + rank[i]] =
           bin[i] < groups || tiles != nullptr ? static_cast<int32_t>(q0 + i * 32 + lane) : -1;
   }
 }
