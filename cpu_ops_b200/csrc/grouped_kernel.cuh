@@ -80,7 +80,9 @@ __host__ __device__ inline int grouped_staging_bytes(int BN, bool two) {
 __host__ __device__ inline int grouped_acc_sets(int BN, int ka, bool two) {
   return 2 * (two ? 2 : 1) * BN + kDecodeSfSlots * 4 * grouped_atoms(BN, ka, two) <= 512 ? 2 : 1;
 }
-__host__ __device__ inline int grouped_table_bytes(int groups) { return (2 * (groups + 1) * 4 + 15) / 16 * 16; }
+// The first items of a CTA are worked out once, by all threads, and looked up by the roles.
+constexpr int kGroupedTable = 64;
+__host__ __device__ inline int grouped_table_bytes(int groups) { return (2 * (groups + 1) * 4 + 15) / 16 * 16 + kGroupedTable * 16; }
 constexpr int kGroupedBarrierBytes = 256;
 __host__ __device__ inline int grouped_smem_bytes(int BN, int stages, int ka, int groups, bool two) {
   return 1024 + stages * (grouped_stage_bytes(BN, two) + grouped_atoms(BN, ka, two) * 512) + grouped_staging_bytes(BN, two) +
@@ -180,7 +182,8 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
   const uint32_t atom_base = smem_base + stages * stage_bytes;
   const uint32_t staging_base = atom_base + stages * atom_bytes;
   const uint32_t table_off = staging_base + static_cast<uint32_t>(grouped_staging_bytes(BN, kTwo)) - smem_base;
-  int32_t* first = reinterpret_cast<int32_t*>(smem + table_off);  // [groups + 1]
+  int4* table = reinterpret_cast<int4*>(smem + table_off);        // [kGroupedTable]
+  int32_t* first = reinterpret_cast<int32_t*>(table + kGroupedTable);  // [groups + 1]
   int32_t* start = first + p.groups + 1;                          // [groups + 1]
   const uint32_t bar_base = smem_base + table_off + static_cast<uint32_t>(grouped_table_bytes(p.groups));
   auto full_bar = [&](int s) { return bar_base + 8u * s; };
@@ -249,25 +252,44 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
     }
     if (lane == 0) first[p.groups] = sum;
   }
+  __syncthreads();
+  if (threadIdx.x < kGroupedTable) {
+    const int64_t it = blockIdx.x + static_cast<int64_t>(threadIdx.x) * gridDim.x;
+    if (it < first[p.groups]) {
+      const GroupedItem item = grouped_item(first, start, p.groups, p.tiles, BN, static_cast<int>(it));
+      table[threadIdx.x] = make_int4(item.group, item.tile, item.p0, item.count);
+    }
+  }
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
-  const int n_items = first[p.groups];
-  const int step = static_cast<int>(gridDim.x);
-  auto item_at = [&](int it) { return grouped_item(first, start, p.groups, p.tiles, BN, it); };
+  const int step = static_cast<int>(gridDim.x), n_all = first[p.groups];
+  const int n_items = n_all > static_cast<int>(blockIdx.x) ? (n_all - 1 - static_cast<int>(blockIdx.x)) / step + 1 : 0;
+  // This CTA's item j: work item blockIdx.x + j gridDim.x.  (Worked out anew it is a search and three
+  // divisions, some 700 cycles of every role.)
+  auto item_at = [&](int j) {
+    if (j < kGroupedTable) {
+      const int4 v = table[j];
+      return GroupedItem{v.x, v.y, v.z, v.w};
+    }
+    return grouped_item(first, start, p.groups, p.tiles, BN, static_cast<int>(blockIdx.x) + j * step);
+  };
   // The pair at place p0 + r of an item's run, or -1.
   auto pair_at = [&](const GroupedItem& item, int r) {
     if (r >= item.count) return -1;
     const int q = p.order[item.p0 + r];
     return q >= 0 && q < p.rows ? q : -1;
   };
-  // The row of X behind the pair at place p0 + r of an item's run, or -1.
-  auto x_row = [&](const GroupedItem& item, int r) {
+  // What finds the row of X behind the pair at place p0 + r of item j: fetched an item ahead ...
+  auto x_pair = [&](int j, int r) {
+    if (j >= n_items) return -1;
+    const GroupedItem item = item_at(j);
     if (p.sorted) return r < item.count ? item.p0 + r : -1;
-    const int q = pair_at(item, r);
-    return q < 0 ? -1 : min(q / p.pairs_per_a_row, p.a_rows - 1);
+    return pair_at(item, r);
   };
+  // ... and the row itself, or -1.
+  auto x_row = [&](int q) { return p.sorted || q < 0 ? q : min(q / p.pairs_per_a_row, p.a_rows - 1); };
   auto columns_of = [&](const GroupedItem& item) { return max(16, (item.count + 15) & ~15); };
 
   if (warp == 0) {
@@ -276,7 +298,7 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
     int s = 0;
     uint32_t ph = 0;
     bool alive = true;
-    for (int it = blockIdx.x; it < n_items && alive; it += step) {
+    for (int it = 0; it < n_items && alive; ++it) {
       const GroupedItem item = item_at(it);
       const int base = item.group * p.b_group_rows;
       for (int kb = 0; kb < p.k_blocks; ++kb) {
@@ -324,21 +346,30 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
     int s = 0, turn = 0;
     uint32_t ph = 0;
     bool alive = true;
-    for (int it = blockIdx.x; it < n_items && alive; it += step) {
+    int pairs[2][4];
+    auto fetch_pairs = [&](int j) {
+      if (p.sorted) return;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pairs[h][i] = x_pair(j, 128 * h + 4 * lane + i);
+    };
+    fetch_pairs(0);
+    for (int it = 0; it < n_items && alive; ++it) {
       const GroupedItem item = item_at(it);
       int row[2][4];
       bool mine[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int r0 = 128 * h + 4 * lane;
-        mine[h] = !p.sorted && r0 < item.count;
+        mine[h] = !p.sorted && 128 * h + 4 * lane < item.count;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) row[h][j] = p.sorted ? -1 : x_row(item, r0 + j);
+        for (int j = 0; j < 4; ++j) row[h][j] = p.sorted ? -1 : x_row(pairs[h][j]);
         if (row[h][0] < 0) row[h][0] = 0;
 #pragma unroll
         for (int j = 1; j < 4; ++j)
           if (row[h][j] < 0) row[h][j] = row[h][0];
       }
+      fetch_pairs(it + 1);
       const bool second = item.count > BN / 2;
       const uint32_t bytes = p.sorted ? static_cast<uint32_t>(BN / 2 * 128 * (second ? 2 : 1))
                                       : static_cast<uint32_t>((item.count + 3) >> 2) * 512u;
@@ -391,7 +422,7 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
     int s = 0, buf = 0, sf_q = 0;
     uint32_t ph = 0, acc_ph = 0;
     bool ok = true;
-    for (int it = blockIdx.x; it < n_items && ok; it += step) {
+    for (int it = 0; it < n_items && ok; ++it) {
       const GroupedItem item = item_at(it);
       const uint32_t idesc = p.idesc | (static_cast<uint32_t>(columns_of(item)) >> 3) << 17;
       if (!__all_sync(kAll, mbar_wait_bounded(acc_empty_bar(buf), acc_ph ^ 1u, abort_flag, budget_ns))) {
@@ -473,8 +504,9 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
     const uint32_t stage_w = staging_base + static_cast<uint32_t>(r) * 16u + static_cast<uint32_t>(set * kFetchAhead) * kStagingSlot;
     // (BN need not reach 128 or 256: threads beyond it have no slot)
     const bool slot0 = r < BN, slot1 = r + 128 < BN;
-    int f_it = blockIdx.x, f_kb = 0;
+    int f_it = 0, f_kb = 0;
     const uint8_t *f_w[kTiles], *f_x0 = nullptr, *f_x1 = nullptr;  // rows of the item being fetched, or null
+    int next0 = x_pair(0, r), next1 = slot1 ? x_pair(0, r + 128) : -1;  // of the item entered next
     auto enter = [&]() {  // the item at the fetch cursor
       f_x0 = f_x1 = nullptr;
 #pragma unroll
@@ -495,12 +527,11 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
         }
         if (col < p.n) f_w[t] = p.sw + (static_cast<int64_t>(item.group) * p.b_group_rows + row) * p.ld_sw;
       }
-      const int a0 = x_row(item, r);
+      const int a0 = x_row(next0), a1 = x_row(next1);
       if (a0 >= 0) f_x0 = p.sx + a0 * p.ld_sx;
-      if (slot1) {
-        const int a1 = x_row(item, r + 128);
-        if (a1 >= 0) f_x1 = p.sx + a1 * p.ld_sx;
-      }
+      if (a1 >= 0) f_x1 = p.sx + a1 * p.ld_sx;
+      next0 = x_pair(f_it + 1, r);
+      if (slot1) next1 = x_pair(f_it + 1, r + 128);
     };
     auto fetch = [&](int slot) {
       if (f_it < n_items) {
@@ -516,7 +547,7 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
         f_kb += kUnitsPerChunk;
         if (f_kb >= p.k_blocks) {
           f_kb = 0;
-          f_it += step;
+          ++f_it;
           enter();
         }
       }
@@ -527,7 +558,7 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
     int s = 0, kb = 0, c_slot = 0, run = 0;  // run: k-blocks so far, modulo two runs
     uint32_t ph = 0;
     bool alive = true;
-    for (int it = blockIdx.x; it < n_items && alive;) {
+    for (int it = 0; it < n_items && alive;) {
       const int in_chunk = min(kUnitsPerChunk, p.k_blocks - kb);
       asm volatile("cp.async.wait_group %0;" ::"n"(kFetchAhead - 1) : "memory");
       uint4 cw[kTiles], cx0 = make_uint4(0, 0, 0, 0), cx1 = make_uint4(0, 0, 0, 0);
@@ -591,7 +622,7 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
       kb += in_chunk;
       if (kb == p.k_blocks) {
         kb = 0;
-        it += step;
+        ++it;
       }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -607,7 +638,7 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
     const bool weighted = p.row_weights != nullptr;
     int buf = 0;
     uint32_t acc_ph = 0;
-    for (int it = blockIdx.x; it < n_items; it += step) {
+    for (int it = 0; it < n_items; ++it) {
       const GroupedItem item = item_at(it);
       const int c0 = kTurns ? 16 * half : 0;
       int q_next = pair_at(item, c0 + (lane & 15));
