@@ -43,8 +43,9 @@ constexpr int kGroupedEpilogueWarp = 12;
 __host__ __device__ constexpr int grouped_threads(bool two) { return 32 * (kGroupedEpilogueWarp + (two ? 8 : 4)); }
 constexpr int kGroupedMaxStages = 8;
 constexpr int kGroupedMaxBN = 192;   // two accumulators and four slots of scales fit tensor memory
-// 16-byte scale chunks that each of the two sets of scale writers has in flight
-__host__ __device__ constexpr int grouped_fetch_ahead(bool two) { return two ? 1 : 2; }
+// 16-byte scale chunks that each of the two sets of scale writers has in flight: of two k-blocks for e2m1
+// (ka = 2 atoms), of four else.  (One token, 8 of 64 experts, 2048 x 4096 e2m1: with half as many TBD us.)
+__host__ __device__ constexpr int grouped_fetch_ahead(bool two, int ka) { return (two ? 1 : 2) * ka; }
 
 struct GroupedParams {
   const uint8_t* sw;          // W's scales, row-major
@@ -73,8 +74,8 @@ struct GroupedParams {
 // W tiles of a CTA: one, or (kTwo) two that share X.
 __host__ __device__ inline int grouped_stage_bytes(int BN, bool two) { return (two ? 2 : 1) * kTileM * 128 + BN * 128; }
 __host__ __device__ inline int grouped_atoms(int BN, int ka, bool two) { return ka * ((two ? 2 : 1) + (BN > 128 ? 2 : 1)); }
-__host__ __device__ inline int grouped_staging_bytes(int BN, bool two) {
-  return 2 * grouped_fetch_ahead(two) * ((two ? 2 : 1) * kTileM + BN) * 16;
+__host__ __device__ inline int grouped_staging_bytes(int BN, int ka, bool two) {
+  return 2 * grouped_fetch_ahead(two, ka) * ((two ? 2 : 1) * kTileM + BN) * 16;
 }
 // Tensor memory: accumulators of BN columns (two sets of them, where they fit), four slots of scales.
 __host__ __device__ inline int grouped_acc_sets(int BN, int ka, bool two) {
@@ -82,10 +83,13 @@ __host__ __device__ inline int grouped_acc_sets(int BN, int ka, bool two) {
 }
 // The first items of a CTA are worked out once, by all threads, and looked up by the roles.
 constexpr int kGroupedTable = 64;
-__host__ __device__ inline int grouped_table_bytes(int groups) { return (2 * (groups + 1) * 4 + 15) / 16 * 16 + kGroupedTable * 16; }
+// Then the epilogue's list of an item's pairs and weights, for two items.
+__host__ __device__ inline int grouped_table_bytes(int groups) {
+  return (2 * (groups + 1) * 4 + 15) / 16 * 16 + kGroupedTable * 16 + 2 * kGroupedMaxBN * 8;
+}
 constexpr int kGroupedBarrierBytes = 256;
 __host__ __device__ inline int grouped_smem_bytes(int BN, int stages, int ka, int groups, bool two) {
-  return 1024 + stages * (grouped_stage_bytes(BN, two) + grouped_atoms(BN, ka, two) * 512) + grouped_staging_bytes(BN, two) +
+  return 1024 + stages * (grouped_stage_bytes(BN, two) + grouped_atoms(BN, ka, two) * 512) + grouped_staging_bytes(BN, ka, two) +
          grouped_table_bytes(groups) + kGroupedBarrierBytes;
 }
 
@@ -163,7 +167,7 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
   constexpr int kUnitsPerChunk = 16 / kSfBytes;        // k-blocks served by one 16-byte fetch of a scale row
   constexpr int kTiles = kTwo ? 2 : 1;
   constexpr int kTileCols = 128 * kTiles / (kGated ? 2 : 1);  // columns of D per item
-  constexpr int kThreads = grouped_threads(kTwo), kFetchAhead = grouped_fetch_ahead(kTwo);
+  constexpr int kThreads = grouped_threads(kTwo), kFetchAhead = grouped_fetch_ahead(kTwo, kKa);
   constexpr uint32_t kWBytes = kTiles * kTileM * 128;
   constexpr unsigned kAll = 0xffffffffu;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -181,9 +185,10 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
   const uint32_t atom_bytes = atoms * 512u;
   const uint32_t atom_base = smem_base + stages * stage_bytes;
   const uint32_t staging_base = atom_base + stages * atom_bytes;
-  const uint32_t table_off = staging_base + static_cast<uint32_t>(grouped_staging_bytes(BN, kTwo)) - smem_base;
+  const uint32_t table_off = staging_base + static_cast<uint32_t>(grouped_staging_bytes(BN, kKa, kTwo)) - smem_base;
   int4* table = reinterpret_cast<int4*>(smem + table_off);        // [kGroupedTable]
-  int32_t* first = reinterpret_cast<int32_t*>(table + kGroupedTable);  // [groups + 1]
+  int2* lists = reinterpret_cast<int2*>(table + kGroupedTable);   // [2][kGroupedMaxBN]: pair, weight
+  int32_t* first = reinterpret_cast<int32_t*>(lists + 2 * kGroupedMaxBN);  // [groups + 1]
   int32_t* start = first + p.groups + 1;                          // [groups + 1]
   const uint32_t bar_base = smem_base + table_off + static_cast<uint32_t>(grouped_table_bytes(p.groups));
   auto full_bar = [&](int s) { return bar_base + 8u * s; };
@@ -628,28 +633,46 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
     asm volatile("cp.async.wait_group 0;" ::: "memory");
   } else {
     // -------------------------------- epilogue --------------------------------
-    // 16 columns (pairs) at a time; their pairs and weights are fetched one step ahead, those of an
-    // item's first step before its accumulator is waited for.  kTwo: two warps to a lane quarter;
-    // gated they take the steps in turn, else a W tile each.
+    // 16 columns (pairs) at a time.  The item's pairs and weights are put into a list in shared memory before its
+    // accumulator is waited for (fetched step by step they took most of the epilogue's time).  kTwo: two
+    // warps to a lane quarter; gated they take the steps in turn, else a W tile each.
     const int quarter = warp & 3;  // the TMEM lane quarter this warp can read
     const int half = (warp - kGroupedEpilogueWarp) >> 2;
     constexpr bool kTurns = kTwo && kGated;
     constexpr int kStep = kTurns ? 32 : 16;
     const bool weighted = p.row_weights != nullptr;
+    bool alive = true;
     int buf = 0;
     uint32_t acc_ph = 0;
     for (int it = 0; it < n_items; ++it) {
       const GroupedItem item = item_at(it);
-      const int c0 = kTurns ? 16 * half : 0;
-      int q_next = pair_at(item, c0 + (lane & 15));
-      float w_next = weighted && q_next >= 0 ? p.row_weights[q_next] : 1.0f;
+      int2* list = lists + (it & 1) * kGroupedMaxBN;
+      for (int r = static_cast<int>(threadIdx.x) - 32 * kGroupedEpilogueWarp; r < item.count; r += 128 * kTiles) {
+        const int q = pair_at(item, r);
+        list[r] = make_int2(q, __float_as_int(weighted && q >= 0 ? p.row_weights[q] : 1.0f));
+      }
+      // the list is complete (and everyone is done with the one before the last); a warp that gave up
+      // waiting takes the others along here, none waits for one that has left
+      uint32_t all_alive;
+      asm volatile(
+          "{\n\t"
+          ".reg .pred p, q;\n\t"
+          "setp.ne.b32 p, %1, 0;\n\t"
+          "bar.red.and.pred q, 1, %2, p;\n\t"
+          "selp.u32 %0, 1, 0, q;\n\t"
+          "}\n"
+          : "=r"(all_alive)
+          : "r"(alive ? 1u : 0u), "n"(128 * kTiles)
+          : "memory");
+      if (!all_alive) break;
       const bool got = mbar_wait_bounded(acc_full_bar(buf), acc_ph, abort_flag, budget_ns);
       if (!__all_sync(kAll, got)) {
         if (lane == 0) {
           leave_error(p.error, kErrEpilogueWait);
           *abort_flag = 1;
         }
-        break;
+        alive = false;
+        continue;
       }
       tc_fence_after_sync();
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
@@ -659,10 +682,7 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
       else col += kGated ? quarter * 16 + (lane & 15) : quarter * 32 + lane;
       float* const d_col = p.d + col;
       const bool in = col < p.n;
-      for (int c = c0; c < item.count; c += kStep) {
-        const int q_mine = q_next;
-        const float w_mine = w_next;
-        q_next = pair_at(item, c + kStep + (lane & 15));
+      for (int c = kTurns ? 16 * half : 0; c < item.count; c += kStep) {
         uint32_t acc[16];
         tmem_ld_32x16(taddr + static_cast<uint32_t>(c), acc);
         if constexpr (kTurns) {
@@ -687,24 +707,24 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
               const float other = __uint_as_float(__shfl_xor_sync(kAll, give, 16));
               const float kept = __uint_as_float(lane < 16 ? acc[j] : acc[j + 1]);
               float y = silu_f32(lane < 16 ? kept : other) * (lane < 16 ? other : kept);
-              const int from = j + (lane >> 4);
-              const int q = __shfl_sync(kAll, q_mine, from);
-              const float w = __shfl_sync(kAll, w_mine, from);
-              if (weighted) y *= w;
-              if (in && q >= 0) d_col[q * p.ldd] = y;
+              if (c + j + (lane >> 4) < item.count) {
+                const int2 to = list[c + j + (lane >> 4)];
+                if (weighted) y *= __int_as_float(to.y);
+                if (in && to.x >= 0) d_col[to.x * p.ldd] = y;
+              }
             }
           } else {
 #pragma unroll
             for (int j = j0; j < j0 + 4; ++j) {
-              const int q = __shfl_sync(kAll, q_mine, j);
-              const float w = __shfl_sync(kAll, w_mine, j);
-              float y = __uint_as_float(acc[j]);
-              if (weighted) y *= w;
-              if (in && q >= 0) d_col[q * p.ldd] = y;
+              if (c + j < item.count) {
+                const int2 to = list[c + j];
+                float y = __uint_as_float(acc[j]);
+                if (weighted) y *= __int_as_float(to.y);
+                if (in && to.x >= 0) d_col[to.x * p.ldd] = y;
+              }
             }
           }
         }
-        w_next = weighted && q_next >= 0 ? p.row_weights[q_next] : 1.0f;
       }
       tc_fence_before_sync();
       __syncwarp();
