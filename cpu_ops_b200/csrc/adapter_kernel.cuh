@@ -72,87 +72,156 @@ __device__ __forceinline__ void load8(const T* row, int i, int len, bool wide, f
   }
 }
 
+// Sixteen elements of a row of B as they are stored, `left` of which exist.
+template <typename W>
+struct Sixteen {
+  uint4 lo, hi;
+  __device__ __forceinline__ void load(const W* row, int left, bool wide) {
+    lo = hi = make_uint4(0, 0, 0, 0);
+    if (wide && left >= 16) {
+      lo = reinterpret_cast<const uint4*>(row)[0];
+      hi = reinterpret_cast<const uint4*>(row)[1];
+    } else {
+      __align__(16) W v[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[j] = j < left ? row[j] : W(0.0f);
+      lo = reinterpret_cast<const uint4*>(v)[0];
+      hi = reinterpret_cast<const uint4*>(v)[1];
+    }
+  }
+  // sum + the product with 16 floats (shared memory, 16-byte aligned); what does not exist on either side is zero
+  __device__ __forceinline__ float dot(const float* u, float sum) const {
+    const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float4 f = reinterpret_cast<const float4*>(u)[j];
+      const W* h = reinterpret_cast<const W*>(&w[2 * j]);
+      sum = __fmaf_rn(f.x, to_f32<W>(h[0]), sum);
+      sum = __fmaf_rn(f.y, to_f32<W>(h[1]), sum);
+      sum = __fmaf_rn(f.z, to_f32<W>(h[2]), sum);
+      sum = __fmaf_rn(f.w, to_f32<W>(h[3]), sum);
+    }
+    return sum;
+  }
+};
+
+// What bounds it is latency (one row: two reads from memory after one another, the exchange between them),
+// with many rows the traffic; so a thread has the B of four columns, and their C, on their way before u is known.
+constexpr int kRowCols = 4;  // columns a thread works on at a time
 template <typename X, typename W>
 __global__ void __launch_bounds__(kAdapterThreads) __cluster_dims__(kAdapterCluster, 1, 1)
     adapter_rows_kernel(const AdapterParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  // Shared memory of another CTA exists once that CTA has started: the waits below, before the first
-  // store to it, are for every CTA's arrival here.
+  // Shared memory of another CTA exists once that CTA has started: the wait below, before the first
+  // store to it, is for every CTA's arrival here.
   cluster_arrive();
   asm volatile("griddepcontrol.wait;" ::: "memory");
   __shared__ float part[kAdapterCluster][kMaxRank];  // [CTA the sum comes from][rank]
-  __shared__ float u[kMaxRank];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __shared__ __align__(16) float u[kMaxRank];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cta = static_cast<int>(cluster_cta_rank());
   const int row = static_cast<int>(blockIdx.x) / kAdapterCluster;
   const int g = p.ids[row];
   const bool has = g >= 0 && g < p.adapters;  // (the same in the whole cluster)
+  cluster_wait();
+
+  // This CTA's columns; of a thread: n0 + tid, + 256, ...
+  const int per_n = (p.n + kAdapterCluster - 1) / kAdapterCluster;
+  const int n0 = cta * per_n, n1 = min(n0 + per_n, p.n);
+  const W* b = static_cast<const W*>(p.b) + (has ? g * p.b_stride : 0);
+  const float* c_row = p.c + row * p.ldc;
+  float* d_row = p.d + row * p.ldd;
+  const bool wide_r = p.align_r == 16;
+  Sixteen<W> bv[kRowCols];
+  float cv[kRowCols];
+  auto load = [&](int col0) {
+#pragma unroll
+    for (int j = 0; j < kRowCols; ++j) {
+      const int col = col0 + j * kAdapterThreads;
+      cv[j] = col < n1 ? c_row[col] : 0.0f;
+      bv[j].lo = bv[j].hi = make_uint4(0, 0, 0, 0);
+      if (has && col < n1) bv[j].load(b + col * p.ldb, p.rank, wide_r);
+    }
+  };
+  if (has || p.c != p.d) load(n0 + tid);
 
   if (has) {
-    // u, this CTA's part of k (whole groups of eight elements)
+    // u, this CTA's part of k (whole groups of eight elements), two ranks of a warp at a time
     const int per = ((p.k + kAdapterCluster - 1) / kAdapterCluster + 7) / 8 * 8;
     const int k0 = min(cta * per, p.k), k1 = min(k0 + per, p.k);
     const X* x = static_cast<const X*>(p.x) + row * p.ldx;
     const W* a = static_cast<const W*>(p.a) + g * p.a_stride;
-    for (int j = warp; j < p.rank; j += kAdapterThreads / 32) {
-      const W* aj = a + j * p.lda;
-      float sum = 0.0f;
+    const bool wide_k = p.align_k == 16;
+    for (int j = 2 * warp; j < p.rank; j += 2 * kAdapterThreads / 32) {
+      const bool two = j + 1 < p.rank;
+      const W *a0 = a + j * p.lda, *a1 = two ? a0 + p.lda : a0;
+      float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll 2
       for (int i = k0 + lane * 8; i < k1; i += 256) {
-        float xv[8], av[8];
-        load8<X>(x, i, k1, p.align_k == 16, xv);
-        load8<W>(aj, i, k1, p.align_k == 16, av);
+        float xv[8], v0[8], v1[8];
+        load8<X>(x, i, k1, wide_k, xv);
+        load8<W>(a0, i, k1, wide_k, v0);
+        load8<W>(a1, i, k1, wide_k, v1);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum = __fmaf_rn(xv[e], av[e], sum);
+        for (int e = 0; e < 8; ++e) {
+          sum0 = __fmaf_rn(xv[e], v0[e], sum0);
+          sum1 = __fmaf_rn(xv[e], v1[e], sum1);
+        }
       }
 #pragma unroll
-      for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-      if (lane == 0) part[cta][j] = sum;
-    }
-  }
-  __syncwarp();
-  cluster_wait();
-  __syncthreads();
-  if (has) {
-    // this CTA's sums to the seven others
-    for (int i = threadIdx.x; i < p.rank * kAdapterCluster; i += kAdapterThreads) {
-      const int j = i / kAdapterCluster, to_cta = i % kAdapterCluster;
-      if (to_cta == cta) continue;
-      const uint32_t to = map_to_cta(smem_u32(&part[cta][j]), static_cast<uint32_t>(to_cta));
-      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(part[cta][j]) : "memory");
+      for (int s = 16; s > 0; s >>= 1) {
+        sum0 += __shfl_xor_sync(0xffffffffu, sum0, s);
+        sum1 += __shfl_xor_sync(0xffffffffu, sum1, s);
+      }
+      // to all eight CTAs: lane l to CTA l % 8, lanes 8-15 the second rank
+      if (lane < kAdapterCluster || (two && lane < 2 * kAdapterCluster)) {
+        const int rank = j + lane / kAdapterCluster;
+        const uint32_t to = map_to_cta(smem_u32(&part[cta][rank]), static_cast<uint32_t>(lane % kAdapterCluster));
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(lane < kAdapterCluster ? sum0 : sum1) : "memory");
+      }
     }
   }
   // all partial sums are in place; and no CTA has left while another still writes to it
   __syncwarp();
   cluster_sync_all();
+  if (!has && p.c == p.d) return;
+  const int rank_pad = (p.rank + 15) / 16 * 16;
   if (has) {
     const float scale = p.scales != nullptr ? p.scales[g] : 1.0f;
-    for (int j = threadIdx.x; j < p.rank; j += kAdapterThreads) {
-      float sum = part[0][j];
+    for (int j = tid; j < rank_pad; j += kAdapterThreads) {
+      float sum = 0.0f;
+      if (j < p.rank) {
+        sum = part[0][j];
 #pragma unroll
-      for (int c = 1; c < kAdapterCluster; ++c) sum += part[c][j];
+        for (int c = 1; c < kAdapterCluster; ++c) sum += part[c][j];
+      }
       u[j] = sum * scale;
     }
     __syncthreads();
-  } else if (p.c == p.d) {
-    return;
   }
-  const int per_n = (p.n + kAdapterCluster - 1) / kAdapterCluster;
-  const int n0 = cta * per_n, n1 = min(n0 + per_n, p.n);
-  const W* b = static_cast<const W*>(p.b) + (has ? g * p.b_stride : 0);
-  for (int col = n0 + threadIdx.x; col < n1; col += kAdapterThreads) {
-    float sum = 0.0f;
-    if (has) {
-      const W* bj = b + col * p.ldb;
-      for (int i = 0; i < p.rank; i += 8) {
-        float bv[8];
-        load8<W>(bj, i, p.rank, p.align_r == 16, bv);
+  for (int col0 = n0 + tid; col0 < n1; col0 += kRowCols * kAdapterThreads) {
+    if (col0 != n0 + tid) load(col0);
+    float sum[kRowCols];
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (i + e < p.rank) sum = __fmaf_rn(u[i + e], bv[e], sum);
+    for (int j = 0; j < kRowCols; ++j) sum[j] = 0.0f;
+    if (has) {
+      for (int r0 = 0; r0 < p.rank; r0 += 16) {
+        if (r0 > 0) {
+#pragma unroll
+          for (int j = 0; j < kRowCols; ++j) {
+            const int col = col0 + j * kAdapterThreads;
+            if (col < n1) bv[j].load(b + col * p.ldb + r0, p.rank - r0, wide_r);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < kRowCols; ++j) sum[j] = bv[j].dot(u + r0, sum[j]);
       }
-      p.d[row * p.ldd + col] = p.c[row * p.ldc + col] + sum;
-    } else {
-      p.d[row * p.ldd + col] = p.c[row * p.ldc + col];
+    }
+#pragma unroll
+    for (int j = 0; j < kRowCols; ++j) {
+      const int col = col0 + j * kAdapterThreads;
+      // (a row without an adapter is C itself: no zero is added to it)
+      if (col < n1) d_row[col] = has ? cv[j] + sum[j] : cv[j];
     }
   }
 }
