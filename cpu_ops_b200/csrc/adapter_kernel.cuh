@@ -106,10 +106,10 @@ struct Sixteen {
 };
 
 // What bounds it is latency (one row: two reads from memory after one another, the exchange between them),
-// with many rows the traffic; so a thread has the B of four columns, and their C, on their way before u is known.
-constexpr int kRowCols = 4;  // columns a thread works on at a time
+// with many rows the traffic; so a thread has the B of two columns, and their C, on their way before u is known.
+constexpr int kRowCols = 2;  // columns a thread works on at a time
 template <typename X, typename W>
-__global__ void __launch_bounds__(kAdapterThreads) __cluster_dims__(kAdapterCluster, 1, 1)
+__global__ void __launch_bounds__(kAdapterThreads, 4) __cluster_dims__(kAdapterCluster, 1, 1)
     adapter_rows_kernel(const AdapterParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // Shared memory of another CTA exists once that CTA has started: the wait below, before the first

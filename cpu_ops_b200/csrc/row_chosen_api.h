@@ -540,6 +540,21 @@ int adapters_by_tiles(RowCall& call, const AdapterParams& p, int x_type, int w_t
                       256, static_cast<size_t>(adapter_up_smem(w_type, t.rank_pad)), call.stream, t);
 }
 
+// Whether rows are taken tile by tile.  By themselves they read their adapters anew, row by row, from L2 where rows
+// share one: 3.3 TB/s of that were seen.  A step of a tile (64 columns, or 64 elements of k) takes its time
+// however few rows the tile has, and an adapter in use has a tile at least.  us, tiles / rows by themselves:
+//   rank 16, 4096 x 4096, 16 adapters: 128 rows 21 / 11.5, 256 22 / 23, 1024 30 / 82
+//   the same of 128 adapters: 256 rows 63 / 27, 512 64 / 48, 1024 65 / 86
+//   rank 64, 2048 x 2048, 64 adapters: 128 rows 35 / 28, 256 36 / 49
+bool adapters_want_tiles(const AdapterParams& p, int sms) {
+  const int64_t tiles = plan_max_tiles(p.m, p.adapters);
+  if (p.adapters > kMaxGroups || tiles > 65535) return false;
+  const double rows_us = 4.0 + 2.0 * p.m * static_cast<double>(p.rank) * (static_cast<double>(p.n) + p.k) / 3.3e6;
+  const double up = static_cast<double>(tiles) * ((p.n + kUpCols - 1) / kUpCols) / (2.0 * sms);
+  const double down = static_cast<double>(tiles) * ((p.k + kDownDepth - 1) / kDownDepth) * ((p.rank + 63) / 64) / (3.0 * sms);
+  return 12.0 + 1.2 * (1.0 + p.rank / 64.0) * up + 0.5 * down < rows_us;
+}
+
 int adapters_call(const cpuops_b200_adapters_desc* d) {
   if (int rc = check_desc(d)) return rc;
   if (!type_ok(d->x_type) || !type_ok(d->w_type)) {
@@ -596,8 +611,7 @@ int adapters_call(const cpuops_b200_adapters_desc* d) {
   p.align_r = align(d->b, d->ldb, d->b_stride, 2);
   p.align_c = align(d->c, d->ldc, 0, 4);
   p.align_d = align(d->d, d->ldd, 0, 4);
-  // Few rows: each reads its adapter by itself (from L2, where rows share one).
-  if (p.adapters > 0 && p.adapters <= kMaxGroups && p.m >= 256 && plan_max_tiles(p.m, p.adapters) <= 65535) {
+  if (any && adapters_want_tiles(p, call.st->sms())) {
     if (int rc = adapters_by_tiles(call, p, d->x_type, d->w_type)) return rc;
     return call.finish();
   }

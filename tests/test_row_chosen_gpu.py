@@ -446,6 +446,86 @@ def test_adapters_keep_f32_accuracy(gpu):
         assert (D == 2.0 ** -12).all()
 
 
+# Many rows go tile by tile: several launches instead of one.
+
+
+def check_many_rows(*args, **kw):
+    before = c.launch_count()
+    check_adapters(*args, **kw)
+    assert c.launch_count() - before >= 3, "these rows were to go tile by tile"
+
+
+@pytest.mark.parametrize("kx,kw", TYPES)
+def test_adapters_many_rows_types(gpu, kx, kw):
+    check_many_rows(kx, kw, 2500, 264, 520, 16, 5, seed=1)
+    check_many_rows(kx, kw, 4200, 260, 500, 15, 5, seed=2)
+
+
+@pytest.mark.parametrize("m,n,k,rank,count", [(1500, 300, 2048, 64, 6), (4000, 65, 33, 256, 2), (6000, 130, 100, 17, 3),
+                                              (2048, 1024, 64, 48, 1), (5000, 64, 1000, 8, 9), (3000, 128, 256, 129, 30),
+                                              (4097, 500, 300, 65, 1000)])
+def test_adapters_many_rows_sizes(gpu, m, n, k, rank, count):
+    if count == 1000:   # (a plan of nearly as many groups as there may be; the rows all in a few of them)
+        ids = W.rng_for(3, 8).integers(0, 1000, 12)[W.rng_for(4, 8).integers(0, 12, m)]
+        got, want, err, _ = run_adapters("bf16", "bf16", m, n, k, rank, count, ids=ids)
+        assert np.all(np.abs(got - want) <= err)
+    else:
+        check_many_rows("bf16", "bf16", m, n, k, rank, count, seed=n)
+        check_many_rows("f32", "f16", m, n, k, rank, count, seed=k)
+
+
+@pytest.mark.parametrize("pad", [(3, 0, 1), (8, 8, 4), (0, 5, 3), (1, 1, 0), (2, 2, 2)])
+def test_adapters_many_rows_strides(gpu, pad):
+    for kx, kw in TYPES:
+        check_many_rows(kx, kw, 4000, 97, 168, 24, 4, pad=pad, gap=2, scaled=False, seed=5)
+        check_many_rows(kx, kw, 4000, 96, 168, 24, 4, pad=pad, in_place=True, seed=6)
+
+
+def test_adapters_many_rows_without(gpu):
+    m = 4000
+    ids = np.where(np.arange(m) % 3 == 0, -1, np.arange(m) % 2)
+    ids[1] = 1 << 30
+
+    def spoil(x, A, B, C):
+        x[::3] = float("nan")
+        x[1] = float("inf")
+        A[2] = float("nan")
+        B[2] = float("nan")
+
+    for in_place in (False, True):
+        before = c.launch_count()
+        got, want, err, C = run_adapters("bf16", "bf16", m, 256, 256, 16, 3, ids=ids, in_place=in_place, spoil=spoil)
+        assert c.launch_count() - before >= 3
+        none = (ids < 0) | (ids >= 3)
+        assert np.array_equal(got[none], C[none])
+        assert np.all(np.abs(got - want)[~none] <= err[~none])
+    check_many_rows("bf16", "bf16", m, 256, 256, 16, 3, ids=np.full(m, -1))
+    check_many_rows("f16", "f16", m, 256, 256, 16, 3, ids=np.full(m, 2), in_place=True)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_adapters_many_rows_keep_f32_accuracy(gpu, kind):
+    """As above: 256 + 2^-12 and 256 cancel in the second product; in f16 also beside a number near the
+    top of u's range, and with all of u tiny."""
+    m, k, rank, n = 4000, 256, 16, 256
+    t, storage = FLOATS[kind]
+    for size in (1.0, 2.0 ** -40, 2.0 ** 30):
+        x = torch.full((m, k), size, dtype=torch.float32, device="cuda")
+        A = torch.zeros((1, rank, k), dtype=t, device="cuda")
+        A[0, 0, 0], A[0, 0, 1], A[0, 1, 0] = 256.0, 2.0 ** -12, 256.0
+        B = torch.zeros((1, n, rank), dtype=t, device="cuda")
+        B[0, :, 0], B[0, :, 1] = 1.0, -1.0
+        C = torch.zeros((m, n), device="cuda")
+        D = torch.empty_like(C)
+        op = c.LowRankAdapters(c.f32_t, storage)
+        before = c.launch_count()
+        check(op(op.Arguments(c.AdapterCoord(m, n, k, rank, 1), c.TensorRef(x, k), c.AdapterRef(A, k, rank * k),
+                              c.AdapterRef(B, rank, n * rank), torch.zeros(m, dtype=torch.int32, device="cuda"),
+                              c.TensorRef(C, n), c.TensorRef(D, n))))
+        assert c.launch_count() - before >= 3
+        assert (D == size * 2.0 ** -12).all()
+
+
 # ---- together, on streams and in graphs ------------------------------------------------------------
 
 
