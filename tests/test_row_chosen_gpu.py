@@ -233,6 +233,65 @@ def test_grouped_formats(gpu, fa, fb, gated):
     Experts(fa, fb, 70, 200, 640, 5, gated=gated, share=2, seed=1).check()
 
 
+# Many pairs per group: A is copied in plan order first.  Narrow outputs take one tile per CTA, wide ones two.
+MANY = [(260, 200, 640, 3), (400, 6000, 96, 4), (777, 1000, 320, 2), (650, 5000, 224, 13)]
+
+
+@pytest.mark.parametrize("fa,fb", PAIRS)
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("rows,n,k,groups", MANY)
+def test_grouped_many_pairs(gpu, fa, fb, gated, rows, n, k, groups):
+    if fb == F4 and fa != F4:
+        k = 128 * (-(-k // 128))
+    before = c.launch_count()
+    Experts(fa, fb, rows, n // 2 if gated else n, k, groups, gated=gated, share=2, seed=rows).check()
+    assert c.launch_count() - before == 2
+
+
+@pytest.mark.parametrize("rows,n,k,groups", MANY[:2])
+@pytest.mark.parametrize("summed,share", [(1, 1), (2, 1), (4, 4)])
+def test_grouped_many_pairs_weights_and_sums(gpu, rows, n, k, groups, summed, share):
+    rng = W.rng_for(rows, 7)
+    ids = rng.integers(-1, groups, rows)
+    ids[:20] = -1
+    e = Experts(E4, E4, rows, n, k, groups, share=share, ids=ids, seed=3, gap=5, pad=64)
+    e.check(True, summed, ldd=n + 3)
+    Experts(F4, F4, rows, n // 3, k, groups, gated=True, share=share, ids=ids, seed=4).check(True, summed)
+
+
+@pytest.mark.parametrize("rows,n,k,groups", MANY[:2])
+@pytest.mark.parametrize("lds,offset", [(32, 0), (32, 4), (21, 3)])
+def test_grouped_many_pairs_scales_anywhere(gpu, rows, n, k, groups, lds, offset):
+    for fmt, gated in ((E4, True), (F4, False)):
+        Experts(fmt, fmt, rows, n, k, groups, gated=gated, share=2, lds=lds, offset=offset, seed=lds).check()
+
+
+@pytest.mark.parametrize("k", [2, 34, 130, 258, 1002])
+def test_grouped_many_pairs_k_inside_a_block(gpu, k):
+    for fmt in (E5, F4):
+        Experts(fmt, fmt, 200, 5000, k, 2, seed=k).check()
+
+
+def test_grouped_many_pairs_of_a_plan_that_lies(gpu):
+    e = Experts(E4, E4, 300, 72, 128, 4, share=3, seed=8)
+    offsets, order = H.plan_of(e.ids, 4)
+    bad = order.copy()
+    bad[::5] = np.array([1 << 30, -5, 300, -(1 << 31)], np.int64)[np.arange(bad[::5].size) % 4]
+    D = e.run(plan=(offsets, bad)).cpu().numpy()
+    left = np.setdiff1d(np.arange(300), order[np.arange(300) % 5 != 0])
+    assert (D[left] == 7.5).all()
+    A, B = e.dense()
+    want, err = H.grouped(A, B, np.where(np.isin(np.arange(300), left), -1, e.ids), 72, False, 3, None, 1, np.full((300, 72), 7.5))
+    assert np.all(np.abs(D - want) <= err)
+
+
+def test_grouped_one_large_group_among_many(gpu):
+    """Far more pairs in one group than the average the call is planned for."""
+    ids = np.where(np.arange(2000) % 50 == 0, np.arange(2000) % 7, 5)
+    Experts(E4, E4, 2000, 300, 256, 40, ids=ids, seed=5).check()
+    Experts(E4, E4, 2000, 300, 256, 20, gated=True, ids=ids, seed=5).check()
+
+
 @pytest.mark.parametrize("rows,n,k,groups", [(1, 1, 32, 1), (1, 128, 128, 4), (2, 129, 4096, 3), (16, 64, 96, 1),
                                              (17, 300, 1056, 2), (193, 130, 256, 1), (385, 65, 544, 2),
                                              (1000, 40, 64, 300), (64, 127, 8192, 2), (5, 257, 288, 1024)])
