@@ -54,7 +54,7 @@ struct GroupedParams {
   const int32_t* order;
   const float* row_weights;   // or null
   float* d;
-  int64_t ldd;
+  int32_t ldd;
   int64_t ld_sw, ld_sx;
   int32_t rows, groups;       // pairs; groups of the plan
   int32_t n;                  // columns of D
@@ -647,7 +647,8 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
     for (int it = 0; it < n_items; ++it) {
       const GroupedItem item = item_at(it);
       int2* list = lists + (it & 1) * kGroupedMaxBN;
-      for (int r = static_cast<int>(threadIdx.x) - 32 * kGroupedEpilogueWarp; r < item.count; r += 128 * kTiles) {
+      const uint32_t list_at = smem_u32(list);
+      for (int r = static_cast<int>(threadIdx.x) - 32 * kGroupedEpilogueWarp; r < ((item.count + 15) & ~15); r += 128 * kTiles) {
         const int q = pair_at(item, r);
         list[r] = make_int2(q, __float_as_int(weighted && q >= 0 ? p.row_weights[q] : 1.0f));
       }
@@ -696,33 +697,33 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
           tmem_ld_wait();
         }
 #pragma unroll
-        for (int j0 = 0; j0 < 16; j0 += 4) {
+        for (int j0 = 0; j0 < 16; j0 += 8) {
           if (c + j0 >= item.count) break;
-          if constexpr (kGated && !kTwo) {
-            // lanes 0-15 hold the gate, 16-31 the up product: the lower lanes finish the even columns,
-            // the upper ones the odd
+          // eight pairs and weights, before any store (behind one the compiler would have to load them again)
+          int q[8];
+          float w[8];
 #pragma unroll
-            for (int j = j0; j < j0 + 4; j += 2) {
-              const uint32_t give = lane < 16 ? acc[j + 1] : acc[j];
-              const float other = __uint_as_float(__shfl_xor_sync(kAll, give, 16));
-              const float kept = __uint_as_float(lane < 16 ? acc[j] : acc[j + 1]);
-              float y = silu_f32(lane < 16 ? kept : other) * (lane < 16 ? other : kept);
-              if (c + j + (lane >> 4) < item.count) {
-                const int2 to = list[c + j + (lane >> 4)];
-                if (weighted) y *= __int_as_float(to.y);
-                if (in && to.x >= 0) d_col[to.x * p.ldd] = y;
-              }
-            }
-          } else {
+          for (int j = 0; j < 8; j += 2)
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(q[j]), "=f"(w[j]), "=r"(q[j + 1]), "=f"(w[j + 1])
+                         : "r"(list_at + static_cast<uint32_t>(c + j0 + j) * 8u));
 #pragma unroll
-            for (int j = j0; j < j0 + 4; ++j) {
-              if (c + j < item.count) {
-                const int2 to = list[c + j];
-                float y = __uint_as_float(acc[j]);
-                if (weighted) y *= __int_as_float(to.y);
-                if (in && to.x >= 0) d_col[to.x * p.ldd] = y;
-              }
+          for (int j = 0; j < 8; j += kGated && !kTwo ? 2 : 1) {
+            float y = __uint_as_float(acc[j0 + j]);
+            int to = q[j];
+            float weight = w[j];
+            if constexpr (kGated && !kTwo) {
+              // lanes 0-15 hold the gate, 16-31 the up product: the lower lanes finish the even columns,
+              // the upper ones the odd
+              const bool upper = lane >= 16;
+              const float other = __shfl_xor_sync(kAll, upper ? y : __uint_as_float(acc[j0 + j + 1]), 16);
+              const float kept = upper ? __uint_as_float(acc[j0 + j + 1]) : y;
+              y = silu_f32(upper ? other : kept) * (upper ? kept : other);
+              to = upper ? q[j + 1] : to;
+              weight = upper ? w[j + 1] : weight;
             }
+            if (weighted) y *= weight;
+            if (in && to >= 0) d_col[static_cast<int64_t>(to) * p.ldd] = y;
           }
         }
       }
