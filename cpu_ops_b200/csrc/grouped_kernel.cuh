@@ -16,8 +16,8 @@
 //     lane of a warp for every four rows; their scales by the scale-writer warps, which read them by
 //     row anyway.  A gather costs the TMA unit about 38 cycles whatever its rows, which W's own time hides
 //     while items have few pairs.  With many, gather_rows_kernel copies the rows in plan order once,
-//     and X comes in boxes of 16 rows (2048 rows x 4 of 32 experts, 4096 x 4096 e4m3: 650 us
-//     gathered, TBD copied, the copy's 10 included).
+//     and X comes in boxes of BN / 2 rows (2048 rows x 4 of 32 experts, 4096 x 4096 e4m3: 650 us
+//     gathered, 275 copied, the copy's 10 included).
 //   * Gated: a tile holds 64 gate rows and their 64 up rows, 16 and 16 in each warp's lane quarter, so
 //     that the two accumulators of an output meet in one warp (lane l and l + 16): one exchange
 //     between lanes, and D is written once, at its final size.
@@ -44,7 +44,7 @@ __host__ __device__ constexpr int grouped_threads(bool two) { return 32 * (kGrou
 constexpr int kGroupedMaxStages = 8;
 constexpr int kGroupedMaxBN = 192;   // two accumulators and four slots of scales fit tensor memory
 // 16-byte scale chunks that each of the two sets of scale writers has in flight: of two k-blocks for e2m1
-// (ka = 2 atoms), of four else.  (One token, 8 of 64 experts, 2048 x 4096 e2m1: with half as many TBD us.)
+// (ka = 2 atoms), of four else.  (One token, 8 of 64 experts, 2048 x 4096 e2m1: with half as many 13.1 us, so 12.6.)
 __host__ __device__ constexpr int grouped_fetch_ahead(bool two, int ka) { return (two ? 1 : 2) * ka; }
 
 struct GroupedParams {
@@ -157,7 +157,7 @@ __device__ __forceinline__ void fetch_scales(uint32_t dst, const uint8_t* src, i
 // kTwo: two W tiles share a stage's X (gated: the gate's and the up projection's 128 rows).  A stage's
 // loads take some 2000 cycles from the moment it is free, so the ring has to hold that much work:
 // with one tile five stages of 144 pairs hold 1440 cycles of it, with two four stages hold 2300, and every
-// role has twice the time for a k-block.  (275 -> TBD us, 2048 rows x 4 of 32 experts, 4096 x 4096 e4m3.)
+// role has twice the time for a k-block.  (275 -> 193 us, 2048 rows x 4 of 32 experts, 4096 x 4096 e4m3.)
 template <int KIND, bool kGated, bool kTwo>
 __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
     grouped_mx_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,

@@ -10,7 +10,7 @@
 // differ by less than a rounding come out in an order that depends on how exp was rounded, about
 // once in a batch of 8192 tokens x 256 experts.  So a token is routed by f32 scores, with a check that
 // neighbours in the order are further apart than the scores' errors, and only where they are not (one token in
-// some hundred) by double ones (8192 tokens, 256 experts in 8 groups, sigmoid, bias: TBD us, all in double
+// some hundred) by double ones (8192 tokens, 256 experts in 8 groups, sigmoid, bias: 28 us, all in double
 // precision 42).  Weights are always formed in double precision.
 #pragma once
 
@@ -212,16 +212,20 @@ __device__ __forceinline__ unsigned groups_kept(const RouteParams& p, const T (&
   }
   const T score = p.group_best == 2 && second != kOut ? best + second : best;
   int ahead = 0;
-  bool close = false;
+  unsigned close = 0;  // groups that are no further away
   for (int j = 0; j < p.n_groups; ++j) {
     const T other = __shfl_sync(kAll, score, j * share);
     ahead += other > score || (other == score && j < g);
     const T size = (other < 0 ? -other : other) + (score < 0 ? -score : score);
     const T gap = other < score ? score - other : other - score;
-    close = close || (j != g && other != kOut && score != kOut && !(gap > slack * size + least));
+    if (other != kOut && score != kOut && !(gap > slack * size + least)) close |= 1u << j;
   }
-  near = __any_sync(kAll, mine && close);
-  return __ballot_sync(kAll, mine && ahead < p.top_groups && part == 0);
+  const bool stays = mine && ahead < p.top_groups;
+  const unsigned kept = __ballot_sync(kAll, stays && part == 0);
+  bool across = false;  // ... and on the other side
+  for (; close != 0; close &= close - 1) across = across || ((kept >> ((__ffs(close) - 1) * share) & 1u) != 0) != stays;
+  near = __any_sync(kAll, mine && across);
+  return kept;
 }
 
 // Lane j's choice of expert `id` in double precision (softmax: `total` is the sum of exponentials).
@@ -258,13 +262,13 @@ __device__ __noinline__ unsigned groups_kept_exact(const RouteParams& p, int64_t
   return groups_kept<double, kPerLane>(p, v, scratch, magic, share, 0.0, 0.0, near);
 }
 
-// The choice from f32 scores, with doubles only where those do not settle it: experts are picked by their f32
-// choice until the next one is further below the last of the top_k than both scores' errors; where two
-// neighbours are no further apart than that, the picked ones are put in order in double precision.
+// The choice from f32 scores, with doubles only where those do not settle it: the experts that may be among the
+// top_k are those not further below the last of these than both scores' errors; where two neighbours
+// are no further apart than that, all of these are put in order in double precision.  list: 32 entries of this warp.
 // False: more than 32 are that close (route_exact decides).
 // Without a bias the order is that of the logits themselves, which f32 holds exactly.
 template <int kPerLane>
-__device__ __forceinline__ bool route_fast(const RouteParams& p, int64_t row, double* scratch, float& top, int& my_id) {
+__device__ __forceinline__ bool route_fast(const RouteParams& p, int64_t row, double* scratch, uint2* list, float& top, int& my_id) {
   constexpr unsigned kAll = 0xffffffffu;
   const int lane = threadIdx.x & 31;
   const bool by_logit = p.bias == nullptr && p.n_groups == 1;
@@ -273,7 +277,7 @@ __device__ __forceinline__ bool route_fast(const RouteParams& p, int64_t row, do
   top = -INFINITY;
   my_id = -1;
   route_logits<kPerLane>(p, row, x);
-  float bias[kPerLane], largest_bias = 0.0f;
+  float bias[kPerLane];
 #pragma unroll
   for (int i = 0; i < kPerLane; ++i) bias[i] = 0.0f;
   if (p.bias != nullptr) {
@@ -281,11 +285,8 @@ __device__ __forceinline__ bool route_fast(const RouteParams& p, int64_t row, do
     for (int i = 0; i < kPerLane; ++i)
       if (lane + 32 * i < p.experts) bias[i] = p.bias[lane + 32 * i];
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
+    for (int i = 0; i < kPerLane; ++i)
       if (!(bias[i] > -INFINITY)) x[i] = -INFINITY;
-      if (x[i] != -INFINITY) largest_bias = fmaxf(largest_bias, fabsf(bias[i]));
-    }
-    largest_bias = __uint_as_float(__reduce_max_sync(kAll, __float_as_uint(largest_bias)));
   }
   if (!p.sigmoid) {
 #pragma unroll
@@ -309,11 +310,11 @@ __device__ __forceinline__ bool route_fast(const RouteParams& p, int64_t row, do
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) x[i] = x[i] != -INFINITY ? x[i] * inverse + bias[i] : -INFINITY;
   }
-  // How far two f32 choices of a summed size have to be apart.  Scores (at most 1, and at most the choice and the
-  // bias together) are within 5e-6 of themselves (an exponential's argument of up to 60 within 2^-24; below
-  // exp(-60) is `least`), sums within 1.2e-7; twice that for either.
-  const float least = 1e-25f + 4e-5f * fminf(largest_bias, 1.0f);
-  const float slack = 1.1e-5f;
+  // How far two f32 choices of a summed size have to be apart: slack times it, and least.  An exponential is within
+  // |argument| 2^-24 + 2^-22 of itself and a quotient within 2^-22, so scores are within 5e-6 of
+  // themselves (down to exp(-60)), and, being at most 1, within 5e-7; sums are within 2^-24.
+  const float slack = p.bias == nullptr ? 1.1e-5f : 4e-7f;
+  const float least = p.bias == nullptr ? 1e-25f : 2e-6f;
   if (p.n_groups > 1) {
     if (p.n_groups > 32) return false;  // (a group to a lane at least)
     const uint32_t magic = ((1u << 20) + p.experts / p.n_groups - 1) / (p.experts / p.n_groups);
@@ -331,45 +332,92 @@ __device__ __forceinline__ bool route_fast(const RouteParams& p, int64_t row, do
 #pragma unroll
   for (int i = 0; i < kPerLane; ++i) key[i] = order_key(x[i]);
   const uint32_t out = order_key(-INFINITY);
-  float my_value = -INFINITY, last = -INFINITY;  // last: the choice of slot top_k - 1
-  bool apart = true;                             // every pick so far from the one before it
+  // How far a choice has to be below the one before it for their order to be settled.
+  auto settled = [&](float above, float value) {
+    // equal logits are equal; others differ in double precision too, unless it has run out of digits
+    if (by_logit) return above == value || above - value > 1e-8f;
+    return above - value > slack * (fabsf(above) + fabsf(value)) + least;
+  };
+  // ... and, by logit, where scores end at 0 or 1, it has.
+  auto in_range = [&](float value) { return !by_logit || (p.sigmoid ? fabsf(value) < 15.0f : value - top > -600.0f); };
+  bool apart = true;  // every choice of the top_k settled against the next one
   int picked = 0;
-  float before = INFINITY;
-  while (true) {
-    uint32_t best = out;
+  if (p.top_k < 32) {
+    // The lanes' best ones in order: of 32 lanes' maxima the top_k + 1st is no larger than the top_k + 1st
+    // of all.  What is not settled below it is listed (a dozen or so, of top_k 8), ranked by counting.
+    uint32_t most = out;
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) best = max(best, key[i]);
-    best = __reduce_max_sync(kAll, best);
-    if (best == out) break;
-    const float value = key_value(best);
-    bool far;
-    if (by_logit) {
-      // equal logits are equal; others differ in double precision too, unless it has run out of digits:
-      // close to one another, or where scores end at 0 or 1
-      far = before == INFINITY || before == value || before - value > 1e-8f;
-      if (picked < p.top_k && !(p.sigmoid ? fabsf(value) < 15.0f : value - top > -600.0f)) return false;
-    } else {
-      far = picked == 0 || before - value > slack * (fabsf(before) + fabsf(value)) + least;
-    }
-    if (picked >= p.top_k) {  // left out, if it is far enough below the last one in
-      const bool enough = by_logit ? far : last - value > slack * (fabsf(last) + fabsf(value)) + least;
-      if (enough) break;
-      if (picked == 32) return false;
-    }
-    apart = apart && far;
-    uint32_t at = kMaxGroups;
+    for (int i = 0; i < kPerLane; ++i) most = max(most, key[i]);
 #pragma unroll
-    for (int i = kPerLane - 1; i >= 0; --i) at = key[i] == best ? lane + 32 * i : at;
-    at = __reduce_min_sync(kAll, at);
-    if (lane == picked) {
-      my_id = static_cast<int>(at);
-      my_value = value;
-    }
+    for (int size = 2; size <= 32; size *= 2) {
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i)
-      if (at == lane + 32 * i) key[i] = out;
-    before = value;
-    if (++picked == p.top_k) last = value;
+      for (int s = size / 2; s > 0; s /= 2) {
+        const uint32_t other = __shfl_xor_sync(kAll, most, s);
+        const bool larger = ((lane & s) == 0) == ((lane & size) == 0 || size == 32);
+        most = larger ? max(most, other) : min(most, other);
+      }
+    }
+    const float bar = key_value(__shfl_sync(kAll, most, p.top_k));
+    const float low = by_logit ? bar - 1e-8f : bar - (slack * 2.0f * fabsf(bar) + least) * 1.01f;
+    const uint32_t at_least = max(order_key(low), out + 1);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+      const bool in = key[i] >= at_least;
+      const unsigned who = __ballot_sync(kAll, in);
+      const int place = picked + __popc(who & ((1u << lane) - 1u));
+      if (in && place < 32) list[place] = make_uint2(key[i], static_cast<uint32_t>(lane + 32 * i));
+      picked += __popc(who);
+    }
+    if (picked > 32) {
+      picked = 0;
+    } else if (picked > 0) {
+      __syncwarp();
+      const uint2 mine = lane < picked ? list[lane] : make_uint2(0u, 0u);
+      int place = 0;
+      for (int j = 0; j < picked; ++j) {
+        const uint2 other = list[j];
+        place += other.x > mine.x || (other.x == mine.x && other.y < mine.y);
+      }
+      __syncwarp();
+      if (lane < picked) list[place] = mine;
+      __syncwarp();
+      const uint2 sorted = lane < picked ? list[lane] : make_uint2(out, 0u);
+      const float value = key_value(sorted.x);
+      const float next = __shfl_down_sync(kAll, value, 1);
+      if (lane < picked) my_id = static_cast<int>(sorted.y);
+      const bool in = lane < picked && lane < p.top_k;
+      if (!__all_sync(kAll, !in || in_range(value))) return false;
+      apart = __all_sync(kAll, !in || lane + 1 == picked || settled(value, next));
+    }
+  }
+  if (picked == 0) {  // one after another
+    float before = INFINITY, last = INFINITY;  // last: the choice of slot top_k - 1
+    while (true) {
+      uint32_t best = out;
+#pragma unroll
+      for (int i = 0; i < kPerLane; ++i) best = max(best, key[i]);
+      best = __reduce_max_sync(kAll, best);
+      if (best == out) break;
+      const float value = key_value(best);
+      if (picked < p.top_k && !in_range(value)) return false;
+      if (picked >= p.top_k) {  // left out, if it is far enough below the last one in
+        if (by_logit ? settled(before, value) && before != value : settled(last, value)) break;
+        if (by_logit && last == value && before == value) break;  // (equal logits: the lower indices are in)
+        if (picked == 32) return false;
+      }
+      if (picked > 0) apart = apart && settled(before, value);
+      uint32_t at = kMaxGroups;
+#pragma unroll
+      for (int i = kPerLane - 1; i >= 0; --i) at = key[i] == best ? lane + 32 * i : at;
+      at = __reduce_min_sync(kAll, at);
+      if (lane == picked) my_id = static_cast<int>(at);
+#pragma unroll
+      for (int i = 0; i < kPerLane; ++i)
+        if (at == lane + 32 * i) key[i] = out;
+      before = value;
+      if (++picked == p.top_k) last = value;
+    }
   }
   if (!apart) {
     const double total = p.sigmoid ? 1.0 : exact_total(p, row, top);
@@ -399,7 +447,8 @@ __device__ __forceinline__ void route_token(const RouteParams& p, int token, dou
   const int64_t row = static_cast<int64_t>(token) * p.ld;
   float top;
   int my_id;
-  if (!route_fast<kPerLane>(p, row, scratch, top, my_id)) my_id = route_exact<kPerLane>(p, row, scratch);
+  __shared__ uint2 lists[kRouteWarps][32];
+  if (!route_fast<kPerLane>(p, row, scratch, lists[threadIdx.x >> 5], top, my_id)) my_id = route_exact<kPerLane>(p, row, scratch);
 
   // Weights: the chosen experts' scores in double precision.
   const double total = !p.sigmoid && !p.renormalize ? exact_total(p, row, top) : 1.0;
@@ -440,8 +489,15 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RoutePara
 // warp owns a contiguous run), so the sort is stable and its result does not depend on which warp came first.
 
 constexpr int kPlanThreads = 1024;
-constexpr int kPlanRounds = 4;  // 32-pair steps of a warp
+constexpr int kPlanRounds = 4;  // 32-pair steps of a warp: of the only block, or of many; of some blocks one step
 constexpr int kPlanPairs = kPlanThreads * kPlanRounds;
+// Blocks of one step spread the scattered stores of `order` over more SMs (65536 pairs of 256 groups: 12.2 us with
+// 16 blocks, 10.7 with 64; 6148 of 60: 9.0, 6.1); each block reads all blocks' counts, so there are not too many of them.
+__host__ __device__ inline int plan_rounds(int64_t rows) { return rows > kPlanPairs && rows <= 128 * kPlanThreads ? 1 : kPlanRounds; }
+__host__ __device__ inline int64_t plan_blocks(int64_t rows) {
+  const int64_t per = static_cast<int64_t>(kPlanThreads) * plan_rounds(rows);
+  return rows > 0 ? (rows + per - 1) / per : 1;
+}
 
 // The bin of pair q: its group, or `groups` for none.
 __device__ __forceinline__ int plan_bin(const int32_t* ids, int64_t q, int groups) {
@@ -457,8 +513,9 @@ __global__ void __launch_bounds__(kPlanThreads) count_ids_kernel(const int32_t* 
   __shared__ int32_t bins[kMaxGroups + 1];
   for (int g = threadIdx.x; g <= groups; g += kPlanThreads) bins[g] = 0;
   __syncthreads();
-  for (int i = 0; i < kPlanRounds; ++i) {
-    const int64_t q = static_cast<int64_t>(blockIdx.x) * kPlanPairs + i * kPlanThreads + threadIdx.x;
+  const int rounds = plan_rounds(rows);
+  for (int i = 0; i < rounds; ++i) {
+    const int64_t q = (static_cast<int64_t>(blockIdx.x) * rounds + i) * kPlanThreads + threadIdx.x;
     if (q < rows) atomicAdd(&bins[plan_bin(ids, q, groups)], 1);  // (whole numbers: any order gives the same)
   }
   __syncthreads();
@@ -645,13 +702,14 @@ __device__ __forceinline__ void plan_block(const int32_t* ids, int64_t rows, int
   }
 }
 
+template <int kRounds>
 __global__ void __launch_bounds__(kPlanThreads) group_rows_kernel(const int32_t* ids, int64_t rows, int groups,
                                                                   const int32_t* counts, int32_t* offsets,
                                                                   int32_t* order, int4* tiles) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   extern __shared__ int32_t plan_smem[];
-  plan_block<kPlanThreads, kPlanRounds>(ids, rows, groups, counts, offsets, order, tiles, plan_smem);
+  plan_block<kPlanThreads, kRounds>(ids, rows, groups, counts, offsets, order, tiles, plan_smem);
 }
 
 // Few tokens: routing and plan in one launch of one block.

@@ -153,7 +153,8 @@ int row_kernels_ready(DeviceState& st) {
     CUDA_TRY(cudaFuncSetAttribute(route_kernel_for(experts), kMost, static_cast<int>(route_smem_bytes(experts, experts))));
     CUDA_TRY(cudaFuncSetAttribute(route_few_kernel_for(experts), kMost, static_cast<int>(route_few_smem_bytes(experts, experts))));
   }
-  CUDA_TRY(cudaFuncSetAttribute(group_rows_kernel, kMost, plan_smem_bytes(kMaxGroups)));
+  CUDA_TRY(cudaFuncSetAttribute(group_rows_kernel<1>, kMost, plan_smem_bytes(kMaxGroups)));
+  CUDA_TRY(cudaFuncSetAttribute(group_rows_kernel<kPlanRounds>, kMost, plan_smem_bytes(kMaxGroups)));
   for (int kind : {kKindMxf8, kKindMxf4})
     for (bool gated : {false, true})
       for (bool two : {false, true}) CUDA_TRY(cudaFuncSetAttribute(grouped_kernel(kind, gated, two), kMost, st.smem_optin));
@@ -177,17 +178,17 @@ int row_kernels_ready(DeviceState& st) {
 
 size_t plan_workspace(int64_t rows, int groups) {
   if (rows <= kPlanPairs) return 0;
-  return static_cast<size_t>((rows + kPlanPairs - 1) / kPlanPairs) * (groups + 1) * sizeof(int32_t);
+  return static_cast<size_t>(plan_blocks(rows)) * (groups + 1) * sizeof(int32_t);
 }
 
 // `counts`: plan_workspace() bytes.
 int launch_plan(const int32_t* ids, int64_t rows, int groups, int32_t* offsets, int32_t* order,
                 int32_t* counts, int4* tiles, cudaStream_t stream) {
-  const unsigned blocks = static_cast<unsigned>(std::max<int64_t>(1, (rows + kPlanPairs - 1) / kPlanPairs));
+  const unsigned blocks = static_cast<unsigned>(plan_blocks(rows));
   if (blocks > 1) {
     if (int rc = launch_after(count_ids_kernel, dim3(blocks), kPlanThreads, 0, stream, ids, rows, groups, counts)) return rc;
   }
-  return launch_after(group_rows_kernel, dim3(blocks), kPlanThreads, static_cast<size_t>(plan_smem_bytes(groups)), stream, ids, rows, groups,
+  return launch_after(plan_rounds(rows) == 1 ? group_rows_kernel<1> : group_rows_kernel<kPlanRounds>, dim3(blocks), kPlanThreads, static_cast<size_t>(plan_smem_bytes(groups)), stream, ids, rows, groups,
                       static_cast<const int32_t*>(blocks > 1 ? counts : nullptr), offsets, order, tiles);
 }
 

@@ -144,7 +144,7 @@ def test_route_padded_rows_and_no_plan(gpu):
 
 
 @pytest.mark.parametrize("rows,groups", [(0, 5), (1, 1), (31, 3), (1000, 64), (4096, 1024), (4097, 7), (30000, 255),
-                                         (70000, 1023)])
+                                         (70000, 1023), (131072, 3), (131073, 37)])
 def test_group_rows(gpu, rows, groups):
     ids = W.rng_for(rows, 6).integers(-2, groups + 2, rows).astype(np.int32)
     offsets = torch.full((groups + 1,), -7, dtype=torch.int32, device="cuda")
