@@ -36,6 +36,8 @@ struct RowCall {
     t_tm_cache = st->tm_cache;
     stream = d.stream ? static_cast<cudaStream_t>(d.stream) : st->stream;
     async = (d.flags & CPUOPS_B200_FLAG_ASYNC) != 0;
+    // (a synchronous call ends with a wait, which would end the capture)
+    if (!async && stream_is_capturing(stream)) return refuse("a call on a stream that is being captured needs FLAG_ASYNC");
     return row_kernels_ready(*st);
   }
   // Every pointer given (nulls apart) is this device's memory.
@@ -366,7 +368,7 @@ int gemm_grouped_call(const cpuops_b200_gemm_grouped_desc* d) {
   if (!d->a || !d->b || !d->a_scales || !d->b_scales || !d->offsets || !d->order || !d->d || (summed && !d->ids))
     return refuse("gemm_grouped: a buffer is missing");
   const int64_t n_b = d->gated ? 2 * static_cast<int64_t>(n) : n;
-  const int blocks32 = (k + 31) / 32;
+  const int blocks32 = static_cast<int>((static_cast<int64_t>(k) + 31) / 32);
   if (d->lda < k || d->ldb < k || d->ld_scales_a < blocks32 || d->ld_scales_b < blocks32 || d->ldd < n ||
       d->b_group_rows < n_b)
     return refuse("gemm_grouped: a leading dimension (or b_group_rows) is too small");
@@ -404,7 +406,7 @@ int gemm_grouped_call(const cpuops_b200_gemm_grouped_desc* d) {
   p.a_rows = d->a_rows;
   p.pairs_per_a_row = d->pairs_per_a_row;
   const int ka = kind == kKindMxf4 ? 2 : 1;
-  p.k_blocks = (k + (kind == kKindMxf4 ? 255 : 127)) / (kind == kKindMxf4 ? 256 : 128);
+  p.k_blocks = static_cast<int>((static_cast<int64_t>(k) + (kind == kKindMxf4 ? 255 : 127)) / (kind == kKindMxf4 ? 256 : 128));
   p.kblocks32 = blocks32;
   const GroupedChoice choice = choose_grouped(st, rows, n, groups, p.k_blocks, ka, d->gated != 0);
   p.BN = choice.BN;
@@ -568,6 +570,7 @@ int adapters_call(const cpuops_b200_adapters_desc* d) {
   }
   if (d->m < 0 || d->n < 0 || d->k < 0 || d->rank < 0 || d->adapters < 0) return CPUOPS_B200_STATUS_INVALID_PROBLEM;
   if (d->m == 0 || d->n == 0) return CPUOPS_B200_STATUS_SUCCESS;
+  if (d->n > (1 << 30) || d->k > (1 << 30)) return refuse("adapters: n and k are at most 2^30");
   if (d->rank > kMaxRank) {
     set_error("adapters: rank %d, at most %d is supported", d->rank, kMaxRank);
     return CPUOPS_B200_STATUS_UNSUPPORTED;

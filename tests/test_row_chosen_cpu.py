@@ -104,6 +104,7 @@ def test_grouped_refuses(lib, change, status):
     (dict(ids=None), S.kErrorInvalidArguments), (dict(c=None), S.kErrorInvalidArguments), (dict(d=None), S.kErrorInvalidArguments),
     (dict(ldx=31), S.kErrorInvalidArguments), (dict(lda=31), S.kErrorInvalidArguments), (dict(ldb=7), S.kErrorInvalidArguments),
     (dict(ldc=15), S.kErrorInvalidArguments), (dict(ldd=15), S.kErrorInvalidArguments), (dict(a_stride=-1), S.kErrorInvalidArguments),
+    (dict(k=(1 << 30) + 1, ldx=(1 << 30) + 1, lda=(1 << 30) + 1), S.kErrorInvalidArguments),
     (dict(d=BASE, ldd=20), S.kErrorInvalidArguments)])
 def test_adapters_refuse(lib, change, status):
     assert adapters(**change) == status

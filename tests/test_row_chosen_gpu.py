@@ -680,3 +680,80 @@ def test_host_memory_is_refused(gpu):
     out = torch.zeros(4, dtype=torch.int32, device="cuda")
     st = op(op.Arguments(4, 2, ids, c.RowPlan(out, out)))
     assert st == c.Status.kErrorInvalidArguments and "device memory" in _capi.last_error()
+
+
+def test_synchronous_call_under_capture_is_refused(gpu):
+    """... and leaves the capture as it is."""
+    stream = torch.cuda.Stream()
+    ids = torch.zeros(4, dtype=torch.int32, device="cuda")
+    offsets = torch.zeros(3, dtype=torch.int32, device="cuda")
+    order = torch.zeros(4, dtype=torch.int32, device="cuda")
+    sync = c.GroupRows(stream=stream.cuda_stream)
+    queued = c.GroupRows(stream=stream.cuda_stream, asynchronous=True)
+    args = sync.Arguments(4, 2, ids, c.RowPlan(offsets, order))
+    check(sync(args))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        assert sync(args) == c.Status.kErrorInvalidArguments
+        check(queued(args))
+    ids.fill_(1)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert offsets.tolist() == [0, 0, 4] and order.tolist() == [0, 1, 2, 3]
+
+
+def test_calls_from_threads_on_their_own_streams(gpu):
+    """Workspaces belong to streams: calls of several threads do not meet in one."""
+    import threading
+    jobs = []
+    for t in range(4):
+        e = Experts(E4, E4, 600 + 30 * t, 200 + 64 * t, 256, 3 + t, share=3, seed=20 + t)
+        stream = torch.cuda.Stream()
+        want = e.run(weighted=True, summed=3).clone()
+        jobs.append((e, stream, want, torch.empty_like(want)))
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(e, stream, want, D):
+        op = c.GemmMxGrouped(stream=stream.cuda_stream, asynchronous=True)
+        e.args.ref_D = c.TensorRef(D, e.n)
+        desc = op.describe(e.args)
+        for _ in range(50):
+            if op.run(desc) != OK:
+                bad.append(_capi.last_error())
+        if c.stream_status(stream.cuda_stream) != OK:
+            bad.append("stream status")
+
+    threads = [threading.Thread(target=work, args=job) for job in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not bad
+    for e, stream, want, D in jobs:
+        assert torch.equal(want, D)
+
+
+def test_memory_space_given(gpu):
+    """With MEM_DEVICE the pointers are taken as they are."""
+    ids = dev(np.array([1, 0, 1, -1], np.int32))
+    offsets = torch.zeros(3, dtype=torch.int32, device="cuda")
+    order = torch.zeros(4, dtype=torch.int32, device="cuda")
+    op = c.GroupRows(memory_space=_capi.MEM_DEVICE, device=0)
+    check(op(op.Arguments(4, 2, ids, c.RowPlan(offsets, order))))
+    assert offsets.tolist() == [0, 1, 3] and order.tolist() == [1, 0, 2, -1]
+
+
+@pytest.mark.parametrize("budget", [1000])
+def test_waits_have_time_in_a_long_call(gpu, lib, budget):
+    """The bounded waits of the experts' kernel are for a stage, not for the call: a budget of a
+    millisecond is enough for one that takes longer."""
+    e = Experts(E4, E4, 3000, 2048, 2048, 24, seed=30)
+    want = e.run().clone()
+    try:
+        lib.cpuops_b200_set_wait_budget_us(budget)
+        assert torch.equal(want, e.run())
+    finally:
+        lib.cpuops_b200_set_wait_budget_us(0)
