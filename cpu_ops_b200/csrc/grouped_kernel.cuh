@@ -509,6 +509,7 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
     const uint32_t stage_w = staging_base + static_cast<uint32_t>(r) * 16u + static_cast<uint32_t>(set * kFetchAhead) * kStagingSlot;
     // (BN need not reach 128 or 256: threads beyond it have no slot)
     const bool slot0 = r < BN, slot1 = r + 128 < BN;
+    const bool aligned = p.align_w == 16 && p.align_x == 16;
     int f_it = 0, f_kb = 0;
     const uint8_t *f_w[kTiles], *f_x0 = nullptr, *f_x1 = nullptr;  // rows of the item being fetched, or null
     int next0 = x_pair(0, r), next1 = slot1 ? x_pair(0, r + 128) : -1;  // of the item entered next
@@ -543,12 +544,28 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
         const int col = (f_kb * kSfBytes) & ~15;
         const int valid = min(16, p.kblocks32 - col);
         const uint32_t dst = stage_w + slot * kStagingSlot;
+        if (aligned) {
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + t * kTileM * 16u),
+                         "l"(f_w[t] != nullptr ? f_w[t] + col : p.sw), "r"(f_w[t] != nullptr ? valid : 0)
+                         : "memory");
+          if (slot0)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + x_slot),
+                         "l"(f_x0 != nullptr ? f_x0 + col : p.sx), "r"(f_x0 != nullptr ? valid : 0)
+                         : "memory");
+          if (slot1)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + x_slot + kTileM * 16u),
+                         "l"(f_x1 != nullptr ? f_x1 + col : p.sx), "r"(f_x1 != nullptr ? valid : 0)
+                         : "memory");
+        } else {
 #pragma unroll
         for (int t = 0; t < kTiles; ++t)
           fetch_scales(dst + t * kTileM * 16u, f_w[t] != nullptr ? f_w[t] + col : p.sw, f_w[t] != nullptr ? valid : 0, p.align_w);
         if (slot0) fetch_scales(dst + x_slot, f_x0 != nullptr ? f_x0 + col : p.sx, f_x0 != nullptr ? valid : 0, p.align_x);
         if (slot1)
           fetch_scales(dst + x_slot + kTileM * 16u, f_x1 != nullptr ? f_x1 + col : p.sx, f_x1 != nullptr ? valid : 0, p.align_x);
+        }
         f_kb += kUnitsPerChunk;
         if (f_kb >= p.k_blocks) {
           f_kb = 0;
@@ -581,6 +598,62 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
         asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                      : "=r"(cx1.x), "=r"(cx1.y), "=r"(cx1.z), "=r"(cx1.w)
                      : "r"(from + x_slot + kTileM * 16u));
+      if (in_chunk == kUnitsPerChunk && run == 0) {
+        // the usual case, a whole chunk of two whole runs, without the bookkeeping of the general one below
+        int s1 = s;
+        uint32_t ph1 = ph;
+        if (set == 1) {
+          s1 += kRun;
+          if (s1 >= stages) { s1 -= stages; ph1 ^= 1u; }
+        }
+        const int first_s = s1;
+#pragma unroll
+        for (int u = 0; u < kRun; ++u) {
+          if (!__all_sync(kAll, mbar_wait_bounded(empty_bar(s1), ph1 ^ 1u, abort_flag, budget_ns))) alive = false;
+          if (!alive) break;
+          const uint32_t aw = atom_base + s1 * atom_bytes + slot_off, ax = aw + kTiles * kKa * 512u;
+#pragma unroll
+          for (int a = 0; a < kKa; ++a) {
+            const int lo = u * kKa + a, hi = lo + kRun * kKa;  // this set's word: one of two
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+              asm volatile("st.shared.u32 [%0], %1;" ::"r"(aw + 512u * (t * kKa + a)),
+                           "r"(set == 0 ? pick_word(cw[t], lo) : pick_word(cw[t], hi))
+                           : "memory");
+            asm volatile("st.shared.u32 [%0], %1;" ::"r"(ax + 512u * (a * x_halves)),
+                         "r"(set == 0 ? pick_word(cx0, lo) : pick_word(cx0, hi))
+                         : "memory");
+            if (x_halves == 2)
+              asm volatile("st.shared.u32 [%0], %1;" ::"r"(ax + 512u * (a * 2 + 1)),
+                           "r"(set == 0 ? pick_word(cx1, lo) : pick_word(cx1, hi))
+                           : "memory");
+          }
+          if (++s1 == stages) { s1 = 0; ph1 ^= 1u; }
+        }
+        if (!alive) {
+          if (lane == 0) {
+            leave_error(p.error, kErrProducerWait);
+            *abort_flag = 1;
+          }
+          break;
+        }
+        fence_proxy_async_shared_cta();
+        __syncwarp();
+        if (lane < kRun) {
+          const int mine = first_s + lane;
+          mbar_arrive(full_bar(mine >= stages ? mine - stages : mine));
+        }
+        s += kUnitsPerChunk;
+        while (s >= stages) { s -= stages; ph ^= 1u; }
+        fetch(c_slot);
+        if (++c_slot == kFetchAhead) c_slot = 0;
+        kb += kUnitsPerChunk;
+        if (kb == p.k_blocks) {
+          kb = 0;
+          ++it;
+        }
+        continue;
+      }
       int first_s = s, pending = 0;  // stages written and not yet handed over
       for (int u = 0; u < in_chunk; ++u) {
         if (run / kRun == set) {
