@@ -378,9 +378,15 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
       const bool second = item.count > BN / 2;
       const uint32_t bytes = p.sorted ? static_cast<uint32_t>(BN / 2 * 128 * (second ? 2 : 1))
                                       : static_cast<uint32_t>((item.count + 3) >> 2) * 512u;
-      for (int kb = 0; kb < p.k_blocks; ++kb) {
-        if (turn == warp - 10) {
-          if (!__all_sync(kAll, mbar_wait_bounded(empty_bar(s), ph ^ 1u, abort_flag, budget_ns))) {
+      for (int kb = 0; kb < p.k_blocks; kb += 2) {
+        // of two k-blocks the first or the second is this warp's (the second may not be there)
+        const bool later = turn != warp - 10;
+        int mine_s = s;
+        uint32_t mine_ph = ph;
+        if (later && ++mine_s == stages) { mine_s = 0; mine_ph ^= 1u; }
+        const int x_kb = kb + (later ? 1 : 0);
+        if (x_kb < p.k_blocks) {
+          if (!__all_sync(kAll, mbar_wait_bounded(empty_bar(mine_s), mine_ph ^ 1u, abort_flag, budget_ns))) {
             if (el) {
               leave_error(p.error, kErrProducerWait);
               *abort_flag = 1;
@@ -388,22 +394,24 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
             alive = false;
             break;
           }
-          mbar_expect_tx_p(full_bar(s), bytes, el);
-          const uint32_t x_base = smem_base + s * stage_bytes + kWBytes;
+          mbar_expect_tx_p(full_bar(mine_s), bytes, el);
+          const uint32_t x_base = smem_base + mine_s * stage_bytes + kWBytes;
           if (p.sorted) {
-            tma_load_2d_g<false>(x_base, &tmX, full_bar(s), kb * 128, item.p0, el);
-            tma_load_2d_g<false>(x_base + BN / 2 * 128, &tmX, full_bar(s), kb * 128, item.p0 + BN / 2, second ? el : 0u);
+            tma_load_2d_g<false>(x_base, &tmX, full_bar(mine_s), x_kb * 128, item.p0, el);
+            tma_load_2d_g<false>(x_base + BN / 2 * 128, &tmX, full_bar(mine_s), x_kb * 128, item.p0 + BN / 2, second ? el : 0u);
           } else {
             __syncwarp();  // (the bytes are announced before any can arrive)
             const uint32_t dst = x_base + static_cast<uint32_t>(lane) * 512u;
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-              if (mine[h])
-                tma_gather4(dst + h * 128u * 128u, &tmX, full_bar(s), kb * 128, row[h][0], row[h][1], row[h][2], row[h][3]);
+            if (mine[0])
+              tma_gather4(dst, &tmX, full_bar(mine_s), x_kb * 128, row[0][0], row[0][1], row[0][2], row[0][3]);
+            if (mine[1])
+              tma_gather4(dst + 128u * 128u, &tmX, full_bar(mine_s), x_kb * 128, row[1][0], row[1][1], row[1][2], row[1][3]);
           }
         }
-        turn ^= 1;
-        if (++s == stages) { s = 0; ph ^= 1u; }
+        const int done = min(2, p.k_blocks - kb);
+        turn = (turn + done) & 1;
+        s += done;
+        if (s >= stages) { s -= stages; ph ^= 1u; }
       }
     }
     if (*abort_flag != 0) {
