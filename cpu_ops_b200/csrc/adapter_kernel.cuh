@@ -289,6 +289,18 @@ __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, int by
     asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(bytes), "n"(kBytes) : "memory");
   }
 }
+// Such a piece by plain loads, and its way into shared memory.
+template <typename T>
+__device__ __forceinline__ uint4 load_piece(const T* row, int i, int left) {
+  constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+  __align__(16) T v[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) v[j] = j < left ? row[i + j] : T(0.0f);
+  return *reinterpret_cast<const uint4*>(v);
+}
+__device__ __forceinline__ void store_piece(uint32_t dst, const uint4& w) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
+}
 template <typename T>
 __device__ __forceinline__ void fill_piece(uint32_t dst, const T* row, int i, int left, int align) {
   constexpr int kPer = 16 / static_cast<int>(sizeof(T));
@@ -304,11 +316,7 @@ __device__ __forceinline__ void fill_piece(uint32_t dst, const T* row, int i, in
 #pragma unroll
     for (int j = 0; j < 16; j += 4) copy_async<4>(dst + j, from + (bytes > j ? j : 0), min(4, max(0, bytes - j)));
   } else {
-    __align__(16) T v[kPer];
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) v[j] = j < valid ? row[i + j] : T(0.0f);
-    const uint4 w = *reinterpret_cast<const uint4*>(v);
-    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
+    store_piece(dst, load_piece<T>(row, i, valid));
   }
 }
 
@@ -362,6 +370,32 @@ __global__ void __launch_bounds__(128) adapter_down_kernel(const AdapterTilePara
   }
   auto fill = [&](int stage, int k) {
     const uint32_t xs = base + stage * kStage, as = xs + kXBytes;
+    if (!kWide && align == 2) {
+      // rows on odd elements: all of this thread's pieces are loaded before the first is stored (piece by piece
+      // a stage took eight memory latencies: 8192 rows, rank 64, 2000 x 2000, bf16 157 us, 138 so, f32 267, 184)
+      uint4 vx[kXTurns], va[kATurns];
+#pragma unroll
+      for (int i = 0; i < kXTurns; ++i) {
+        const int at = k + (tid + 128 * i) % kXPieces * (16 / static_cast<int>(sizeof(X)));
+        vx[i] = load_piece<X>(xrow[i], at, xrow[i] ? k1 - at : 0);
+      }
+#pragma unroll
+      for (int i = 0; i < kATurns; ++i) {
+        const int at = k + ((tid + 128 * i) & 7) * 8;
+        va[i] = load_piece<W>(arow[i], at, arow[i] ? k1 - at : 0);
+      }
+#pragma unroll
+      for (int i = 0; i < kXTurns; ++i) {
+        const int piece = tid + 128 * i, r = piece / kXPieces, c = piece % kXPieces;
+        store_piece(xs + r * (kXPieces * 16) + ((c ^ (r & 7)) << 4), vx[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < kATurns; ++i) {
+        const int piece = tid + 128 * i, j = piece >> 3, c = piece & 7;
+        store_piece(as + j * 128 + ((c ^ (j & 7)) << 4), va[i]);
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < kXTurns; ++i) {
       const int piece = tid + 128 * i, r = piece / kXPieces, c = piece % kXPieces;
