@@ -348,7 +348,9 @@ CPUOPS_B200_API int cpuops_b200_group_rows(const cpuops_b200_group_rows_desc* de
  *     D[q]   = y       if pairs_per_d_row == 1 (rows of pairs in no group are left as they were)
  *     D[t]   = the sum of y over t's pairs_per_d_row pairs, ascending, otherwise (pairs in no group
  *              add nothing; a row without any is zero).  `ids` are then the ids the plan was
- *              made from, and the call uses the stream's workspace (rows * n floats).
+ *              made from.
+ * Uses the stream's workspace when it sums (rows * n floats) and when there are 48 pairs per group
+ * or more (their rows of A in the plan's order).
  * B_g is n (gated: 2n, the gate's rows first) rows of k, the first of them row g * b_group_rows
  * of B.  A and B: 16-byte aligned, rows a multiple of 16 bytes apart, an even k for e2m1.  A
  * and B may both be 8-bit formats, both e2m1, or e2m1 weights under 8-bit rows (then B 32-byte
@@ -387,7 +389,8 @@ CPUOPS_B200_API int cpuops_b200_gemm_grouped(const cpuops_b200_gemm_grouped_desc
  * adapters a_stride elements apart), B_g n rows of `rank` (ldb, b_stride).  An adapter of a smaller
  * rank is padded with zeros.  X may be f32 with A and B f16 or bf16, or all three the same
  * 16-bit type; C, D and every sum are f32.  D may be C.  16-byte aligned rows of X, A and B are read
- * fastest.  Uses the stream's workspace from a few hundred rows on. */
+ * fastest.  n and k are at most 2^30.  Uses the stream's workspace where rows are taken in tiles sorted by
+ * adapter, which an estimate of both times decides (a few hundred rows and more). */
 typedef struct cpuops_b200_adapters_desc {
   uint32_t struct_size;
   int32_t m, n, k, rank, adapters;
