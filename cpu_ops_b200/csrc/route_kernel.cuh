@@ -310,11 +310,21 @@ __device__ __forceinline__ bool route_fast(const RouteParams& p, int64_t row, do
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) x[i] = x[i] != -INFINITY ? x[i] * inverse + bias[i] : -INFINITY;
   }
-  // How far two f32 choices of a summed size have to be apart: slack times it, and least.  An exponential is within
-  // |argument| 2^-24 + 2^-22 of itself and a quotient within 2^-22, so scores are within 5e-6 of
-  // themselves (down to exp(-60)), and, being at most 1, within 5e-7; sums are within 2^-24.
+  // How far two f32 choices of a summed size have to be apart: slack times it, and least.  u = 2^-24 below.
+  // An exponential is within (2 + 1.173 |argument|) 2u of itself (CUDA's bound for __expf), the rounding of
+  // an argument of size a moves it by another a u (a < 64: by 2^-19 at most), a quotient is within 4u.
+  //   No bias: a softmax's quotient is common to all of a token's scores, so it does not count.  Down to
+  //   1e-25 = exp(-57.6), below which `least` holds, a score is within 139 u + 32 u + 2 u = 1.03e-5 of itself.
+  //   Bias, softmax: scores are at most 1, and so is the sum of those compared.  The total is common to
+  //   them: it counts once, for their difference.  Its terms' errors: at most 5 2u = 5.9e-7 of a largest score
+  //   (2 + 1.67 sum of p_j |argument j|, which with 1024 experts is below 1.77 of it); its sum, kPerLane numbers
+  //   one after another and five steps across the lanes: kPerLane + 4 roundings; the quotient 2.4e-7.
+  //   The exponentials of the scores themselves: 2.5 2u = 2.9e-7, of four scores of two groups 3.0 2u; the products
+  //   6e-8.  Together 1.26e-6 + (kPerLane + 4) u.
+  //   Bias, sigmoid: s (1 - s) (2 + 1.173 |argument|) 2u + 5u, together 3.8e-7 for each score, which is less.
+  //   The sum with the bias: u of the choice, which slack covers.
   const float slack = p.bias == nullptr ? 1.1e-5f : 4e-7f;
-  const float least = p.bias == nullptr ? 1e-25f : 2e-6f;
+  const float least = p.bias == nullptr ? 1e-25f : 1.3e-6f + static_cast<float>(kPerLane + 5) * 6e-8f;
   if (p.n_groups > 1) {
     if (p.n_groups > 32) return false;  // (a group to a lane at least)
     const uint32_t magic = ((1u << 20) + p.experts / p.n_groups - 1) / (p.experts / p.n_groups);
