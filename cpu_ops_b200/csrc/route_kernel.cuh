@@ -177,8 +177,8 @@ __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(
 
 // Which groups stay, in the precision of T: bit g * share of the result, share lanes to a group (n_groups <=
 // 32).  `v`: a lane's choices (-inf: out); scratch: experts + n_groups numbers of this warp.  `near`: the
-// last group that stays and the first that does not are no further apart than `slack` times their size and
-// `least`.
+// last group that stays and the first that does not are no further apart than `slack` times the sizes of the
+// choices in them (a group's two may cancel: its score may be far smaller than their roundings) and `least`.
 template <typename T, int kPerLane>
 __device__ __forceinline__ unsigned groups_kept(const RouteParams& p, const T (&v)[kPerLane], T* scratch, uint32_t magic,
                                                 int share, T slack, T least, bool& near) {
@@ -210,15 +210,16 @@ __device__ __forceinline__ unsigned groups_kept(const RouteParams& p, const T (&
     second = most < less ? less : most;
     best = best < b2 ? b2 : best;
   }
-  const T score = p.group_best == 2 && second != kOut ? best + second : best;
+  const bool both = p.group_best == 2 && second != kOut;
+  const T score = both ? best + second : best;
+  const T reach = slack * ((best < 0 ? -best : best) + (both ? second < 0 ? -second : second : T(0)));
   int ahead = 0;
   unsigned close = 0;  // groups that are no further away
   for (int j = 0; j < p.n_groups; ++j) {
-    const T other = __shfl_sync(kAll, score, j * share);
+    const T other = __shfl_sync(kAll, score, j * share), other_reach = __shfl_sync(kAll, reach, j * share);
     ahead += other > score || (other == score && j < g);
-    const T size = (other < 0 ? -other : other) + (score < 0 ? -score : score);
     const T gap = other < score ? score - other : other - score;
-    if (other != kOut && score != kOut && !(gap > slack * size + least)) close |= 1u << j;
+    if (other != kOut && score != kOut && !(gap > reach + other_reach + least)) close |= 1u << j;
   }
   const bool stays = mine && ahead < p.top_groups;
   const unsigned kept = __ballot_sync(kAll, stays && part == 0);

@@ -27,3 +27,15 @@ def test_route_softmax_sum_that_loses_its_small_terms(gpu):
     bias[37] = np.float32(-2.08e-6)
     check_route(dev(x), "f32", 1, bias=bias)
     check_route(dev(x), "f32", 2, bias=bias, n_groups=16, top_groups=2)
+
+
+def test_route_groups_whose_two_best_cancel(gpu):
+    """A group's two best choices are +100 and -100 and a little: each is rounded to 8e-6 in f32, their sum is
+    below one."""
+    rng = W.rng_for(2000, 9)
+    x = rng.standard_normal((2000, 8)).astype(np.float32)
+    x[:, 4:] = x[:, :4]
+    x[:, 4:6] += (4e-5 * (2 * rng.random((2000, 2)) - 1)).astype(np.float32)
+    bias = np.array([100, -100, -np.inf, -np.inf] * 2, np.float32)
+    for sigmoid in (False, True):
+        check_route(dev(x), "f32", 1, bias=bias, sigmoid=sigmoid, n_groups=2, top_groups=1, group_best=2)
