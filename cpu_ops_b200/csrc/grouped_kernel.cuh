@@ -852,6 +852,17 @@ __global__ void __launch_bounds__(256) gather_rows_kernel(const uint8_t* a, int6
   }
 }
 
+// Zeros in the rows of D whose only pair is in no group.  A warp for every row in turn.
+__global__ void __launch_bounds__(256) zero_rows_kernel(const int32_t* ids, int groups, int rows, int n, float* d, int64_t ldd) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (int64_t row = blockIdx.x * 8 + (threadIdx.x >> 5); row < rows; row += gridDim.x * 8) {
+    const int id = ids[row];
+    if (id >= 0 && id < groups) continue;
+    for (int64_t col = threadIdx.x & 31; col < n; col += 32) d[row * ldd + col] = 0.0f;
+  }
+}
+
 // D[t] = the sum of row t's `per` pairs, ascending; pairs in no group add nothing.
 __global__ void __launch_bounds__(256) sum_pairs_kernel(const float* pairs, const int32_t* ids, int groups, int per,
                                                         int64_t rows, int n, float* d, int64_t ldd) {

@@ -425,6 +425,14 @@ int gemm_grouped_call(const cpuops_b200_gemm_grouped_desc* d) {
   p.wait_budget_us = g_wait_budget_us.load();
   p.error = st.error_dev;
 
+  const int64_t most_items = (static_cast<int64_t>(std::min(groups, rows)) + rows / p.BN) * p.tiles;
+  if (most_items > INT32_MAX) return refuse("gemm_grouped: the problem has more tiles than fit 31 bits");
+  const unsigned row_blocks = static_cast<unsigned>(std::min<int64_t>((static_cast<int64_t>(rows) + 7) / 8, 8 * st.sm_count));
+  if (!summed && d->ids) {  // rows without a group are zeros, as in a sum
+    if (int rc = launch_after(zero_rows_kernel, dim3(row_blocks), 256, 0, call.stream, d->ids, groups, rows, n, d->d,
+                              static_cast<int64_t>(d->ldd)))
+      return rc;
+  }
   const int row_bytes = fp4_a ? k / 2 : k;
   const int64_t x_pitch = align_up(row_bytes, 16), sx_pitch = align_up(blocks32, 16);
   Plan plan;
@@ -439,8 +447,7 @@ int gemm_grouped_call(const cpuops_b200_gemm_grouped_desc* d) {
     p.sx = ws + off_sx;
     p.ld_sx = sx_pitch;
     p.align_x = 16;
-    const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((static_cast<int64_t>(rows) + 7) / 8, 8 * st.sm_count));
-    if (int rc = launch_after(gather_rows_kernel, dim3(blocks), 256, 0, call.stream, static_cast<const uint8_t*>(d->a), a_pitch,
+    if (int rc = launch_after(gather_rows_kernel, dim3(row_blocks), 256, 0, call.stream, static_cast<const uint8_t*>(d->a), a_pitch,
                               static_cast<const uint8_t*>(d->a_scales), static_cast<int64_t>(d->ld_scales_a), d->order, rows,
                               d->a_rows, d->pairs_per_a_row, row_bytes, blocks32, ws + off_x, x_pitch, ws + off_sx, sx_pitch))
       return rc;
@@ -448,8 +455,6 @@ int gemm_grouped_call(const cpuops_b200_gemm_grouped_desc* d) {
   p.d = summed ? reinterpret_cast<float*>(ws + off_sum) : d->d;
   p.ldd = summed ? n : d->ldd;
 
-  const int64_t most_items = (static_cast<int64_t>(std::min(groups, rows)) + rows / p.BN) * p.tiles;
-  if (most_items > INT32_MAX) return refuse("gemm_grouped: the problem has more tiles than fit 31 bits");
   if (groups > 0) {
     CUtensorMap tmW, tmX;
     const uint32_t box = d->gated && !choice.two ? 16 : 128;

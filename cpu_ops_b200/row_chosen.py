@@ -110,7 +110,8 @@ class GroupRowsArguments:
 @dataclass
 class GemmGroupedArguments:
     """``ref_B`` covers all groups; group g starts at its row ``g * b_group_rows`` (0: the rows
-    of one group).  ``a_rows`` 0: as many as the pairs need."""
+    of one group).  ``a_rows`` 0: as many as the pairs need.  With ``ids`` (those of the plan; needed
+    where ``pairs_per_d_row`` > 1) rows of D without a group become zeros, without they are left."""
     problem_size: GroupedCoord = field(default_factory=GroupedCoord)
     ref_A: MxTensorRef = field(default_factory=MxTensorRef)
     ref_B: MxTensorRef = field(default_factory=MxTensorRef)

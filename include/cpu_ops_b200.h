@@ -345,10 +345,11 @@ CPUOPS_B200_API int cpuops_b200_group_rows(const cpuops_b200_group_rows_desc* de
  *     acc[j] = sum_k A[q / pairs_per_a_row][k] * B_g[j][k]                 (f32 sums)
  *     y[j]   = acc[j],  or  silu(acc[j]) * acc[n + j]  with `gated`
  *     y[j]  *= row_weights[q]                                              (if given)
- *     D[q]   = y       if pairs_per_d_row == 1 (rows of pairs in no group are left as they were)
+ *     D[q]   = y       if pairs_per_d_row == 1; rows of pairs in no group are zeros if `ids` are given
+ *              (a layer with one expert per row), and left as they were if they are NULL
  *     D[t]   = the sum of y over t's pairs_per_d_row pairs, ascending, otherwise (pairs in no group
- *              add nothing; a row without any is zero).  `ids` are then the ids the plan was
- *              made from.
+ *              add nothing; a row without any is zero); `ids` are needed then
+ * `ids` are the ids the plan was made from.
  * Uses the stream's workspace when it sums (rows * n floats) and when there are 48 pairs per group
  * or more (their rows of A in the plan's order).
  * B_g is n (gated: 2n, the gate's rows first) rows of k, the first of them row g * b_group_rows
@@ -373,7 +374,7 @@ typedef struct cpuops_b200_gemm_grouped_desc {
   const void* b_scales;
   const int32_t* offsets;     /* groups + 1                                  */
   const int32_t* order;       /* rows                                        */
-  const int32_t* ids;         /* rows; pairs_per_d_row > 1 only              */
+  const int32_t* ids;         /* rows, or NULL (pairs_per_d_row == 1 only)   */
   const float* row_weights;   /* rows, or NULL                               */
   float* d;                   /* rows / pairs_per_d_row rows of n, row-major */
   void* stream;
