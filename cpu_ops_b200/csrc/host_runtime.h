@@ -20,6 +20,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <map>
+#include <memory>
 #include <mutex>
 #include <vector>
 
@@ -101,13 +102,17 @@ struct DeviceState {
   // Grow-only workspaces, one per stream that ever called in.  A buffer that was handed to
   // kernels while its stream was being captured into a CUDA graph is never freed (the graph
   // keeps its address); when such a stream later needs more room the old buffer is retired,
-  // not released.
+  // not released.  A handle alone does not say which stream it is: cudaStreamPerThread is another
+  // one in every thread (its workspaces are found by thread too), and a destroyed stream's
+  // handle may come back as a new stream's (told by the stream's id).
   struct Workspace {
     void* ptr = nullptr;
     size_t bytes = 0;
     bool captured = false;
+    unsigned long long stream_id = 0;
+    std::weak_ptr<const uint64_t> thread;  // cudaStreamPerThread: expired once the thread has ended
   };
-  std::map<cudaStream_t, Workspace> ws;
+  std::map<std::pair<cudaStream_t, uint64_t>, Workspace> ws;  // by handle and, if need be, thread number
   std::vector<void*> retired;
   // Host-operand calls are cut into row panels that run on these streams, so that one
   // panel's upload, another's GEMM and a third's download overlap (see gemm_body).
@@ -330,14 +335,70 @@ bool stream_is_capturing(cudaStream_t stream) {
   return cs != cudaStreamCaptureStatusNone;
 }
 
+// A number of the calling thread that no other thread of the process ever has.
+const std::shared_ptr<const uint64_t>& thread_number() {
+  static std::atomic<uint64_t> threads{0};
+  thread_local const std::shared_ptr<const uint64_t> number = std::make_shared<const uint64_t>(threads.fetch_add(1) + 1);
+  return number;
+}
+
+// The entry of the stream that `stream` names.  A workspace whose stream is gone, a destroyed one with the same
+// handle or an ended thread's, is taken over after a wait for the device, whose work may still use it; one
+// that a graph may hold is retired instead.  Under capture nothing can be waited for, and asking for the
+// stream's id would end the capture: the call that has to come before it has settled both.
+int find_workspace(DeviceState& st, cudaStream_t stream, bool capturing, DeviceState::Workspace** out) {
+  const bool per_thread = stream == cudaStreamPerThread;
+  const auto at = st.ws.try_emplace({stream, per_thread ? *thread_number() : 0});
+  DeviceState::Workspace& w = at.first->second;
+  if (per_thread && at.second) w.thread = thread_number();
+  *out = &w;
+  if (capturing) return 0;
+  auto release = [&](DeviceState::Workspace& gone) {  // what a graph may hold of a stream that is gone
+    if (!gone.captured) return;
+    st.retired.push_back(gone.ptr);
+    gone = DeviceState::Workspace{};
+  };
+  if (!per_thread) {
+    unsigned long long id = 0;
+    CUDA_TRY(cudaStreamGetId(stream, &id));
+    if (w.stream_id == id) return 0;
+    release(w);
+    if (w.ptr) CUDA_TRY(cudaDeviceSynchronize());
+    w.stream_id = id;
+    return 0;
+  }
+  if (w.ptr) return 0;
+  for (auto it = st.ws.begin(); it != st.ws.end();) {
+    DeviceState::Workspace& other = it->second;
+    if (it->first.first != stream || !other.thread.expired()) {
+      ++it;
+      continue;
+    }
+    release(other);
+    if (other.ptr) {
+      CUDA_TRY(cudaDeviceSynchronize());
+      if (w.ptr) {
+        CUDA_TRY(cudaFree(other.ptr));
+      } else {
+        w.ptr = other.ptr;
+        w.bytes = other.bytes;
+      }
+    }
+    it = st.ws.erase(it);
+  }
+  return 0;
+}
+
 // The stream's workspace, grown to `bytes` if need be.  While the stream is being captured
 // nothing can be allocated or synchronised: a call that needs more room than the stream's
 // workspace has fails with a message (run the call once outside capture first).  A
 // workspace that was used under capture stays allocated for good, because graphs made
 // from that capture hold its address.
 int ensure_workspace(DeviceState& st, cudaStream_t stream, size_t bytes, uint8_t** out) {
-  DeviceState::Workspace& w = st.ws[stream];
   const bool capturing = stream_is_capturing(stream);
+  DeviceState::Workspace* entry = nullptr;
+  if (int rc = find_workspace(st, stream, capturing, &entry)) return rc;
+  DeviceState::Workspace& w = *entry;
   if (w.bytes < bytes) {
     if (capturing) {
       set_error("this call needs a %zu-byte workspace but the stream being captured has %zu: issue the "

@@ -161,6 +161,9 @@ typedef struct cpuops_b200_gemm_desc {
  * then finds its workspace in place; one that would have to allocate during capture
  * returns CPUOPS_B200_STATUS_INVALID_ARGUMENTS instead).  A workspace used under capture
  * is never freed, so graphs stay valid when later calls on the stream need more room.
+ * Workspaces belong to streams, not to handles: cudaStreamPerThread is a stream of its own in
+ * every thread, and a stream with a destroyed one's handle does not share that one's (that one's
+ * graphs stay valid).
  * Large operands in pageable host memory are copied through 16 MB of pinned memory per
  * device and by up to three threads besides the caller's, both kept until the process
  * ends; the threads take no signals, and from then on the library cannot be unloaded. */

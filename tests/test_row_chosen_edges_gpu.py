@@ -1,14 +1,16 @@
 """Calls of the operators whose weights are chosen per row in which a bound, a mask, an infinity or
 the sharing of a stream decides the result."""
 import math
+import threading
 
 import numpy as np
 import pytest
 import torch
 
 import cpu_ops_b200 as c
-from cpu_ops_b200 import workloads as W
+from cpu_ops_b200 import _capi, workloads as W
 from tests import row_chosen_helpers as H
+from tests.gpu_helpers import MX_TOL, gather, normwise, run_mx_gpu
 from tests.test_row_chosen_gpu import E4, Experts, check, check_route, dev
 
 pytestmark = pytest.mark.gpu
@@ -81,3 +83,143 @@ def test_grouped_one_pair_per_row_with_ids_writes_every_row(gpu, rows, n, k, gro
     # without ids they are left as they were
     D = torch.full((rows, n), 7.5, device="cuda")
     assert (e.run(weighted, D=D).cpu().numpy()[none] == 7.5).all()
+
+
+# ---- workspaces belong to streams, whatever their handles say ------------------------------------
+
+
+PER_THREAD = 2   # cudaStreamPerThread
+
+
+def many_async(jobs, turns, results):
+    """Runs every job's call `turns` times, asynchronously, and its stream's status at the end."""
+    for e, stream, D, op in jobs:
+        e.args.ref_D = c.TensorRef(D, e.n)
+        desc = op.describe(e.args)
+        for _ in range(turns):
+            if op.run(desc) != c.Status.kSuccess:
+                results.append(_capi.last_error())
+        if c.stream_status(stream) != c.Status.kSuccess:
+            results.append("stream status")
+
+
+def expert_job(t, stream):
+    e = Experts(E4, E4, 600 + 30 * t, 200 + 64 * t, 256, 3 + t, share=3, seed=20 + t)
+    want = e.run(weighted=True, summed=3).clone()
+    return e, stream, torch.empty_like(want), c.GemmMxGrouped(stream=stream, asynchronous=True), want
+
+
+def test_the_per_thread_stream_is_another_in_every_thread(gpu):
+    """Threads that all pass cudaStreamPerThread run side by side, each in a workspace of its own."""
+    jobs = [expert_job(t, PER_THREAD) for t in range(4)]
+    torch.cuda.synchronize()
+    for generation in range(3):    # (workspaces of threads that have ended are taken over)
+        for job in jobs:
+            job[2].fill_(float("nan"))
+        torch.cuda.synchronize()
+        bad = []
+        threads = [threading.Thread(target=many_async, args=([job[:4]], 50, bad)) for job in jobs]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        assert not bad
+        for job in jobs:
+            assert torch.equal(job[2], job[4])
+
+
+def test_a_gemm_on_the_per_thread_stream(gpu):
+    """The GEMMs' workspaces are found the same way."""
+    P = W.mx_problem(_capi.FMT_E4M3, 512, 384, 4096, True, seed=3)
+    status, want = run_mx_gpu(P, 1.0, 0.5)
+    assert status == c.Status.kSuccess
+    found = [None] * 4
+
+    def work(i):
+        op = c.GemmMxE4M3(stream=PER_THREAD, asynchronous=True)
+        A, B, SA, SB, C = (dev(x) for x in (P.A, P.B, P.SA, P.SB, P.C))
+        D = torch.empty_like(C)
+        torch.cuda.synchronize()
+        desc = op.describe(op.Arguments(c.GemmCoord(P.m, P.n, P.k), c.MxTensorRef(A, SA, P.lda, P.ldsa),
+                                        c.MxTensorRef(B, SB, P.ldb, P.ldsb), c.TensorRef(C, P.ldc), c.TensorRef(D, P.ldc),
+                                        c.LinearCombination(1.0, 0.5)))
+        ok = all(op.run(desc) == c.Status.kSuccess for _ in range(40)) and c.stream_status(PER_THREAD) == c.Status.kSuccess
+        found[i] = (ok, D.cpu().numpy())
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for ok, D in found:
+        assert ok and normwise(*(gather(x, P.m, P.n, P.ldc, P.c_row_major) for x in (D, want))) <= MX_TOL
+
+
+def test_a_stream_with_a_destroyed_streams_handle(gpu):
+    """Work of a destroyed stream may still run when a new stream has its handle."""
+    runtime = pytest.importorskip("cuda.bindings.runtime")
+    jobs = [expert_job(t, None) for t in range(2)]
+    torch.cuda.synchronize()
+    for turn in range(6):
+        for e, _, D, _, _ in jobs:
+            D.fill_(float("nan"))
+        torch.cuda.synchronize()
+        bad = []
+        for e, _, D, _, _ in jobs:
+            status, stream = runtime.cudaStreamCreateWithFlags(runtime.cudaStreamNonBlocking)
+            assert int(status) == 0
+            op = c.GemmMxGrouped(stream=int(stream), asynchronous=True)
+            e.args.ref_D = c.TensorRef(D, e.n)
+            desc = op.describe(e.args)
+            bad += [_capi.last_error() for _ in range(30) if op.run(desc) != c.Status.kSuccess]
+            assert int(runtime.cudaStreamDestroy(stream)[0]) == 0
+        torch.cuda.synchronize()
+        assert not bad
+        for job in jobs:
+            assert torch.equal(job[2], job[4])
+
+
+def test_capture_on_the_per_thread_stream(gpu):
+    """A captured call keeps its workspace for the graph, and one that has none is refused."""
+    runtime = pytest.importorskip("cuda.bindings.runtime")
+    e, stream, D, op, want = expert_job(1, PER_THREAD)
+    e.args.ref_D = c.TensorRef(D, e.n)
+    desc = op.describe(e.args)
+    torch.cuda.synchronize()
+    seen = {}
+
+    def capture(warm):
+        handle = runtime.cudaStream_t(PER_THREAD)
+        if warm:
+            seen["warm"] = op.run(desc)
+        mode = runtime.cudaStreamCaptureMode.cudaStreamCaptureModeThreadLocal
+        seen["begin"] = int(runtime.cudaStreamBeginCapture(handle, mode)[0])
+        seen["call"] = op.run(desc)
+        status, seen["graph"] = runtime.cudaStreamEndCapture(handle)
+        seen["end"] = int(status)
+
+    for warm in (False, True):
+        t = threading.Thread(target=capture, args=(warm,))
+        t.start()
+        t.join()
+        assert seen["begin"] == 0 and seen["end"] == 0
+        if not warm:
+            assert seen["call"] == c.Status.kErrorInvalidArguments
+    assert seen["warm"] == seen["call"] == c.Status.kSuccess
+    status, graph = runtime.cudaGraphInstantiate(seen["graph"], 0)
+    assert int(status) == 0
+    # the capturing thread has ended: another one must not take the graph's workspace over
+    other = expert_job(2, PER_THREAD)
+    bad = []
+    D.fill_(float("nan"))
+    other[2].fill_(float("nan"))
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    t = threading.Thread(target=many_async, args=([other[:4]], 100, bad))
+    t.start()
+    for _ in range(100):
+        assert int(runtime.cudaGraphLaunch(graph, runtime.cudaStream_t(side.cuda_stream))[0]) == 0
+    t.join()
+    torch.cuda.synchronize()
+    assert not bad and torch.equal(D, want) and torch.equal(other[2], other[4])
