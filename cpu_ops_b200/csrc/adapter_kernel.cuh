@@ -320,6 +320,21 @@ __device__ __forceinline__ void fill_piece(uint32_t dst, const T* row, int i, in
   }
 }
 
+// The product of a factor in f32 (the sum of `parts` arrays `step` apart, times `scale`) and one of 16 bits, not cut
+// into terms.  With an infinity in the 16-bit factor the terms' products may be of either sign or, of a term of
+// zero, NaN, and so may those of a term that is an infinity and others that are beyond f16's range; what came
+// out as NaN is made anew here.
+template <typename W>
+__device__ __noinline__ float whole_product(const float* f, int parts, int64_t step, float scale, const W* w, int count) {
+  float y = 0.0f;
+  for (int j = 0; j < count && y == y; ++j) {
+    float v = 0.0f;
+    for (int s = 0; s < parts; ++s) v += f[s * step + j];
+    y = __fmaf_rn(v * scale, to_f32<W>(w[j]), y);
+  }
+  return y;
+}
+
 struct AdapterTileParams {
   AdapterParams a;
   const int4* tiles;      // {adapter, first place, rows, -}
@@ -496,8 +511,16 @@ __global__ void __launch_bounds__(128) adapter_down_kernel(const AdapterTilePara
 #pragma unroll
     for (int j = 0; j < kRanks / 8; ++j) {
       const int at = rank0 + j * 8 + 2 * (lane & 3);
-      if (at < t.rank_pad)
-        *reinterpret_cast<float2*>(u + static_cast<int64_t>(r) * t.rank_pad + at) = make_float2(sum[j][2 * h] + acc[j][2 * h], sum[j][2 * h + 1] + acc[j][2 * h + 1]);
+      float2 v = make_float2(sum[j][2 * h] + acc[j][2 * h], sum[j][2 * h + 1] + acc[j][2 * h + 1]);
+      if constexpr (sizeof(X) == 4) {
+        if (__builtin_expect(v.x != v.x || v.y != v.y, 0)) {
+          const X* x = static_cast<const X*>(p.x) + t.order[tile.y + r] * p.ldx + k0;
+          const W* a = static_cast<const W*>(p.a) + tile.x * p.a_stride + at * p.lda + k0;
+          if (v.x != v.x && at < p.rank) v.x = whole_product<W>(x, 1, 0, 1.0f, a, k1 - k0);
+          if (v.y != v.y && at + 1 < p.rank) v.y = whole_product<W>(x, 1, 0, 1.0f, a + p.lda, k1 - k0);
+        }
+      }
+      if (at < t.rank_pad) *reinterpret_cast<float2*>(u + static_cast<int64_t>(r) * t.rank_pad + at) = v;
     }
   }
 }
@@ -705,6 +728,24 @@ __global__ void __launch_bounds__(256, 2) adapter_up_kernel(const AdapterTilePar
         for (int j = 0; j < 4; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[j][e] *= row_scale[row0 + g + 8 * (e >> 1)];
+      }
+      float any = 0.0f;  // NaN where one of them is
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) any += acc[j][e];
+      if (__builtin_expect(any != any, 0)) {
+        const float scale = p.scales != nullptr ? p.scales[tile.x] : 1.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = row0 + g + 8 * (e >> 1), col = col0 + half + j * 8 + 2 * i + (e & 1);
+            if (acc[j][e] != acc[j][e] && r < tile.z && col < p.n)
+              acc[j][e] = whole_product<W>(t.u + static_cast<int64_t>(tile.y + r) * t.rank_pad, t.splits,
+                                           static_cast<int64_t>(p.m) * t.rank_pad, scale,
+                                           static_cast<const W*>(p.b) + tile.x * p.b_stride + col * p.ldb, p.rank);
+          }
       }
     }
     // D takes C's place in the stage (a row without an adapter is C itself: no zero is added to it) ...

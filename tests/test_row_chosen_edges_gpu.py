@@ -11,7 +11,7 @@ import cpu_ops_b200 as c
 from cpu_ops_b200 import _capi, workloads as W
 from tests import row_chosen_helpers as H
 from tests.gpu_helpers import MX_TOL, gather, normwise, run_mx_gpu
-from tests.test_row_chosen_gpu import E4, Experts, check, check_route, dev
+from tests.test_row_chosen_gpu import E4, Experts, check, check_route, dev, run_adapters
 
 pytestmark = pytest.mark.gpu
 
@@ -83,6 +83,43 @@ def test_grouped_one_pair_per_row_with_ids_writes_every_row(gpu, rows, n, k, gro
     # without ids they are left as they were
     D = torch.full((rows, n), 7.5, device="cuda")
     assert (e.run(weighted, D=D).cpu().numpy()[none] == 7.5).all()
+
+
+# ---- adapters: infinities ----------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("kx,kw", [("bf16", "bf16"), ("f16", "f16"), ("f32", "bf16"), ("f32", "f16")])
+@pytest.mark.parametrize("m", [6, 4000])
+@pytest.mark.parametrize("where", ["x", "a", "b"])
+def test_adapters_infinities(gpu, kx, kw, m, where):
+    """An infinity reaches what it is multiplied with as the formula says, in few rows as in many (whose factors are
+    multiplied in parts, one of which may be zero or of the other sign)."""
+
+    def spoil(x, A, B, C):
+        if kx == "f32":
+            x *= 1e6            # u beyond f16's range
+            x[:, ::2] = x[:, ::2].bfloat16().float()      # (whose second part is zero)
+        if where == "x":
+            x[2::5, 3] = float("inf")
+            x[1, 7] = -float("inf")
+        elif where == "a":
+            A[1, 2, 5] = float("inf")
+            A[0, 0, 100] = -float("inf")
+        else:
+            B[1, 9, 3] = float("inf")
+            B[0, 130, 0] = -float("inf")
+            B[2, 64:, 7] = float("inf")
+
+    ids = np.arange(m) % 4 - 1
+    before = c.launch_count()
+    with np.errstate(invalid="ignore"):
+        got, want, err, _ = run_adapters(kx, kw, m, 200, 160, 16, 3, ids=ids, spoil=spoil, seed=m)
+    assert (c.launch_count() - before >= 3) == (m > 100)
+    assert not np.isfinite(want).all()
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    finite = np.isfinite(want)
+    assert np.array_equal(got[~finite & ~np.isnan(want)], want[~finite & ~np.isnan(want)])
+    assert np.all(np.abs(got - want)[finite] <= err[finite])
 
 
 # ---- workspaces belong to streams, whatever their handles say ------------------------------------
