@@ -43,6 +43,7 @@ constexpr int kGroupedEpilogueWarp = 12;
 __host__ __device__ constexpr int grouped_threads(bool two) { return 32 * (kGroupedEpilogueWarp + (two ? 8 : 4)); }
 constexpr int kGroupedMaxStages = 8;
 constexpr int kGroupedMaxBN = 192;   // two accumulators and four slots of scales fit tensor memory
+constexpr int kGroupedMaxGathered = 96;  // ... of launches that gather X row by row
 // 16-byte scale chunks that each of the two sets of scale writers has in flight: of two k-blocks for e2m1
 // (ka = 2 atoms), of four else.  (One token, 8 of 64 experts, 2048 x 4096 e2m1: with half as many 13.1 us, so 12.6.)
 __host__ __device__ constexpr int grouped_fetch_ahead(bool two, int ka) { return (two ? 1 : 2) * ka; }
@@ -344,36 +345,31 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
     // ------------------------------ X ------------------------------
     // Two warps, k-blocks in turn (as for the scale writers' runs, a ring of two stages or more keeps the
     // parities apart).  Rows in plan order: one or two boxes of BN / 2 rows.  Otherwise lane l
-    // gathers rows 4 l .. 4 l + 3 of the item's X, and those 128 further on; rows that do not exist
-    // inside a group of four are read as the group's first one.  What is not loaded is left as it is
-    // (its columns are computed and never read).
+    // gathers rows 4 l .. 4 l + 3 of the item's X (which is kGroupedMaxGathered wide at most); rows that do
+    // not exist inside a group of four are read as the group's first one.  What is not loaded is left
+    // as it is (its columns are computed and never read).
     const uint32_t el = elect_one() ? 1u : 0u;
     int s = 0, turn = 0;
     uint32_t ph = 0;
     bool alive = true;
-    int pairs[2][4];
+    static_assert(kGroupedMaxGathered <= 128, "four rows to a lane");
+    int pairs[4];
     auto fetch_pairs = [&](int j) {
       if (p.sorted) return;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) pairs[h][i] = x_pair(j, 128 * h + 4 * lane + i);
+      for (int i = 0; i < 4; ++i) pairs[i] = x_pair(j, 4 * lane + i);
     };
     fetch_pairs(0);
     for (int it = 0; it < n_items && alive; ++it) {
       const GroupedItem item = item_at(it);
-      int row[2][4];
-      bool mine[2];
+      const bool mine = !p.sorted && 4 * lane < item.count;
+      int row[4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        mine[h] = !p.sorted && 128 * h + 4 * lane < item.count;
+      for (int j = 0; j < 4; ++j) row[j] = p.sorted ? -1 : x_row(pairs[j]);
+      if (row[0] < 0) row[0] = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) row[h][j] = p.sorted ? -1 : x_row(pairs[h][j]);
-        if (row[h][0] < 0) row[h][0] = 0;
-#pragma unroll
-        for (int j = 1; j < 4; ++j)
-          if (row[h][j] < 0) row[h][j] = row[h][0];
-      }
+      for (int j = 1; j < 4; ++j)
+        if (row[j] < 0) row[j] = row[0];
       fetch_pairs(it + 1);
       const bool second = item.count > BN / 2;
       const uint32_t bytes = p.sorted ? static_cast<uint32_t>(BN / 2 * 128 * (second ? 2 : 1))
@@ -402,10 +398,7 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
           } else {
             __syncwarp();  // (the bytes are announced before any can arrive)
             const uint32_t dst = x_base + static_cast<uint32_t>(lane) * 512u;
-            if (mine[0])
-              tma_gather4(dst, &tmX, full_bar(mine_s), x_kb * 128, row[0][0], row[0][1], row[0][2], row[0][3]);
-            if (mine[1])
-              tma_gather4(dst + 128u * 128u, &tmX, full_bar(mine_s), x_kb * 128, row[1][0], row[1][1], row[1][2], row[1][3]);
+            if (mine) tma_gather4(dst, &tmX, full_bar(mine_s), x_kb * 128, row[0], row[1], row[2], row[3]);
           }
         }
         const int done = min(2, p.k_blocks - kb);
@@ -568,11 +561,11 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
                          : "memory");
         } else {
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t)
-          fetch_scales(dst + t * kTileM * 16u, f_w[t] != nullptr ? f_w[t] + col : p.sw, f_w[t] != nullptr ? valid : 0, p.align_w);
-        if (slot0) fetch_scales(dst + x_slot, f_x0 != nullptr ? f_x0 + col : p.sx, f_x0 != nullptr ? valid : 0, p.align_x);
-        if (slot1)
-          fetch_scales(dst + x_slot + kTileM * 16u, f_x1 != nullptr ? f_x1 + col : p.sx, f_x1 != nullptr ? valid : 0, p.align_x);
+          for (int t = 0; t < kTiles; ++t)
+            fetch_scales(dst + t * kTileM * 16u, f_w[t] != nullptr ? f_w[t] + col : p.sw, f_w[t] != nullptr ? valid : 0, p.align_w);
+          if (slot0) fetch_scales(dst + x_slot, f_x0 != nullptr ? f_x0 + col : p.sx, f_x0 != nullptr ? valid : 0, p.align_x);
+          if (slot1)
+            fetch_scales(dst + x_slot + kTileM * 16u, f_x1 != nullptr ? f_x1 + col : p.sx, f_x1 != nullptr ? valid : 0, p.align_x);
         }
         f_kb += kUnitsPerChunk;
         if (f_kb >= p.k_blocks) {
@@ -821,7 +814,7 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
   if (warp == 1) tmem_dealloc(tmem_base, 512u);
 }
 
-// Rows of A (elements, then scales) in plan order: row p of `x` and `sx` belongs to pair order[p].  A block
+// Rows of A (elements, then scales) in plan order: row p of `x` and `sx` belongs to pair order[p].  A warp
 // for every place in turn; places without a pair are left as they are.
 __global__ void __launch_bounds__(256) gather_rows_kernel(const uint8_t* a, int64_t a_pitch, const uint8_t* sa,
                                                           int64_t sa_pitch, const int32_t* order, int rows, int a_rows,

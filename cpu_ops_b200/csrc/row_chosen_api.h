@@ -308,7 +308,8 @@ GroupedChoice choose_grouped(const DeviceState& st, int rows, int n, int groups,
   GroupedChoice best;
   const int average = rows / std::max(1, groups), sms = st.sms();
   if (average < 48) {
-    best.BN = std::max(32, std::min(kGroupedMaxBN, (std::min(rows, 2 * average) + 31) / 32 * 32));
+    static_assert(2 * 47 <= kGroupedMaxGathered && kGroupedMaxGathered % 32 == 0, "twice the average, in steps of 32");
+    best.BN = std::max(32, (std::min(rows, 2 * average) + 31) / 32 * 32);
     best.stages = grouped_stages(st.smem_optin, best.BN, ka, groups, false);
     best.tile_cols = gated ? 64 : 128;
     return best;
