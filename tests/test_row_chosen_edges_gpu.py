@@ -85,6 +85,31 @@ def test_grouped_one_pair_per_row_with_ids_writes_every_row(gpu, rows, n, k, gro
     assert (e.run(weighted, D=D).cpu().numpy()[none] == 7.5).all()
 
 
+def test_waits_are_for_a_stage_not_for_the_call(gpu, lib):
+    """A budget for the bounded waits of 400 us is enough for a call that takes several times as long."""
+    budget = 400
+    e = Experts(E4, E4, 131072, 4096, 4096, 8, share=512, seed=31)
+    want = e.run()
+    D = torch.full_like(want, float("nan"))
+    e.args.ref_D = c.TensorRef(D, e.n)
+    op = c.GemmMxGrouped(stream=torch.cuda.current_stream().cuda_stream, asynchronous=True)
+    desc = op.describe(e.args)
+    check(op.run(desc))   # (this stream's workspace is in place)
+    D.fill_(float("nan"))
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    torch.cuda.synchronize()
+    try:
+        lib.cpuops_b200_set_wait_budget_us(budget)
+        start.record()
+        check(op.run(desc))
+        end.record()
+        check(c.stream_status(torch.cuda.current_stream().cuda_stream))
+    finally:
+        lib.cpuops_b200_set_wait_budget_us(0)
+    assert start.elapsed_time(end) * 1000 > 3 * budget
+    assert torch.equal(want, D)
+
+
 # ---- adapters: infinities ----------------------------------------------------------------------
 
 
