@@ -325,10 +325,12 @@ __device__ __forceinline__ void fill_piece(uint32_t dst, const T* row, int i, in
 // zero, NaN, and so may those of a term that is an infinity and others that are beyond f16's range; what came
 // out as NaN is made anew here.
 template <typename W>
-__device__ __noinline__ float whole_product(const float* f, int parts, int64_t step, float scale, const W* w, int count) {
+__device__ __forceinline__ float whole_product(const float* f, int parts, int64_t step, float scale, const W* w, int count) {
   float y = 0.0f;
+#pragma unroll 1
   for (int j = 0; j < count && y == y; ++j) {
     float v = 0.0f;
+#pragma unroll 1
     for (int s = 0; s < parts; ++s) v += f[s * step + j];
     y = __fmaf_rn(v * scale, to_f32<W>(w[j]), y);
   }
