@@ -320,23 +320,6 @@ __device__ __forceinline__ void fill_piece(uint32_t dst, const T* row, int i, in
   }
 }
 
-// The product of a factor in f32 (the sum of `parts` arrays `step` apart, times `scale`) and one of 16 bits, not cut
-// into terms.  With an infinity in the 16-bit factor the terms' products may be of either sign or, of a term of
-// zero, NaN, and so may those of a term that is an infinity and others that are beyond f16's range; what came
-// out as NaN is made anew here.
-template <typename W>
-__device__ __forceinline__ float whole_product(const float* f, int parts, int64_t step, float scale, const W* w, int count) {
-  float y = 0.0f;
-#pragma unroll 1
-  for (int j = 0; j < count && y == y; ++j) {
-    float v = 0.0f;
-#pragma unroll 1
-    for (int s = 0; s < parts; ++s) v += f[s * step + j];
-    y = __fmaf_rn(v * scale, to_f32<W>(w[j]), y);
-  }
-  return y;
-}
-
 struct AdapterTileParams {
   AdapterParams a;
   const int4* tiles;      // {adapter, first place, rows, -}
@@ -347,6 +330,24 @@ struct AdapterTileParams {
   int32_t up_cols;        // columns of D per CTA of the up kernel (a multiple of kUpCols)
 };
 
+// What the tiles' products make NaN is made anew from the whole factors: with an infinity in the 16-bit factor the
+// products of the other one's terms may be of either sign or, of a term of zero, NaN, and so may those of a
+// term that is an infinity and others that are beyond f16's range.
+//
+// Element j of this CTA's part of u for row r of its tile, of f32 rows (which alone are cut there).
+template <typename W>
+__device__ __forceinline__ void whole_part(const AdapterTileParams& t, int r, int j) {
+  const AdapterParams& p = t.a;
+  const int4 tile = t.tiles[blockIdx.x];
+  const int k0 = static_cast<int>(blockIdx.y) * t.depth, k1 = min(k0 + t.depth, p.k);
+  const float* x = static_cast<const float*>(p.x) + t.order[tile.y + r] * p.ldx;
+  const W* a = static_cast<const W*>(p.a) + tile.x * p.a_stride + j * p.lda;
+  float u = 0.0f;
+#pragma unroll 1
+  for (int i = k0; i < k1 && u == u; ++i) u = __fmaf_rn(x[i], to_f32<W>(a[i]), u);
+  t.u[(static_cast<int64_t>(blockIdx.y) * p.m + tile.y + r) * t.rank_pad + j] = u;
+}
+
 template <typename X>
 __host__ __device__ constexpr int down_x_bytes() { return kPlanTileRows * kDownDepth * static_cast<int>(sizeof(X)); }
 template <typename X, int kRanks>
@@ -356,7 +357,7 @@ __host__ __device__ constexpr int down_smem_bytes() { return kDownStages * (down
 // every 16 rows.  kWide: rows of x and A start on 16-byte boundaries (the other kinds of copy in the
 // same loop cost 2 us of 28).
 template <typename X, typename W, int kRanks, bool kWide>
-__global__ void __launch_bounds__(128) adapter_down_kernel(const AdapterTileParams t) {
+__global__ void __launch_bounds__(128) adapter_down_kernel(const __grid_constant__ AdapterTileParams t) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   extern __shared__ __align__(128) uint8_t down_smem[];
@@ -506,6 +507,7 @@ __global__ void __launch_bounds__(128) adapter_down_kernel(const AdapterTilePara
   cp_async_wait<0>();
   // (row g or g + 8, ranks 2 i and 2 i + 1 of eight)
   float* u = t.u + (static_cast<int64_t>(blockIdx.y) * p.m + tile.y) * t.rank_pad;
+  float any = 0.0f;  // NaN where one of this thread's is
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int r = warp * 16 + (lane >> 2) + 8 * h;
@@ -513,16 +515,21 @@ __global__ void __launch_bounds__(128) adapter_down_kernel(const AdapterTilePara
 #pragma unroll
     for (int j = 0; j < kRanks / 8; ++j) {
       const int at = rank0 + j * 8 + 2 * (lane & 3);
-      float2 v = make_float2(sum[j][2 * h] + acc[j][2 * h], sum[j][2 * h + 1] + acc[j][2 * h + 1]);
-      if constexpr (sizeof(X) == 4) {
-        if (__builtin_expect(v.x != v.x || v.y != v.y, 0)) {
-          const X* x = static_cast<const X*>(p.x) + t.order[tile.y + r] * p.ldx + k0;
-          const W* a = static_cast<const W*>(p.a) + tile.x * p.a_stride + at * p.lda + k0;
-          if (v.x != v.x && at < p.rank) v.x = whole_product<W>(x, 1, 0, 1.0f, a, k1 - k0);
-          if (v.y != v.y && at + 1 < p.rank) v.y = whole_product<W>(x, 1, 0, 1.0f, a + p.lda, k1 - k0);
-        }
-      }
+      const float2 v = make_float2(sum[j][2 * h] + acc[j][2 * h], sum[j][2 * h + 1] + acc[j][2 * h + 1]);
       if (at < t.rank_pad) *reinterpret_cast<float2*>(u + static_cast<int64_t>(r) * t.rank_pad + at) = v;
+      any += v.x + v.y;
+    }
+  }
+  if constexpr (sizeof(X) == 4) {
+    if (any != any) {
+      // (this thread's own stores, read back)
+#pragma unroll 1
+      for (int at = 0; at < kRanks / 2; ++at) {
+        const int r = warp * 16 + (lane >> 2) + 8 * (at & 1), e = rank0 + (at >> 2) * 8 + 2 * (lane & 3) + (at >> 1 & 1);
+        if (r >= tile.z || e >= p.rank) continue;
+        const float v = u[static_cast<int64_t>(r) * t.rank_pad + e];
+        if (v != v) whole_part<W>(t, r, e);
+      }
     }
   }
 }
@@ -566,6 +573,24 @@ __host__ __device__ inline int up_smem_bytes(int rank_pad, int terms) {
   return terms * kPlanTileRows * (rank_pad + 8) * 2 + up_stages(rank_pad) * up_stage_bytes(rank_pad) + kPlanTileRows * 4;
 }
 
+// As whole_part, of the second product: column col of scale * u B^T for row r of this CTA's tile.
+template <typename W>
+__device__ __forceinline__ float whole_product(const AdapterTileParams& t, int r, int col) {
+  const AdapterParams& p = t.a;
+  const int4 tile = t.tiles[blockIdx.y];
+  const float scale = p.scales != nullptr ? p.scales[tile.x] : 1.0f;
+  const W* b = static_cast<const W*>(p.b) + tile.x * p.b_stride + col * p.ldb;
+  float y = 0.0f;
+#pragma unroll 1
+  for (int j = 0; j < p.rank && y == y; ++j) {
+    float u = 0.0f;
+#pragma unroll 1
+    for (int s = 0; s < t.splits; ++s) u += t.u[(static_cast<int64_t>(s) * p.m + tile.y + r) * t.rank_pad + j];
+    y = __fmaf_rn(u * scale, to_f32<W>(b[j]), y);
+  }
+  return y;
+}
+
 // D = C + u B^T for tile blockIdx.y and t.up_cols columns from blockIdx.x * t.up_cols on, 64 at a time;
 // 256 threads, a warp for 16 rows x 32 columns of a step.  The time is that of the traffic, C in and D
 // out, so B and C come through a ring in shared memory, a step or two ahead.  (C one step ahead in
@@ -574,7 +599,7 @@ __host__ __device__ inline int up_smem_bytes(int rank_pad, int terms) {
 // kWhole: 16-byte aligned rows of B, C and D, whole steps of 64 columns and ranks in eights, so nothing
 // needs a check: a step is 400 instructions of a warp with them, 200 without (85 / 70 us of the above).
 template <typename W, int kUpStages, bool kWhole>
-__global__ void __launch_bounds__(256, 2) adapter_up_kernel(const AdapterTileParams t) {
+__global__ void __launch_bounds__(256, 2) adapter_up_kernel(const __grid_constant__ AdapterTileParams t) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   extern __shared__ __align__(128) uint8_t up_smem[];
@@ -731,24 +756,6 @@ __global__ void __launch_bounds__(256, 2) adapter_up_kernel(const AdapterTilePar
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[j][e] *= row_scale[row0 + g + 8 * (e >> 1)];
       }
-      float any = 0.0f;  // NaN where one of them is
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) any += acc[j][e];
-      if (__builtin_expect(any != any, 0)) {
-        const float scale = p.scales != nullptr ? p.scales[tile.x] : 1.0f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = row0 + g + 8 * (e >> 1), col = col0 + half + j * 8 + 2 * i + (e & 1);
-            if (acc[j][e] != acc[j][e] && r < tile.z && col < p.n)
-              acc[j][e] = whole_product<W>(t.u + static_cast<int64_t>(tile.y + r) * t.rank_pad, t.splits,
-                                           static_cast<int64_t>(p.m) * t.rank_pad, scale,
-                                           static_cast<const W*>(p.b) + tile.x * p.b_stride + col * p.ldb, p.rank);
-          }
-      }
     }
     // D takes C's place in the stage (a row without an adapter is C itself: no zero is added to it) ...
     if (has) {
@@ -774,6 +781,18 @@ __global__ void __launch_bounds__(256, 2) adapter_up_kernel(const AdapterTilePar
                    : "=f"(y.x), "=f"(y.y), "=f"(y.z), "=f"(y.w)
                    : "r"(at + c_to + 16 * j * kUpCWords * 4));
       if ((tid >> 4) + 16 * j < tile.z) {
+        const float any = y.x + y.y + y.z + y.w;  // (NaN where one of them is)
+        if (any != any && has) {
+#pragma unroll 1
+          for (int e = 0; e < 4; ++e) {
+            const float v = e == 0 ? y.x : e == 1 ? y.y : e == 2 ? y.z : y.w;
+            const int r = (tid >> 4) + 16 * j, col = col0 + (tid & 15) * 4 + e;
+            if (v == v || col >= p.n) continue;
+            // (of a D that is C this thread alone writes the element, below)
+            const float made = p.c[t.order[tile.y + r] * p.ldc + col] + whole_product<W>(t, r, col);
+            y = make_float4(e == 0 ? made : y.x, e == 1 ? made : y.y, e == 2 ? made : y.z, e == 3 ? made : y.w);
+          }
+        }
         const int left = kWhole ? 4 : p.n - col0 - (tid & 15) * 4;  // columns from here on
         if (wide_d && left >= 4) {
           *reinterpret_cast<float4*>(d_to[j]) = y;
