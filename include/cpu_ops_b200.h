@@ -230,7 +230,8 @@ CPUOPS_B200_API int cpuops_b200_stream_status(void* stream);
  * persistent, one CTA per SM, and hold their SMs until they end: a caller that wants a
  * communication kernel to run beside a GEMM (the all-gather of D on a second stream) leaves
  * it some SMs with this setting.  Results do not depend on it for int8; for MX it can change
- * the automatic split-k choice like any change of problem size does. */
+ * the automatic split-k choice like any change of problem size does, and for low-rank adapters of
+ * many rows the parts in which k is summed. */
 CPUOPS_B200_API int cpuops_b200_set_sm_limit(int32_t device, int32_t sms);
 
 /* Budget of every bounded device-side wait (mbarrier waits of the GEMM kernels' roles), in
@@ -275,8 +276,10 @@ CPUOPS_B200_API int cpuops_b200_release_b(void* handle);
  * host never reads.  `stream`, `flags` (CPUOPS_B200_FLAG_ASYNC), `device` and `memory_space` mean
  * what they mean in cpuops_b200_gemm_desc (MEM_DEVICE skips the check of the pointers), locking
  * and stream capture are the same too.  Calls whose comment says so use the stream's workspace:
- * graphs captured from one stream share it, so replay such graphs one after another, not side by
- * side.  Results are bit-identical from run to run.  Outputs must not overlap inputs or one
+ * graphs captured from one stream share it with each other and with that stream's own calls, so replay
+ * such graphs one after another, not side by side, nor beside those calls.  Results are
+ * bit-identical from run to run, for one setting of cpuops_b200_set_sm_limit (the adapters' products of
+ * many rows are summed in parts of k that depend on it).  Outputs must not overlap inputs or one
  * another, except where a comment allows it. */
 
 /* Element types of rows that are not quantised. */
@@ -345,7 +348,9 @@ CPUOPS_B200_API int cpuops_b200_group_rows(const cpuops_b200_group_rows_desc* de
 
 /* The experts' products, on MX operands (the formats, scales and leading dimensions of
  * cpuops_b200_gemm_desc).  For every pair q of group g in the plan
- *     acc[j] = sum_k A[q / pairs_per_a_row][k] * B_g[j][k]                 (f32 sums)
+ *     acc[j] = sum_k A[q / pairs_per_a_row][k] * B_g[j][k]
+ *              (one running f32 sum of the tensor cores, whose roundings grow with k: of random 8-bit
+ *              operands 2.5e-6 of the result's norm at k = 4096, 1e-5 at 16384)
  *     y[j]   = acc[j],  or  silu(acc[j]) * acc[n + j]  with `gated`
  *     y[j]  *= row_weights[q]                                              (if given)
  *     D[q]   = y       if pairs_per_d_row == 1; rows of pairs in no group are zeros if `ids` are given
@@ -392,7 +397,8 @@ CPUOPS_B200_API int cpuops_b200_gemm_grouped(const cpuops_b200_gemm_grouped_desc
  * and D[t] = C[t] where ids[t] lies outside [0, adapters).  A_g is `rank` rows of k (rows lda,
  * adapters a_stride elements apart), B_g n rows of `rank` (ldb, b_stride).  An adapter of a smaller
  * rank is padded with zeros.  X may be f32 with A and B f16 or bf16, or all three the same
- * 16-bit type; C, D and every sum are f32.  D may be C.  16-byte aligned rows of X, A and B are read
+ * 16-bit type; C, D and every sum are f32 (of f16 adapters, where rows are taken in tiles, the elements of
+ * X A_g^T are kept to 22 bits, small ones to 2^-39 of the row's largest).  D may be C.  16-byte aligned rows of X, A and B are read
  * fastest.  n and k are at most 2^30.  Uses the stream's workspace where rows are taken in tiles sorted by
  * adapter, which an estimate of both times decides (a few hundred rows and more). */
 typedef struct cpuops_b200_adapters_desc {
