@@ -44,10 +44,13 @@ void set_error(const char* fmt, ...) {
   va_end(ap);
 }
 
+// (The runtime keeps a failed call's error for whoever asks next, here or in the caller's program: it has been
+// reported with this call's status, so it is taken back.)
 #define CUDA_TRY(expr)                                                                       \
   do {                                                                                       \
     cudaError_t err__ = (expr);                                                              \
     if (err__ != cudaSuccess) {                                                              \
+      cudaGetLastError();                                                                    \
       set_error("%s failed: %s (%s:%d)", #expr, cudaGetErrorString(err__), __FILE__, __LINE__); \
       return CPUOPS_B200_STATUS_CUDA_ERROR;                                                  \
     }                                                                                        \

@@ -110,6 +110,25 @@ def test_waits_are_for_a_stage_not_for_the_call(gpu, lib):
     assert torch.equal(want, D)
 
 
+def test_a_call_after_one_without_memory(gpu):
+    """A workspace that does not fit the device fails its call, and only that one."""
+    rows, n, k = 1 << 16, 1 << 20, 32          # the pairs' rows: 275 GB
+    A = torch.zeros((1, k), dtype=torch.uint8, device="cuda")
+    B = torch.zeros((n, k), dtype=torch.uint8, device="cuda")
+    ones = torch.full((n, 1), 127, dtype=torch.uint8, device="cuda")
+    ids = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    order = torch.arange(rows, dtype=torch.int32, device="cuda")
+    offsets = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
+    D = torch.full((rows // 32, n), 7.5, device="cuda")
+    op = c.GemmMxGrouped()
+    st = op(op.Arguments(c.GroupedCoord(rows, n, k, 1), c.MxTensorRef(A, ones, k, 1), c.MxTensorRef(B, ones, k, 1),
+                         c.RowPlan(offsets, order), c.TensorRef(D, n), pairs_per_a_row=rows, pairs_per_d_row=32, ids=ids))
+    assert st not in (c.Status.kSuccess, c.Status.kErrorInvalidArguments) and "memory" in _capi.last_error()
+    assert (D == 7.5).all()
+    del D
+    Experts(E4, E4, 40, 96, 128, 5, seed=32).check(summed=2)
+
+
 # ---- adapters: infinities ----------------------------------------------------------------------
 
 
