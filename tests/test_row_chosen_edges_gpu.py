@@ -1,5 +1,6 @@
 """Calls of the operators whose weights are chosen per row in which a bound, a mask, an infinity or
 the sharing of a stream decides the result."""
+import ctypes
 import math
 import threading
 
@@ -127,6 +128,20 @@ def test_a_call_after_one_without_memory(gpu):
     assert (D == 7.5).all()
     del D
     Experts(E4, E4, 40, 96, 128, 5, seed=32).check(summed=2)
+
+
+def test_a_call_after_an_error_of_the_program(gpu):
+    """An error that the program's own runtime call left behind is not this call's."""
+    e = Experts(E4, E4, 40, 96, 128, 5, seed=33)
+    e.check(summed=2)
+    runtime = ctypes.CDLL("libcudart.so.12")
+    pointer = ctypes.c_void_p()
+    assert runtime.cudaMalloc(ctypes.byref(pointer), ctypes.c_size_t(1 << 50)) != 0
+    try:
+        status = c.GemmMxGrouped(memory_space=_capi.MEM_DEVICE)(e.args)
+    finally:
+        runtime.cudaGetLastError()
+    check(status)
 
 
 # ---- adapters: infinities ----------------------------------------------------------------------
