@@ -332,7 +332,8 @@ struct AdapterTileParams {
 
 // What the tiles' products make NaN is made anew from the whole factors: with an infinity in the 16-bit factor the
 // products of the other one's terms may be of either sign or, of a term of zero, NaN, and so may those of a
-// term that is an infinity and others that are beyond f16's range.
+// term that is an infinity and others that are beyond f16's range.  (The check costs 1 us of 98, 8192 rows,
+// rank 64, n 4096; beside the products, in their loops, it cost f32 rows 7 of 146.)
 //
 // Element j of this CTA's part of u for row r of its tile, of f32 rows (which alone are cut there).
 template <typename W>
