@@ -56,6 +56,11 @@ EXPORTED_SYMBOLS = (
     "cpuops_b200_group_rows",
     "cpuops_b200_gemm_grouped",
     "cpuops_b200_adapters",
+    "cpuops_b200_gemm16",
+    "cpuops_b200_epilogue_grad",
+    "cpuops_b200_layer_norm",
+    "cpuops_b200_layer_norm_grad",
+    "cpuops_b200_balance_loss",
     "cpuops_b200_last_error",
     "cpuops_b200_abi_version",
     "cpuops_b200_device_count",
@@ -126,6 +131,34 @@ class AdaptersDesc(C.Structure):
                 _fields(C.c_int64, "a_stride b_stride") + _fields(C.c_void_p, "x a b ids scales c d") + _PLACE)
 
 
+class Gemm16Desc(C.Structure):
+    _fields_ = ([("struct_size", C.c_uint32)] +
+                _fields(C.c_int32, "type c_type d_type m n k a_row_major b_row_major activation lda ldb ldc ldd ldz") +
+                _fields(C.c_float, "alpha beta") + _fields(C.c_void_p, "a b bias c d z") +
+                _fields(C.c_int32, "split_k_slices tile_n") + _PLACE)
+
+
+class EpilogueGradDesc(C.Structure):
+    _fields_ = ([("struct_size", C.c_uint32)] + _fields(C.c_int32, "type m n activation lddy ldz lddz") +
+                _fields(C.c_void_p, "dy z dz dbias") + _PLACE)
+
+
+class LayerNormDesc(C.Structure):
+    _fields_ = ([("struct_size", C.c_uint32)] + _fields(C.c_int32, "x_type y_type m n ldx ldy") +
+                [("eps", C.c_float)] + _fields(C.c_void_p, "x gamma beta y mean rstd") + _PLACE)
+
+
+class LayerNormGradDesc(C.Structure):
+    _fields_ = ([("struct_size", C.c_uint32)] + _fields(C.c_int32, "x_type y_type m n lddy ldx lddr lddx") +
+                _fields(C.c_void_p, "dy x dr gamma mean rstd dx dgamma dbeta") + _PLACE)
+
+
+class BalanceLossDesc(C.Structure):
+    _fields_ = ([("struct_size", C.c_uint32)] + _fields(C.c_int32, "tokens experts top_k scoring") +
+                [("coefficient", C.c_float)] + _fields(C.c_int32, "logits_type ld_logits ld_dlogits") +
+                _fields(C.c_void_p, "logits ids upstream counts loss dlogits") + _PLACE)
+
+
 _lib = None
 
 
@@ -169,7 +202,9 @@ def load() -> C.CDLL:
     lib.cpuops_b200_release_b.restype = C.c_int
     lib.cpuops_b200_release_b.argtypes = [C.c_void_p]
     for name, desc in (("route", RouteDesc), ("group_rows", GroupRowsDesc), ("gemm_grouped", GemmGroupedDesc),
-                       ("adapters", AdaptersDesc)):
+                       ("adapters", AdaptersDesc), ("gemm16", Gemm16Desc), ("epilogue_grad", EpilogueGradDesc),
+                       ("layer_norm", LayerNormDesc), ("layer_norm_grad", LayerNormGradDesc),
+                       ("balance_loss", BalanceLossDesc)):
         entry = getattr(lib, "cpuops_b200_" + name)
         entry.restype = C.c_int
         entry.argtypes = [C.POINTER(desc)]

@@ -20,7 +20,7 @@ OUT_INSTRUMENT = PKG_DIR / "libcpu_ops_b200_instrument.so"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-    "-Xcompiler", "-fPIC,-fvisibility=hidden", "-shared",
+    "-Xcompiler", "-fPIC,-fvisibility=hidden", "-shared", "--threads", "0",  # (sources side by side)
 ]
 
 

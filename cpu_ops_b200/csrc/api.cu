@@ -1799,3 +1799,4 @@ CPUOPS_B200_API int cpuops_b200_gemm_i8_noalloc(const cpuops_b200_gemm_desc* d) 
 }  // extern "C"
 
 #include "row_chosen_api.h"
+#include "dense_api.h"

@@ -422,8 +422,152 @@ typedef struct cpuops_b200_adapters_desc {
 #define CPUOPS_B200_MAX_RANK 256
 CPUOPS_B200_API int cpuops_b200_adapters(const cpuops_b200_adapters_desc* desc);
 
+/* ---- 16-bit layers and their gradients -------------------------------------------------------
+ * What a program that trains the dense parts of a model, or its router, needs beside the quantised products:
+ * the reference has 16-bit GEMMs and layer norm on the CPU, no gradients.  As the entry points above, these take
+ * device memory only, and `stream`, `flags`, `device`, `memory_space`, locking, stream capture and the
+ * stream's workspace mean the same (comments say which calls use the workspace).  Matrices are rows of
+ * contiguous elements, ld elements apart; types are CPUOPS_B200_TYPE_*.  Sums are f32 throughout and
+ * every stored 16-bit value is rounded once.  Results are bit-identical from run to run, for one setting of
+ * cpuops_b200_set_sm_limit (on which the parts that are summed depend).  Outputs must not overlap inputs or
+ * one another, except where a comment allows it. */
+
+/* z = alpha * A B + bias,  D = act(z) + beta * C,  Z = z (where Z is given: what cpuops_b200_epilogue_grad wants).
+ * A is m x k, B k x n, both f16 or both bf16, each row-major or column-major, so that the products of a backward
+ * pass are calls of this entry too: with Y = X W^T (W by rows: B column-major), dX = dY W has B row-major and
+ * dW = dY^T X has A column-major and B row-major.  C, D and Z are row-major; C and D f32 or of A's type, Z of D's.
+ * activation: 0 or CPUOPS_B200_OP_RELU, _GELU (tanh form), _SILU.  C is not read and may be NULL when beta == 0;
+ * D may be C (same ld and type).  k == 0: the product is zero.
+ * A sum is one running f32 sum of the tensor cores (up to eight parts of k, added in order, where there are few tiles).
+ * 16-byte aligned rows are read and written fastest.  Uses the stream's workspace where rows of A or B are not
+ * 16-byte aligned (a copy of them).  m, n and k are at most 2^30. */
+typedef struct cpuops_b200_gemm16_desc {
+  uint32_t struct_size; /* sizeof(cpuops_b200_gemm16_desc), checked */
+  int32_t type;         /* of A and B: CPUOPS_B200_TYPE_F16, _BF16 */
+  int32_t c_type, d_type;
+  int32_t m, n, k;
+  int32_t a_row_major, b_row_major;
+  int32_t activation;
+  int32_t lda, ldb, ldc, ldd, ldz;
+  float alpha, beta;
+  const void* a;
+  const void* b;
+  const float* bias;      /* n, or NULL                              */
+  const void* c;
+  void* d;
+  void* z;                /* or NULL                                 */
+  int32_t split_k_slices; /* 0 automatic; else 1, 2, 4 or 8          */
+  int32_t tile_n;         /* 0 automatic; else force (testing/tuning, as the FLAG_PAIR_ flags) */
+  void* stream;
+  uint32_t flags;
+  int32_t device;
+  int32_t memory_space;
+} cpuops_b200_gemm16_desc;
+CPUOPS_B200_API int cpuops_b200_gemm16(const cpuops_b200_gemm16_desc* desc);
+
+/* The gradient of that epilogue: dZ = dY * act'(Z), dbias[j] = the sum over i of dZ[i][j] before its rounding.
+ * dY, Z and dZ are m x n of one type.  (dC of the residual is beta * dY itself; the products' gradients are
+ * calls of cpuops_b200_gemm16 on dZ.)  Without an activation Z is not read, and dZ may be NULL.  relu'(z) is 0
+ * for z <= 0; where z is infinite gelu' and silu' are their limits, 0 and 1.
+ * dZ may be dY or Z.  dbias may be NULL.  Uses the stream's workspace for dbias. */
+typedef struct cpuops_b200_epilogue_grad_desc {
+  uint32_t struct_size;
+  int32_t type;
+  int32_t m, n;
+  int32_t activation;
+  int32_t lddy, ldz, lddz;
+  const void* dy;
+  const void* z;
+  void* dz;
+  float* dbias;         /* n, or NULL */
+  void* stream;
+  uint32_t flags;
+  int32_t device;
+  int32_t memory_space;
+} cpuops_b200_epilogue_grad_desc;
+CPUOPS_B200_API int cpuops_b200_epilogue_grad(const cpuops_b200_epilogue_grad_desc* desc);
+
+/* Layer norm, row by row (the reference's ops/norm.h layernorm):
+ *     mean = sum x / n,  rstd = 1 / sqrt(sum (x - mean)^2 / n + eps),  Y = (x - mean) * rstd * gamma + beta
+ * Y is of X's type, or of any type where X is f32.  gamma (NULL: 1) and beta (NULL: 0) hold n floats; mean and rstd
+ * (NULL: not wanted) m floats, which cpuops_b200_layer_norm_grad reads.  Y may be X (same ld and type). */
+typedef struct cpuops_b200_layer_norm_desc {
+  uint32_t struct_size;
+  int32_t x_type, y_type;
+  int32_t m, n;
+  int32_t ldx, ldy;
+  float eps;            /* >= 0 */
+  const void* x;
+  const float* gamma;
+  const float* beta;
+  void* y;
+  float* mean;
+  float* rstd;
+  void* stream;
+  uint32_t flags;
+  int32_t device;
+  int32_t memory_space;
+} cpuops_b200_layer_norm_desc;
+CPUOPS_B200_API int cpuops_b200_layer_norm(const cpuops_b200_layer_norm_desc* desc);
+
+/* Its gradient, from the mean and rstd that the forward call left: with g = dY * gamma, xhat = (x - mean) * rstd
+ *     dX = rstd * (g - sum g / n - xhat * sum(g * xhat) / n) + dR,   dgamma = sum dY * xhat,   dbeta = sum dY
+ * (sums of dX's along the row, of dgamma's and dbeta's over the rows).  dR (NULL: 0), of X's type, is the gradient that
+ * comes past the norm on the residual stream.  x_type is X's, dR's and dX's, y_type dY's.  dX may be X, dR or
+ * (of the same type) dY.  dgamma and dbeta may be NULL.  Uses the stream's workspace for dgamma and dbeta. */
+typedef struct cpuops_b200_layer_norm_grad_desc {
+  uint32_t struct_size;
+  int32_t x_type, y_type;
+  int32_t m, n;
+  int32_t lddy, ldx, lddr, lddx;
+  const void* dy;
+  const void* x;
+  const void* dr;
+  const float* gamma;
+  const float* mean;
+  const float* rstd;
+  void* dx;
+  float* dgamma;
+  float* dbeta;
+  void* stream;
+  uint32_t flags;
+  int32_t device;
+  int32_t memory_space;
+} cpuops_b200_layer_norm_grad_desc;
+CPUOPS_B200_API int cpuops_b200_layer_norm_grad(const cpuops_b200_layer_norm_grad_desc* desc);
+
+/* The balance loss of a router, beside cpuops_b200_route and on its ids:
+ *     counts[e] = pairs whose id is e,  f_e = counts[e] / sum counts
+ *     p_te = softmax(logits[t])[e],  or with SCORE_SIGMOID s_te / sum_j s_tj of s = 1 / (1 + exp(-logits))
+ *     P_e = the mean of p_te over the tokens that have an id in [0, experts)
+ *     loss = coefficient * experts * sum_e f_e P_e        (coefficient where the load is even)
+ * and dlogits = upstream * d loss / d logits, of the logits' type (counts have no gradient).  Tokens without an id
+ * (padding, ids of -1) count nowhere and have a gradient of zero; without any such token the loss is 0.
+ * An expert whose logit is NaN or -inf is out of its token's sum; +inf counts as the largest number.
+ * upstream: the loss's own gradient, one float on the device (NULL: 1).  counts, loss and dlogits may each be NULL;
+ * dlogits may be logits (same ld).  Uses the stream's workspace beyond 32 tokens. */
+typedef struct cpuops_b200_balance_loss_desc {
+  uint32_t struct_size;
+  int32_t tokens, experts, top_k;
+  int32_t scoring;       /* CPUOPS_B200_SCORE_*           */
+  float coefficient;
+  int32_t logits_type;
+  int32_t ld_logits, ld_dlogits;
+  const void* logits;
+  const int32_t* ids;    /* tokens x top_k, contiguous    */
+  const float* upstream;
+  int32_t* counts;       /* experts                       */
+  float* loss;           /* 1                             */
+  void* dlogits;
+  void* stream;
+  uint32_t flags;
+  int32_t device;
+  int32_t memory_space;
+} cpuops_b200_balance_loss_desc;
+CPUOPS_B200_API int cpuops_b200_balance_loss(const cpuops_b200_balance_loss_desc* desc);
+
 /* What the calling thread's last cpuops_b200_gemm call that reached a tensor-core kernel
- * launched (diagnostics for tests and benchmarks): */
+ * launched, or cpuops_b200_gemm16 call (diagnostics for tests and benchmarks): */
 typedef struct cpuops_b200_plan {
   int32_t swapped;   /* 1: the caller's B went on the MMA M side (small m)          */
   int32_t tile_n;    /* N tile                                                    */
