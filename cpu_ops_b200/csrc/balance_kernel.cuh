@@ -7,7 +7,8 @@
 // which differ from one another as much as f_e do: an even load leaves nothing of the f_e themselves.
 //
 // A kernel counts, block by block; the other needs all counts (its CTAs add the blocks' up), takes a token
-// per warp, logits read once, and keeps sums of p in registers; its last CTA adds those up.
+// per warp, logits read once, and keeps sums of p in registers; its last CTA adds those up.  Bound by latencies: two launches, two hand-overs through L2, a token's three sums
+// across a warp.
 #pragma once
 
 #include "dense_params.h"
@@ -17,8 +18,9 @@
 
 namespace b200 {
 
-constexpr int kBalanceWarps = 8;
-constexpr int kBalanceThreads = 32 * kBalanceWarps;
+constexpr int kBalanceCountThreads = 256;
+// Warps of a CTA of the main kernel, as many as its registers (a token's scores, its next logits, the sums) leave.
+__host__ __device__ constexpr int balance_warps(int per_lane) { return per_lane <= 8 ? 32 : 16; }
 
 // Counts of the tokens [begin, end) into shared memory: counts[0 .. experts), and counts[experts]
 // of tokens that have an expert.  All threads of the CTA.
@@ -39,7 +41,7 @@ __device__ __forceinline__ void count_pairs(const BalanceParams& p, int begin, i
   __syncthreads();
 }
 
-__global__ void __launch_bounds__(kBalanceThreads) balance_count_kernel(const BalanceParams p) {
+__global__ void __launch_bounds__(kBalanceCountThreads) balance_count_kernel(const BalanceParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ int32_t counts[1025];
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -50,44 +52,43 @@ __global__ void __launch_bounds__(kBalanceThreads) balance_count_kernel(const Ba
   for (int i = threadIdx.x; i <= p.experts; i += blockDim.x) p.part_counts[static_cast<int64_t>(blockIdx.x) * (p.experts + 1) + i] = counts[i];
 }
 
-__device__ __forceinline__ float logit_of(const BalanceParams& p, int64_t token, int e) {
-  const int64_t i = token * p.ld + e;
-  const float x = p.type == kF32 ? __ldg(static_cast<const float*>(p.logits) + i)
-                  : p.type == kF16 ? __half2float(static_cast<const __half*>(p.logits)[i])
-                                   : __bfloat162float(static_cast<const __nv_bfloat16*>(p.logits)[i]);
-  return x > FLT_MAX ? FLT_MAX : x;  // (+inf counts as the largest number, as it does in routing)
-}
-__device__ __forceinline__ void put_gradient(const BalanceParams& p, int64_t token, int e, float v) {
-  const int64_t i = token * p.ldg + e;
-  if (p.type == kF32) {
-    static_cast<float*>(p.dlogits)[i] = v;
-  } else if (p.type == kF16) {
-    static_cast<__half*>(p.dlogits)[i] = __float2half_rn(v);
-  } else {
-    static_cast<__nv_bfloat16*>(p.dlogits)[i] = __float2bfloat16_rn(v);
-  }
+// exp(v), v <= 0: exp2 of a rounded product, off by |v| eps / 2 of itself, which the sums of the larger terms dwarf.
+__device__ __forceinline__ float exp_fast(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v * 1.4426950408889634f));
+  return r;
 }
 
 // kPer: experts per lane.  p.count_blocks == 0: one CTA, which counts itself.
-template <int kPer>
-__global__ void __launch_bounds__(kBalanceThreads) balance_kernel(const BalanceParams p) {
+template <typename T, int kPer>
+__global__ void __launch_bounds__(32 * balance_warps(kPer)) balance_kernel(const BalanceParams p) {
+  constexpr int kWarps = balance_warps(kPer), kThreads = 32 * kWarps;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ int32_t counts[32 * kPer + 1];
   __shared__ float share[32 * kPer];             // f_e - 1 / E
-  __shared__ float join[kBalanceWarps][32 * kPer <= 256 ? 32 * kPer : 256];
-  __shared__ double terms[kBalanceWarps];
+  __shared__ float join[kWarps][32 * kPer <= 256 ? 32 * kPer : 256];
+  __shared__ double terms[kWarps];
   __shared__ int32_t last, all_pairs;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, experts = p.experts;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (p.count_blocks == 0) {
     count_pairs(p, 0, p.tokens, counts);
   } else {
-    for (int i = threadIdx.x; i <= experts; i += kBalanceThreads) {
-      int32_t sum = 0;
-#pragma unroll 8
-      for (int b = 0; b < p.count_blocks; ++b) sum += __ldcg(p.part_counts + static_cast<int64_t>(b) * (experts + 1) + i);
-      counts[i] = sum;
+    // the blocks' counts, each warp its share of the blocks (all of its loads in flight together)
+    for (int i = threadIdx.x; i <= experts; i += kThreads) counts[i] = 0;
+    __syncthreads();
+    int32_t some[kPer + 1];
+#pragma unroll
+    for (int j = 0; j <= kPer; ++j) some[j] = 0;
+#pragma unroll 2
+    for (int b = warp; b < p.count_blocks; b += kWarps) {
+#pragma unroll
+      for (int j = 0; j <= kPer; ++j)
+        if (lane + 32 * j <= experts) some[j] += __ldcg(p.part_counts + static_cast<int64_t>(b) * (experts + 1) + lane + 32 * j);
     }
+#pragma unroll
+    for (int j = 0; j <= kPer; ++j)
+      if (some[j] != 0) atomicAdd(counts + lane + 32 * j, some[j]);
     __syncthreads();
   }
   if (warp == 0) {
@@ -100,10 +101,10 @@ __global__ void __launch_bounds__(kBalanceThreads) balance_kernel(const BalanceP
   __syncthreads();
   const int64_t pairs = all_pairs;
   const int live_tokens = counts[experts];
-  for (int i = threadIdx.x; i < experts; i += kBalanceThreads) {
-    // a whole number over a whole number: one rounding
+  for (int i = threadIdx.x; i < experts; i += kThreads) {
+    // a whole number over a whole number: nothing cancels behind this difference
     const int64_t above = static_cast<int64_t>(counts[i]) * experts - pairs;
-    share[i] = pairs > 0 ? static_cast<float>(static_cast<double>(above) / (static_cast<double>(pairs) * experts)) : 0.0f;
+    share[i] = pairs > 0 ? static_cast<float>(above) / (static_cast<float>(pairs) * static_cast<float>(experts)) : 0.0f;
     if (blockIdx.x == 0 && p.counts) p.counts[i] = counts[i];
   }
   __syncthreads();
@@ -113,27 +114,36 @@ __global__ void __launch_bounds__(kBalanceThreads) balance_kernel(const BalanceP
   float sums[kPer];
 #pragma unroll
   for (int j = 0; j < kPer; ++j) sums[j] = 0.0f;
-  const int step = gridDim.x * kBalanceWarps;
-  for (int64_t t = blockIdx.x * kBalanceWarps + warp; t < p.tokens; t += step) {
-    bool any = false;
-    for (int k = lane; k < p.top_k; k += 32) {
-      const int32_t id = __ldg(p.ids + t * p.top_k + k);
-      any |= id >= 0 && id < experts;
-    }
-    if (!__any_sync(0xffffffffu, any)) {  // a padding token
-      if (p.dlogits) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps;
+  const T* logits = static_cast<const T*>(p.logits);
+  T* dlogits = static_cast<T*>(p.dlogits);
+  T next[kPer];
+  int32_t next_id = -1;
+  auto fetch = [&](int64_t t) {  // (top_k is at most 32)
+    next_id = lane < p.top_k ? __ldg(p.ids + t * p.top_k + lane) : -1;
 #pragma unroll
-        for (int j = 0; j < kPer; ++j)
-          if (lane + 32 * j < experts) put_gradient(p, t, lane + 32 * j, 0.0f);
-      }
-      continue;
-    }
+    for (int j = 0; j < kPer; ++j) next[j] = lane + 32 * j < experts ? logits[t * p.ld + lane + 32 * j] : from_f32<T>(-INFINITY);
+  };
+  int64_t t = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
+  if (t < p.tokens) fetch(t);
+  for (; t < p.tokens; t += step) {
     float x[kPer], most = -INFINITY;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-      x[j] = lane + 32 * j < experts ? logit_of(p, t, lane + 32 * j) : -INFINITY;
-      if (!(x[j] > -INFINITY)) x[j] = -INFINITY;  // (NaN: the expert is out)
+      const float v = to_f32(next[j]);
+      // (NaN: the expert is out; +inf counts as the largest number, as it does in routing)
+      x[j] = v > -INFINITY ? fminf(v, FLT_MAX) : -INFINITY;
       most = fmaxf(most, x[j]);
+    }
+    const bool live = __any_sync(0xffffffffu, next_id >= 0 && next_id < experts);
+    if (t + step < p.tokens) fetch(t + step);
+    if (!live) {  // a padding token
+      if (dlogits) {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+          if (lane + 32 * j < experts) dlogits[t * p.ldg + lane + 32 * j] = from_f32<T>(0.0f);
+      }
+      continue;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
@@ -146,11 +156,11 @@ __global__ void __launch_bounds__(kBalanceThreads) balance_kernel(const BalanceP
       rest[j] = 1.0f;
       float s;
       if (p.sigmoid) {
-        const float small = expf(-fabsf(x[j])), d = 1.0f + small;
-        s = expf(fminf(x[j], 0.0f) - shift) / d;
-        rest[j] = (x[j] >= 0.0f ? small : 1.0f) / d;  // 1 - s
+        const float small = exp_fast(-fabsf(x[j])), r = __fdividef(1.0f, 1.0f + small);
+        s = exp_fast(fminf(x[j], 0.0f) - shift) * r;
+        rest[j] = (x[j] >= 0.0f ? small : 1.0f) * r;  // 1 - s
       } else {
-        s = expf(x[j] - shift);
+        s = exp_fast(x[j] - shift);
       }
       x[j] = out ? 0.0f : s;
       total += x[j];
@@ -163,11 +173,12 @@ __global__ void __launch_bounds__(kBalanceThreads) balance_kernel(const BalanceP
       sums[j] += x[j];
       if (lane + 32 * j < experts) along = __fmaf_rn(x[j], share[lane + 32 * j], along);
     }
-    if (p.dlogits) {
+    if (dlogits) {
       along = warp_sum(along);
 #pragma unroll
       for (int j = 0; j < kPer; ++j)
-        if (lane + 32 * j < experts) put_gradient(p, t, lane + 32 * j, factor * (x[j] * rest[j] * (share[lane + 32 * j] - along)));
+        if (lane + 32 * j < experts)
+          dlogits[t * p.ldg + lane + 32 * j] = from_f32<T>(factor * (x[j] * rest[j] * (share[lane + 32 * j] - along)));
     }
   }
   if (p.loss == nullptr) return;
@@ -182,12 +193,12 @@ __global__ void __launch_bounds__(kBalanceThreads) balance_kernel(const BalanceP
     for (int j = 0; j < kPer; ++j)
       if (j >= j0 && j < j0 + kAtOnce) join[warp][lane + 32 * (j - j0)] = sums[j];
     __syncthreads();
-    for (int i = threadIdx.x; i < 32 * kAtOnce; i += kBalanceThreads) {
+    for (int i = threadIdx.x; i < 32 * kAtOnce; i += kThreads) {
       const int e = 32 * j0 + i;
       if (e >= experts) continue;
       float s = join[0][i];
 #pragma unroll
-      for (int w = 1; w < kBalanceWarps; ++w) s += join[w][i];
+      for (int w = 1; w < kWarps; ++w) s += join[w][i];
       if (alone) {
         term += static_cast<double>(counts[e]) * s;
       } else {
@@ -202,12 +213,18 @@ __global__ void __launch_bounds__(kBalanceThreads) balance_kernel(const BalanceP
     __syncthreads();
     if (!last) return;
     __threadfence();
-    for (int e = threadIdx.x; e < experts; e += kBalanceThreads) {
-      double s = 0.0;
-#pragma unroll 8
-      for (int b = 0; b < static_cast<int>(gridDim.x); ++b) s += __ldcg(p.part_scores + static_cast<int64_t>(b) * experts + e);
-      term += static_cast<double>(counts[e]) * s;
+    float own[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) own[j] = 0.0f;
+#pragma unroll 4
+    for (int b = warp; b < static_cast<int>(gridDim.x); b += kWarps) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j)
+        if (lane + 32 * j < experts) own[j] += __ldcg(p.part_scores + static_cast<int64_t>(b) * experts + lane + 32 * j);
     }
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+      if (lane + 32 * j < experts) term += static_cast<double>(counts[lane + 32 * j]) * own[j];
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) term += __shfl_xor_sync(0xffffffffu, term, o);
@@ -215,7 +232,7 @@ __global__ void __launch_bounds__(kBalanceThreads) balance_kernel(const BalanceP
   __syncthreads();
   if (threadIdx.x == 0) {
     double sum = 0.0;
-    for (int w = 0; w < kBalanceWarps; ++w) sum += terms[w];
+    for (int w = 0; w < kWarps; ++w) sum += terms[w];
     const double scale = pairs > 0 ? static_cast<double>(experts) / (static_cast<double>(pairs) * live_tokens) : 0.0;
     *p.loss = static_cast<float>(static_cast<double>(p.coefficient) * scale * sum);
   }

@@ -355,8 +355,8 @@ int gemm16_call(const cpuops_b200_gemm16_desc* d) {
 // ---- columns' sums -------------------------------------------------------------------------
 
 int launch_column_sum(const float* in, float* out0, float* out1, int parts, int n, int count, cudaStream_t stream) {
-  ColumnSumParams s{in, {out0, out1}, parts, n, count};
-  return launch_after(column_sum(), dim3(static_cast<unsigned>((n + 31) / 32), static_cast<unsigned>(count)), 1024, 0, stream, s);
+  ColumnSumParams s{in, out0, out1, parts, n};
+  return launch_after(column_sum(), dim3(static_cast<unsigned>((n + 31) / 32), static_cast<unsigned>(count)), 32 * std::min(16, parts), 0, stream, s);
 }
 
 // ---- gradient of bias and activation ----------------------------------------------------------
@@ -413,7 +413,7 @@ int epilogue_grad_call(const cpuops_b200_epilogue_grad_desc* d) {
   p.sums = d->dbias ? (parts ? parts : d->dbias) : nullptr;
   const bool wide = rows_aligned(d->dy, d->lddy, d->type) && (!act || rows_aligned(d->z, d->ldz, d->type)) &&
                     (!d->dz || rows_aligned(d->dz, d->lddz, d->type));
-  if (int rc = launch_after(epilogue_grad_of(d->type, wide), dim3(static_cast<unsigned>(strips), static_cast<unsigned>(blocks)), 256, 0,
+  if (int rc = launch_after(epilogue_grad_of(d->type, p.act, wide), dim3(static_cast<unsigned>(strips), static_cast<unsigned>(blocks)), 256, 0,
                             call.stream, p))
     return rc;
   if (parts)
@@ -462,10 +462,10 @@ int layer_norm_call(const cpuops_b200_layer_norm_desc* d) {
   p.n = d->n;
   p.eps = d->eps;
   const bool wide = rows_aligned(d->x, d->ldx, d->x_type) && rows_aligned(d->y, d->ldy, d->y_type);
-  const NormChoice c = norm_choice(d->x_type, d->y_type, d->n, wide, false);
+  const NormChoice c = norm_choice(d->x_type, d->y_type, d->n, wide, d->m >= 4 * call.st->sms(), false);
   const int rows = (d->m + c.rows_at_once - 1) / c.rows_at_once;
   const int grid = std::min(rows, call.st->sms() * std::max(1, std::min(16, 1024 / c.threads)));
-  if (int rc = launch_after(c.kernel, dim3(static_cast<unsigned>(grid)), c.threads, 0, call.stream, p)) return rc;
+  if (int rc = launch_after(c.kernel, dim3(static_cast<unsigned>(grid)), c.threads, static_cast<size_t>(c.smem), call.stream, p)) return rc;
   return call.finish();
 }
 
@@ -513,7 +513,7 @@ int layer_norm_grad_call(const cpuops_b200_layer_norm_grad_desc* d) {
   p.n = d->n;
   const bool wide = rows_aligned(d->x, d->ldx, d->x_type) && rows_aligned(d->dy, d->lddy, d->y_type) &&
                     rows_aligned(d->dx, d->lddx, d->x_type) && (!d->dr || rows_aligned(d->dr, d->lddr, d->x_type));
-  const NormChoice c = norm_choice(d->x_type, d->y_type, d->n, wide, true);
+  const NormChoice c = norm_choice(d->x_type, d->y_type, d->n, wide, d->m >= 4 * call.st->sms(), true);
   const int rows = std::max(1, (d->m + c.rows_at_once - 1) / c.rows_at_once);
   const int grid = std::min(rows, call.st->sms() * std::max(1, std::min(16, 512 / c.threads)));
   const bool sums = d->dgamma || d->dbeta, is_long = norm_is_long(d->n);
@@ -586,8 +586,9 @@ int balance_loss_call(const cpuops_b200_balance_loss_desc* d) {
   p.sigmoid = d->scoring == CPUOPS_B200_SCORE_SIGMOID ? 1 : 0;
   p.coefficient = d->coefficient;
   int grid = 1;
+  const int warps = balance_warps_of(d->experts);
   if (d->tokens > 32) {
-    grid = std::min((d->tokens + 7) / 8, 2 * call.st->sms());
+    grid = std::min((d->tokens + warps - 1) / warps, call.st->sms());
     p.count_blocks = std::min(64, (d->tokens + 255) / 256);
     Plan plan;
     const size_t off_ticket = plan.take(sizeof(int32_t));
@@ -600,7 +601,7 @@ int balance_loss_call(const cpuops_b200_balance_loss_desc* d) {
     p.part_scores = reinterpret_cast<float*>(ws + off_scores);
     if (int rc = launch_after(balance_count(), dim3(static_cast<unsigned>(p.count_blocks)), 256, 0, call.stream, p)) return rc;
   }
-  if (int rc = launch_after(balance_of(d->experts), dim3(static_cast<unsigned>(grid)), 256, 0, call.stream, p)) return rc;
+  if (int rc = launch_after(balance_of(d->logits_type, d->experts), dim3(static_cast<unsigned>(grid)), 32 * warps, 0, call.stream, p)) return rc;
   return call.finish();
 }
 

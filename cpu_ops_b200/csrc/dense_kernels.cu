@@ -19,7 +19,7 @@ int product_threads(int form, int epi_warps) { return form == kProductParts ? 22
 namespace {
 
 template <typename X, typename Y, bool kGradient>
-NormChoice norm_choice_for(int n, bool wide) {
+NormChoice norm_choice_for(int n, bool wide, bool many) {
   NormChoice c{};
   c.rows_at_once = 1;
   if (n > kNormMaxHeld) {
@@ -31,43 +31,71 @@ NormChoice norm_choice_for(int n, bool wide) {
     }
     return c;
   }
-  if (n <= 256) {
-    c.threads = 128;
-    c.rows_at_once = 4;
-    if constexpr (kGradient) {
-      c.kernel = wide ? norm_grad_kernel<X, Y, true, true, 1> : norm_grad_kernel<X, Y, false, true, 1>;
-    } else {
-      c.kernel = wide ? norm_kernel<X, Y, true, true, 1> : norm_kernel<X, Y, false, true, 1>;
-    }
-    return c;
-  }
-  const bool one = n <= 8 * kNormMaxThreads;
-  const int per = one ? 8 : 16;
-  c.threads = ((n + per - 1) / per + 31) / 32 * 32;
   if constexpr (kGradient) {
-    c.kernel = one ? (wide ? norm_grad_kernel<X, Y, true, false, 1> : norm_grad_kernel<X, Y, false, false, 1>)
-                   : (wide ? norm_grad_kernel<X, Y, true, false, 2> : norm_grad_kernel<X, Y, false, false, 2>);
+    if (n <= 256) {
+      c.threads = 128;
+      c.rows_at_once = 4;
+      c.kernel = wide ? norm_grad_kernel<X, Y, true, true, 1> : norm_grad_kernel<X, Y, false, true, 1>;
+      return c;
+    }
+    // (many rows: sixteen elements per thread, so that half as many threads share in a row's two sums)
+    const bool two = n > 8 * kNormMaxThreads || (many && n > 1024 && sizeof(X) == 2);
+    const int per = two ? 16 : 8;
+    c.threads = ((n + per - 1) / per + 31) / 32 * 32;
+    c.kernel = two ? (wide ? norm_grad_kernel<X, Y, true, false, 2> : norm_grad_kernel<X, Y, false, false, 2>)
+                   : (wide ? norm_grad_kernel<X, Y, true, false, 1> : norm_grad_kernel<X, Y, false, false, 1>);
   } else {
-    c.kernel = one ? (wide ? norm_kernel<X, Y, true, false, 1> : norm_kernel<X, Y, false, false, 1>)
-                   : (wide ? norm_kernel<X, Y, true, false, 2> : norm_kernel<X, Y, false, false, 2>);
+    if (n <= 256 || (many && n <= kNormWarpMost)) {
+      c.threads = 32 * kNormWarps;
+      c.rows_at_once = kNormWarps;
+      c.smem = 2 * ((n + 7) / 8 * 8) * static_cast<int>(sizeof(float));
+      c.kernel = n <= 256    ? (wide ? norm_rows_kernel<X, Y, true, 1> : norm_rows_kernel<X, Y, false, 1>)
+                 : n <= 1024 ? (wide ? norm_rows_kernel<X, Y, true, 4> : norm_rows_kernel<X, Y, false, 4>)
+                             : (wide ? norm_rows_kernel<X, Y, true, 16> : norm_rows_kernel<X, Y, false, 16>);
+      return c;
+    }
+    const bool two = n > 8 * kNormMaxThreads;
+    const int per = two ? 16 : 8;
+    c.threads = ((n + per - 1) / per + 31) / 32 * 32;
+    c.kernel = two ? (wide ? norm_kernel<X, Y, true, 2> : norm_kernel<X, Y, false, 2>)
+                   : (wide ? norm_kernel<X, Y, true, 1> : norm_kernel<X, Y, false, 1>);
   }
   return c;
 }
 
 template <bool kGradient>
-NormChoice norm_choice_of(int x_type, int y_type, int n, bool wide) {
-  if (x_type == kF16) return norm_choice_for<__half, __half, kGradient>(n, wide);
-  if (x_type == kBf16) return norm_choice_for<__nv_bfloat16, __nv_bfloat16, kGradient>(n, wide);
-  if (y_type == kF16) return norm_choice_for<float, __half, kGradient>(n, wide);
-  if (y_type == kBf16) return norm_choice_for<float, __nv_bfloat16, kGradient>(n, wide);
-  return norm_choice_for<float, float, kGradient>(n, wide);
+NormChoice norm_choice_of(int x_type, int y_type, int n, bool wide, bool many) {
+  if (x_type == kF16) return norm_choice_for<__half, __half, kGradient>(n, wide, many);
+  if (x_type == kBf16) return norm_choice_for<__nv_bfloat16, __nv_bfloat16, kGradient>(n, wide, many);
+  if (y_type == kF16) return norm_choice_for<float, __half, kGradient>(n, wide, many);
+  if (y_type == kBf16) return norm_choice_for<float, __nv_bfloat16, kGradient>(n, wide, many);
+  return norm_choice_for<float, float, kGradient>(n, wide, many);
+}
+
+template <typename T, bool kWide>
+EpilogueGradKernel epilogue_grad_for(int act) {
+  return act == kOpRelu   ? epilogue_grad_kernel<T, kOpRelu, kWide>
+         : act == kOpGelu ? epilogue_grad_kernel<T, kOpGelu, kWide>
+         : act == kOpSilu ? epilogue_grad_kernel<T, kOpSilu, kWide>
+                          : epilogue_grad_kernel<T, 0, kWide>;
+}
+
+template <typename T>
+BalanceKernel balance_for(int experts) {
+  const int per_lane = (experts + 31) / 32;
+  return per_lane <= 1   ? balance_kernel<T, 1>
+         : per_lane <= 2 ? balance_kernel<T, 2>
+         : per_lane <= 4 ? balance_kernel<T, 4>
+         : per_lane <= 8 ? balance_kernel<T, 8>
+         : per_lane <= 16 ? balance_kernel<T, 16>
+                          : balance_kernel<T, 32>;
 }
 
 }  // namespace
 
 bool norm_is_long(int n) { return n > kNormMaxHeld; }
-NormChoice norm_choice(int x_type, int y_type, int n, bool wide, bool gradient) {
-  return gradient ? norm_choice_of<true>(x_type, y_type, n, wide) : norm_choice_of<false>(x_type, y_type, n, wide);
+NormChoice norm_choice(int x_type, int y_type, int n, bool wide, bool many, bool gradient) {
+  return gradient ? norm_choice_of<true>(x_type, y_type, n, wide, many) : norm_choice_of<false>(x_type, y_type, n, wide, many);
 }
 NormColumnsKernel norm_grad_columns(int x_type, int y_type) {
   if (x_type == kF16) return norm_grad_columns_kernel<__half, __half>;
@@ -77,18 +105,17 @@ NormColumnsKernel norm_grad_columns(int x_type, int y_type) {
   return norm_grad_columns_kernel<float, float>;
 }
 
-EpilogueGradKernel epilogue_grad_of(int type, bool wide) {
-  if (type == kF32) return wide ? epilogue_grad_kernel<float, true> : epilogue_grad_kernel<float, false>;
-  if (type == kF16) return wide ? epilogue_grad_kernel<__half, true> : epilogue_grad_kernel<__half, false>;
-  return wide ? epilogue_grad_kernel<__nv_bfloat16, true> : epilogue_grad_kernel<__nv_bfloat16, false>;
+EpilogueGradKernel epilogue_grad_of(int type, int act, bool wide) {
+  if (type == kF32) return wide ? epilogue_grad_for<float, true>(act) : epilogue_grad_for<float, false>(act);
+  if (type == kF16) return wide ? epilogue_grad_for<__half, true>(act) : epilogue_grad_for<__half, false>(act);
+  return wide ? epilogue_grad_for<__nv_bfloat16, true>(act) : epilogue_grad_for<__nv_bfloat16, false>(act);
 }
 ColumnSumKernel column_sum() { return column_sum_kernel; }
 
 BalanceKernel balance_count() { return balance_count_kernel; }
-BalanceKernel balance_of(int experts) {
-  const int per_lane = (experts + 31) / 32;
-  return per_lane <= 1 ? balance_kernel<1> : per_lane <= 2 ? balance_kernel<2> : per_lane <= 4 ? balance_kernel<4>
-       : per_lane <= 8 ? balance_kernel<8> : per_lane <= 16 ? balance_kernel<16> : balance_kernel<32>;
+int balance_warps_of(int experts) { return balance_warps((experts + 31) / 32); }
+BalanceKernel balance_of(int type, int experts) {
+  return type == kF32 ? balance_for<float>(experts) : type == kF16 ? balance_for<__half>(experts) : balance_for<__nv_bfloat16>(experts);
 }
 
 }  // namespace b200

@@ -19,19 +19,22 @@ struct NormChoice {
   NormKernel kernel;
   int threads;
   int rows_at_once;  // of a CTA
+  int smem;
 };
-NormChoice norm_choice(int x_type, int y_type, int n, bool wide, bool gradient);
+// `many`: rows enough to give every warp one of its own (forward).
+NormChoice norm_choice(int x_type, int y_type, int n, bool wide, bool many, bool gradient);
 using NormColumnsKernel = void (*)(NormParams, int);
 NormColumnsKernel norm_grad_columns(int x_type, int y_type);
 bool norm_is_long(int n);
 
 using EpilogueGradKernel = void (*)(EpilogueGradParams);
-EpilogueGradKernel epilogue_grad_of(int type, bool wide);
+EpilogueGradKernel epilogue_grad_of(int type, int act, bool wide);
 using ColumnSumKernel = void (*)(ColumnSumParams);
 ColumnSumKernel column_sum();
 
 using BalanceKernel = void (*)(BalanceParams);
 BalanceKernel balance_count();
-BalanceKernel balance_of(int experts);
+BalanceKernel balance_of(int type, int experts);
+int balance_warps_of(int experts);  // of its CTAs
 
 }  // namespace b200

@@ -64,8 +64,9 @@ struct EpilogueGradParams {
 // Sum of `parts` rows of n, `parts * count` floats apart from one result to the next.
 struct ColumnSumParams {
   const float* in;
-  float* out[2];
-  int32_t parts, n, count;
+  float* out0;
+  float* out1;
+  int32_t parts, n;
 };
 
 // ---- layer norm ---------------------------------------------------------------------------------

@@ -21,7 +21,9 @@
 namespace b200 {
 
 constexpr int kNormMaxThreads = 512;
-constexpr int kNormMaxHeld = 16 * kNormMaxThreads;  // longest row that is held in registers
+constexpr int kNormMaxHeld = 16 * kNormMaxThreads;  // longest row that a CTA holds in registers
+constexpr int kNormWarpMost = 4096;                 // ... that a warp does
+constexpr int kNormWarps = 8;                       // rows that a CTA of norm_rows_kernel has in flight
 constexpr int kNormLongThreads = 1024;
 constexpr int kNormStrip = 256;      // columns of a CTA of the column kernels
 
@@ -41,9 +43,20 @@ __device__ __forceinline__ T from_f32(float v) {  // (rounded to nearest even)
 
 // Eight elements of a row in flight.  kWide: rows are 16-byte aligned; thread t of T holds the elements
 // 8 (t + T j) .. + 7; otherwise t + T i.  `left`: elements of the row from `p` on.
+// (held as the words they came in: an element takes a register of its own only while it is worked on)
 template <typename T>
-struct alignas(16) Eight {
-  T v[8];
+struct Eight {
+  uint32_t w[2 * sizeof(T)];
+  __device__ __forceinline__ float operator[](int i) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w[i]);
+    } else if constexpr (std::is_same<T, __half>::value) {
+      const __half2 h = *reinterpret_cast<const __half2*>(&w[i / 2]);
+      return i % 2 ? __high2float(h) : __low2float(h);
+    } else {
+      return __uint_as_float(i % 2 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+    }
+  }
 };
 template <typename T, bool kWide>
 __device__ __forceinline__ int element_of(int t, int threads, int j, int i) {
@@ -51,21 +64,33 @@ __device__ __forceinline__ int element_of(int t, int threads, int j, int i) {
 }
 template <typename T, bool kWide>
 __device__ __forceinline__ Eight<T> load_eight(const T* row, int n, int t, int threads, int j) {
+  using Word = typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type;
   Eight<T> e;
   if constexpr (kWide) {
     const int c = 8 * (t + threads * j);
     if (c + 8 <= n) {
       const uint4* src = reinterpret_cast<const uint4*>(row + c);
-      uint4* dst = reinterpret_cast<uint4*>(e.v);
 #pragma unroll
-      for (int w = 0; w < static_cast<int>(sizeof(T) / 2); ++w) dst[w] = src[w];
+      for (int h = 0; h < static_cast<int>(sizeof(T) / 2); ++h) {
+        const uint4 v = src[h];
+        e.w[4 * h] = v.x;
+        e.w[4 * h + 1] = v.y;
+        e.w[4 * h + 2] = v.z;
+        e.w[4 * h + 3] = v.w;
+      }
       return e;
     }
   }
+  const Word* words = reinterpret_cast<const Word*>(row);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int c = element_of<T, kWide>(t, threads, j, i);
-    e.v[i] = c < n ? row[c] : from_f32<T>(0.0f);
+    const uint32_t v = c < n ? static_cast<uint32_t>(words[c]) : 0u;
+    if constexpr (sizeof(T) == 4) {
+      e.w[i] = v;
+    } else {
+      e.w[i / 2] = i % 2 ? e.w[i / 2] | (v << 16) : v;
+    }
   }
   return e;
 }
@@ -74,13 +99,22 @@ __device__ __forceinline__ void store_eight(T* row, int n, int t, int threads, i
   if constexpr (kWide) {
     const int c = 8 * (t + threads * j);
     if (c + 8 <= n) {
-      Eight<T> e;
+      uint32_t w[2 * sizeof(T)];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) e.v[i] = from_f32<T>(v[i]);
+      for (int i = 0; i < static_cast<int>(2 * sizeof(T)); ++i) {
+        if constexpr (sizeof(T) == 4) {
+          w[i] = __float_as_uint(v[i]);
+        } else if constexpr (std::is_same<T, __half>::value) {
+          const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+          w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+          w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+      }
       uint4* dst = reinterpret_cast<uint4*>(row + c);
-      const uint4* src = reinterpret_cast<const uint4*>(e.v);
 #pragma unroll
-      for (int w = 0; w < static_cast<int>(sizeof(T) / 2); ++w) dst[w] = src[w];
+      for (int h = 0; h < static_cast<int>(sizeof(T) / 2); ++h) dst[h] = make_uint4(w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]);
       return;
     }
   }
@@ -115,53 +149,61 @@ __device__ __forceinline__ float block_sum(float v, float* slot) {
   return warp_sum(lane < warps ? slot[lane] : 0.0f);
 }
 
-// kWarp: every warp takes rows of its own (n <= 256 * kV); otherwise the CTA takes one row at a time.
-template <typename X, typename Y, bool kWide, bool kWarp, int kV>
-__global__ void __launch_bounds__(kWarp ? 128 : kNormMaxThreads) norm_kernel(const NormParams p) {
+// Subtracts the mean from eight elements (those beyond the row stay zero) and adds their squares up.
+template <typename X, bool kWide>
+__device__ __forceinline__ float centred_squares(float (&v)[8], float mean, int n, int t, int threads, int j, float square) {
+  if (kWide && 8 * (t + threads * j) + 8 <= n) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[i] -= mean;
+      square = __fmaf_rn(v[i], v[i], square);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[i] = element_of<X, kWide>(t, threads, j, i) < n ? v[i] - mean : 0.0f;
+      square = __fmaf_rn(v[i], v[i], square);
+    }
+  }
+  return square;
+}
+
+// One row per CTA at a time: few rows, or rows longer than a warp holds.
+template <typename X, typename Y, bool kWide, int kV>
+__global__ void __launch_bounds__(kNormMaxThreads) norm_kernel(const NormParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ float slots[4][32];
-  const int threads = kWarp ? 32 : static_cast<int>(blockDim.x);
-  const int t = kWarp ? threadIdx.x & 31 : threadIdx.x;
-  const int first = kWarp ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
-  const int step = kWarp ? gridDim.x * 4 : gridDim.x;
+  const int threads = blockDim.x, t = threadIdx.x;
   const float inverse = 1.0f / static_cast<float>(p.n);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (first >= p.m) return;
   float gamma[kV][8], beta[kV][8];
   Eight<X> next[kV];
   const X* x = static_cast<const X*>(p.x);
 #pragma unroll
-  for (int j = 0; j < kV; ++j) next[j] = load_eight<X, kWide>(x + first * p.ldx, p.n, t, threads, j);
+  for (int j = 0; j < kV; ++j) next[j] = load_eight<X, kWide>(x + blockIdx.x * p.ldx, p.n, t, threads, j);
 #pragma unroll
   for (int j = 0; j < kV; ++j) {
     load_vector<kWide>(p.gamma, p.n, t, threads, j, 1.0f, gamma[j]);
     load_vector<kWide>(p.beta, p.n, t, threads, j, 0.0f, beta[j]);
   }
   int turn = 0;
-  for (int64_t row = first; row < p.m; row += step, turn ^= 2) {
-    float v[kV][8], sum = 0.0f;
+  for (int64_t row = blockIdx.x; row < p.m; row += gridDim.x, turn ^= 2) {
+    float v[kV][8], sum = 0.0f, square = 0.0f;
 #pragma unroll
     for (int j = 0; j < kV; ++j)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        v[j][i] = to_f32(next[j].v[i]);
+        v[j][i] = next[j][i];
         sum += v[j][i];
       }
-    if (row + step < p.m) {
+    if (row + gridDim.x < p.m) {
 #pragma unroll
-      for (int j = 0; j < kV; ++j) next[j] = load_eight<X, kWide>(x + (row + step) * p.ldx, p.n, t, threads, j);
+      for (int j = 0; j < kV; ++j) next[j] = load_eight<X, kWide>(x + (row + gridDim.x) * p.ldx, p.n, t, threads, j);
     }
-    const float mean = (kWarp ? warp_sum(sum) : block_sum(sum, slots[turn])) * inverse;
-    float square = 0.0f;
+    const float mean = block_sum(sum, slots[turn]) * inverse;
 #pragma unroll
-    for (int j = 0; j < kV; ++j)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[j][i] = element_of<X, kWide>(t, threads, j, i) < p.n ? v[j][i] - mean : 0.0f;
-        square = __fmaf_rn(v[j][i], v[j][i], square);
-      }
-    const float var = (kWarp ? warp_sum(square) : block_sum(square, slots[turn + 1])) * inverse;
-    const float rstd = 1.0f / sqrtf(var + p.eps);
+    for (int j = 0; j < kV; ++j) square = centred_squares<X, kWide>(v[j], mean, p.n, t, threads, j, square);
+    const float rstd = 1.0f / sqrtf(block_sum(square, slots[turn + 1]) * inverse + p.eps);
     if (t == 0) {
       if (p.mean) p.mean[row] = mean;
       if (p.rstd) p.rstd[row] = rstd;
@@ -173,6 +215,83 @@ __global__ void __launch_bounds__(kWarp ? 128 : kNormMaxThreads) norm_kernel(con
 #pragma unroll
       for (int i = 0; i < 8; ++i) r[i] = __fmaf_rn(v[j][i] * rstd, gamma[j][i], beta[j][i]);
       store_eight<Y, kWide>(y, p.n, t, threads, j, r);
+    }
+  }
+}
+
+// One row per warp at a time, n <= 256 * kV: sums need no barrier, and each of the SM's warps has a whole row on its
+// way.  gamma and beta lie in shared memory (2 n floats).
+template <typename X, typename Y, bool kWide, int kV>
+__global__ void __launch_bounds__(32 * kNormWarps, sizeof(X) == 2 || kV < 16 ? 2 : 1) norm_rows_kernel(const NormParams p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  extern __shared__ __align__(16) float weights[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float inverse = 1.0f / static_cast<float>(p.n);
+  const int room = (p.n + 7) / 8 * 8;  // (whole vectors of eight)
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (int c = threadIdx.x; c < room; c += 32 * kNormWarps) {
+    weights[c] = p.gamma != nullptr && c < p.n ? __ldg(p.gamma + c) : 1.0f;
+    weights[room + c] = p.beta != nullptr && c < p.n ? __ldg(p.beta + c) : 0.0f;
+  }
+  __syncthreads();
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kNormWarps;
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kNormWarps + warp; row < p.m; row += step) {
+    const X* x = static_cast<const X*>(p.x) + row * p.ldx;
+    Eight<X> raw[kV];
+#pragma unroll
+    for (int j = 0; j < kV; ++j)
+      if (256 * j < p.n) raw[j] = load_eight<X, kWide>(x, p.n, lane, 32, j);
+    float sum = 0.0f, square = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kV; ++j) {
+      if (256 * j >= p.n) continue;
+      float part = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) part += raw[j][i];
+      sum += part;
+    }
+    const float mean = warp_sum(sum) * inverse;
+#pragma unroll
+    for (int j = 0; j < kV; ++j) {
+      if (256 * j >= p.n) continue;
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = raw[j][i];
+      square += centred_squares<X, kWide>(v, mean, p.n, lane, 32, j, 0.0f);
+    }
+    const float rstd = 1.0f / sqrtf(warp_sum(square) * inverse + p.eps);
+    if (lane == 0) {
+      if (p.mean) p.mean[row] = mean;
+      if (p.rstd) p.rstd[row] = rstd;
+    }
+    Y* y = static_cast<Y*>(p.y) + row * p.ldy;
+#pragma unroll
+    for (int j = 0; j < kV; ++j) {
+      if (256 * j >= p.n) continue;
+      float r[8];
+      if constexpr (kWide) {
+        const int c = 8 * (lane + 32 * j);
+        if (c < p.n) {
+          const float4* g = reinterpret_cast<const float4*>(weights + c);
+          const float4* b = reinterpret_cast<const float4*>(weights + room + c);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float4 gg = g[h], bb = b[h];
+            r[4 * h] = __fmaf_rn((raw[j][4 * h] - mean) * rstd, gg.x, bb.x);
+            r[4 * h + 1] = __fmaf_rn((raw[j][4 * h + 1] - mean) * rstd, gg.y, bb.y);
+            r[4 * h + 2] = __fmaf_rn((raw[j][4 * h + 2] - mean) * rstd, gg.z, bb.z);
+            r[4 * h + 3] = __fmaf_rn((raw[j][4 * h + 3] - mean) * rstd, gg.w, bb.w);
+          }
+          store_eight<Y, kWide>(y, p.n, lane, 32, j, r);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int c = min(element_of<X, kWide>(lane, 32, j, i), p.n - 1);
+          r[i] = __fmaf_rn((raw[j][i] - mean) * rstd, weights[c], weights[room + c]);
+        }
+        store_eight<Y, kWide>(y, p.n, lane, 32, j, r);
+      }
     }
   }
 }
@@ -208,11 +327,13 @@ __global__ void __launch_bounds__(kNormLongThreads) norm_long_kernel(const NormP
   }
 }
 
-// X: the type of x, dx and dr; Y: of dy.  The columns' sums of a CTA's rows go to its row of p.sums.
+// X: the type of x, dx and dr; Y: of dy.  The columns' sums of a CTA's rows go to its row of p.sums.  A row's elements
+// stay as they were loaded between its sums and its result, and the next row is on its way meanwhile.
+// kWarp: every warp takes rows of its own (n <= 256).
 template <typename X, typename Y, bool kWide, bool kWarp, int kV>
 __global__ void __launch_bounds__(kWarp ? 128 : kNormMaxThreads) norm_grad_kernel(const NormParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  __shared__ float slots[4][32];
+  __shared__ float2 slots[2][32];
   __shared__ float join[kWarp ? 4 : 1][kWarp ? 256 : 1];
   const int threads = kWarp ? 32 : static_cast<int>(blockDim.x);
   const int t = kWarp ? threadIdx.x & 31 : threadIdx.x;
@@ -220,16 +341,9 @@ __global__ void __launch_bounds__(kWarp ? 128 : kNormMaxThreads) norm_grad_kerne
   const int step = kWarp ? gridDim.x * 4 : gridDim.x;
   const float inverse = 1.0f / static_cast<float>(p.n);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  float gamma[kV][8], dgamma[kV][8], dbeta[kV][8];
-#pragma unroll
-  for (int j = 0; j < kV; ++j) {
-    load_vector<kWide>(p.gamma, p.n, t, threads, j, 1.0f, gamma[j]);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) dgamma[j][i] = dbeta[j][i] = 0.0f;
-  }
   const X* x = static_cast<const X*>(p.x);
   const Y* dy = static_cast<const Y*>(p.dy);
-  Eight<X> next_x[kV];
+  Eight<X> next_x[kV], next_dr[kV];
   Eight<Y> next_dy[kV];
   float next_mean = 0.0f, next_rstd = 0.0f;
   auto fetch = [&](int64_t row) {
@@ -237,47 +351,52 @@ __global__ void __launch_bounds__(kWarp ? 128 : kNormMaxThreads) norm_grad_kerne
     for (int j = 0; j < kV; ++j) {
       next_x[j] = load_eight<X, kWide>(x + row * p.ldx, p.n, t, threads, j);
       next_dy[j] = load_eight<Y, kWide>(dy + row * p.lddy, p.n, t, threads, j);
+      if (p.dr) next_dr[j] = load_eight<X, kWide>(static_cast<const X*>(p.dr) + row * p.lddr, p.n, t, threads, j);
     }
     next_mean = __ldg(p.mean_in + row);
     next_rstd = __ldg(p.rstd_in + row);
   };
   if (first < p.m) fetch(first);
-  int turn = 0;
-  for (int64_t row = first; row < p.m; row += step, turn ^= 2) {
-    float xhat[kV][8], g[kV][8], sum = 0.0f, along = 0.0f;
-    const float mean = next_mean, rstd = next_rstd;
-    Eight<X> dr[kV];
-    if (p.dr) {
+  float gamma[kV][8], dgamma[kV][8], dbeta[kV][8];
 #pragma unroll
-      for (int j = 0; j < kV; ++j) dr[j] = load_eight<X, kWide>(static_cast<const X*>(p.dr) + row * p.lddr, p.n, t, threads, j);
+  for (int j = 0; j < kV; ++j) {
+    load_vector<kWide>(p.gamma, p.n, t, threads, j, 1.0f, gamma[j]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dgamma[j][i] = dbeta[j][i] = 0.0f;
+  }
+  int turn = 0;
+  for (int64_t row = first; row < p.m; row += step, turn ^= 1) {
+    float sum = 0.0f, along = 0.0f;
+    const float mean = next_mean, rstd = next_rstd;
+    Eight<X> this_x[kV], this_dr[kV];
+    Eight<Y> this_dy[kV];
+#pragma unroll
+    for (int j = 0; j < kV; ++j) {
+      this_x[j] = next_x[j];
+      this_dy[j] = next_dy[j];
+      if (p.dr) this_dr[j] = next_dr[j];
     }
+    if (row + step < p.m) fetch(row + step);
+    // (elements beyond the row: dy is zero, and with it all that is added up)
 #pragma unroll
     for (int j = 0; j < kV; ++j)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float d = to_f32(next_dy[j].v[i]);
-        xhat[j][i] = element_of<X, kWide>(t, threads, j, i) < p.n ? (to_f32(next_x[j].v[i]) - mean) * rstd : 0.0f;
-        g[j][i] = d * gamma[j][i];
-        dgamma[j][i] = __fmaf_rn(d, xhat[j][i], dgamma[j][i]);
+        const float d = this_dy[j][i], xhat = (this_x[j][i] - mean) * rstd, g = d * gamma[j][i];
+        dgamma[j][i] = __fmaf_rn(d, xhat, dgamma[j][i]);
         dbeta[j][i] += d;
-        sum += g[j][i];
-        along = __fmaf_rn(g[j][i], xhat[j][i], along);
+        sum += g;
+        along = __fmaf_rn(g, xhat, along);
       }
-    if (row + step < p.m) fetch(row + step);
-    if constexpr (kWarp) {
-      sum = warp_sum(sum);
-      along = warp_sum(along);
-    } else {
-      sum = warp_sum(sum);
-      along = warp_sum(along);
+    sum = warp_sum(sum);
+    along = warp_sum(along);
+    if constexpr (!kWarp) {
       const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-      if (lane == 0) {
-        slots[turn][warp] = sum;
-        slots[turn + 1][warp] = along;
-      }
+      if (lane == 0) slots[turn][warp] = make_float2(sum, along);
       __syncthreads();
-      sum = warp_sum(lane < warps ? slots[turn][lane] : 0.0f);
-      along = warp_sum(lane < warps ? slots[turn + 1][lane] : 0.0f);
+      const float2 v = lane < warps ? slots[turn][lane] : make_float2(0.0f, 0.0f);
+      sum = warp_sum(v.x);
+      along = warp_sum(v.y);
     }
     sum *= inverse;
     along *= inverse;
@@ -287,8 +406,9 @@ __global__ void __launch_bounds__(kWarp ? 128 : kNormMaxThreads) norm_grad_kerne
       float r[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        r[i] = rstd * (g[j][i] - __fmaf_rn(xhat[j][i], along, sum));
-        if (p.dr) r[i] += to_f32(dr[j].v[i]);
+        const float xhat = (this_x[j][i] - mean) * rstd;
+        r[i] = rstd * (this_dy[j][i] * gamma[j][i] - __fmaf_rn(xhat, along, sum));
+        if (p.dr) r[i] += this_dr[j][i];
       }
       store_eight<X, kWide>(dx, p.n, t, threads, j, r);
     }
@@ -309,7 +429,7 @@ __global__ void __launch_bounds__(kWarp ? 128 : kNormMaxThreads) norm_grad_kerne
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < kV; ++j)
+    for (int j = 0; j < kV; ++j) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int c = element_of<X, kWide>(t, threads, j, i);
@@ -318,6 +438,7 @@ __global__ void __launch_bounds__(kWarp ? 128 : kNormMaxThreads) norm_grad_kerne
           out[c + other] = dbeta[j][i];
         }
       }
+    }
   }
 }
 
@@ -376,29 +497,47 @@ __global__ void __launch_bounds__(kNormStrip) norm_grad_columns_kernel(const Nor
 
 // ---- gradient of bias and activation --------------------------------------------------------
 
+// min and max that keep a NaN.
+__device__ __forceinline__ float clamp_nan(float v, float most) {
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(v) : "f"(most));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(v) : "f"(-most));
+  return v;
+}
 // act'(z).  Beyond the clamps the slopes are 0 or 1 to the last bit of f32, and the products of an infinity
 // and a zero that the formulas have there are not formed.  t = exp(-|v|) gives both the logistic and one
-// minus it without a cancellation.
-__device__ __forceinline__ float activation_slope(float z, int act) {
-  if (act == kOpRelu) return z <= 0.0f ? 0.0f : 1.0f;
-  const bool gelu = act == kOpGelu;
-  const float most = gelu ? 12.0f : 100.0f;
-  z = z > most ? most : (z < -most ? -most : z);  // (NaN stays)
-  float v = z, slope = 1.0f;
-  if (gelu) {
-    const float c = 2.0f * 0.7978845608028654f, zz = z * z;
-    v = c * z * __fmaf_rn(0.044715f, zz, 1.0f);
-    slope = c * __fmaf_rn(3.0f * 0.044715f, zz, 1.0f);
+// minus it without a cancellation.  exp2 of a rounded product is exact enough: the product's rounding, |v| eps / 2 of t,
+// is at most eps / 5 of one, and the approximate exp2 and reciprocal are within 2 ulp: together 3e-7 of dy.
+template <int kAct>
+__device__ __forceinline__ float activation_slope(float z) {
+  if constexpr (kAct == kOpRelu) return z <= 0.0f ? 0.0f : 1.0f;
+  constexpr bool kGelu = kAct == kOpGelu;
+  z = clamp_nan(z, kGelu ? 12.0f : 100.0f);
+  float v = z, w = z;  // the logistic's argument, and z times its slope
+  if constexpr (kGelu) {
+    constexpr float c = 2.0f * 0.7978845608028654f;
+    const float zz = z * z;
+    v = z * __fmaf_rn(c * 0.044715f, zz, c);
+    w = z * __fmaf_rn(c * 3.0f * 0.044715f, zz, c);
   }
-  const float t = expf(-fabsf(v)), big = __fdividef(1.0f, 1.0f + t), small = t * big;
+  float t, big;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fabsf(v) * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(big) : "f"(1.0f + t));
+  const float small = t * big;
   const float s = v >= 0.0f ? big : small, rest = v >= 0.0f ? small : big;
-  return s * __fmaf_rn(z * slope, rest, 1.0f);
+  return s * __fmaf_rn(w, rest, 1.0f);
+}
+
+template <int kAct>
+__device__ __forceinline__ float slope_times(float dy, float z) {
+  if constexpr (kAct == 0) return dy;
+  if constexpr (kAct == kOpRelu) return z <= 0.0f ? 0.0f : dy;
+  return dy * activation_slope<kAct>(z);
 }
 
 // A warp takes rows of the CTA's strip of 256 columns in turn, eight columns per lane: loads and stores of whole
 // rows' pieces, the columns' sums in registers until the CTA's rows are done.
-template <typename T, bool kWide>
-__global__ void __launch_bounds__(256) epilogue_grad_kernel(const EpilogueGradParams p) {
+template <typename T, int kAct, bool kWide>
+__global__ void __launch_bounds__(256, sizeof(T) == 2 && kWide ? 4 : 3) epilogue_grad_kernel(const EpilogueGradParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ float join[8][kNormStrip];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -407,36 +546,35 @@ __global__ void __launch_bounds__(256) epilogue_grad_kernel(const EpilogueGradPa
   const int64_t begin = static_cast<int64_t>(blockIdx.y) * p.block_rows;
   const int64_t end = min(begin + p.block_rows, static_cast<int64_t>(p.m));
   const T* dy = static_cast<const T*>(p.dy) + c0;
-  const T* z = static_cast<const T*>(p.z) + c0;
-  T* dz = static_cast<T*>(p.dz) + c0;
+  const T* z = kAct ? static_cast<const T*>(p.z) + c0 : nullptr;
+  T* dz = p.dz ? static_cast<T*>(p.dz) + c0 : nullptr;
   float sums[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  auto finish = [&](int64_t row, const Eight<T>& a, const Eight<T>& b) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[i] = slope_times<kAct>(a[i], kAct ? b[i] : 0.0f);
+      sums[i] += v[i];
+    }
+    if (kAct || dz) store_eight<T, kWide>(dz + row * p.lddz, n, lane, 32, 0, v);
+  };
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  constexpr int kRows = 4;  // in flight per warp
-  for (int64_t r0 = begin + warp; r0 < end; r0 += 8 * kRows) {
-    Eight<T> a[kRows], b[kRows];
+  int64_t row = begin + warp;
+  for (; row + 8 < end; row += 16) {  // two rows in flight
+    Eight<T> a[2], b[2];
 #pragma unroll
-    for (int k = 0; k < kRows; ++k) {
-      const int64_t row = r0 + 8 * k;
-      if (row >= end) break;
-      a[k] = load_eight<T, kWide>(dy + row * p.lddy, n, lane, 32, 0);
-      if (p.z) b[k] = load_eight<T, kWide>(z + row * p.ldz, n, lane, 32, 0);
+    for (int k = 0; k < 2; ++k) {
+      a[k] = load_eight<T, kWide>(dy + (row + 8 * k) * p.lddy, n, lane, 32, 0);
+      if (kAct) b[k] = load_eight<T, kWide>(z + (row + 8 * k) * p.ldz, n, lane, 32, 0);
     }
 #pragma unroll
-    for (int k = 0; k < kRows; ++k) {
-      const int64_t row = r0 + 8 * k;
-      if (row >= end) break;
-      float v[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[i] = to_f32(a[k].v[i]);
-        if (p.z) {
-          const float s = activation_slope(to_f32(b[k].v[i]), p.act);
-          v[i] = p.act == kOpRelu && s == 0.0f ? 0.0f : v[i] * s;
-        }
-        sums[i] += v[i];
-      }
-      if (p.dz) store_eight<T, kWide>(dz + row * p.lddz, n, lane, 32, 0, v);
-    }
+    for (int k = 0; k < 2; ++k) finish(row + 8 * k, a[k], b[k]);
+  }
+  if (row < end) {
+    const Eight<T> a = load_eight<T, kWide>(dy + row * p.lddy, n, lane, 32, 0);
+    Eight<T> b = a;
+    if (kAct) b = load_eight<T, kWide>(z + row * p.ldz, n, lane, 32, 0);
+    finish(row, a, b);
   }
   if (p.sums == nullptr) return;
 #pragma unroll
@@ -452,25 +590,26 @@ __global__ void __launch_bounds__(256) epilogue_grad_kernel(const EpilogueGradPa
 }
 
 // Block (x, y): 32 columns of result y; its warps take the parts in turn.
-__global__ void __launch_bounds__(1024) column_sum_kernel(const ColumnSumParams p) {
+__global__ void __launch_bounds__(512) column_sum_kernel(const ColumnSumParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  __shared__ float join[32][33];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ float join[16][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  float* out = p.out[blockIdx.y];
+  float* out = blockIdx.y == 0 ? p.out0 : p.out1;
   if (out == nullptr) return;
   float sum = 0.0f;
   if (c < p.n) {
     const float* in = p.in + static_cast<int64_t>(blockIdx.y) * p.parts * p.n + c;
-#pragma unroll 4
-    for (int i = warp; i < p.parts; i += 32) sum += __ldcg(in + static_cast<int64_t>(i) * p.n);
+#pragma unroll 8
+    for (int i = warp; i < p.parts; i += warps) sum += __ldcg(in + static_cast<int64_t>(i) * p.n);
   }
   join[warp][lane] = sum;
   __syncthreads();
-  sum = warp_sum(join[lane][warp]);  // warp w: column w
-  const int64_t column = static_cast<int64_t>(blockIdx.x) * 32 + warp;
-  if (lane == 0 && column < p.n) out[column] = sum;
+  if (warp == 0 && c < p.n) {
+    for (int w = 1; w < warps; ++w) sum += join[w][lane];
+    out[c] = sum;
+  }
 }
 
 }  // namespace b200

@@ -83,6 +83,19 @@ __device__ __forceinline__ ProductTile product_tile(const ProductParams& p, int 
   return c;
 }
 
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_float(float v) {
+  if constexpr (std::is_same<T, float>::value) {
+    return v;
+  } else if constexpr (std::is_same<T, __half>::value) {
+    return __float2half_rn(v);
+  } else {
+    return __float2bfloat16_rn(v);
+  }
+}
 __device__ __forceinline__ float load_as_f32(const void* base, int64_t i, int type) {
   if (type == kF32) return static_cast<const float*>(base)[i];
   if (type == kF16) return __half2float(static_cast<const __half*>(base)[i]);
@@ -210,28 +223,50 @@ __device__ __forceinline__ void activate_chunk(uint32_t (&r)[32], int act) {
 }
 
 // Where C, D or Z cannot be addressed by TMA: a chunk's f32 values (in shared memory, put there by
-// put_chunk_row) leave row by row, lane = column, and C is read the same way.
+// put_chunk_row) leave row by row, lane = column, and C is read the same way, all of a chunk's rows at once.
+template <int kRows>
+__device__ __forceinline__ void load_c_rows(const ProductParams& p, int row0, int col0, int lane, float (&c)[kRows]) {
+  const int nrows = lane < p.Nk - col0 ? p.Mk - row0 : 0;
+  const int64_t at = static_cast<int64_t>(row0) * p.ldc + col0 + lane;
+  auto rows = [&](auto* base) {
+    base += at;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) c[r] = r < nrows ? to_float(base[r * p.ldc]) : 0.0f;
+  };
+  if (p.c_type == kF32) {
+    rows(static_cast<const float*>(p.C));
+  } else if (p.c_type == kF16) {
+    rows(static_cast<const __half*>(p.C));
+  } else {
+    rows(static_cast<const __nv_bfloat16*>(p.C));
+  }
+}
+// Rows r0 .. r0 + kRows of the chunk whose first row and column are row0 and col0.
+template <int kRows>
 __device__ __forceinline__ void write_chunk_rows(const ProductParams& p, uint32_t buf, void* dst, int64_t ld, bool add_c,
-                                                 int row0, int col0, int lane) {
-  const int nrows = lane < p.Nk - col0 ? min(32, p.Mk - row0) : 0;
-#pragma unroll 1
-  for (int r0 = 0; r0 < 32; r0 += 8) {
-    float v[8], c[8];
+                                                 const float (&c)[kRows], int r0, int row0, int col0, int lane) {
+  const int nrows = lane < p.Nk - col0 ? p.Mk - row0 - r0 : 0;
+  const int64_t at = static_cast<int64_t>(row0 + r0) * ld + col0 + lane;
+  auto rows = [&](auto* base) {
+    using T = std::remove_pointer_t<decltype(base)>;
+    base += at;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int r = r0 + j;
+    for (int i = 0; i < kRows; ++i) {
+      const int r = r0 + i;
+      float v;
       asm volatile("ld.shared.f32 %0, [%1];"
-                   : "=f"(v[j])
+                   : "=f"(v)
                    : "r"(buf + static_cast<uint32_t>(r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4)));
-      c[j] = 0.0f;
-      if (add_c && r < nrows) c[j] = load_as_f32(p.C, static_cast<int64_t>(row0 + r) * p.ldc + col0 + lane, p.c_type);
+      if (add_c) v = __fmaf_rn(p.beta, c[i], v);
+      if (i < nrows) base[i * ld] = from_float<T>(v);
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (r0 + j >= nrows) continue;
-      store_from_f32(dst, static_cast<int64_t>(row0 + r0 + j) * ld + col0 + lane, p.d_type,
-                     add_c ? __fmaf_rn(p.beta, c[j], v[j]) : v[j]);
-    }
+  };
+  if (p.d_type == kF32) {
+    rows(static_cast<float*>(dst));
+  } else if (p.d_type == kF16) {
+    rows(static_cast<__half*>(dst));
+  } else {
+    rows(static_cast<__nv_bfloat16*>(dst));
   }
 }
 
@@ -543,17 +578,26 @@ __global__ void __launch_bounds__(kForm == kProductParts ? 224 : kProductThreads
         }
         if (++d_b == depth) d_b = 0;
       } else if (inside) {
+        // (the pieces' sums leave registers for a few rows of C at a time only)
+        constexpr int kRows = kPieces ? 4 : 32;
+        float cc[kRows];
+        if (!kPieces && has_c) load_c_rows(p, row0, col0, lane, cc);
         __syncwarp();  // every lane has read the chunk before
         if (has_z) {
           put_chunk_row(ring, lane, r, kF32);
           __syncwarp();
-          write_chunk_rows(p, ring, p.Z, p.ldz, false, row0, col0, lane);
+#pragma unroll 1
+          for (int r0 = 0; r0 < 32; r0 += kRows) write_chunk_rows(p, ring, p.Z, p.ldz, false, cc, r0, row0, col0, lane);
           __syncwarp();
         }
         activate_chunk(r, p.act);
         put_chunk_row(ring, lane, r, kF32);
         __syncwarp();
-        write_chunk_rows(p, ring, p.D, p.ldd, has_c, row0, col0, lane);
+#pragma unroll 1
+        for (int r0 = 0; r0 < 32; r0 += kRows) {
+          if (kPieces && has_c) load_c_rows(p, row0 + r0, col0, lane, cc);
+          write_chunk_rows(p, ring, p.D, p.ldd, has_c, cc, r0, row0, col0, lane);
+        }
       }
       return true;
     };
