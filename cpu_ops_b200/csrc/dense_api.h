@@ -77,17 +77,18 @@ int product_clusters(DeviceState& st, int form, int size) {
 
 struct ProductChoice {
   int form = kProductTiles, BN = 128, parts = 1, stages = 0, epi_warps = kProductEpiWarps, ring_bytes = 0, ring_depth = 1;
+  int tile_rows = 128;
   bool swapped = false;
 };
 
 // Shared memory of a choice: stages, epilogue warps and their buffers.  `chunks`: bytes of one chunk each of C, D and
 // Z (0: not by TMA).  False: it does not fit.
 bool fit_product(ProductChoice& c, int smem_optin, int chunks, int k_blocks, bool pieces) {
-  const int room = smem_optin - 1024 - kProductBarrierBytes;
+  const int room = smem_optin - 1024 - kProductBarrierBytes - 4 * kProductBiasFloats;
   const int stage = (kTileM + c.BN / (c.form == kProductPairs ? 2 : 1)) * 128;
   if (c.form == kProductParts) {
-    c.epi_warps = 4;  // the owners' sums: a slab per part, rows of own + 1 columns at most
-    c.ring_bytes = ((c.BN + c.parts) * 512 / 4 + 1023) / 1024 * 1024;
+    c.epi_warps = 4;  // (together: the sums of an owner's columns from all parts)
+    c.ring_bytes = c.BN * kTileM;
     c.stages = (room - 4 * c.ring_bytes) / stage;
   } else {
     // Eight epilogue warps with two buffers for each matrix, unless that leaves the ring of stages short: then one
@@ -106,7 +107,7 @@ bool fit_product(ProductChoice& c, int smem_optin, int chunks, int k_blocks, boo
 
 // Estimated cycles; the least of all choices is taken.
 double product_cycles(const ProductChoice& c, const DeviceState& st, int Mk, int Nk, int k_blocks) {
-  const int tile_m = c.form == kProductPairs ? 256 : 128;
+  const int tile_m = c.form == kProductPairs ? 256 : c.tile_rows;
   const int64_t tiles = static_cast<int64_t>((Mk + tile_m - 1) / tile_m) * ((Nk + c.BN - 1) / c.BN);
   const int ctas = c.form == kProductPairs ? 2 : c.parts;
   const int64_t slots = std::max(1, st.sms() / ctas);
@@ -177,6 +178,7 @@ int gemm16_call(const cpuops_b200_gemm16_desc* d) {
   p.ldc = d->ldc;
   p.ldd = d->ldd;
   p.ldz = d->ldz;
+  p.type = d->type;
   p.c_type = d->c_type;
   p.d_type = d->d_type;
   p.error = st.error_dev;
@@ -225,7 +227,16 @@ int gemm16_call(const cpuops_b200_gemm16_desc* d) {
     if ((d->flags & CPUOPS_B200_FLAG_PAIR_OFF) && form == kProductPairs) return;
     if (form != kProductTiles && product_clusters(st, form, form == kProductPairs ? 2 : parts) < 1) return;
     if (!fit_product(c, st.smem_optin, chunks, k_blocks, pieces)) return;
-    const double cycles = product_cycles(c, st, swapped ? d->n : d->m, swapped ? d->m : d->n, k_blocks);
+    const int Mk = swapped ? d->n : d->m, Nk = swapped ? d->m : d->n;
+    if (form == kProductParts && !(swapped ? b.mn : a.mn)) {
+      // Tiles of fewer rows where that gives every cluster one (a tile's other rows are neither loaded nor used):
+      // 8 x 14336 x 4096 as 138 tiles of 104 rows instead of 112 of 128.
+      const int64_t columns = (Nk + BN - 1) / BN, clusters = std::max<int64_t>(1, std::min(product_clusters(st, form, parts), st.sms() / parts));
+      const int64_t tiles = (Mk + 127) / 128 * columns, rounds = (tiles + clusters - 1) / clusters;
+      const int64_t along_m = std::max<int64_t>(1, rounds * clusters / columns);
+      c.tile_rows = static_cast<int>(std::min<int64_t>(128, ((Mk + along_m - 1) / along_m + 7) / 8 * 8));
+    }
+    const double cycles = product_cycles(c, st, Mk, Nk, k_blocks);
     if (!found || cycles < least) {
       best = c;
       least = cycles;
@@ -283,7 +294,9 @@ int gemm16_call(const cpuops_b200_gemm16_desc* d) {
   p.swapped = c.swapped ? 1 : 0;
   p.Mk = c.swapped ? d->n : d->m;
   p.Nk = c.swapped ? d->m : d->n;
-  p.m_tiles = (p.Mk + tile_m - 1) / tile_m;
+  const int tile_rows = c.form == kProductParts ? c.tile_rows : tile_m;
+  p.tile_rows = tile_rows;
+  p.m_tiles = (p.Mk + tile_rows - 1) / tile_rows;
   p.n_tiles = (p.Nk + c.BN - 1) / c.BN;
   p.BN = c.BN;
   p.stages = c.stages;
@@ -304,7 +317,7 @@ int gemm16_call(const cpuops_b200_gemm16_desc* d) {
   p.raster_m = std::max(1, std::min(p.m_tiles, static_cast<int>(std::lround(std::sqrt(static_cast<double>(at_once) * c.BN / tile_m)))));
 
   CUtensorMap tmA, tmB, tmC, tmD, tmZ;
-  if (int rc = make_tensor_map_elements(&tmA, ka.base, d->type, ka.inner, ka.outer, ka.ld * 2, 64, ka.mn ? 64 : 128)) return rc;
+  if (int rc = make_tensor_map_elements(&tmA, ka.base, d->type, ka.inner, ka.outer, ka.ld * 2, 64, ka.mn ? 64 : std::min(tile_rows, 128))) return rc;
   if (int rc = make_tensor_map_elements(&tmB, kb.base, d->type, kb.inner, kb.outer, kb.ld * 2, 64, kb.mn ? 64 : b_rows)) return rc;
   tmC = tmD = tmZ = tmA;
   if (by_tma && c.form != kProductParts) {
@@ -316,7 +329,7 @@ int gemm16_call(const cpuops_b200_gemm16_desc* d) {
   }
   const int stage_bytes = (kTileM + b_rows) * 128;
   // At least 120 KB so that two CTAs never share an SM: each allocates all of tensor memory.
-  const int smem = std::max(1024 + c.stages * stage_bytes + c.epi_warps * c.ring_bytes + kProductBarrierBytes, 120 * 1024);
+  const int smem = std::max(1024 + c.stages * stage_bytes + c.epi_warps * c.ring_bytes + kProductBarrierBytes + 4 * kProductBiasFloats, 120 * 1024);
   cudaLaunchConfig_t cfg = {};
   int64_t grid = std::min<int64_t>(total_tiles, st.sms());
   if (c.form == kProductPairs)

@@ -17,9 +17,10 @@ __host__ __device__ inline int type_bytes(int type) { return type == kF32 ? 4 : 
 enum : int32_t { kProductTiles = 0, kProductPairs = 1, kProductParts = 2 };
 
 constexpr int kProductEpiWarps = 8;    // at most; 4 where shared memory is short of stages otherwise, and in kProductParts
-constexpr int kProductMaxStages = 8;
+constexpr int kProductMaxStages = 12;
 constexpr int kProductMaxParts = 8;
 constexpr int kProductBarrierBytes = 512;
+constexpr int kProductBiasFloats = 1024;  // 128 for each of eight epilogue warps, 256 for each of four; behind the barriers
 constexpr int kProductPieceBlocks = 8;   // k-blocks of a piece of k (kPieces)
 
 struct ProductParams {
@@ -28,6 +29,7 @@ struct ProductParams {
   int32_t Mk, Nk, K;
   int32_t m_tiles, n_tiles, k_blocks;   // tiles of 128 (pairs: 256) x BN; k-blocks of 64
   int32_t BN, stages, nacc, raster_m, parts;
+  int32_t tile_rows;                    // kProductParts: rows of Ak per tile, at most 128 (others: 128)
   int32_t a_mn, b_mn;                   // 1: the m (n) direction is contiguous in memory
   int32_t swapped;
   uint32_t idesc;
@@ -40,7 +42,7 @@ struct ProductParams {
   void* D;
   void* Z;                              // alpha A B + bias, or null
   int64_t ldc, ldd, ldz;
-  int32_t c_type, d_type;               // (Z has D's)
+  int32_t type, c_type, d_type;         // of A and B, of C, of D and Z
   int32_t ring_bytes, ring_depth;       // epilogue buffers of one warp, and how many chunks of each matrix they hold
   int32_t* error;
   uint32_t wait_budget_us;

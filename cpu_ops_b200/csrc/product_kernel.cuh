@@ -12,7 +12,6 @@
 #pragma once
 
 #include "dense_params.h"
-#include "epilogue.cuh"
 #include "gemm_params.h"
 #include "ptx_sm100.cuh"
 #include "ptx_sm100_pair.cuh"
@@ -179,34 +178,45 @@ __device__ __forceinline__ void add_chunk_row(uint32_t buf, int lane, uint32_t (
   }
 }
 
+// z / (1 + exp(-v)) from one exp2 and one reciprocal, both within 2 ulp: 3e-7 of z.  (silu_f32 and gelu_f32, to the last
+// bit, take some 90 instructions an element: 8192 x 4096 x 1024 with gelu and Z 88 us, 49 in this form.)  Where
+// exp(-v) overflows the quotient is 0 (of -inf: NaN).
+__device__ __forceinline__ float times_logistic(float z, float v) {
+  float t, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(v * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + t));
+  return z * r;
+}
+// The tanh form: 0.5 z (1 + tanh(u)) = z / (1 + exp(-2 u)).
+__device__ __forceinline__ float gelu_fast(float z) {
+  constexpr float c = 2.0f * 0.7978845608028654f;
+  return times_logistic(z, z * __fmaf_rn(c * 0.044715f, z * z, c));
+}
 __device__ __forceinline__ float activate(float z, int act) {
   switch (act) {
     case kOpRelu: return z < 0.0f ? 0.0f : z;
-    case kOpGelu: return gelu_f32(z);
-    case kOpSilu: return silu_f32(z);
+    case kOpGelu: return gelu_fast(z);
+    case kOpSilu: return times_logistic(z, z);
     default: return z;
   }
 }
 
-// z of a chunk: alpha acc + bias by column (columns at or beyond `ncols` are computed on harmlessly).
-__device__ __forceinline__ void product_z(const ProductParams& p, uint32_t (&r)[32], int col0, int ncols) {
+// z of a chunk: alpha acc + bias by column (`bias`: 32 floats of shared memory, or null).
+__device__ __forceinline__ void product_z(float alpha, const float* bias, uint32_t (&r)[32]) {
+  if (bias == nullptr) {
+    if (alpha != 1.0f) {
 #pragma unroll
-  for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(p.alpha * __uint_as_float(r[i]));
-  if (p.bias == nullptr) return;
-  const float* b = p.bias + col0;
-  if (ncols == 32 && (reinterpret_cast<uintptr_t>(b) & 15u) == 0) {
-#pragma unroll
-    for (int i = 0; i < 32; i += 4) {
-      const float4 v = __ldg(reinterpret_cast<const float4*>(b + i));
-      r[i] = __float_as_uint(__uint_as_float(r[i]) + v.x);
-      r[i + 1] = __float_as_uint(__uint_as_float(r[i + 1]) + v.y);
-      r[i + 2] = __float_as_uint(__uint_as_float(r[i + 2]) + v.z);
-      r[i + 3] = __float_as_uint(__uint_as_float(r[i + 3]) + v.w);
+      for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(alpha * __uint_as_float(r[i]));
     }
-  } else {
+    return;
+  }
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (i < ncols) r[i] = __float_as_uint(__uint_as_float(r[i]) + __ldg(b + i));
+  for (int i = 0; i < 32; i += 4) {
+    const float4 v = *reinterpret_cast<const float4*>(bias + i);
+    r[i] = __float_as_uint(__fmaf_rn(alpha, __uint_as_float(r[i]), v.x));
+    r[i + 1] = __float_as_uint(__fmaf_rn(alpha, __uint_as_float(r[i + 1]), v.y));
+    r[i + 2] = __float_as_uint(__fmaf_rn(alpha, __uint_as_float(r[i + 2]), v.z));
+    r[i + 3] = __float_as_uint(__fmaf_rn(alpha, __uint_as_float(r[i + 3]), v.w));
   }
 }
 __device__ __forceinline__ void activate_chunk(uint32_t (&r)[32], int act) {
@@ -215,10 +225,10 @@ __device__ __forceinline__ void activate_chunk(uint32_t (&r)[32], int act) {
     for (int i = 0; i < 32; ++i) r[i] = __uint_as_float(r[i]) < 0.0f ? 0u : r[i];
   } else if (act == kOpGelu) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(gelu_f32(__uint_as_float(r[i])));
+    for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(gelu_fast(__uint_as_float(r[i])));
   } else if (act == kOpSilu) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(silu_f32(__uint_as_float(r[i])));
+    for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(times_logistic(__uint_as_float(r[i]), __uint_as_float(r[i])));
   }
 }
 
@@ -278,12 +288,122 @@ __device__ __forceinline__ void store_lane_row(void* dst, int64_t ld, int row, i
     if (i < ncols) store_from_f32(dst, at + i, type, __uint_as_float(r[i]));
 }
 
+// The owner's part of kProductParts' epilogue: its columns' sums, [part][column][row] from `base`, `slab` bytes a
+// part.  A warp takes 32 rows and kCols columns at a time, a lane a row, so that shared memory is read without
+// conflicts; where rows are contiguous in D (swapped) a warp's stores are whole lines, otherwise a lane's eight
+// columns leave as one or two 16-byte stores where D's rows allow it.
+template <typename T, typename TC, int kCols>
+__device__ __forceinline__ void finish_columns(const ProductParams& p, uint32_t base, uint32_t slab, const float* bias, int row, int col,
+                                               int kr, int kc, int ncols) {
+  float v[kCols], c[kCols];
+  const int64_t i = p.swapped ? kc : kr, j = p.swapped ? kr : kc;  // the caller's row and column of the first element
+  if (p.C) {
+    const TC* from = static_cast<const TC*>(p.C) + (i * p.ldc + j);
+    const int64_t step = p.swapped ? p.ldc : 1;
+#pragma unroll
+    for (int u = 0; u < kCols; ++u) c[u] = u < ncols ? to_float(from[u * step]) : 0.0f;
+  }
+  const uint32_t at = base + static_cast<uint32_t>((col * kTileM + row) * 4);
+#pragma unroll
+  for (int u = 0; u < kCols; ++u) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[u]) : "r"(at + 512u * u));
+  for (int s = 1; s < p.parts; ++s) {
+    float x[kCols];
+#pragma unroll
+    for (int u = 0; u < kCols; ++u) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x[u]) : "r"(at + static_cast<uint32_t>(s) * slab + 512u * u));
+#pragma unroll
+    for (int u = 0; u < kCols; ++u) v[u] += x[u];
+  }
+  if (p.bias) {
+#pragma unroll
+    for (int u = 0; u < kCols; ++u) v[u] = __fmaf_rn(p.alpha, v[u], bias[p.swapped ? row : col + u]);
+  } else {
+#pragma unroll
+    for (int u = 0; u < kCols; ++u) v[u] *= p.alpha;
+  }
+  auto store = [&](void* matrix, int64_t ld) {
+    T* to = static_cast<T*>(matrix) + (i * ld + j);
+    if constexpr (kCols == 8) {
+      if (!p.swapped && ncols >= 8 && (reinterpret_cast<uintptr_t>(to) & 15u) == 0) {
+        uint4* out = reinterpret_cast<uint4*>(to);
+        if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            out[h] = make_uint4(__float_as_uint(v[4 * h]), __float_as_uint(v[4 * h + 1]), __float_as_uint(v[4 * h + 2]), __float_as_uint(v[4 * h + 3]));
+        } else {
+          constexpr int type = std::is_same<T, __half>::value ? kF16 : kBf16;
+          *out = make_uint4(pack2(v[0], v[1], type), pack2(v[2], v[3], type), pack2(v[4], v[5], type), pack2(v[6], v[7], type));
+        }
+        return;
+      }
+    }
+    const int64_t step = p.swapped ? ld : 1;
+#pragma unroll
+    for (int u = 0; u < kCols; ++u)
+      if (u < ncols) to[u * step] = from_float<T>(v[u]);
+  };
+  if (p.Z) store(p.Z, p.ldz);
+  if (p.act == kOpRelu) {
+#pragma unroll
+    for (int u = 0; u < kCols; ++u) v[u] = v[u] < 0.0f ? 0.0f : v[u];
+  } else if (p.act == kOpGelu) {
+#pragma unroll
+    for (int u = 0; u < kCols; ++u) v[u] = gelu_fast(v[u]);
+  } else if (p.act == kOpSilu) {
+#pragma unroll
+    for (int u = 0; u < kCols; ++u) v[u] = times_logistic(v[u], v[u]);
+  }
+  if (p.C) {
+#pragma unroll
+    for (int u = 0; u < kCols; ++u) v[u] = __fmaf_rn(p.beta, c[u], v[u]);
+  }
+  store(p.D, p.ldd);
+}
+// By warp `warp` of `warps`, all of them on one CTA's columns.
+__device__ __forceinline__ void finish_parts(const ProductParams& p, uint32_t base, uint32_t slab, const float* bias, int warp, int warps,
+                                             int lane, int tile, int part) {
+  const int own = p.BN / p.parts;
+  const ProductTile tc = product_tile(p, tile, part);
+  const int row0 = tc.m_tile * p.tile_rows, col0 = tc.n_tile * p.BN + part * own;
+  const int nrows = min(p.tile_rows, p.Mk - row0), ncols = min(own, p.Nk - col0);  // (ncols may be negative)
+  auto finish = [&](auto type, auto c_type, auto cols) {
+    constexpr int kCols = decltype(cols)::value;
+    for (int item = warp; item < 4 * (own / kCols); item += warps) {
+      const int row = (item & 3) * 32 + lane, col = (item >> 2) * kCols;
+      if (row < nrows && col < ncols)
+        finish_columns<decltype(type), decltype(c_type), kCols>(p, base, slab, bias, row, col, row0 + row, col0 + col, ncols - col);
+    }
+  };
+  auto with_cols = [&](auto type, auto c_type) {
+    if (own >= 8) {
+      finish(type, c_type, std::integral_constant<int, 8>{});
+    } else {
+      finish(type, c_type, std::integral_constant<int, 2>{});
+    }
+  };
+  // (C is f32 or of the operands' type, as D is)
+  const bool c_f32 = p.c_type == kF32;
+  if (p.type == kF16) {
+    if (p.d_type == kF32) {
+      if (c_f32) with_cols(0.0f, 0.0f); else with_cols(0.0f, __half{});
+    } else {
+      if (c_f32) with_cols(__half{}, 0.0f); else with_cols(__half{}, __half{});
+    }
+  } else {
+    if (p.d_type == kF32) {
+      if (c_f32) with_cols(0.0f, 0.0f); else with_cols(0.0f, __nv_bfloat16{});
+    } else {
+      if (c_f32) with_cols(__nv_bfloat16{}, 0.0f); else with_cols(__nv_bfloat16{}, __nv_bfloat16{});
+    }
+  }
+}
+
 // kProductPairs: clusters of two CTAs compute 256-row tiles with the cta_group::2 instructions; each CTA
 // stages its own 128 rows of A and its half of B's BN rows, and drains its own 128 rows of the accumulator.
 //
 // kProductParts: few tiles.  The CTAs of a cluster take a part of k each; then each of them owns an equal
-// share of the tile's columns, to which all CTAs write their sums in distributed shared memory, and adds them in
-// the order of k.  No workspace, no second launch, and the same result on every run.
+// share of the tile's columns, of which all CTAs send it their sums by bulk copies between shared memories, and adds
+// them in the order of k.  No workspace, no second launch, and the same result on every run.  (Stored element by element
+// into the owner's memory, a warp's store took some 65 cycles: 256 x 4096 x 4096 in two parts 35 us.)
 //
 // kPieces (D is f32): the accumulator is taken down every kProductPieceBlocks k-blocks and the pieces added in
 // f32 registers.  The tensor cores drop the low bits of a running sum: against float64 it is off by 1e-9 of the result per
@@ -311,7 +431,7 @@ __global__ void __launch_bounds__(kForm == kProductParts ? 224 : kProductThreads
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint64_t budget_ns = static_cast<uint64_t>(p.wait_budget_us) * 1000ull;
   const int stages = p.stages, b_rows = p.BN / kCtas;
-  const int stage_bytes = (kTileM + b_rows) * 128;
+  const int stage_bytes = (kTileM + b_rows) * 128, tile_rows = kParts ? p.tile_rows : kTileM;
   const uint32_t ring_base = smem_base + static_cast<uint32_t>(stages * stage_bytes);
   const int n_epi = p.epi_warps, warp_producer2 = 2 + n_epi;
   const uint32_t bar_base = ring_base + static_cast<uint32_t>(n_epi * p.ring_bytes);
@@ -321,8 +441,10 @@ __global__ void __launch_bounds__(kForm == kProductParts ? 224 : kProductThreads
   auto acc_empty_bar = [&](int b) { return bar_base + 8u * (2 * kProductMaxStages + 2 + b); };
   const uint32_t drain_bar = bar_base + 8u * (2 * kProductMaxStages + 4);
   auto c_full_bar = [&](int w, int b) { return bar_base + 8u * (2 * kProductMaxStages + 5 + 2 * w + b); };
-  constexpr int kBarriers = 2 * kProductMaxStages + 5 + 2 * kProductEpiWarps;
+  constexpr int kRecvBar = 2 * kProductMaxStages + 5 + 2 * kProductEpiWarps, kBarriers = kRecvBar + 1;
+  const uint32_t recv_bar = bar_base + 8u * kRecvBar;
   static_assert(8 * kBarriers + 8 <= kProductBarrierBytes, "barriers, tensor memory slot, abort flag");
+  float* bias_smem = reinterpret_cast<float*>(smem + (bar_base - smem_base) + kProductBarrierBytes);  // a warp's chunks' bias
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (bar_base - smem_base) + 8 * kBarriers);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -333,6 +455,8 @@ __global__ void __launch_bounds__(kForm == kProductParts ? 224 : kProductThreads
     }
     if (lane == 0) *abort_flag = 0;
     fence_mbar_init_cluster();
+    __syncwarp();
+    if (kParts && lane == 0) mbar_expect_tx(recv_bar, static_cast<uint32_t>(p.BN * kTileM * 4));  // its columns' sums from all parts
   }
   if (warp == 1) {
     tmem_alloc_g<kPair>(smem_u32(tmem_slot), kTmemCols512);
@@ -365,14 +489,14 @@ __global__ void __launch_bounds__(kForm == kProductParts ? 224 : kProductThreads
       int s = me, g_par = 0;
       uint32_t ph = 0, armed = 0, armed_parity = 0, peek = 0;
       bool ok = true;
-      const uint32_t tx_bytes = static_cast<uint32_t>(stage_bytes) * kCtas;
+      const uint32_t tx_bytes = static_cast<uint32_t>(tile_rows + b_rows) * 128u * kCtas;
       // pair: every load of both CTAs credits the leader's barrier, which the leader arms with the bytes of both
       const uint32_t full0 = kPair ? map_to_cta(full_bar(0), 0) : full_bar(0), empty0 = empty_bar(0);
       const int a_mn = p.a_mn, b_mn = p.b_mn, b_chunks = b_rows / 64;
       asm volatile("griddepcontrol.wait;" ::: "memory");
       for (int t = work0; t < total_tiles && ok; t += work_step) {
         const ProductTile tc = product_tile(p, t, part);
-        const int m0 = (tc.m_tile * kCtas + (kPair ? static_cast<int>(cta_rank) : 0)) * kTileM;
+        const int m0 = (tc.m_tile * kCtas + (kPair ? static_cast<int>(cta_rank) : 0)) * tile_rows;
         const int n0 = tc.n_tile * p.BN + (kPair ? static_cast<int>(cta_rank) * b_rows : 0);
         const int i0 = np == 1 ? 0 : ((me ^ g_par) & 1);
         int kx = (tc.kb0 + i0) * 64;
@@ -532,11 +656,12 @@ __global__ void __launch_bounds__(kForm == kProductParts ? 224 : kProductThreads
         c_ph ^= 1u;
       }
     };
+    float* my_bias = bias_smem + ew * (kProductBiasFloats / n_epi);
     // Sums of one chunk -> D (and Z).  False: C did not arrive.
     auto finish_chunk = [&](uint32_t (&r)[32], int row0, int n0, int c, int nchunks) -> bool {
       const int col0 = n0 + c * 32, ncols = min(32, p.Nk - col0);
       const bool inside = row0 < p.Mk && ncols > 0;
-      product_z(p, r, col0, ncols);
+      product_z(p.alpha, p.bias ? my_bias + (c - c0) / cstep * 32 : nullptr, r);
       if (by_tma) {
         const bool ragged = col0 >= whole_cols, mine = inside && row0 + lane < p.Mk;
         if (!ragged || has_c) {
@@ -629,6 +754,14 @@ __global__ void __launch_bounds__(kForm == kProductParts ? 224 : kProductThreads
         // the tile's first chunks of C, before the accumulator is ready
         for (int c = c0; c < min(nchunks, c0 + static_cast<int>(depth) * cstep); c += cstep) request_c(n0 + c * 32, row0);
       }
+      if (p.bias) {  // the tile's bias, likewise (as loads of a chunk their latency followed every accumulator)
+        __syncwarp();
+        for (int c = c0, j = 0; c < nchunks; c += cstep, ++j) {
+          const int col = n0 + c * 32 + lane;
+          my_bias[32 * j + lane] = col < p.Nk ? __ldg(p.bias + col) : 0.0f;
+        }
+        __syncwarp();
+      }
       uint32_t taddr = 0;
       int buf = 0;
       if constexpr (kPieces) {
@@ -685,19 +818,20 @@ __global__ void __launch_bounds__(kForm == kProductParts ? 224 : kProductThreads
   } else {
     // ------------------- sums of a part of k, to the columns' owners ------------------
     const int q = warp & 3;
-    // (powers of two both)
-    const int own = p.BN / p.parts, own_log = 31 - __clz(own), row = q * 32 + lane;
-    // in the owner's buffer: [part][column][row] (rows are contiguous in D), or [part][row][own + 1 columns]
-    const int pitch_c = p.swapped ? kTileM : 1, pitch_r = p.swapped ? 1 : own + 1;
-    const uint32_t slab = static_cast<uint32_t>((p.swapped ? own * kTileM : kTileM * (own + 1)) * 4);
-    const uint32_t mine = ring_base + static_cast<uint32_t>(part) * slab + static_cast<uint32_t>(row * pitch_r * 4);
-    auto send = [&](const uint32_t (&r)[16], int c) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // before bias and C are read, D or Z written
+    if (p.bias) {  // of this tile's rows (swapped), or of the columns that this CTA will own
+      const ProductTile tc = product_tile(p, work0, part);
+      const int i = static_cast<int>(threadIdx.x) - 64, own = p.BN / p.parts;
+      const int at = p.swapped ? tc.m_tile * tile_rows + i : tc.n_tile * p.BN + part * own + i;
+      bias_smem[i] = (p.swapped || i < own) && at < (p.swapped ? p.Mk : p.Nk) ? __ldg(p.bias + at) : 0.0f;
+    }
+    // The sums as [column][row] where the stages were: every load has landed and every MMA has read it
+    // once the last accumulator is there (two stages hold BN <= 128 columns).
+    const uint32_t mine = smem_base + static_cast<uint32_t>((q * 32 + lane) * 4);
+    auto put = [&](const uint32_t (&r)[16], int c) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int owner = (c + i) >> own_log, local = (c + i) & (own - 1);
-        const uint32_t at = mine + static_cast<uint32_t>(local * pitch_c * 4);
-        asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(map_to_cta(at, static_cast<uint32_t>(owner))), "r"(r[i]) : "memory");
-      }
+      for (int i = 0; i < 16; ++i)
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(mine + static_cast<uint32_t>((c + i) * kTileM * 4)), "r"(r[i]) : "memory");
     };
     constexpr int kGroups = kPieces ? 8 : 1;  // of 16 columns
     [[maybe_unused]] uint32_t sum[kGroups][16];
@@ -732,7 +866,7 @@ __global__ void __launch_bounds__(kForm == kProductParts ? 224 : kProductThreads
           uint32_t r[16];
           tmem_ld_32x16(taddr + static_cast<uint32_t>(c), r);
           tmem_ld_wait();
-          send(r, c);
+          put(r, c);
         }
         tc_fence_before_sync();
       }
@@ -740,44 +874,37 @@ __global__ void __launch_bounds__(kForm == kProductParts ? 224 : kProductThreads
     if constexpr (kPieces) {
 #pragma unroll
       for (int g = 0; g < kGroups; ++g)
-        if (alive && 16 * g < p.BN) send(sum[g], 16 * g);
+        if (alive && 16 * g < p.BN) put(sum[g], 16 * g);
+    }
+    // (a CTA that gave up sends as well: the others do not wait for it)
+    fence_proxy_async_shared_cta();
+    asm volatile("bar.sync 1, 128;" ::: "memory");  // the four epilogue warps
+    const uint32_t slab = static_cast<uint32_t>(p.BN / p.parts * kTileM * 4);
+    if (warp == 2 && lane < p.parts) {
+      const uint32_t to = ring_base + static_cast<uint32_t>(part) * slab;
+      asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                       map_to_cta(to, static_cast<uint32_t>(lane))),
+                   "r"(smem_base + static_cast<uint32_t>(lane) * slab), "r"(slab), "r"(map_to_cta(recv_bar, static_cast<uint32_t>(lane)))
+                   : "memory");
     }
   }
 
   if constexpr (kParts) {
-    __syncwarp();
-    cluster_sync_all();  // every CTA's sums are where they belong
-    if (warp >= 2 && warp < warp_producer2 && *abort_flag == 0) {
-      asm volatile("griddepcontrol.wait;" ::: "memory");
-      const int own = p.BN / p.parts, own_log = 31 - __clz(own), n_threads = 32 * n_epi, tid = static_cast<int>(threadIdx.x) - 64;
-      const int pitch_c = p.swapped ? kTileM : 1, pitch_r = p.swapped ? 1 : own + 1;
-      const uint32_t slab = static_cast<uint32_t>((p.swapped ? own * kTileM : kTileM * (own + 1)) * 4);
-      const ProductTile tc = product_tile(p, work0, part);
-      const int row0 = tc.m_tile * kTileM, col0 = tc.n_tile * p.BN + part * own;
-      for (int e = tid; e < own * kTileM; e += n_threads) {
-        const int row = p.swapped ? e & (kTileM - 1) : e >> own_log, col = p.swapped ? e >> 7 : e & (own - 1);
-        const int kr = row0 + row, kc = col0 + col;
-        if (kr >= p.Mk || kc >= p.Nk) continue;
-        const uint32_t at = ring_base + static_cast<uint32_t>((row * pitch_r + col * pitch_c) * 4);
-        float v = 0.0f;
-        for (int i = 0; i < p.parts; ++i) {
-          float x;
-          asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(at + static_cast<uint32_t>(i) * slab));
-          v = i == 0 ? x : v + x;
-        }
-        const int64_t i = p.swapped ? kc : kr, j = p.swapped ? kr : kc;  // the caller's row and column
-        v *= p.alpha;
-        if (p.bias) v += __ldg(p.bias + j);
-        if (p.Z) store_from_f32(p.Z, i * p.ldz + j, p.d_type, v);
-        v = activate(v, p.act);
-        if (p.C) v = __fmaf_rn(p.beta, load_as_f32(p.C, i * p.ldc + j, p.c_type), v);
-        store_from_f32(p.D, i * p.ldd + j, p.d_type, v);
-      }
+    // This CTA's columns, by all warps: the parts' sums added in the order of k, and the epilogue.
+    __syncthreads();  // (the bias is there)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    int dummy = 0;
+    const bool got = mbar_wait_bounded(recv_bar, 0, &dummy, budget_ns);
+    if (!__all_sync(0xffffffffu, got)) {
+      if (lane == 0) product_error(p, abort_flag, kErrEpilogueWait);
+    } else if (*abort_flag == 0) {
+      finish_parts(p, ring_base, static_cast<uint32_t>(p.BN / p.parts * kTileM * 4), bias_smem, warp, 7, lane, work0, part);
     }
   }
   tc_fence_before_sync();
-  if constexpr (kPair) {
-    // neither CTA may leave while the other can still touch its shared memory, barriers or accumulator
+  if constexpr (kForm != kProductTiles) {
+    // no CTA may leave while another can still touch its shared memory, barriers or accumulator
+    __syncwarp();
     cluster_sync_all();
   } else {
     __syncthreads();
