@@ -105,18 +105,29 @@ bool fit_product(ProductChoice& c, int smem_optin, int chunks, int k_blocks, boo
   return c.stages >= 2;
 }
 
-// Estimated cycles; the least of all choices is taken.
-double product_cycles(const ProductChoice& c, const DeviceState& st, int Mk, int Nk, int k_blocks) {
-  const int tile_m = c.form == kProductPairs ? 256 : c.tile_rows;
+// Estimated time in us; the choice whose is least is taken.  Measured on B200 at K = 1024 .. 8192 (a k-block of one tile,
+// rounds of tiles, and what does not shrink with k); us, estimated / measured:
+//   XXXEST
+// chunk_us: an epilogue warp's time for 32 x 32 elements; hbm_us: the bytes that the call cannot do without.
+double product_us(const ProductChoice& c, const DeviceState& st, int Mk, int Nk, int k_blocks, bool pieces, double chunk_us, double hbm_us) {
+  const bool pair = c.form == kProductPairs;
+  const int tile_m = pair ? 256 : c.tile_rows;
   const int64_t tiles = static_cast<int64_t>((Mk + tile_m - 1) / tile_m) * ((Nk + c.BN - 1) / c.BN);
-  const int ctas = c.form == kProductPairs ? 2 : c.parts;
-  const int64_t slots = std::max(1, st.sms() / ctas);
+  const int64_t slots = std::max(1, c.form == kProductTiles ? st.sms() : st.sms() / (pair ? 2 : c.parts));
   const double rounds = static_cast<double>((tiles + slots - 1) / slots);
-  const double stage = (kTileM + c.BN / (c.form == kProductPairs ? 2 : 1)) * 128.0;
-  const double block = std::max(std::max(2.0 * c.BN, 128.0), stage / 56.0);
+  double block = pair ? (c.BN == 128 ? 0.215 : c.BN == 192 ? 0.285 : 0.345)
+                      : (c.BN <= 16 ? 0.13 : c.BN == 32 ? 0.145 : c.BN == 64 ? 0.185 : c.BN == 128 ? 0.26 : 0.45);
+  if (pieces) block += 0.05;
   const double kb = static_cast<double>((k_blocks + c.parts - 1) / c.parts);
-  if (c.form == kProductParts) return rounds * (kb * block + 2500.0 + 12.0 * c.BN + (c.parts > 1 ? 1500.0 : 0.0));
-  return rounds * std::max(kb * block, 10.0 * c.BN) + 2500.0 + 14.0 * c.BN;
+  // (a short loop does not reach the memory's rate from its first load on)
+  auto together = [&](double us) { return std::max(hbm_us, us) + 0.25 * std::min(hbm_us, us); };
+  if (c.form == kProductParts) {
+    const int own = c.BN / c.parts, items = own >= 8 ? (4 * own / 8 + 6) / 7 : 1;
+    const double tail = 0.6 * items + (c.parts > 1 ? 1.6 + 0.011 * c.BN : 0.0);
+    return together(rounds * kb * block + (rounds - 1.0) * 3.0) + 3.3 + rounds * tail;
+  }
+  const double epilogue = 0.6 + (c.BN + 63) / 64 * chunk_us * (c.epi_warps == 8 ? 1.0 : 1.6) * (pair ? 1.0 : 1.1);
+  return together(rounds * std::max(kb * block, epilogue)) + 1.2 + epilogue + (pair ? 1.0 : 0.0);
 }
 
 int dense_kernels_ready(DeviceState& st) {
@@ -209,6 +220,9 @@ int gemm16_call(const cpuops_b200_gemm16_desc* d) {
   const bool pieces = d->d_type == kF32 && k_blocks > kProductPieceBlocks;
 
   // The choice of form and tile.
+  const double c_size = use_c ? type_bytes(d->c_type) : 0, d_size = type_bytes(d->d_type) * (d->z ? 2 : 1);
+  const double hbm_us = (2.0 * d->k * (static_cast<double>(d->m) + d->n) + static_cast<double>(d->m) * d->n * (c_size + d_size)) / 6.4e6;
+  const double chunk_us = 1.15 + (d->activation > CPUOPS_B200_OP_RELU ? 0.5 : 0.0) + 0.1 * (d_size + c_size) * (by_tma ? 1.0 : 4.0);
   ProductChoice best;
   double least = 0.0;
   bool found = false;
@@ -236,10 +250,10 @@ int gemm16_call(const cpuops_b200_gemm16_desc* d) {
       const int64_t along_m = std::max<int64_t>(1, rounds * clusters / columns);
       c.tile_rows = static_cast<int>(std::min<int64_t>(128, ((Mk + along_m - 1) / along_m + 7) / 8 * 8));
     }
-    const double cycles = product_cycles(c, st, Mk, Nk, k_blocks);
-    if (!found || cycles < least) {
+    const double us = product_us(c, st, Mk, Nk, k_blocks, pieces, chunk_us, hbm_us);
+    if (!found || us < least) {
       best = c;
-      least = cycles;
+      least = us;
       found = true;
     }
   };

@@ -30,6 +30,13 @@ __device__ __forceinline__ void product_error(const ProductParams& p, volatile i
   __threadfence_block();
 }
 
+// Hands an accumulator back to the pair's leader.  Its reads are complete (tcgen05.wait::ld), nothing else is published:
+// with release semantics the arrival waits for all the thread's stores, TMA's among them, which took 1000 to 2500 cycles
+// (4096 x 2048 x 8192 in pieces 120 us, XXX so).
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
 template <bool kPair>
 __device__ __forceinline__ void mma_f16_g(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
                                           uint32_t idesc, uint32_t accumulate, uint32_t issue) {
@@ -234,6 +241,12 @@ __device__ __forceinline__ void activate_chunk(uint32_t (&r)[32], int act) {
 
 // Where C, D or Z cannot be addressed by TMA: a chunk's f32 values (in shared memory, put there by
 // put_chunk_row) leave row by row, lane = column, and C is read the same way, all of a chunk's rows at once.
+// Asks for a chunk's C ahead of its use, a row per lane.
+__device__ __forceinline__ void prefetch_c_rows(const ProductParams& p, int row0, int col0, int lane) {
+  if (row0 + lane >= p.Mk || col0 >= p.Nk) return;
+  const char* at = static_cast<const char*>(p.C) + (static_cast<int64_t>(row0 + lane) * p.ldc + col0) * type_bytes(p.c_type);
+  asm volatile("prefetch.global.L1 [%0];" ::"l"(at));
+}
 template <int kRows>
 __device__ __forceinline__ void load_c_rows(const ProductParams& p, int row0, int col0, int lane, float (&c)[kRows]) {
   const int nrows = lane < p.Nk - col0 ? p.Mk - row0 : 0;
@@ -241,7 +254,7 @@ __device__ __forceinline__ void load_c_rows(const ProductParams& p, int row0, in
   auto rows = [&](auto* base) {
     base += at;
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) c[r] = r < nrows ? to_float(base[r * p.ldc]) : 0.0f;
+    for (int r = 0; r < kRows; ++r, base += p.ldc) c[r] = r < nrows ? to_float(*base) : 0.0f;
   };
   if (p.c_type == kF32) {
     rows(static_cast<const float*>(p.C));
@@ -260,15 +273,22 @@ __device__ __forceinline__ void write_chunk_rows(const ProductParams& p, uint32_
   auto rows = [&](auto* base) {
     using T = std::remove_pointer_t<decltype(base)>;
     base += at;
+    constexpr int kAtOnce = kRows < 8 ? kRows : 8;
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      const int r = r0 + i;
-      float v;
-      asm volatile("ld.shared.f32 %0, [%1];"
-                   : "=f"(v)
-                   : "r"(buf + static_cast<uint32_t>(r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4)));
-      if (add_c) v = __fmaf_rn(p.beta, c[i], v);
-      if (i < nrows) base[i * ld] = from_float<T>(v);
+    for (int i0 = 0; i0 < kRows; i0 += kAtOnce) {
+      float v[kAtOnce];
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int r = r0 + i0 + i;
+        asm volatile("ld.shared.f32 %0, [%1];"
+                     : "=f"(v[i])
+                     : "r"(buf + static_cast<uint32_t>(r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4)));
+      }
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i, base += ld) {
+        if (add_c) v[i] = __fmaf_rn(p.beta, c[i0 + i], v[i]);
+        if (i0 + i < nrows) *base = from_float<T>(v[i]);
+      }
     }
   };
   if (p.d_type == kF32) {
@@ -740,7 +760,7 @@ __global__ void __launch_bounds__(kForm == kProductParts ? 224 : kProductThreads
       __syncwarp();
       if (lane == 0) {
         if constexpr (kPair) {
-          mbar_arrive_cluster(acc_empty0 + 8u * buf);
+          mbar_arrive_cluster_relaxed(acc_empty0 + 8u * buf);
         } else {
           mbar_arrive(acc_empty_bar(buf));
         }
@@ -753,6 +773,9 @@ __global__ void __launch_bounds__(kForm == kProductParts ? 224 : kProductThreads
       if (has_c && by_tma && lane == 0) {
         // the tile's first chunks of C, before the accumulator is ready
         for (int c = c0; c < min(nchunks, c0 + static_cast<int>(depth) * cstep); c += cstep) request_c(n0 + c * 32, row0);
+      }
+      if (has_c && !by_tma) {
+        for (int c = c0; c < nchunks; c += cstep) prefetch_c_rows(p, row0, n0 + c * 32, lane);
       }
       if (p.bias) {  // the tile's bias, likewise (as loads of a chunk their latency followed every accumulator)
         __syncwarp();
