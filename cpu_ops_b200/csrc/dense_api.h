@@ -136,6 +136,13 @@ int dense_kernels_ready(DeviceState& st) {
   for (int form : {kProductTiles, kProductPairs, kProductParts})
     for (bool pieces : {false, true})
       CUDA_TRY(cudaFuncSetAttribute(product_kernel_of(form, pieces), cudaFuncAttributeMaxDynamicSharedMemorySize, st.smem_optin));
+  for (int x : {kF32, kF16, kBf16})
+    for (int y : {kF32, kF16, kBf16})
+      for (bool gradient : {false, true}) {
+        if (x != y && x != kF32) continue;
+        const NormChoice c = norm_choice(x, y, 2048, true, true, true, gradient);  // (the one with shared memory)
+        CUDA_TRY(cudaFuncSetAttribute(c.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kNormMostSmem));
+      }
   ready[st.device] = true;
   return 0;
 }
@@ -383,7 +390,7 @@ int gemm16_call(const cpuops_b200_gemm16_desc* d) {
 
 int launch_column_sum(const float* in, float* out0, float* out1, int parts, int n, int count, cudaStream_t stream) {
   ColumnSumParams s{in, out0, out1, parts, n};
-  return launch_after(column_sum(), dim3(static_cast<unsigned>((n + 31) / 32), static_cast<unsigned>(count)), 32 * std::min(16, parts), 0, stream, s);
+  return launch_after(column_sum(), dim3(static_cast<unsigned>((n + 63) / 64), static_cast<unsigned>(count)), 32 * std::min(32, parts), 0, stream, s);
 }
 
 // ---- gradient of bias and activation ----------------------------------------------------------
@@ -475,6 +482,7 @@ int layer_norm_call(const cpuops_b200_layer_norm_desc* d) {
   RowCall call;
   if (int rc = call.enter(*d)) return rc;
   if (int rc = call.check(d->memory_space, {d->x, d->gamma, d->beta, d->y, d->mean, d->rstd})) return rc;
+  if (int rc = dense_kernels_ready(*call.st)) return rc;
   NormParams p;
   memset(&p, 0, sizeof(p));
   p.x = d->x;
@@ -489,9 +497,12 @@ int layer_norm_call(const cpuops_b200_layer_norm_desc* d) {
   p.n = d->n;
   p.eps = d->eps;
   const bool wide = rows_aligned(d->x, d->ldx, d->x_type) && rows_aligned(d->y, d->ldy, d->y_type);
-  const NormChoice c = norm_choice(d->x_type, d->y_type, d->n, wide, d->m >= 4 * call.st->sms(), false);
+  const NormChoice c = norm_choice(d->x_type, d->y_type, d->n, wide, d->m >= 4 * call.st->sms(), false, false);
   const int rows = (d->m + c.rows_at_once - 1) / c.rows_at_once;
-  const int grid = std::min(rows, call.st->sms() * std::max(1, std::min(16, 1024 / c.threads)));
+  const int grid = std::min(rows, call.st->sms() * (c.ring ? 1 : std::max(1, std::min(16, 1024 / c.threads))));
+  p.ring = c.ring;
+  p.error = call.st->error_dev;
+  p.wait_budget_us = g_wait_budget_us.load();
   if (int rc = launch_after(c.kernel, dim3(static_cast<unsigned>(grid)), c.threads, static_cast<size_t>(c.smem), call.stream, p)) return rc;
   return call.finish();
 }
@@ -523,6 +534,7 @@ int layer_norm_grad_call(const cpuops_b200_layer_norm_grad_desc* d) {
   RowCall call;
   if (int rc = call.enter(*d)) return rc;
   if (int rc = call.check(d->memory_space, {d->x, d->dy, d->dr, d->gamma, d->mean, d->rstd, d->dx, d->dgamma, d->dbeta})) return rc;
+  if (int rc = dense_kernels_ready(*call.st)) return rc;
   NormParams p;
   memset(&p, 0, sizeof(p));
   p.x = d->x;
@@ -540,9 +552,12 @@ int layer_norm_grad_call(const cpuops_b200_layer_norm_grad_desc* d) {
   p.n = d->n;
   const bool wide = rows_aligned(d->x, d->ldx, d->x_type) && rows_aligned(d->dy, d->lddy, d->y_type) &&
                     rows_aligned(d->dx, d->lddx, d->x_type) && (!d->dr || rows_aligned(d->dr, d->lddr, d->x_type));
-  const NormChoice c = norm_choice(d->x_type, d->y_type, d->n, wide, d->m >= 4 * call.st->sms(), true);
+  const NormChoice c = norm_choice(d->x_type, d->y_type, d->n, wide, d->m >= 4 * call.st->sms(), d->dr != nullptr, true);
   const int rows = std::max(1, (d->m + c.rows_at_once - 1) / c.rows_at_once);
   const int grid = std::min(rows, call.st->sms() * std::max(1, std::min(16, 512 / c.threads)));
+  p.ring = c.ring;
+  p.error = call.st->error_dev;
+  p.wait_budget_us = g_wait_budget_us.load();
   const bool sums = d->dgamma || d->dbeta, is_long = norm_is_long(d->n);
   int parts = grid, block_rows = 0;
   if (is_long) {
@@ -559,7 +574,7 @@ int layer_norm_grad_call(const cpuops_b200_layer_norm_grad_desc* d) {
     if (int rc = launch_after(norm_grad_columns(d->x_type, d->y_type), dim3(static_cast<unsigned>((d->n + 255) / 256), static_cast<unsigned>(parts)),
                               256, 0, call.stream, p, block_rows))
       return rc;
-  if (int rc = launch_after(c.kernel, dim3(static_cast<unsigned>(grid)), c.threads, 0, call.stream, p)) return rc;
+  if (int rc = launch_after(c.kernel, dim3(static_cast<unsigned>(grid)), c.threads, static_cast<size_t>(c.smem), call.stream, p)) return rc;
   if (sums)
     if (int rc = launch_column_sum(p.sums, d->dgamma, d->dbeta, parts, d->n, 2, call.stream)) return rc;
   return call.finish();

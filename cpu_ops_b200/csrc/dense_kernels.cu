@@ -2,6 +2,8 @@
 // own, compiled beside api.cu.
 #include "dense_kernels.h"
 
+#include <algorithm>
+
 #include "balance_kernel.cuh"
 #include "norm_kernel.cuh"
 #include "product_kernel.cuh"
@@ -19,7 +21,7 @@ int product_threads(int form, int epi_warps) { return form == kProductParts ? 22
 namespace {
 
 template <typename X, typename Y, bool kGradient>
-NormChoice norm_choice_for(int n, bool wide, bool many) {
+NormChoice norm_choice_for(int n, bool wide, bool many, bool dr) {
   NormChoice c{};
   c.rows_at_once = 1;
   if (n > kNormMaxHeld) {
@@ -38,6 +40,15 @@ NormChoice norm_choice_for(int n, bool wide, bool many) {
       c.kernel = wide ? norm_grad_kernel<X, Y, true, true, 1> : norm_grad_kernel<X, Y, false, true, 1>;
       return c;
     }
+    const int row_bytes = n * static_cast<int>((dr ? 2 : 1) * sizeof(X) + sizeof(Y));
+    if (wide && many && n % 8 == 0 && n > 1024 && n <= 4096) {
+      // sixteen elements per thread, so that half as many threads share in a row's two sums; two CTAs per SM
+      c.threads = (n / 16 + 31) / 32 * 32;
+      c.ring = std::min(kNormMaxRing, 100 * 1024 / row_bytes);
+      c.smem = c.ring * row_bytes;
+      c.kernel = norm_grad_ring_kernel<X, Y, 2>;
+      return c;
+    }
     // (many rows: sixteen elements per thread, so that half as many threads share in a row's two sums)
     const bool two = n > 8 * kNormMaxThreads || (many && n > 1024 && sizeof(X) == 2);
     const int per = two ? 16 : 8;
@@ -45,6 +56,15 @@ NormChoice norm_choice_for(int n, bool wide, bool many) {
     c.kernel = two ? (wide ? norm_grad_kernel<X, Y, true, false, 2> : norm_grad_kernel<X, Y, false, false, 2>)
                    : (wide ? norm_grad_kernel<X, Y, true, false, 1> : norm_grad_kernel<X, Y, false, false, 1>);
   } else {
+    const int ring_smem = 2 * n * static_cast<int>(sizeof(float)) + 2 * kNormWarps * n * static_cast<int>(sizeof(X));
+    if (wide && many && n % 8 == 0 && n > 1024 && n <= kNormWarpMost && ring_smem <= kNormMostSmem) {
+      c.threads = 32 * kNormWarps;
+      c.rows_at_once = kNormWarps;
+      c.ring = 2;
+      c.smem = ring_smem;
+      c.kernel = norm_ring_kernel<X, Y, 16>;
+      return c;
+    }
     if (n <= 256 || (many && n <= kNormWarpMost)) {
       c.threads = 32 * kNormWarps;
       c.rows_at_once = kNormWarps;
@@ -64,12 +84,12 @@ NormChoice norm_choice_for(int n, bool wide, bool many) {
 }
 
 template <bool kGradient>
-NormChoice norm_choice_of(int x_type, int y_type, int n, bool wide, bool many) {
-  if (x_type == kF16) return norm_choice_for<__half, __half, kGradient>(n, wide, many);
-  if (x_type == kBf16) return norm_choice_for<__nv_bfloat16, __nv_bfloat16, kGradient>(n, wide, many);
-  if (y_type == kF16) return norm_choice_for<float, __half, kGradient>(n, wide, many);
-  if (y_type == kBf16) return norm_choice_for<float, __nv_bfloat16, kGradient>(n, wide, many);
-  return norm_choice_for<float, float, kGradient>(n, wide, many);
+NormChoice norm_choice_of(int x_type, int y_type, int n, bool wide, bool many, bool dr) {
+  if (x_type == kF16) return norm_choice_for<__half, __half, kGradient>(n, wide, many, dr);
+  if (x_type == kBf16) return norm_choice_for<__nv_bfloat16, __nv_bfloat16, kGradient>(n, wide, many, dr);
+  if (y_type == kF16) return norm_choice_for<float, __half, kGradient>(n, wide, many, dr);
+  if (y_type == kBf16) return norm_choice_for<float, __nv_bfloat16, kGradient>(n, wide, many, dr);
+  return norm_choice_for<float, float, kGradient>(n, wide, many, dr);
 }
 
 template <typename T, bool kWide>
@@ -94,8 +114,8 @@ BalanceKernel balance_for(int experts) {
 }  // namespace
 
 bool norm_is_long(int n) { return n > kNormMaxHeld; }
-NormChoice norm_choice(int x_type, int y_type, int n, bool wide, bool many, bool gradient) {
-  return gradient ? norm_choice_of<true>(x_type, y_type, n, wide, many) : norm_choice_of<false>(x_type, y_type, n, wide, many);
+NormChoice norm_choice(int x_type, int y_type, int n, bool wide, bool many, bool dr, bool gradient) {
+  return gradient ? norm_choice_of<true>(x_type, y_type, n, wide, many, dr) : norm_choice_of<false>(x_type, y_type, n, wide, many, dr);
 }
 NormColumnsKernel norm_grad_columns(int x_type, int y_type) {
   if (x_type == kF16) return norm_grad_columns_kernel<__half, __half>;

@@ -20,9 +20,11 @@ struct NormChoice {
   int threads;
   int rows_at_once;  // of a CTA
   int smem;
+  int ring;          // rows on their way by bulk copies (0: none)
 };
-// `many`: rows enough to give every warp one of its own (forward).
-NormChoice norm_choice(int x_type, int y_type, int n, bool wide, bool many, bool gradient);
+// `many`: rows enough for several on every SM; `dr`: the gradient adds one.
+NormChoice norm_choice(int x_type, int y_type, int n, bool wide, bool many, bool dr, bool gradient);
+constexpr int kNormMostSmem = 200 * 1024;  // of a choice
 using NormColumnsKernel = void (*)(NormParams, int);
 NormColumnsKernel norm_grad_columns(int x_type, int y_type);
 bool norm_is_long(int n);

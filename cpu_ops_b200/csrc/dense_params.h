@@ -87,7 +87,10 @@ struct NormParams {
   float* sums;           // gradient: per CTA, n sums of dy xhat, then (from n * gridDim.x on) n of dy; or null
   int64_t ldx, lddy, lddr, ldy;
   int32_t m, n;
+  int32_t ring;          // gradient by bulk copies: rows on their way
   float eps;
+  int32_t* error;        // kernels that wait for bulk copies
+  uint32_t wait_budget_us;
 };
 
 // ---- balance loss -------------------------------------------------------------------------------

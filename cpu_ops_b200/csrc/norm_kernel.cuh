@@ -12,6 +12,7 @@
 
 #include "dense_params.h"
 #include "gemm_params.h"
+#include "ptx_sm100.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -24,6 +25,7 @@ constexpr int kNormMaxThreads = 512;
 constexpr int kNormMaxHeld = 16 * kNormMaxThreads;  // longest row that a CTA holds in registers
 constexpr int kNormWarpMost = 4096;                 // ... that a warp does
 constexpr int kNormWarps = 8;                       // rows that a CTA of norm_rows_kernel has in flight
+constexpr int kNormMaxRing = 4;                     // rows on their way of norm_grad_ring_kernel
 constexpr int kNormLongThreads = 1024;
 constexpr int kNormStrip = 256;      // columns of a CTA of the column kernels
 
@@ -57,7 +59,32 @@ struct Eight {
       return __uint_as_float(i % 2 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
     }
   }
+  __device__ __forceinline__ float2 pair(int i) const {  // elements 2 i and 2 i + 1
+    if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    return make_float2((*this)[2 * i], (*this)[2 * i + 1]);
+  }
 };
+// Two f32 operations per instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{ .reg .b64 a, b, r; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; add.rn.f32x2 r, a, b; mov.b64 {%0, %1}, r; }"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{ .reg .b64 a, b, r; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; mul.rn.f32x2 r, a, b; mov.b64 {%0, %1}, r; }"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{ .reg .b64 a, b, c, r; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; mov.b64 c, {%6, %7}; fma.rn.f32x2 r, a, b, c; mov.b64 {%0, %1}, r; }"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
 template <typename T, bool kWide>
 __device__ __forceinline__ int element_of(int t, int threads, int j, int i) {
   return kWide ? 8 * (t + threads * j) + i : t + threads * (8 * j + i);
@@ -296,6 +323,114 @@ __global__ void __launch_bounds__(32 * kNormWarps, sizeof(X) == 2 || kV < 16 ? 2
   }
 }
 
+// The same with a warp's rows on their way by bulk copies, two rows ahead of the one that is worked on: the loads
+// do not wait for the arithmetic (8192 x 4096 bf16 44 us without, XXX in this form).  Rows are whole vectors of eight,
+// 16-byte aligned.  Shared memory: gamma and beta, two rows per warp.
+template <typename X, typename Y, int kV>
+__global__ void __launch_bounds__(32 * kNormWarps, 1) norm_ring_kernel(const NormParams p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  extern __shared__ __align__(16) float weights[];
+  __shared__ __align__(8) uint64_t barriers[kNormWarps][2];
+  __shared__ int abort_flag;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = p.n;
+  const float inverse = 1.0f / static_cast<float>(n);
+  const uint32_t row_bytes = static_cast<uint32_t>(n) * sizeof(X);
+  const uint32_t ring = smem_u32(weights + 2 * n) + static_cast<uint32_t>(2 * warp) * row_bytes, bar = smem_u32(&barriers[warp][0]);
+  if (threadIdx.x == 0) abort_flag = 0;
+  if (lane < 2) mbar_init(bar + 8u * lane, 1);
+  fence_mbar_init();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kNormWarps;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kNormWarps + warp;
+  auto request = [&](int64_t r, uint32_t slot) {
+    if (lane == 0 && r < p.m) {
+      mbar_expect_tx(bar + 8u * slot, row_bytes);
+      bulk_load(ring + slot * row_bytes, static_cast<const X*>(p.x) + r * p.ldx, row_bytes, bar + 8u * slot);
+    }
+  };
+  __syncwarp();
+  request(row, 0);
+  request(row + step, 1);
+  for (int c = threadIdx.x; c < n; c += 32 * kNormWarps) {
+    weights[c] = p.gamma != nullptr ? __ldg(p.gamma + c) : 1.0f;
+    weights[n + c] = p.beta != nullptr ? __ldg(p.beta + c) : 0.0f;
+  }
+  __syncthreads();
+  const uint64_t budget_ns = static_cast<uint64_t>(p.wait_budget_us) * 1000ull;
+  uint32_t slot = 0, phase = 0;
+  for (; row < p.m; row += step) {
+    if (!__all_sync(0xffffffffu, mbar_wait_bounded(bar + 8u * slot, phase, &abort_flag, budget_ns))) {
+      if (lane == 0) leave_error(p.error, kErrProducerWait);
+      break;
+    }
+    Eight<X> raw[kV];
+    const uint32_t from = ring + slot * row_bytes;
+#pragma unroll
+    for (int j = 0; j < kV; ++j) {
+      const int c = 8 * (lane + 32 * j);
+#pragma unroll
+      for (int h = 0; h < static_cast<int>(sizeof(X) / 2); ++h) {
+        uint32_t w[4] = {0, 0, 0, 0};
+        if (c < n)
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                       : "r"(from + static_cast<uint32_t>(c * static_cast<int>(sizeof(X)) + 16 * h)));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) raw[j].w[4 * h + i] = w[i];
+      }
+    }
+    __syncwarp();  // every lane has read the slot
+    fence_proxy_async_shared_cta();
+    request(row + 2 * step, slot);
+    if (++slot == 2) {
+      slot = 0;
+      phase ^= 1u;
+    }
+    float2 sum = both(0.0f), square = both(0.0f);
+#pragma unroll
+    for (int j = 0; j < kV; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum = add2(sum, raw[j].pair(i));  // (zeros beyond the row)
+    const float mean = warp_sum(sum.x + sum.y) * inverse;
+#pragma unroll
+    for (int j = 0; j < kV; ++j) {
+      if (8 * (lane + 32 * j) < n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 d = add2(raw[j].pair(i), both(-mean));
+          square = fma2(d, d, square);
+        }
+      }
+    }
+    const float rstd = 1.0f / sqrtf(warp_sum(square.x + square.y) * inverse + p.eps);
+    if (lane == 0) {
+      if (p.mean) p.mean[row] = mean;
+      if (p.rstd) p.rstd[row] = rstd;
+    }
+    Y* y = static_cast<Y*>(p.y) + row * p.ldy;
+#pragma unroll
+    for (int j = 0; j < kV; ++j) {
+      const int c = 8 * (lane + 32 * j);
+      if (c < n) {
+        const float4* g = reinterpret_cast<const float4*>(weights + c);
+        const float4* b = reinterpret_cast<const float4*>(weights + n + c);
+        float r[8];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float4 gg = g[h], bb = b[h];
+          const float2 lo = fma2(mul2(add2(raw[j].pair(2 * h), both(-mean)), both(rstd)), make_float2(gg.x, gg.y), make_float2(bb.x, bb.y));
+          const float2 hi = fma2(mul2(add2(raw[j].pair(2 * h + 1), both(-mean)), both(rstd)), make_float2(gg.z, gg.w), make_float2(bb.z, bb.w));
+          r[4 * h] = lo.x;
+          r[4 * h + 1] = lo.y;
+          r[4 * h + 2] = hi.x;
+          r[4 * h + 3] = hi.y;
+        }
+        store_eight<Y, true>(y, n, lane, 32, j, r);
+      }
+    }
+  }
+}
+
 // Rows too long for registers: three passes, the second and third out of L2.
 template <typename X, typename Y>
 __global__ void __launch_bounds__(kNormLongThreads) norm_long_kernel(const NormParams p) {
@@ -442,6 +577,143 @@ __global__ void __launch_bounds__(kWarp ? 128 : kNormMaxThreads) norm_grad_kerne
   }
 }
 
+// The same with rows on their way by bulk copies, p.ring rows ahead (rows of whole vectors of eight, 16-byte aligned):
+// a thread holds no row but the one it works on.  Shared memory: p.ring times the rows of x, dy and dr.
+template <typename X, typename Y, int kV>
+__global__ void __launch_bounds__(kNormMaxThreads / kV, sizeof(X) == 2 ? 2 : 1) norm_grad_ring_kernel(const NormParams p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  extern __shared__ __align__(16) uint8_t rows[];
+  __shared__ float2 slots[2][32];
+  __shared__ __align__(8) uint64_t barriers[kNormMaxRing];
+  __shared__ int abort_flag, failed;
+  const int t = threadIdx.x, threads = blockDim.x, n = p.n, lane = t & 31, warp = t >> 5, warps = threads >> 5;
+  const float inverse = 1.0f / static_cast<float>(n);
+  const uint32_t x_bytes = static_cast<uint32_t>(n) * sizeof(X), dy_bytes = static_cast<uint32_t>(n) * sizeof(Y);
+  const uint32_t slot_bytes = (p.dr ? 2u : 1u) * x_bytes + dy_bytes, bar = smem_u32(barriers), ring0 = smem_u32(rows);
+  if (t == 0) {
+    abort_flag = failed = 0;
+    for (int i = 0; i < p.ring; ++i) mbar_init(bar + 8u * i, 1);
+    fence_mbar_init();
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int64_t step = gridDim.x;
+  auto request = [&](int64_t r, uint32_t slot) {  // thread 0
+    if (r >= p.m) return;
+    const uint32_t to = ring0 + slot * slot_bytes, b = bar + 8u * slot;
+    mbar_expect_tx(b, slot_bytes);
+    bulk_load(to, static_cast<const X*>(p.x) + r * p.ldx, x_bytes, b);
+    bulk_load(to + x_bytes, static_cast<const Y*>(p.dy) + r * p.lddy, dy_bytes, b);
+    if (p.dr) bulk_load(to + x_bytes + dy_bytes, static_cast<const X*>(p.dr) + r * p.lddr, x_bytes, b);
+  };
+  int64_t row = blockIdx.x;
+  if (t == 0)
+    for (int i = 0; i < p.ring; ++i) request(row + i * step, static_cast<uint32_t>(i));
+  float2 gamma[kV][4], dgamma[kV][4], dbeta[kV][4];
+#pragma unroll
+  for (int j = 0; j < kV; ++j) {
+    float g[8];
+    load_vector<true>(p.gamma, n, t, threads, j, 1.0f, g);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      gamma[j][i] = make_float2(g[2 * i], g[2 * i + 1]);
+      dgamma[j][i] = dbeta[j][i] = both(0.0f);
+    }
+  }
+  float next_mean = row < p.m ? __ldg(p.mean_in + row) : 0.0f, next_rstd = row < p.m ? __ldg(p.rstd_in + row) : 0.0f;
+  __syncthreads();
+  const uint64_t budget_ns = static_cast<uint64_t>(p.wait_budget_us) * 1000ull;
+  uint32_t slot = 0, phase = 0, turn = 0;
+  for (; row < p.m; row += step, turn ^= 1u) {
+    const float mean = next_mean, rstd = next_rstd;
+    if (row + step < p.m) {
+      next_mean = __ldg(p.mean_in + row + step);
+      next_rstd = __ldg(p.rstd_in + row + step);
+    }
+    if (!mbar_wait_bounded(bar + 8u * slot, phase, &abort_flag, budget_ns)) failed = 1;
+    const uint32_t from = ring0 + slot * slot_bytes;
+    Eight<X> xs[kV], drs[kV];
+    Eight<Y> dys[kV];
+    auto take = [&](auto& e, uint32_t base, int c) {
+      constexpr int kWords = sizeof(e.w) / 4;
+#pragma unroll
+      for (int h = 0; h < kWords / 4; ++h) {
+        uint32_t w[4] = {0, 0, 0, 0};
+        if (c < n)
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                       : "r"(base + static_cast<uint32_t>(c * (kWords / 2) + 16 * h)));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e.w[4 * h + i] = w[i];
+      }
+    };
+#pragma unroll
+    for (int j = 0; j < kV; ++j) {
+      const int c = 8 * (t + threads * j);
+      take(xs[j], from, c);
+      take(dys[j], from + x_bytes, c);
+      if (p.dr) take(drs[j], from + x_bytes + dy_bytes, c);
+    }
+    // (elements beyond the row: dy is zero, and with it all that is added up)
+    float2 sum = both(0.0f), along = both(0.0f);
+#pragma unroll
+    for (int j = 0; j < kV; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 d = dys[j].pair(i), xhat = mul2(add2(xs[j].pair(i), both(-mean)), both(rstd)), g = mul2(d, gamma[j][i]);
+        dgamma[j][i] = fma2(d, xhat, dgamma[j][i]);
+        dbeta[j][i] = add2(dbeta[j][i], d);
+        sum = add2(sum, g);
+        along = fma2(g, xhat, along);
+      }
+    float s1 = warp_sum(sum.x + sum.y), s2 = warp_sum(along.x + along.y);
+    if (lane == 0) slots[turn][warp] = make_float2(s1, s2);
+    fence_proxy_async_shared_cta();  // the slot has been read: before it is filled again
+    __syncthreads();
+    if (failed) break;
+    if (t == 0) request(row + p.ring * step, slot);
+    if (++slot == static_cast<uint32_t>(p.ring)) {
+      slot = 0;
+      phase ^= 1u;
+    }
+    const float2 v = lane < warps ? slots[turn][lane] : make_float2(0.0f, 0.0f);
+    s1 = warp_sum(v.x) * inverse;
+    s2 = warp_sum(v.y) * inverse;
+    X* dx = static_cast<X*>(p.y) + row * p.ldy;
+#pragma unroll
+    for (int j = 0; j < kV; ++j) {
+      float r[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 xhat = mul2(add2(xs[j].pair(i), both(-mean)), both(rstd));
+        const float2 even = fma2(xhat, both(s2), both(s1));
+        float2 v2 = mul2(both(rstd), add2(mul2(dys[j].pair(i), gamma[j][i]), make_float2(-even.x, -even.y)));
+        if (p.dr) v2 = add2(v2, drs[j].pair(i));
+        r[2 * i] = v2.x;
+        r[2 * i + 1] = v2.y;
+      }
+      store_eight<X, true>(dx, n, t, threads, j, r);
+    }
+  }
+  if (failed) {
+    if (t == 0) leave_error(p.error, kErrProducerWait);
+    return;
+  }
+  if (p.sums == nullptr) return;
+  float* out = p.sums + static_cast<int64_t>(blockIdx.x) * n;
+  const int64_t other = static_cast<int64_t>(gridDim.x) * n;
+#pragma unroll
+  for (int j = 0; j < kV; ++j) {
+    const int c = 8 * (t + threads * j);
+    if (c < n) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        *reinterpret_cast<float2*>(out + c + 2 * i) = dgamma[j][i];
+        *reinterpret_cast<float2*>(out + other + c + 2 * i) = dbeta[j][i];
+      }
+    }
+  }
+}
+
 // Rows too long for registers: dx in two passes, the columns' sums in a kernel of their own.
 template <typename X, typename Y>
 __global__ void __launch_bounds__(kNormLongThreads) norm_grad_long_kernel(const NormParams p) {
@@ -503,35 +775,35 @@ __device__ __forceinline__ float clamp_nan(float v, float most) {
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(v) : "f"(-most));
   return v;
 }
-// act'(z).  Beyond the clamps the slopes are 0 or 1 to the last bit of f32, and the products of an infinity
-// and a zero that the formulas have there are not formed.  t = exp(-|v|) gives both the logistic and one
-// minus it without a cancellation.  exp2 of a rounded product is exact enough: the product's rounding, |v| eps / 2 of t,
-// is at most eps / 5 of one, and the approximate exp2 and reciprocal are within 2 ulp: together 3e-7 of dy.
+// dy act'(z) of two elements.  gelu and silu are z s with s = 1 / (1 + t), t = exp(-v): their slope is
+// s (1 + z v' (1 - s)) with 1 - s = t s, which does not cancel.  z is clamped where the slope is 0 or 1 to the last
+// bit of f32 and t still a number (exp(88.5)): beyond, the products of an infinity and a zero that the formulas have there
+// are not formed.  exp2 of a rounded product is exact enough: the product's rounding, |v| eps / 2 of t, is at most
+// eps / 5 of one in t s, and the approximate exp2 and reciprocal are within 2 ulp: together 3e-7 of dy.
 template <int kAct>
-__device__ __forceinline__ float activation_slope(float z) {
-  if constexpr (kAct == kOpRelu) return z <= 0.0f ? 0.0f : 1.0f;
+__device__ __forceinline__ float2 slope_times(float2 dy, float2 z) {
+  if constexpr (kAct == 0) return dy;
+  if constexpr (kAct == kOpRelu) return make_float2(z.x <= 0.0f ? 0.0f : dy.x, z.y <= 0.0f ? 0.0f : dy.y);
   constexpr bool kGelu = kAct == kOpGelu;
-  z = clamp_nan(z, kGelu ? 12.0f : 100.0f);
-  float v = z, w = z;  // the logistic's argument, and z times its slope
+  constexpr float most = kGelu ? 10.05f : 88.4f, log2e = 1.4426950408889634f;
+  z = make_float2(clamp_nan(z.x, most), clamp_nan(z.y, most));
+  float2 v, w;  // -v log2(e), and z v'
   if constexpr (kGelu) {
     constexpr float c = 2.0f * 0.7978845608028654f;
-    const float zz = z * z;
-    v = z * __fmaf_rn(c * 0.044715f, zz, c);
-    w = z * __fmaf_rn(c * 3.0f * 0.044715f, zz, c);
+    const float2 zz = mul2(z, z);
+    v = mul2(z, fma2(both(-c * 0.044715f * log2e), zz, both(-c * log2e)));
+    w = mul2(z, fma2(both(c * 3.0f * 0.044715f), zz, both(c)));
+  } else {
+    v = mul2(z, both(-log2e));
+    w = z;
   }
-  float t, big;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fabsf(v) * -1.4426950408889634f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(big) : "f"(1.0f + t));
-  const float small = t * big;
-  const float s = v >= 0.0f ? big : small, rest = v >= 0.0f ? small : big;
-  return s * __fmaf_rn(w, rest, 1.0f);
-}
-
-template <int kAct>
-__device__ __forceinline__ float slope_times(float dy, float z) {
-  if constexpr (kAct == 0) return dy;
-  if constexpr (kAct == kOpRelu) return z <= 0.0f ? 0.0f : dy;
-  return dy * activation_slope<kAct>(z);
+  float2 t, s;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t.x) : "f"(v.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t.y) : "f"(v.y));
+  const float2 d = add2(t, both(1.0f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.x) : "f"(d.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.y) : "f"(d.y));
+  return mul2(mul2(dy, s), fma2(w, mul2(t, s), both(1.0f)));
 }
 
 // A warp takes rows of the CTA's strip of 256 columns in turn, eight columns per lane: loads and stores of whole
@@ -548,13 +820,15 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 && kWide ? 4 : 3) epilogue
   const T* dy = static_cast<const T*>(p.dy) + c0;
   const T* z = kAct ? static_cast<const T*>(p.z) + c0 : nullptr;
   T* dz = p.dz ? static_cast<T*>(p.dz) + c0 : nullptr;
-  float sums[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  float2 sums[4] = {both(0.0f), both(0.0f), both(0.0f), both(0.0f)};
   auto finish = [&](int64_t row, const Eight<T>& a, const Eight<T>& b) {
     float v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      v[i] = slope_times<kAct>(a[i], kAct ? b[i] : 0.0f);
-      sums[i] += v[i];
+    for (int i = 0; i < 4; ++i) {
+      const float2 r = slope_times<kAct>(a.pair(i), kAct ? b.pair(i) : both(0.0f));
+      sums[i] = add2(sums[i], r);
+      v[2 * i] = r.x;
+      v[2 * i + 1] = r.y;
     }
     if (kAct || dz) store_eight<T, kWide>(dz + row * p.lddz, n, lane, 32, 0, v);
   };
@@ -578,7 +852,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 && kWide ? 4 : 3) epilogue
   }
   if (p.sums == nullptr) return;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) join[warp][element_of<T, kWide>(lane, 32, 0, i)] = sums[i];
+  for (int i = 0; i < 8; ++i) join[warp][element_of<T, kWide>(lane, 32, 0, i)] = i % 2 ? sums[i / 2].y : sums[i / 2].x;
   __syncthreads();
   const int c = threadIdx.x;
   if (c < n) {
@@ -589,26 +863,36 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 && kWide ? 4 : 3) epilogue
   }
 }
 
-// Block (x, y): 32 columns of result y; its warps take the parts in turn.
-__global__ void __launch_bounds__(512) column_sum_kernel(const ColumnSumParams p) {
+// Block (x, y): 64 columns of result y, two to a lane; its warps take the parts in turn.
+__global__ void __launch_bounds__(1024) column_sum_kernel(const ColumnSumParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  __shared__ float join[16][32];
+  __shared__ float2 join[32][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * 64 + 2 * lane;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   float* out = blockIdx.y == 0 ? p.out0 : p.out1;
   if (out == nullptr) return;
-  float sum = 0.0f;
-  if (c < p.n) {
-    const float* in = p.in + static_cast<int64_t>(blockIdx.y) * p.parts * p.n + c;
-#pragma unroll 8
-    for (int i = warp; i < p.parts; i += warps) sum += __ldcg(in + static_cast<int64_t>(i) * p.n);
+  float2 sum = both(0.0f);
+  const float* in = p.in + static_cast<int64_t>(blockIdx.y) * p.parts * p.n + c;
+  if (p.n % 2 == 0) {
+    if (c < p.n) {
+#pragma unroll 10
+      for (int i = warp; i < p.parts; i += warps) sum = add2(sum, __ldcg(reinterpret_cast<const float2*>(in + static_cast<int64_t>(i) * p.n)));
+    }
+  } else if (c < p.n) {
+    const bool two = c + 1 < p.n;
+#pragma unroll 5
+    for (int i = warp; i < p.parts; i += warps) {
+      const float* at = in + static_cast<int64_t>(i) * p.n;
+      sum = add2(sum, make_float2(__ldcg(at), two ? __ldcg(at + 1) : 0.0f));
+    }
   }
   join[warp][lane] = sum;
   __syncthreads();
   if (warp == 0 && c < p.n) {
-    for (int w = 1; w < warps; ++w) sum += join[w][lane];
-    out[c] = sum;
+    for (int w = 1; w < warps; ++w) sum = add2(sum, join[w][lane]);
+    out[c] = sum.x;
+    if (c + 1 < p.n) out[c + 1] = sum.y;
   }
 }
 
