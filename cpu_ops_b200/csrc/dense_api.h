@@ -140,8 +140,10 @@ int dense_kernels_ready(DeviceState& st) {
     for (int y : {kF32, kF16, kBf16})
       for (bool gradient : {false, true}) {
         if (x != y && x != kF32) continue;
-        const NormChoice c = norm_choice(x, y, 2048, true, true, true, gradient);  // (the one with shared memory)
-        CUDA_TRY(cudaFuncSetAttribute(c.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kNormMostSmem));
+        for (int n : {2048, 8192}) {  // (those with shared memory)
+          const NormChoice c = norm_choice(x, y, n, true, true, true, gradient);
+          CUDA_TRY(cudaFuncSetAttribute(c.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kNormMostSmem));
+        }
       }
   ready[st.device] = true;
   return 0;
@@ -431,12 +433,16 @@ int epilogue_grad_call(const cpuops_b200_epilogue_grad_desc* d) {
   p.type = d->type;
   p.act = d->activation == CPUOPS_B200_OP_RELU ? kOpRelu : d->activation == CPUOPS_B200_OP_GELU ? kOpGelu
         : d->activation == CPUOPS_B200_OP_SILU ? kOpSilu : 0;
+  const bool wide = rows_aligned(d->dy, d->lddy, d->type) && (!act || rows_aligned(d->z, d->ldz, d->type)) &&
+                    (!d->dz || rows_aligned(d->dz, d->lddz, d->type));
+  // 16-bit rows on odd elements: every second one begins in the middle of a word, and a block takes those or the others.
+  p.every = !wide && d->type != kF32 && d->m > 1 && (d->dz ? d->lddz : d->lddy) % 2 != 0 ? 2 : 1;
   // Blocks of rows: enough CTAs for six on every SM, at least 32 rows each.
-  const int strips = (d->n + 255) / 256;
+  const int strips = (d->n + (wide || d->type == kF32 ? 255 : 256)) / 256;
   const int want = std::max(1, 6 * call.st->sms() / strips);
   int block_rows = std::max(32, (d->m + want - 1) / want);
-  block_rows = std::max(block_rows, (d->m + 65534) / 65535);
-  const int blocks = std::max(1, (d->m + block_rows - 1) / block_rows);
+  block_rows = std::max(block_rows, (d->m + 32766) / 32767);
+  const int blocks = p.every * std::max(1, (d->m + block_rows * p.every - 1) / (block_rows * p.every));
   p.block_rows = block_rows;
   float* parts = nullptr;
   if (d->dbias && blocks > 1) {
@@ -445,8 +451,6 @@ int epilogue_grad_call(const cpuops_b200_epilogue_grad_desc* d) {
     parts = reinterpret_cast<float*>(ws);
   }
   p.sums = d->dbias ? (parts ? parts : d->dbias) : nullptr;
-  const bool wide = rows_aligned(d->dy, d->lddy, d->type) && (!act || rows_aligned(d->z, d->ldz, d->type)) &&
-                    (!d->dz || rows_aligned(d->dz, d->lddz, d->type));
   if (int rc = launch_after(epilogue_grad_of(d->type, p.act, wide), dim3(static_cast<unsigned>(strips), static_cast<unsigned>(blocks)), 256, 0,
                             call.stream, p))
     return rc;
@@ -499,7 +503,7 @@ int layer_norm_call(const cpuops_b200_layer_norm_desc* d) {
   const bool wide = rows_aligned(d->x, d->ldx, d->x_type) && rows_aligned(d->y, d->ldy, d->y_type);
   const NormChoice c = norm_choice(d->x_type, d->y_type, d->n, wide, d->m >= 4 * call.st->sms(), false, false);
   const int rows = (d->m + c.rows_at_once - 1) / c.rows_at_once;
-  const int grid = std::min(rows, call.st->sms() * (c.ring ? 1 : std::max(1, std::min(16, 1024 / c.threads))));
+  const int grid = std::min(rows, call.st->sms() * (c.ring ? 1 : std::max(1, std::min(16, 1536 / c.threads))));
   p.ring = c.ring;
   p.error = call.st->error_dev;
   p.wait_budget_us = g_wait_budget_us.load();
@@ -554,7 +558,8 @@ int layer_norm_grad_call(const cpuops_b200_layer_norm_grad_desc* d) {
                     rows_aligned(d->dx, d->lddx, d->x_type) && (!d->dr || rows_aligned(d->dr, d->lddr, d->x_type));
   const NormChoice c = norm_choice(d->x_type, d->y_type, d->n, wide, d->m >= 4 * call.st->sms(), d->dr != nullptr, true);
   const int rows = std::max(1, (d->m + c.rows_at_once - 1) / c.rows_at_once);
-  const int grid = std::min(rows, call.st->sms() * std::max(1, std::min(16, 512 / c.threads)));
+  int grid = std::min(rows, call.st->sms() * std::max(1, std::min(4, 512 / c.threads)));  // (a row of sums each)
+  if (c.even && grid > 1) grid &= ~1;
   p.ring = c.ring;
   p.error = call.st->error_dev;
   p.wait_budget_us = g_wait_budget_us.load();

@@ -41,44 +41,57 @@ NormChoice norm_choice_for(int n, bool wide, bool many, bool dr) {
       return c;
     }
     const int row_bytes = n * static_cast<int>((dr ? 2 : 1) * sizeof(X) + sizeof(Y));
-    if (wide && many && n % 8 == 0 && n > 1024 && n <= 4096) {
-      // sixteen elements per thread, so that half as many threads share in a row's two sums; two CTAs per SM
-      c.threads = (n / 16 + 31) / 32 * 32;
-      c.ring = std::min(kNormMaxRing, 100 * 1024 / row_bytes);
+    if (wide && many && n % 8 == 0) {
+      // sixteen elements per thread, so that few threads share in a row's two sums; two CTAs per SM and more, or one of
+      // rows beyond 4096
+      const bool one = n > 4096;
+      c.threads = ((n + 15) / 16 + 31) / 32 * 32;
+      c.ring = std::min(kNormMaxRing, (one ? kNormMostSmem : std::min(100 * 1024, c.threads * 400)) / row_bytes);
       c.smem = c.ring * row_bytes;
-      c.kernel = norm_grad_ring_kernel<X, Y, 2>;
+      c.kernel = one ? norm_grad_ring_kernel<X, Y, 2, 512> : norm_grad_ring_kernel<X, Y, 2, 256>;
+      if (c.ring >= 2) return c;
+      c.ring = c.smem = 0;
+    }
+    if (!wide) {
+      c.threads = kNormGradPairThreads;
+      c.even = true;
+      c.kernel = n <= 2048 ? norm_grad_pairs_kernel<X, Y, 5> : n <= 4096 ? norm_grad_pairs_kernel<X, Y, 9> : norm_grad_pairs_kernel<X, Y, 17>;
       return c;
     }
     // (many rows: sixteen elements per thread, so that half as many threads share in a row's two sums)
     const bool two = n > 8 * kNormMaxThreads || (many && n > 1024 && sizeof(X) == 2);
     const int per = two ? 16 : 8;
     c.threads = ((n + per - 1) / per + 31) / 32 * 32;
-    c.kernel = two ? (wide ? norm_grad_kernel<X, Y, true, false, 2> : norm_grad_kernel<X, Y, false, false, 2>)
-                   : (wide ? norm_grad_kernel<X, Y, true, false, 1> : norm_grad_kernel<X, Y, false, false, 1>);
+    c.kernel = two ? norm_grad_kernel<X, Y, true, false, 2> : norm_grad_kernel<X, Y, true, false, 1>;
   } else {
-    const int ring_smem = 2 * n * static_cast<int>(sizeof(float)) + 2 * kNormWarps * n * static_cast<int>(sizeof(X));
-    if (wide && many && n % 8 == 0 && n > 1024 && n <= kNormWarpMost && ring_smem <= kNormMostSmem) {
+    constexpr int kSlots = sizeof(X) == 2 ? 2 : 1;
+    if (wide && many && n % 8 == 0 && n > 1024 && n <= kNormWarpMost) {
       c.threads = 32 * kNormWarps;
       c.rows_at_once = kNormWarps;
-      c.ring = 2;
-      c.smem = ring_smem;
-      c.kernel = norm_ring_kernel<X, Y, 16>;
+      c.ring = 1;
+      c.smem = 2 * n * static_cast<int>(sizeof(float)) + kSlots * kNormWarps * n * static_cast<int>(sizeof(X));
+      c.kernel = norm_ring_kernel<X, Y, 16, kNormWarps, kSlots>;
+      return c;
+    }
+    if (!wide && n > 256) {
+      c.threads = kNormPairThreads;
+      c.kernel = n <= 4096 ? norm_pairs_kernel<X, Y, 17> : norm_pairs_kernel<X, Y, 33>;
       return c;
     }
     if (n <= 256 || (many && n <= kNormWarpMost)) {
       c.threads = 32 * kNormWarps;
       c.rows_at_once = kNormWarps;
       c.smem = 2 * ((n + 7) / 8 * 8) * static_cast<int>(sizeof(float));
+      // (rows of whole vectors beyond 1024 took norm_ring_kernel)
       c.kernel = n <= 256    ? (wide ? norm_rows_kernel<X, Y, true, 1> : norm_rows_kernel<X, Y, false, 1>)
-                 : n <= 1024 ? (wide ? norm_rows_kernel<X, Y, true, 4> : norm_rows_kernel<X, Y, false, 4>)
-                             : (wide ? norm_rows_kernel<X, Y, true, 16> : norm_rows_kernel<X, Y, false, 16>);
+                 : n <= 1024 ? norm_rows_kernel<X, Y, true, 4>
+                             : norm_rows_kernel<X, Y, true, 16>;
       return c;
     }
     const bool two = n > 8 * kNormMaxThreads;
     const int per = two ? 16 : 8;
     c.threads = ((n + per - 1) / per + 31) / 32 * 32;
-    c.kernel = two ? (wide ? norm_kernel<X, Y, true, 2> : norm_kernel<X, Y, false, 2>)
-                   : (wide ? norm_kernel<X, Y, true, 1> : norm_kernel<X, Y, false, 1>);
+    c.kernel = two ? norm_kernel<X, Y, true, 2> : norm_kernel<X, Y, true, 1>;
   }
   return c;
 }
@@ -98,6 +111,13 @@ EpilogueGradKernel epilogue_grad_for(int act) {
          : act == kOpGelu ? epilogue_grad_kernel<T, kOpGelu, kWide>
          : act == kOpSilu ? epilogue_grad_kernel<T, kOpSilu, kWide>
                           : epilogue_grad_kernel<T, 0, kWide>;
+}
+template <typename T>
+EpilogueGradKernel epilogue_grad_pairs_for(int act) {
+  return act == kOpRelu   ? epilogue_grad_pairs_kernel<T, kOpRelu>
+         : act == kOpGelu ? epilogue_grad_pairs_kernel<T, kOpGelu>
+         : act == kOpSilu ? epilogue_grad_pairs_kernel<T, kOpSilu>
+                          : epilogue_grad_pairs_kernel<T, 0>;
 }
 
 template <typename T>
@@ -127,8 +147,8 @@ NormColumnsKernel norm_grad_columns(int x_type, int y_type) {
 
 EpilogueGradKernel epilogue_grad_of(int type, int act, bool wide) {
   if (type == kF32) return wide ? epilogue_grad_for<float, true>(act) : epilogue_grad_for<float, false>(act);
-  if (type == kF16) return wide ? epilogue_grad_for<__half, true>(act) : epilogue_grad_for<__half, false>(act);
-  return wide ? epilogue_grad_for<__nv_bfloat16, true>(act) : epilogue_grad_for<__nv_bfloat16, false>(act);
+  if (type == kF16) return wide ? epilogue_grad_for<__half, true>(act) : epilogue_grad_pairs_for<__half>(act);
+  return wide ? epilogue_grad_for<__nv_bfloat16, true>(act) : epilogue_grad_pairs_for<__nv_bfloat16>(act);
 }
 ColumnSumKernel column_sum() { return column_sum_kernel; }
 

@@ -21,8 +21,9 @@ struct NormChoice {
   int rows_at_once;  // of a CTA
   int smem;
   int ring;          // rows on their way by bulk copies (0: none)
+  bool even;         // takes an even number of CTAs (of two rows or more)
 };
-// `many`: rows enough for several on every SM; `dr`: the gradient adds one.
+// wide: 16-byte aligned rows.  `many`: rows enough for several on every SM; `dr`: the gradient adds one.
 NormChoice norm_choice(int x_type, int y_type, int n, bool wide, bool many, bool dr, bool gradient);
 constexpr int kNormMostSmem = 200 * 1024;  // of a choice
 using NormColumnsKernel = void (*)(NormParams, int);

@@ -61,6 +61,7 @@ struct EpilogueGradParams {
   int64_t lddy, ldz, lddz;
   int32_t m, n, act, type;
   int32_t block_rows;
+  int32_t every;      // rows that are not 16-byte aligned: a block takes every row, or every second one
 };
 
 // Sum of `parts` rows of n, `parts * count` floats apart from one result to the next.

@@ -163,7 +163,7 @@ def test_product_infinities_stay_in_their_rows(gpu, m, n, k):
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("name", ["none", "relu", "gelu", "silu"])
 def test_epilogue_grad(gpu, kind, name):
-    for m, n, pad in [(1, 1, 0), (1, 300, 0), (33, 256, 0), (70, 515, 3), (1000, 264, 8), (3000, 40, 1)]:
+    for m, n, pad in [(1, 1, 0), (1, 300, 0), (33, 256, 0), (70, 515, 3), (1000, 264, 8), (3000, 40, 1), (777, 511, 0), (400, 256, 1), (301, 1023, 2)]:
         dy, z = matrix(m, n, pad, kind, 1), matrix(m, n, pad, kind, 2, 3.0)
         dz, dbias = held(m, n, pad, kind), torch.full((n + 1,), GUARD, device="cuda")
         op = c.BiasActivationGrad(STORAGE[kind], ACT[name])
@@ -205,7 +205,8 @@ def test_slopes_of_far_values(gpu, name, limits):
 
 PAIRS = [("f32", "f32"), ("f32", "f16"), ("f32", "bf16"), ("f16", "f16"), ("bf16", "bf16")]
 ROWS = [(1, 1, 0), (3, 5, 0), (1000, 64, 0), (77, 256, 0), (50, 257, 3), (9, 1000, 0), (700, 515, 1), (130, 4096, 0), (5, 4100, 4),
-        (400, 8192, 0), (3, 8193, 0), (6, 20000, 8)]
+        (400, 8192, 0), (3, 8193, 0), (6, 20000, 8), (700, 2048, 0), (1300, 1032, 8), (601, 4096, 8), (640, 3000, 1), (2, 2047, 2), (300, 300, 0),
+        (45, 5001, 0), (640, 264, 0), (600, 5000, 8), (593, 8192, 0)]
 
 
 @pytest.mark.parametrize("x_type,y_type", PAIRS)
