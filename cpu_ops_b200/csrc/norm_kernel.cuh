@@ -324,8 +324,8 @@ __global__ void __launch_bounds__(32 * kNormWarps, sizeof(X) == 2 || kV < 16 ? 2
 }
 
 // The same with a warp's rows on their way by bulk copies, two rows ahead of the one that is worked on: the loads
-// do not wait for the arithmetic (8192 x 4096 bf16 44 us without, XXX in this form).  Rows are whole vectors of eight,
-// 16-byte aligned.  Shared memory: gamma and beta, two rows per warp.
+// do not wait for the arithmetic (8192 x 4096 bf16 44 us without, 31 in this form; 12 warps with two rows each, or 16 with
+// one, 31 and 36).  Rows are whole vectors of eight, 16-byte aligned.  Shared memory: gamma and beta, kSlots rows per warp.
 template <typename X, typename Y, int kV, int kWarps, int kSlots>
 __global__ void __launch_bounds__(32 * kWarps, 1) norm_ring_kernel(const NormParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -360,7 +360,13 @@ __global__ void __launch_bounds__(32 * kWarps, 1) norm_ring_kernel(const NormPar
   uint32_t slot = 0, phase = 0;
   for (; row < p.m; row += step) {
     if (!__all_sync(0xffffffffu, mbar_wait_bounded(bar + 8u * slot, phase, &abort_flag, budget_ns))) {
-      if (lane == 0) leave_error(p.error, kErrProducerWait);
+      if (lane == 0) {
+        leave_error(p.error, kErrProducerWait);
+        // copies that are on their way land before the CTA ends
+        int dummy = 0;
+        for (uint32_t i = 0; i < kSlots; ++i)
+          mbar_wait_bounded(bar + 8u * i, i < slot ? phase ^ 1u : phase, &dummy, budget_ns);
+      }
       break;
     }
     Eight<X> raw[kV];
@@ -783,7 +789,8 @@ __global__ void __launch_bounds__(kWarp ? 128 : kNormMaxThreads) norm_grad_kerne
 }
 
 // The same with rows on their way by bulk copies, p.ring rows ahead (rows of whole vectors of eight, 16-byte aligned):
-// a thread holds no row but the one it works on.  Shared memory: p.ring times the rows of x, dy and dr.
+// a thread holds no row but the one it works on (8192 x 4096 bf16 with dr 76 us with the next row in registers, 51 in this
+// form: 5.2 TB/s).  Shared memory: p.ring times the rows of x, dy and dr.
 template <typename X, typename Y, int kV, int kMaxThreads>
 __global__ void __launch_bounds__(kMaxThreads, kMaxThreads == 256 && sizeof(X) == 2 ? 2 : 1) norm_grad_ring_kernel(const NormParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -900,7 +907,13 @@ __global__ void __launch_bounds__(kMaxThreads, kMaxThreads == 256 && sizeof(X) =
     }
   }
   if (failed) {
-    if (t == 0) leave_error(p.error, kErrProducerWait);
+    if (t == 0) {
+      leave_error(p.error, kErrProducerWait);
+      int dummy = 0;  // copies that are on their way land before the CTA ends
+      for (uint32_t i = 0; i < static_cast<uint32_t>(p.ring); ++i)
+        mbar_wait_bounded(bar + 8u * i, i < slot ? phase ^ 1u : phase, &dummy, budget_ns);
+    }
+    __syncthreads();
     return;
   }
   if (p.sums == nullptr) return;

@@ -31,8 +31,8 @@ __device__ __forceinline__ void product_error(const ProductParams& p, volatile i
 }
 
 // Hands an accumulator back to the pair's leader.  Its reads are complete (tcgen05.wait::ld), nothing else is published:
-// with release semantics the arrival waits for all the thread's stores, TMA's among them, which took 1000 to 2500 cycles
-// (4096 x 2048 x 8192 in pieces 120 us, XXX so).
+// with release semantics the arrival waits for the thread's stores, which took 1000 to 2500 cycles (8192 x 4096 x 1024
+// 53 us, 49 in this form; with gelu, Z and C 91 and 80).
 __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
