@@ -24,10 +24,10 @@ __host__ __device__ constexpr int balance_warps(int per_lane) { return per_lane 
 
 // Counts of the tokens [begin, end) into shared memory: counts[0 .. experts), and counts[experts]
 // of tokens that have an expert.  All threads of the CTA.
-__device__ __forceinline__ void count_pairs(const BalanceParams& p, int begin, int end, int32_t* counts) {
+__device__ __forceinline__ void count_pairs(const BalanceParams& p, int64_t begin, int64_t end, int32_t* counts) {
   for (int i = threadIdx.x; i <= p.experts; i += blockDim.x) counts[i] = 0;
   __syncthreads();
-  for (int64_t t = begin + static_cast<int>(threadIdx.x); t < end; t += blockDim.x) {
+  for (int64_t t = begin + threadIdx.x; t < end; t += blockDim.x) {
     bool any = false;
     for (int k = 0; k < p.top_k; ++k) {
       const int32_t id = __ldg(p.ids + t * p.top_k + k);
@@ -46,9 +46,9 @@ __global__ void __launch_bounds__(kBalanceCountThreads) balance_count_kernel(con
   __shared__ int32_t counts[1025];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (blockIdx.x == 0 && threadIdx.x == 0) *p.ticket = 0;
-  const int per = (p.tokens + p.count_blocks - 1) / p.count_blocks;
-  const int begin = min(static_cast<int>(blockIdx.x) * per, p.tokens);
-  count_pairs(p, begin, min(begin + per, p.tokens), counts);
+  const int64_t tokens = p.tokens, per = (tokens + p.count_blocks - 1) / p.count_blocks;
+  const int64_t begin = min(blockIdx.x * per, tokens);
+  count_pairs(p, begin, min(begin + per, tokens), counts);
   for (int i = threadIdx.x; i <= p.experts; i += blockDim.x) p.part_counts[static_cast<int64_t>(blockIdx.x) * (p.experts + 1) + i] = counts[i];
 }
 

@@ -66,7 +66,7 @@ int product_clusters(DeviceState& st, int form, int size) {
     probe.attrs = attr;
     probe.numAttrs = 1;
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, product_kernel_of(form, true), &probe) != cudaSuccess) {
+    if (cudaOccupancyMaxActiveClusters(&n, product_kernel_of(form, true, true), &probe) != cudaSuccess) {
       cudaGetLastError();
       n = 0;
     }
@@ -82,8 +82,8 @@ struct ProductChoice {
 };
 
 // Shared memory of a choice: stages, epilogue warps and their buffers.  `chunks`: bytes of one chunk each of C, D and
-// Z (0: not by TMA).  False: it does not fit.
-bool fit_product(ProductChoice& c, int smem_optin, int chunks, int k_blocks, bool pieces) {
+// Z (0: not by TMA); `rows`: an epilogue warp's otherwise.  False: it does not fit.
+bool fit_product(ProductChoice& c, int smem_optin, int chunks, int rows, int k_blocks, bool pieces) {
   const int room = smem_optin - 1024 - kProductBarrierBytes - 4 * kProductBiasFloats;
   const int stage = (kTileM + c.BN / (c.form == kProductPairs ? 2 : 1)) * 128;
   if (c.form == kProductParts) {
@@ -96,7 +96,7 @@ bool fit_product(ProductChoice& c, int smem_optin, int chunks, int k_blocks, boo
     for (int attempt = 0; attempt < 3; ++attempt) {
       c.epi_warps = attempt < 2 || pieces ? 8 : 4;
       c.ring_depth = attempt == 0 ? 2 : 1;
-      c.ring_bytes = chunks ? c.ring_depth * chunks : 4096;
+      c.ring_bytes = chunks ? c.ring_depth * chunks : rows;
       c.stages = (room - c.epi_warps * c.ring_bytes) / stage;
       if (c.stages >= 5) break;
     }
@@ -107,7 +107,9 @@ bool fit_product(ProductChoice& c, int smem_optin, int chunks, int k_blocks, boo
 
 // Estimated time in us; the choice whose is least is taken.  Measured on B200 at K = 1024 .. 8192 (a k-block of one tile,
 // rounds of tiles, and what does not shrink with k); us, estimated / measured:
-//   XXXEST
+//   512 x 2048 x 1024: tiles of 64 6.5 / 6.3, of 128 9.2 / 7.4, pairs of 128 9.2 / 7.3, of 256 14.5 / 11.2, two parts 11.7 / 11.4
+//   256 x 4096 x 4096: tiles of 64 16.6 / 16.3, pairs of 128 20.7 / 18.1, two parts of 128 19.1 / 20.4
+//   4096 x 4096 x 4096: pairs of 256 100 / 94, of 192 102 / 95, of 128 106 / 100, tiles of 128 125 / 115
 // chunk_us: an epilogue warp's time for 32 x 32 elements; hbm_us: the bytes that the call cannot do without.
 double product_us(const ProductChoice& c, const DeviceState& st, int Mk, int Nk, int k_blocks, bool pieces, double chunk_us, double hbm_us) {
   const bool pair = c.form == kProductPairs;
@@ -135,7 +137,8 @@ int dense_kernels_ready(DeviceState& st) {
   if (ready[st.device]) return 0;
   for (int form : {kProductTiles, kProductPairs, kProductParts})
     for (bool pieces : {false, true})
-      CUDA_TRY(cudaFuncSetAttribute(product_kernel_of(form, pieces), cudaFuncAttributeMaxDynamicSharedMemorySize, st.smem_optin));
+      for (bool tma : {false, true})
+        CUDA_TRY(cudaFuncSetAttribute(product_kernel_of(form, pieces, tma), cudaFuncAttributeMaxDynamicSharedMemorySize, st.smem_optin));
   for (int x : {kF32, kF16, kBf16})
     for (int y : {kF32, kF16, kBf16})
       for (bool gradient : {false, true}) {
@@ -249,7 +252,7 @@ int gemm16_call(const cpuops_b200_gemm16_desc* d) {
     if ((d->flags & CPUOPS_B200_FLAG_PAIR_ON) && form != kProductPairs) return;
     if ((d->flags & CPUOPS_B200_FLAG_PAIR_OFF) && form == kProductPairs) return;
     if (form != kProductTiles && product_clusters(st, form, form == kProductPairs ? 2 : parts) < 1) return;
-    if (!fit_product(c, st.smem_optin, chunks, k_blocks, pieces)) return;
+    if (!fit_product(c, st.smem_optin, chunks, use_c && d->c_type == kF32 ? 2 * 4096 : 4096, k_blocks, pieces)) return;
     const int Mk = swapped ? d->n : d->m, Nk = swapped ? d->m : d->n;
     if (form == kProductParts && !(swapped ? b.mn : a.mn)) {
       // Tiles of fewer rows where that gives every cluster one (a tile's other rows are neither loaded nor used):
@@ -259,6 +262,10 @@ int gemm16_call(const cpuops_b200_gemm16_desc* d) {
       const int64_t along_m = std::max<int64_t>(1, rounds * clusters / columns);
       c.tile_rows = static_cast<int>(std::min<int64_t>(128, ((Mk + along_m - 1) / along_m + 7) / 8 * 8));
     }
+    // (parts are launched all at once: a limit on the SMs is kept by the other forms)
+    if (form == kProductParts && st.sms() < st.sm_count &&
+        static_cast<int64_t>((Mk + c.tile_rows - 1) / c.tile_rows) * ((Nk + BN - 1) / BN) * parts > st.sms())
+      return;
     const double us = product_us(c, st, Mk, Nk, k_blocks, pieces, chunk_us, hbm_us);
     if (!found || us < least) {
       best = c;
@@ -288,7 +295,7 @@ int gemm16_call(const cpuops_b200_gemm16_desc* d) {
     Side& s = *sides[i];
     if (tma_addressable(s.base, s.ld * 2, s.outer)) continue;
     if (s.inner > INT32_MAX / 2 - 16) return refuse("gemm16: rows longer than 2^30 bytes need 16-byte aligned operands");
-    const int64_t pitch = (static_cast<int64_t>(s.inner) * 2 + 15) / 16 * 16;
+    const int64_t pitch = (static_cast<int64_t>(s.inner) * 2 + 127) / 128 * 128;  // (a box's row is one line then)
     off_copy[n_jobs] = plan.take(static_cast<size_t>(pitch) * s.outer);
     RepackJob& j = jobs[n_jobs++];
     j.src = static_cast<const uint8_t*>(s.base);
@@ -330,7 +337,6 @@ int gemm16_call(const cpuops_b200_gemm16_desc* d) {
   p.epi_warps = c.epi_warps;
   p.ring_bytes = c.ring_bytes;
   p.ring_depth = c.ring_depth;
-  p.by_tma = by_tma ? 1 : 0;
   const uint32_t fmt = d->type == kBf16 ? 1u : 0u;
   p.idesc = make_idesc(1 /*f32*/, fmt, fmt, static_cast<uint32_t>(ka.mn), static_cast<uint32_t>(kb.mn), tile_m, c.BN);
   const int64_t total_tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles;
@@ -383,7 +389,7 @@ int gemm16_call(const cpuops_b200_gemm16_desc* d) {
   g_last_plan.grid = static_cast<int32_t>(grid);
   g_last_plan.c_ring = by_tma && use_c && c.form != kProductParts ? 1 : 0;
   g_last_plan.epilogue_warps = c.epi_warps;
-  CUDA_TRY(cudaLaunchKernelEx(&cfg, product_kernel_of(c.form, pieces), tmA, tmB, tmC, tmD, tmZ, p));
+  CUDA_TRY(cudaLaunchKernelEx(&cfg, product_kernel_of(c.form, pieces, by_tma), tmA, tmB, tmC, tmD, tmZ, p));
   g_launches.fetch_add(1);
   return call.finish();
 }

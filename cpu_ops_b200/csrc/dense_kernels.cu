@@ -10,10 +10,14 @@
 
 namespace b200 {
 
-ProductKernel product_kernel_of(int form, bool pieces) {
-  if (form == kProductPairs) return pieces ? product_kernel<kProductPairs, true> : product_kernel<kProductPairs, false>;
-  if (form == kProductParts) return pieces ? product_kernel<kProductParts, true> : product_kernel<kProductParts, false>;
-  return pieces ? product_kernel<kProductTiles, true> : product_kernel<kProductTiles, false>;
+template <int kForm>
+static ProductKernel product_kernel_for(bool pieces, bool tma) {
+  if (tma) return pieces ? product_kernel<kForm, true, true> : product_kernel<kForm, false, true>;
+  return pieces ? product_kernel<kForm, true, false> : product_kernel<kForm, false, false>;
+}
+ProductKernel product_kernel_of(int form, bool pieces, bool tma) {
+  if (form == kProductParts) return pieces ? product_kernel<kProductParts, true, true> : product_kernel<kProductParts, false, true>;
+  return form == kProductPairs ? product_kernel_for<kProductPairs>(pieces, tma) : product_kernel_for<kProductTiles>(pieces, tma);
 }
 ProductEmptyKernel product_empty() { return product_empty_kernel; }
 int product_threads(int form, int epi_warps) { return form == kProductParts ? 224 : 96 + 32 * epi_warps; }

@@ -8,7 +8,8 @@
 namespace b200 {
 
 using ProductKernel = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, ProductParams);
-ProductKernel product_kernel_of(int form, bool pieces);
+// tma: C, D and Z by TMA (kProductParts: either).
+ProductKernel product_kernel_of(int form, bool pieces, bool tma);
 using ProductEmptyKernel = void (*)(ProductParams);
 ProductEmptyKernel product_empty();
 int product_threads(int form, int epi_warps);

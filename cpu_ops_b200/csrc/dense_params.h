@@ -34,7 +34,6 @@ struct ProductParams {
   int32_t swapped;
   uint32_t idesc;
   int32_t epi_warps;
-  int32_t by_tma;                       // C, D and Z pass through shared memory by TMA (row-major forms)
   int32_t act;                          // kOp* or 0
   float alpha, beta;
   const float* bias;                    // by the caller's column, or null

@@ -264,10 +264,24 @@ __device__ __forceinline__ void load_c_rows(const ProductParams& p, int row0, in
     rows(static_cast<const __nv_bfloat16*>(p.C));
   }
 }
-// Rows r0 .. r0 + kRows of the chunk whose first row and column are row0 and col0.
+// An f32 C's chunk into shared memory, rows of 128 bytes, without registers in between; one group of copies.
+__device__ __forceinline__ void fetch_c_rows(const ProductParams& p, uint32_t buf, int row0, int col0, int lane) {
+  const int nrows = lane < p.Nk - col0 ? p.Mk - row0 : 0;
+  const float* src = static_cast<const float*>(p.C) + (static_cast<int64_t>(row0) * p.ldc + col0 + lane);
+#pragma unroll 8
+  for (int r = 0; r < 32; ++r, src += p.ldc) {
+    const bool valid = r < nrows;
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(buf + static_cast<uint32_t>(r * 128 + lane * 4)),
+                 "l"(valid ? src : static_cast<const float*>(p.C)), "r"(valid ? 4 : 0)
+                 : "memory");
+  }
+  cp_async_commit();
+}
+// Rows r0 .. r0 + kRows of the chunk whose first row and column are row0 and col0; C (add_c) from c, or from shared memory
+// (c_buf: fetch_c_rows').
 template <int kRows>
 __device__ __forceinline__ void write_chunk_rows(const ProductParams& p, uint32_t buf, void* dst, int64_t ld, bool add_c,
-                                                 const float (&c)[kRows], int r0, int row0, int col0, int lane) {
+                                                 const float (&c)[kRows], uint32_t c_buf, int r0, int row0, int col0, int lane) {
   const int nrows = lane < p.Nk - col0 ? p.Mk - row0 - r0 : 0;
   const int64_t at = static_cast<int64_t>(row0 + r0) * ld + col0 + lane;
   auto rows = [&](auto* base) {
@@ -286,7 +300,11 @@ __device__ __forceinline__ void write_chunk_rows(const ProductParams& p, uint32_
       }
 #pragma unroll
       for (int i = 0; i < kAtOnce; ++i, base += ld) {
-        if (add_c) v[i] = __fmaf_rn(p.beta, c[i0 + i], v[i]);
+        if (add_c) {
+          float x = c[i0 + i];
+          if (c_buf) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(c_buf + static_cast<uint32_t>((r0 + i0 + i) * 128 + lane * 4)));
+          v[i] = __fmaf_rn(p.beta, x, v[i]);
+        }
         if (i0 + i < nrows) *base = from_float<T>(v[i]);
       }
     }
@@ -428,7 +446,10 @@ __device__ __forceinline__ void finish_parts(const ProductParams& p, uint32_t ba
 // kPieces (D is f32): the accumulator is taken down every kProductPieceBlocks k-blocks and the pieces added in
 // f32 registers.  The tensor cores drop the low bits of a running sum: against float64 it is off by 1e-9 of the result per
 // element of k (2.1e-6 at k = 2048), by 5e-7 at any k in pieces of 512.  A 16-bit D does not show it.
-template <int kForm, bool kPieces>
+//
+// kTma: C, D and Z pass through shared memory by TMA.  Instances of their own, because next to the pieces' 128 sums either
+// path's registers are at the other's expense (680 bytes of spills with both, 200 with TMA alone).  (kProductParts: true.)
+template <int kForm, bool kPieces, bool kTma>
 __global__ void __launch_bounds__(kForm == kProductParts ? 224 : kProductThreads, 1)
     product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmD,
@@ -485,7 +506,7 @@ __global__ void __launch_bounds__(kForm == kProductParts ? 224 : kProductThreads
   if (warp == 0 && lane == 0) {
     prefetch_tensormap(&tmA);
     prefetch_tensormap(&tmB);
-    if (!kParts && p.by_tma) {
+    if (!kParts && kTma) {
       prefetch_tensormap(&tmD);
       if (p.C) prefetch_tensormap(&tmC);
       if (p.Z) prefetch_tensormap(&tmZ);
@@ -654,7 +675,9 @@ __global__ void __launch_bounds__(kForm == kProductParts ? 224 : kProductThreads
     const uint32_t ring = ring_base + static_cast<uint32_t>(ew * p.ring_bytes), depth = static_cast<uint32_t>(p.ring_depth);
     const uint32_t d_chunk = static_cast<uint32_t>(chunk_bytes(p.d_type)), c_chunk = p.C ? static_cast<uint32_t>(chunk_bytes(p.c_type)) : 0u;
     const uint32_t c_buf0 = ring, d_buf0 = ring + depth * c_chunk, z_buf0 = d_buf0 + depth * d_chunk;
-    const bool by_tma = p.by_tma != 0, has_c = p.C != nullptr, has_z = p.Z != nullptr;
+    constexpr bool by_tma = kTma;
+    const bool has_c = p.C != nullptr, has_z = p.Z != nullptr;
+    const bool c_copied = has_c && !by_tma && p.c_type == kF32;  // by cp.async, before the chunk's turn
     // (a TMA store writes whole 16-byte pieces: the last chunk of rows that end within one is stored lane by lane)
     const int whole_cols = p.Nk % (16 / type_bytes(p.d_type)) == 0 ? p.Nk : p.Nk / 32 * 32;
     asm volatile("griddepcontrol.wait;" ::: "memory");  // before C is read, D or Z written
@@ -682,7 +705,7 @@ __global__ void __launch_bounds__(kForm == kProductParts ? 224 : kProductThreads
       const int col0 = n0 + c * 32, ncols = min(32, p.Nk - col0);
       const bool inside = row0 < p.Mk && ncols > 0;
       product_z(p.alpha, p.bias ? my_bias + (c - c0) / cstep * 32 : nullptr, r);
-      if (by_tma) {
+      if constexpr (by_tma) {
         const bool ragged = col0 >= whole_cols, mine = inside && row0 + lane < p.Mk;
         if (!ragged || has_c) {
           // the stores that last read these buffers are done with them
@@ -724,25 +747,33 @@ __global__ void __launch_bounds__(kForm == kProductParts ? 224 : kProductThreads
         if (++d_b == depth) d_b = 0;
       } else if (inside) {
         // (the pieces' sums leave registers for a few rows of C at a time only)
-        constexpr int kRows = kPieces ? 4 : 32;
+        constexpr int kRows = kPieces ? 8 : 32;
         float cc[kRows];
-        if (!kPieces && has_c) load_c_rows(p, row0, col0, lane, cc);
+        if (!kPieces && has_c && !c_copied) load_c_rows(p, row0, col0, lane, cc);
         __syncwarp();  // every lane has read the chunk before
         if (has_z) {
           put_chunk_row(ring, lane, r, kF32);
           __syncwarp();
 #pragma unroll 1
-          for (int r0 = 0; r0 < 32; r0 += kRows) write_chunk_rows(p, ring, p.Z, p.ldz, false, cc, r0, row0, col0, lane);
+          for (int r0 = 0; r0 < 32; r0 += kRows) write_chunk_rows(p, ring, p.Z, p.ldz, false, cc, 0u, r0, row0, col0, lane);
           __syncwarp();
         }
         activate_chunk(r, p.act);
         put_chunk_row(ring, lane, r, kF32);
+        if (c_copied) cp_async_wait<0>();
         __syncwarp();
 #pragma unroll 1
         for (int r0 = 0; r0 < 32; r0 += kRows) {
-          if (kPieces && has_c) load_c_rows(p, row0 + r0, col0, lane, cc);
-          write_chunk_rows(p, ring, p.D, p.ldd, has_c, cc, r0, row0, col0, lane);
+          if (kPieces && has_c && !c_copied) load_c_rows(p, row0 + r0, col0, lane, cc);
+          write_chunk_rows(p, ring, p.D, p.ldd, has_c, cc, c_copied ? ring + 4096u : 0u, r0, row0, col0, lane);
         }
+      }
+      if (c_copied && c + cstep < nchunks) {
+        // the next chunk's C, as soon as this one's is used (a second buffer would cost stages of operands: 4096 x 4097 x 8192
+        // 296 us, 378 with it)
+        cp_async_wait<0>();
+        __syncwarp();
+        fetch_c_rows(p, ring + 4096u, row0, col0 + cstep * 32, lane);
       }
       return true;
     };
@@ -774,7 +805,13 @@ __global__ void __launch_bounds__(kForm == kProductParts ? 224 : kProductThreads
         // the tile's first chunks of C, before the accumulator is ready
         for (int c = c0; c < min(nchunks, c0 + static_cast<int>(depth) * cstep); c += cstep) request_c(n0 + c * 32, row0);
       }
-      if (has_c && !by_tma) {
+      if (c_copied) {
+        if (c0 < nchunks) {
+          cp_async_wait<0>();
+          __syncwarp();
+          fetch_c_rows(p, ring + 4096u, row0, n0 + c0 * 32, lane);
+        }
+      } else if (has_c && !by_tma) {
         for (int c = c0; c < nchunks; c += cstep) prefetch_c_rows(p, row0, n0 + c * 32, lane);
       }
       if (p.bias) {  // the tile's bias, likewise (as loads of a chunk their latency followed every accumulator)

@@ -214,6 +214,11 @@ def test_few_sms(gpu, lib):
             layer.backward()
             torch.cuda.synchronize()
             check(layer)
+            for m, n in ((3, 9000), (100, 300), (500, 900)):
+                a, w, out = matrix(m, 512, 0, "bf16", 1), matrix(n, 512, 0, "bf16", 2, 0.05), held(m, n, 0, "bf16")
+                layer.gemm(m, n, 512, a, w, out, lb=c.ColumnMajor)
+                assert _capi.last_plan().grid <= sms
+                assert H.worst(out[:m], H.product(d(a), d(w).t(), None, "none", None, 1.0, 0.0, "bf16")[0]) <= 1
     finally:
         lib.cpuops_b200_set_sm_limit(-1, 0)
 
