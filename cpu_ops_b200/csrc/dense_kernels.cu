@@ -44,6 +44,14 @@ NormChoice norm_choice_for(int n, bool wide, bool many, bool dr) {
       c.kernel = wide ? norm_grad_kernel<X, Y, true, true, 1> : norm_grad_kernel<X, Y, false, true, 1>;
       return c;
     }
+    if constexpr (sizeof(X) == 2) {
+      if (wide && many && n <= 1024) {  // (a row per warp: no barrier, and few rows of partial sums)
+        c.threads = 128;
+        c.rows_at_once = 4;
+        c.kernel = norm_grad_kernel<X, Y, true, true, 4>;
+        return c;
+      }
+    }
     const int row_bytes = n * static_cast<int>((dr ? 2 : 1) * sizeof(X) + sizeof(Y));
     if (wide && many && n % 8 == 0) {
       // sixteen elements per thread, so that few threads share in a row's two sums; two CTAs per SM and more, or one of
@@ -69,6 +77,14 @@ NormChoice norm_choice_for(int n, bool wide, bool many, bool dr) {
     c.kernel = two ? norm_grad_kernel<X, Y, true, false, 2> : norm_grad_kernel<X, Y, true, false, 1>;
   } else {
     constexpr int kSlots = sizeof(X) == 2 ? 2 : 1;
+    if (wide && many && n % 8 == 0 && n > 1024 && n <= 2048) {
+      c.threads = 32 * 2 * kNormWarps;
+      c.rows_at_once = 2 * kNormWarps;
+      c.ring = 1;
+      c.smem = 2 * n * static_cast<int>(sizeof(float)) + kSlots * 2 * kNormWarps * n * static_cast<int>(sizeof(X));
+      c.kernel = norm_ring_kernel<X, Y, 8, 2 * kNormWarps, kSlots>;
+      return c;
+    }
     if (wide && many && n % 8 == 0 && n > 1024 && n <= kNormWarpMost) {
       c.threads = 32 * kNormWarps;
       c.rows_at_once = kNormWarps;

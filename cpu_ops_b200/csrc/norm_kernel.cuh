@@ -246,6 +246,10 @@ __global__ void __launch_bounds__(kNormMaxThreads) norm_kernel(const NormParams 
   }
 }
 
+// Where element c of gamma (or beta) lies in a vector of n in shared memory whose eights are read by neighbouring lanes: the
+// fours of all eights' first halves, then those of the second, so that a warp reads whole lines without conflicts.
+__device__ __forceinline__ int weight_at(int c, int n) { return ((c >> 2) & 1) * (n >> 1) + (c >> 3) * 4 + (c & 3); }
+
 // One row per warp at a time, n <= 256 * kV: sums need no barrier, and each of the SM's warps has a whole row on its
 // way.  gamma and beta lie in shared memory (2 n floats).
 template <typename X, typename Y, bool kWide, int kV>
@@ -257,8 +261,9 @@ __global__ void __launch_bounds__(32 * kNormWarps, sizeof(X) == 2 || kV < 16 ? 2
   const int room = (p.n + 7) / 8 * 8;  // (whole vectors of eight)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   for (int c = threadIdx.x; c < room; c += 32 * kNormWarps) {
-    weights[c] = p.gamma != nullptr && c < p.n ? __ldg(p.gamma + c) : 1.0f;
-    weights[room + c] = p.beta != nullptr && c < p.n ? __ldg(p.beta + c) : 0.0f;
+    const int at = kWide ? weight_at(c, room) : c;
+    weights[at] = p.gamma != nullptr && c < p.n ? __ldg(p.gamma + c) : 1.0f;
+    weights[room + at] = p.beta != nullptr && c < p.n ? __ldg(p.beta + c) : 0.0f;
   }
   __syncthreads();
   const int64_t step = static_cast<int64_t>(gridDim.x) * kNormWarps;
@@ -299,11 +304,11 @@ __global__ void __launch_bounds__(32 * kNormWarps, sizeof(X) == 2 || kV < 16 ? 2
       if constexpr (kWide) {
         const int c = 8 * (lane + 32 * j);
         if (c < p.n) {
-          const float4* g = reinterpret_cast<const float4*>(weights + c);
-          const float4* b = reinterpret_cast<const float4*>(weights + room + c);
+          const float4* g = reinterpret_cast<const float4*>(weights + (c >> 1));
+          const float4* b = reinterpret_cast<const float4*>(weights + room + (c >> 1));
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float4 gg = g[h], bb = b[h];
+            const float4 gg = g[h * (room >> 3)], bb = b[h * (room >> 3)];
             r[4 * h] = __fmaf_rn((raw[j][4 * h] - mean) * rstd, gg.x, bb.x);
             r[4 * h + 1] = __fmaf_rn((raw[j][4 * h + 1] - mean) * rstd, gg.y, bb.y);
             r[4 * h + 2] = __fmaf_rn((raw[j][4 * h + 2] - mean) * rstd, gg.z, bb.z);
@@ -352,8 +357,8 @@ __global__ void __launch_bounds__(32 * kWarps, 1) norm_ring_kernel(const NormPar
 #pragma unroll
   for (int i = 0; i < kSlots; ++i) request(row + i * step, static_cast<uint32_t>(i));
   for (int c = threadIdx.x; c < n; c += 32 * kWarps) {
-    weights[c] = p.gamma != nullptr ? __ldg(p.gamma + c) : 1.0f;
-    weights[n + c] = p.beta != nullptr ? __ldg(p.beta + c) : 0.0f;
+    weights[weight_at(c, n)] = p.gamma != nullptr ? __ldg(p.gamma + c) : 1.0f;
+    weights[n + weight_at(c, n)] = p.beta != nullptr ? __ldg(p.beta + c) : 0.0f;
   }
   __syncthreads();
   const uint64_t budget_ns = static_cast<uint64_t>(p.wait_budget_us) * 1000ull;
@@ -418,12 +423,12 @@ __global__ void __launch_bounds__(32 * kWarps, 1) norm_ring_kernel(const NormPar
     for (int j = 0; j < kV; ++j) {
       const int c = 8 * (lane + 32 * j);
       if (c < n) {
-        const float4* g = reinterpret_cast<const float4*>(weights + c);
-        const float4* b = reinterpret_cast<const float4*>(weights + n + c);
+        const float4* g = reinterpret_cast<const float4*>(weights + (c >> 1));
+        const float4* b = reinterpret_cast<const float4*>(weights + n + (c >> 1));
         float r[8];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float4 gg = g[h], bb = b[h];
+          const float4 gg = g[h * (n >> 3)], bb = b[h * (n >> 3)];
           const float2 lo = fma2(mul2(add2(raw[j].pair(2 * h), both(-mean)), both(rstd)), make_float2(gg.x, gg.y), make_float2(bb.x, bb.y));
           const float2 hi = fma2(mul2(add2(raw[j].pair(2 * h + 1), both(-mean)), both(rstd)), make_float2(gg.z, gg.w), make_float2(bb.z, bb.w));
           r[4 * h] = lo.x;
@@ -675,12 +680,12 @@ __global__ void __launch_bounds__(kNormLongThreads) norm_long_kernel(const NormP
 
 // X: the type of x, dx and dr; Y: of dy.  The columns' sums of a CTA's rows go to its row of p.sums.  A row's elements
 // stay as they were loaded between its sums and its result, and the next row is on its way meanwhile.
-// kWarp: every warp takes rows of its own (n <= 256).
+// kWarp: every warp takes rows of its own (n <= 256 * kV).
 template <typename X, typename Y, bool kWide, bool kWarp, int kV>
 __global__ void __launch_bounds__(kWarp ? 128 : kNormMaxThreads) norm_grad_kernel(const NormParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ float2 slots[2][32];
-  __shared__ float join[kWarp ? 4 : 1][kWarp ? 256 : 1];
+  __shared__ float join[kWarp ? 4 : 1][kWarp ? 256 * kV : 1];
   const int threads = kWarp ? 32 : static_cast<int>(blockDim.x);
   const int t = kWarp ? threadIdx.x & 31 : threadIdx.x;
   const int first = kWarp ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
@@ -763,12 +768,14 @@ __global__ void __launch_bounds__(kWarp ? 128 : kNormMaxThreads) norm_grad_kerne
   float* out = p.sums + static_cast<int64_t>(blockIdx.x) * p.n;
   const int64_t other = static_cast<int64_t>(gridDim.x) * p.n;
   if constexpr (kWarp) {
-    // (columns 0 .. 255: the four warps' sums, added in turn)
+    // (the four warps' sums, added in turn)
     const int warp = threadIdx.x >> 5;
     for (int which = 0; which < 2; ++which) {
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < 8; ++i) join[warp][element_of<X, kWide>(t, 32, 0, i)] = which ? dbeta[0][i] : dgamma[0][i];
+      for (int j = 0; j < kV; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) join[warp][element_of<X, kWide>(t, 32, j, i)] = which ? dbeta[j][i] : dgamma[j][i];
       __syncthreads();
       for (int c = threadIdx.x; c < p.n; c += 128)
         out[c + which * other] = ((join[0][c] + join[1][c]) + join[2][c]) + join[3][c];
