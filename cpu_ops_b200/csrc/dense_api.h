@@ -143,7 +143,7 @@ int dense_kernels_ready(DeviceState& st) {
     for (int y : {kF32, kF16, kBf16})
       for (bool gradient : {false, true}) {
         if (x != y && x != kF32) continue;
-        for (int n : {2048, 4096, 8192}) {  // (those with shared memory)
+        for (int n : {1024, 2048, 4096, 8192}) {  // (those with shared memory)
           const NormChoice c = norm_choice(x, y, n, true, true, true, gradient);
           CUDA_TRY(cudaFuncSetAttribute(c.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kNormMostSmem));
         }

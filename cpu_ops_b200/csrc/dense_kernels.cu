@@ -77,12 +77,12 @@ NormChoice norm_choice_for(int n, bool wide, bool many, bool dr) {
     c.kernel = two ? norm_grad_kernel<X, Y, true, false, 2> : norm_grad_kernel<X, Y, true, false, 1>;
   } else {
     constexpr int kSlots = sizeof(X) == 2 ? 2 : 1;
-    if (wide && many && n % 8 == 0 && n > 1024 && n <= 2048) {
+    if (wide && many && n % 8 == 0 && n > 256 && n <= 2048) {
       c.threads = 32 * 2 * kNormWarps;
       c.rows_at_once = 2 * kNormWarps;
       c.ring = 1;
       c.smem = 2 * n * static_cast<int>(sizeof(float)) + kSlots * 2 * kNormWarps * n * static_cast<int>(sizeof(X));
-      c.kernel = norm_ring_kernel<X, Y, 8, 2 * kNormWarps, kSlots>;
+      c.kernel = n <= 1024 ? norm_ring_kernel<X, Y, 4, 2 * kNormWarps, kSlots> : norm_ring_kernel<X, Y, 8, 2 * kNormWarps, kSlots>;
       return c;
     }
     if (wide && many && n % 8 == 0 && n > 1024 && n <= kNormWarpMost) {
@@ -102,7 +102,7 @@ NormChoice norm_choice_for(int n, bool wide, bool many, bool dr) {
       c.threads = 32 * kNormWarps;
       c.rows_at_once = kNormWarps;
       c.smem = 2 * ((n + 7) / 8 * 8) * static_cast<int>(sizeof(float));
-      // (rows of whole vectors beyond 1024 took norm_ring_kernel)
+      // (beyond 256 columns rows of whole vectors took norm_ring_kernel)
       c.kernel = n <= 256    ? (wide ? norm_rows_kernel<X, Y, true, 1> : norm_rows_kernel<X, Y, false, 1>)
                  : n <= 1024 ? norm_rows_kernel<X, Y, true, 4>
                              : norm_rows_kernel<X, Y, true, 16>;
