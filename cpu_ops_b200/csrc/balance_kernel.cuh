@@ -7,8 +7,9 @@
 // which differ from one another as much as f_e do: an even load leaves nothing of the f_e themselves.
 //
 // A kernel counts, block by block; the other needs all counts (its CTAs add the blocks' up), takes a token
-// per warp, logits read once, and keeps sums of p in registers; its last CTA adds those up.  Bound by latencies: two launches, two hand-overs through L2, a token's three sums
-// across a warp.
+// per warp, logits read once, and keeps sums of p in registers; its last CTA adds those up.  Bound by latencies: two
+// launches, two hand-overs through L2, a token's three sums across a warp.  8192 tokens of 256 experts, f32: 16 us of a
+// replayed graph (17 MB, 2.6 us at HBM's rate); 1537 of 60, bf16: 8.5; 32 of 64 in one launch: 4.6.
 #pragma once
 
 #include "dense_params.h"

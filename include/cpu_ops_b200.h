@@ -230,8 +230,9 @@ CPUOPS_B200_API int cpuops_b200_stream_status(void* stream);
  * persistent, one CTA per SM, and hold their SMs until they end: a caller that wants a
  * communication kernel to run beside a GEMM (the all-gather of D on a second stream) leaves
  * it some SMs with this setting.  Results do not depend on it for int8; for MX it can change
- * the automatic split-k choice like any change of problem size does, and for low-rank adapters of
- * many rows the parts in which k is summed. */
+ * the automatic split-k choice like any change of problem size does, for low-rank adapters of
+ * many rows and 16-bit products the parts in which k is summed, and for sums over rows (dbias, dgamma, dbeta, the
+ * balance loss) the parts of rows. */
 CPUOPS_B200_API int cpuops_b200_set_sm_limit(int32_t device, int32_t sms);
 
 /* Budget of every bounded device-side wait (mbarrier waits of the GEMM kernels' roles), in
@@ -438,7 +439,9 @@ CPUOPS_B200_API int cpuops_b200_adapters(const cpuops_b200_adapters_desc* desc);
  * dW = dY^T X has A column-major and B row-major.  C, D and Z are row-major; C and D f32 or of A's type, Z of D's.
  * activation: 0 or CPUOPS_B200_OP_RELU, _GELU (tanh form), _SILU.  C is not read and may be NULL when beta == 0;
  * D may be C (same ld and type).  k == 0: the product is zero.
- * A sum is one running f32 sum of the tensor cores (up to eight parts of k, added in order, where there are few tiles).
+ * Sums are the tensor cores' running f32 sums (of up to eight parts of k, added in order, where there are few tiles); where D is
+ * f32 they are handed over to f32 additions every 512 elements of k (5e-7 of the result's norm at any k; a running sum is off
+ * by 1e-9 per element, which a 16-bit D does not show).
  * 16-byte aligned rows are read and written fastest.  Uses the stream's workspace where rows of A or B are not
  * 16-byte aligned (a copy of them).  m, n and k are at most 2^30. */
 typedef struct cpuops_b200_gemm16_desc {
