@@ -206,7 +206,8 @@ def test_slopes_of_far_values(gpu, name, limits):
 PAIRS = [("f32", "f32"), ("f32", "f16"), ("f32", "bf16"), ("f16", "f16"), ("bf16", "bf16")]
 ROWS = [(1, 1, 0), (3, 5, 0), (1000, 64, 0), (77, 256, 0), (50, 257, 3), (9, 1000, 0), (700, 515, 1), (130, 4096, 0), (5, 4100, 4),
         (400, 8192, 0), (3, 8193, 0), (6, 20000, 8), (700, 2048, 0), (1300, 1032, 8), (601, 4096, 8), (640, 3000, 1), (2, 2047, 2), (300, 300, 0),
-        (45, 5001, 0), (640, 264, 0), (600, 5000, 8), (593, 8192, 0), (900, 1000, 0), (2000, 520, 0), (700, 3064, 0)]
+        (45, 5001, 0), (640, 264, 0), (600, 5000, 8), (593, 8192, 0), (900, 1000, 0), (2000, 520, 0), (700, 3064, 0),
+        (650, 1501, 3), (620, 515, 5), (3, 5001, 7), (600, 5001, 7), (592, 250, 6)]
 
 
 @pytest.mark.parametrize("x_type,y_type", PAIRS)
