@@ -347,3 +347,47 @@ def test_balance_loss_outputs_are_optional(gpu):
     assert torch.equal(other, counts) and torch.equal(alone, loss)
     ok(op(op.Arguments(size, ref(logits), ids, ref_dLogits=ref(logits))))   # in place
     assert torch.equal(logits, d)
+
+
+def shifted(rows, cols, pad, kind, seed, by, sigma=1.0):
+    """A matrix that begins `by` elements behind an aligned address; -> the view and its TensorRef."""
+    flat = torch.full((rows * (cols + pad) + by + 8,), GUARD, dtype=H.TYPES[kind], device="cuda")
+    view = flat[by:by + rows * (cols + pad)].view(rows, cols + pad)
+    if seed is not None:
+        view[:, :cols] = matrix(rows, cols, 0, kind, seed, sigma)
+    return view, c.TensorRef(view, cols + pad)
+
+
+@pytest.mark.parametrize("m,n", [(40, 600), (650, 1200), (650, 200)])
+@pytest.mark.parametrize("pad", [0, 1])
+@pytest.mark.parametrize("offsets", [(1, 0, 1, 0), (0, 1, 0, 1), (3, 3, 2, 5)])
+def test_operands_that_begin_anywhere(gpu, m, n, pad, offsets):
+    """Every operand at its own distance from an aligned address: rows of different shifts in one call."""
+    (x, rx), (dy, rdy), (dr, rdr) = (shifted(m, n, pad, "bf16", i, by) for i, by in enumerate(offsets[:3]))
+    out, rout = shifted(m, n, pad, "bf16", None, offsets[3])
+    x64, dy64, dr64 = (v[:, :n].double().cpu() for v in (x, dy, dr))
+    gamma = matrix(1, n, 0, "f32", 7)[0]
+    mean, rstd = torch.zeros((m,), device="cuda"), torch.zeros((m,), device="cuda")
+    op = c.LayerNorm(c.bf16_t)
+    ok(op(op.Arguments(c.RowsCoord(m, n), rx, gamma, None, rout, mean, rstd, 1e-5)))
+    for got, want in zip((out[:, :n], mean, rstd), H.layer_norm(x64, gamma.double().cpu(), None, 1e-5, "bf16")):
+        assert H.worst(got, want) <= 1
+    dgamma, dbeta, dbias = (torch.zeros((n,), device="cuda") for _ in range(3))
+    op = c.LayerNormGrad(c.bf16_t)
+    ok(op(op.Arguments(c.RowsCoord(m, n), rdy, rx, gamma, mean, rstd, rout, dgamma, dbeta, rdr)))
+    want = H.layer_norm_grad(dy64, x64, gamma.double().cpu(), mean.double().cpu(), rstd.double().cpu(), dr64, "bf16")
+    for got, w in zip((out[:, :n], dgamma, dbeta), want):
+        assert H.worst(got, w) <= 1
+    op = c.BiasActivationGrad(c.bf16_t, c.Gelu())
+    ok(op(op.Arguments(c.RowsCoord(m, n), rdy, rx, rout, dbias)))
+    want, sums = H.epilogue_grad(dy64, x64, "gelu", "bf16")
+    assert H.worst(out[:, :n], want) <= 1 and H.worst(dbias, sums) <= 1
+    w, rw = shifted(n, 72, pad, "bf16", 9, offsets[1], n ** -0.5)
+    d, rd = shifted(m, 72, pad, "bf16", None, offsets[3])
+    r, rr = shifted(m, 72, pad, "bf16", 10, offsets[2])
+    op = c.GemmBF16(c.RowMajor, c.RowMajor)
+    ok(op(op.Arguments(c.GemmCoord(m, 72, n), rx, rw, rr, rd, c.BiasActivation(beta=1.0))))
+    want, _ = H.product(x64, w[:, :72].double().cpu(), None, "none", r[:, :72].double().cpu(), 1.0, 1.0, "bf16")
+    assert H.worst(d[:, :72], want) <= 1
+    for v, cols in ((out, n), (d, 72)):
+        assert pad == 0 or bool((v[:, cols:] == GUARD).all())
