@@ -12,6 +12,7 @@
 #pragma once
 
 #include "dense_params.h"
+#include "exchange.h"
 #include "gemm_params.h"
 #include "ptx_sm100.cuh"
 #include "ptx_sm100_pair.cuh"
@@ -396,6 +397,24 @@ __device__ __forceinline__ void finish_columns(const ProductParams& p, uint32_t 
   }
   store(p.D, p.ldd);
 }
+// leave_exchange's view of a cluster: a warp of one of its `parts` CTAs.
+struct PartsCluster {
+  volatile int* late;  // this CTA's word, which any CTA sets
+  uint32_t received;   // its barrier
+  int parts, lane;
+  __device__ __forceinline__ void tell_late() {
+    if (lane < parts)
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(map_to_cta(smem_u32(const_cast<int*>(late)), static_cast<uint32_t>(lane))), "r"(1)
+                   : "memory");
+  }
+  __device__ __forceinline__ void barrier() {
+    __syncwarp();
+    cluster_sync_all();
+  }
+  __device__ __forceinline__ bool any_late() { return *late != 0; }
+  __device__ __forceinline__ void wait_for_copies() { mbar_drain(received, 0); }
+};
+
 // By warp `warp` of `warps`, all of them on one CTA's columns.
 __device__ __forceinline__ void finish_parts(const ProductParams& p, uint32_t base, uint32_t slab, const float* bias, int warp, int warps,
                                              int lane, int tile, int part) {
@@ -484,17 +503,18 @@ __global__ void __launch_bounds__(kForm == kProductParts ? 224 : kProductThreads
   auto c_full_bar = [&](int w, int b) { return bar_base + 8u * (2 * kProductMaxStages + 5 + 2 * w + b); };
   constexpr int kRecvBar = 2 * kProductMaxStages + 5 + 2 * kProductEpiWarps, kBarriers = kRecvBar + 1;
   const uint32_t recv_bar = bar_base + 8u * kRecvBar;
-  static_assert(8 * kBarriers + 8 <= kProductBarrierBytes, "barriers, tensor memory slot, abort flag");
+  static_assert(8 * kBarriers + 12 <= kProductBarrierBytes, "barriers, tensor memory slot, abort and late flags");
   float* bias_smem = reinterpret_cast<float*>(smem + (bar_base - smem_base) + kProductBarrierBytes);  // a warp's chunks' bias
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (bar_base - smem_base) + 8 * kBarriers);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* late_flag = abort_flag + 1;  // kProductParts: some CTA's wait for the parts' sums ran out
 
   if (warp == 2) {
     for (int i = lane; i < kBarriers; i += 32) {
       const bool acc_empty = i == 2 * kProductMaxStages + 2 || i == 2 * kProductMaxStages + 3;
       mbar_init(bar_base + 8u * static_cast<uint32_t>(i), acc_empty ? static_cast<uint32_t>(n_epi) * kCtas : 1u);
     }
-    if (lane == 0) *abort_flag = 0;
+    if (lane == 0) *abort_flag = *late_flag = 0;
     fence_mbar_init_cluster();
     __syncwarp();
     if (kParts && lane == 0) mbar_expect_tx(recv_bar, static_cast<uint32_t>(p.BN * kTileM * 4));  // its columns' sums from all parts
@@ -953,20 +973,22 @@ __global__ void __launch_bounds__(kForm == kProductParts ? 224 : kProductThreads
     // This CTA's columns, by all warps: the parts' sums added in the order of k, and the epilogue.
     __syncthreads();  // (the bias is there)
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    int dummy = 0;
-    const bool got = mbar_wait_bounded(recv_bar, 0, &dummy, budget_ns);
-    if (!__all_sync(0xffffffffu, got)) {
+    const bool got = __all_sync(0xffffffffu, mbar_wait_bounded(recv_bar, 0, abort_flag, budget_ns));
+    if (!got) {
       if (lane == 0) product_error(p, abort_flag, kErrEpilogueWait);
     } else if (*abort_flag == 0) {
       finish_parts(p, ring_base, static_cast<uint32_t>(p.BN / p.parts * kTileM * 4), bias_smem, warp, 7, lane, work0, part);
     }
-  }
-  tc_fence_before_sync();
-  if constexpr (kForm != kProductTiles) {
+    tc_fence_before_sync();
+    PartsCluster cluster{late_flag, recv_bar, p.parts, lane};
+    leave_exchange(cluster, got);
+  } else if constexpr (kPair) {
+    tc_fence_before_sync();
     // no CTA may leave while another can still touch its shared memory, barriers or accumulator
     __syncwarp();
     cluster_sync_all();
   } else {
+    tc_fence_before_sync();
     __syncthreads();
   }
   if (warp == 1) tmem_dealloc_g<kPair>(tmem_base, kTmemCols512);

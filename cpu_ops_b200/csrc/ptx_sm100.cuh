@@ -102,6 +102,15 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity,
   return true;
 }
 
+// Waits for what was issued and so certainly comes: copies on their way, MMAs under way, before their memory is given up.
+// Its limit is its own: one that a caller may set (cpuops_b200_set_wait_budget_us, down to a microsecond) could end
+// the wait, and the CTA, before a copy has landed in its memory.
+constexpr uint64_t kDrainLimitNs = 1000000000ull;
+__device__ __forceinline__ bool mbar_drain(uint32_t bar, uint32_t parity) {
+  int never = 0;
+  return mbar_wait_bounded(bar, parity, &never, kDrainLimitNs);
+}
+
 // Leaves `code` in the call's error word unless one is there.  The word may be host memory
 // (no atomics over the bus: of two codes at the same moment either may stay).
 __device__ __forceinline__ void leave_error(int32_t* word, int32_t code) {
