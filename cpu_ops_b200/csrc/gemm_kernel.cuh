@@ -595,10 +595,9 @@ __global__ void __launch_bounds__(kGemmThreadsWide + (kRaw ? 32 * kScaleWriterWa
       }
       if (*abort_flag != 0 && el) {
         // Let copies that were already issued land before the CTA exits.
-        int dummy = 0;
         if (!kRaw)
           for (int st = 0; st < stages; ++st)
-            if (armed & (1u << st)) mbar_wait_bounded(full_bar(st), (armed_parity >> st) & 1u, &dummy, budget_ns);
+            if (armed & (1u << st)) mbar_drain(full_bar(st), (armed_parity >> st) & 1u);
         if constexpr (kRaw) {
           // (the full barriers also count the scale writers, which may have given up)
           const uint64_t t_end = global_timer_ns() + 200000;
@@ -754,8 +753,7 @@ __global__ void __launch_bounds__(kGemmThreadsWide + (kRaw ? 32 * kScaleWriterWa
       }
       // Nothing may still be executing when tensor memory is released.
       tc_commit_g<kPair>(drain_bar, el);
-      int dummy = 0;
-      if (!__all_sync(kAll, mbar_wait_bounded(drain_bar, 0, &dummy, budget_ns)) && el)
+      if (!__all_sync(kAll, mbar_drain(drain_bar, 0)) && el)
         record_error(p, abort_flag, kErrDrainWait);
       if (dbg && el) {
         B200_CLK(p)[2] = static_cast<unsigned long long>(clock64() - dbg_start);
@@ -992,9 +990,8 @@ __global__ void __launch_bounds__(kGemmThreadsWide + (kRaw ? 32 * kScaleWriterWa
       if (!kTmaOnly && ring && !c_tma) cp_async_wait<0>();
       if (c_tma && *abort_flag != 0 && lane == 0) {
         // let C chunks that were requested but never consumed land before the CTA exits
-        int dummy = 0;
         for (; cq < cissued; ++cq) {
-          mbar_wait_bounded(c_full_bar(ew, cq_b), cq_ph, &dummy, budget_ns);
+          mbar_drain(c_full_bar(ew, cq_b), cq_ph);
           if (++cq_b == nb) {
             cq_b = 0;
             cq_ph ^= 1u;

@@ -485,8 +485,7 @@ __global__ void __launch_bounds__(grouped_threads(kTwo), 1)
     }
     // nothing may still be executing when tensor memory is released
     tc_commit_g<false>(drain_bar, el);
-    int dummy = 0;
-    if (!__all_sync(kAll, mbar_wait_bounded(drain_bar, 0, &dummy, budget_ns)) && el) {
+    if (!__all_sync(kAll, mbar_drain(drain_bar, 0)) && el) {
       leave_error(p.error, kErrDrainWait);
       *abort_flag = 1;
     }

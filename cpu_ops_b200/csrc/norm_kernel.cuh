@@ -367,10 +367,14 @@ __global__ void __launch_bounds__(32 * kWarps, 1) norm_ring_kernel(const NormPar
     if (!__all_sync(0xffffffffu, mbar_wait_bounded(bar + 8u * slot, phase, &abort_flag, budget_ns))) {
       if (lane == 0) {
         leave_error(p.error, kErrProducerWait);
-        // copies that are on their way land before the CTA ends
-        int dummy = 0;
-        for (uint32_t i = 0; i < kSlots; ++i)
-          mbar_wait_bounded(bar + 8u * i, i < slot ? phase ^ 1u : phase, &dummy, budget_ns);
+        // copies that are on their way (this row's, and the next ones') land before the CTA ends
+        for (int64_t r = row; r < p.m && r < row + kSlots * step; r += step) {
+          mbar_drain(bar + 8u * slot, phase);
+          if (++slot == kSlots) {
+            slot = 0;
+            phase ^= 1u;
+          }
+        }
       }
       break;
     }
@@ -916,9 +920,14 @@ __global__ void __launch_bounds__(kMaxThreads, kMaxThreads == 256 && sizeof(X) =
   if (failed) {
     if (t == 0) {
       leave_error(p.error, kErrProducerWait);
-      int dummy = 0;  // copies that are on their way land before the CTA ends
-      for (uint32_t i = 0; i < static_cast<uint32_t>(p.ring); ++i)
-        mbar_wait_bounded(bar + 8u * i, i < slot ? phase ^ 1u : phase, &dummy, budget_ns);
+      // copies that are on their way (this row's, and the next ones') land before the CTA ends
+      for (int64_t r = row; r < p.m && r < row + p.ring * step; r += step) {
+        mbar_drain(bar + 8u * slot, phase);
+        if (++slot == static_cast<uint32_t>(p.ring)) {
+          slot = 0;
+          phase ^= 1u;
+        }
+      }
     }
     __syncthreads();
     return;

@@ -600,9 +600,8 @@ __global__ void __launch_bounds__(kForm == kProductParts ? 224 : kProductThreads
       }
       if (*abort_flag != 0 && el) {
         // copies that were already issued land before the CTA exits
-        int dummy = 0;
         for (int st = 0; st < stages; ++st)
-          if (armed & (1u << st)) mbar_wait_bounded(full_bar(st), (armed_parity >> st) & 1u, &dummy, budget_ns);
+          if (armed & (1u << st)) mbar_drain(full_bar(st), (armed_parity >> st) & 1u);
         if (kPair && !leader) {  // (the peer cannot watch the leader's barriers: time for its copies)
           const uint64_t t_end = global_timer_ns() + 100000;
           while (global_timer_ns() < t_end) __nanosleep(1000);
@@ -682,8 +681,7 @@ __global__ void __launch_bounds__(kForm == kProductParts ? 224 : kProductThreads
       }
       // nothing may still be executing when tensor memory is released
       tc_commit_g<kPair>(drain_bar, el);
-      int dummy = 0;
-      if (!__all_sync(kAll, mbar_wait_bounded(drain_bar, 0, &dummy, budget_ns)) && el)
+      if (!__all_sync(kAll, mbar_drain(drain_bar, 0)) && el)
         product_error(p, abort_flag, kErrDrainWait);
     }
     __syncwarp();
@@ -889,9 +887,8 @@ __global__ void __launch_bounds__(kForm == kProductParts ? 224 : kProductThreads
     if (!alive && lane == 0) product_error(p, abort_flag, kErrEpilogueWait);
     if (by_tma && lane == 0) {
       bulk_wait_group_all();  // D and Z are complete before the kernel ends
-      int dummy = 0;
       while (taken < asked) {  // (after a failed wait: chunks of C that are on their way)
-        mbar_wait_bounded(c_full_bar(ew, c_b), c_ph, &dummy, budget_ns);
+        mbar_drain(c_full_bar(ew, c_b), c_ph);
         next_c();
       }
     }
