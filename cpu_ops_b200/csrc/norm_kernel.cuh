@@ -808,13 +808,13 @@ __global__ void __launch_bounds__(kMaxThreads, kMaxThreads == 256 && sizeof(X) =
   extern __shared__ __align__(16) uint8_t rows[];
   __shared__ float2 slots[2][32];
   __shared__ __align__(8) uint64_t barriers[kNormMaxRing];
-  __shared__ int abort_flag, failed;
+  __shared__ int abort_flag, failed[2];  // (failed: by turns, so that no thread sets what another has still to read)
   const int t = threadIdx.x, threads = blockDim.x, n = p.n, lane = t & 31, warp = t >> 5, warps = threads >> 5;
   const float inverse = 1.0f / static_cast<float>(n);
   const uint32_t x_bytes = static_cast<uint32_t>(n) * sizeof(X), dy_bytes = static_cast<uint32_t>(n) * sizeof(Y);
   const uint32_t slot_bytes = (p.dr ? 2u : 1u) * x_bytes + dy_bytes, bar = smem_u32(barriers), ring0 = smem_u32(rows);
   if (t == 0) {
-    abort_flag = failed = 0;
+    abort_flag = failed[0] = failed[1] = 0;
     for (int i = 0; i < p.ring; ++i) mbar_init(bar + 8u * i, 1);
     fence_mbar_init();
   }
@@ -852,7 +852,7 @@ __global__ void __launch_bounds__(kMaxThreads, kMaxThreads == 256 && sizeof(X) =
       next_mean = __ldg(p.mean_in + row + step);
       next_rstd = __ldg(p.rstd_in + row + step);
     }
-    if (!mbar_wait_bounded(bar + 8u * slot, phase, &abort_flag, budget_ns)) failed = 1;
+    if (!mbar_wait_bounded(bar + 8u * slot, phase, &abort_flag, budget_ns)) failed[turn] = 1;
     const uint32_t from = ring0 + slot * slot_bytes;
     Eight<X> xs[kV], drs[kV];
     Eight<Y> dys[kV];
@@ -892,7 +892,7 @@ __global__ void __launch_bounds__(kMaxThreads, kMaxThreads == 256 && sizeof(X) =
     if (lane == 0) slots[turn][warp] = make_float2(s1, s2);
     fence_proxy_async_shared_cta();  // the slot has been read: before it is filled again
     __syncthreads();
-    if (failed) break;
+    if (failed[turn]) break;
     if (t == 0) request(row + p.ring * step, slot);
     if (++slot == static_cast<uint32_t>(p.ring)) {
       slot = 0;
@@ -917,7 +917,7 @@ __global__ void __launch_bounds__(kMaxThreads, kMaxThreads == 256 && sizeof(X) =
       store_eight<X, true>(dx, n, t, threads, j, r);
     }
   }
-  if (failed) {
+  if (row < p.m) {  // (a wait ran out)
     if (t == 0) {
       leave_error(p.error, kErrProducerWait);
       // copies that are on their way (this row's, and the next ones') land before the CTA ends
