@@ -628,6 +628,7 @@ __global__ void __launch_bounds__(kForm == kProductParts ? 224 : kProductThreads
       int s = 0, buf = 0;
       uint32_t ph = 0, acc_ph = 0, peek = 0;
       uint32_t a_lo = a_lo0, b_lo = b_lo0, full_addr = full0, empty_addr = empty0;
+      asm volatile("griddepcontrol.wait;" ::: "memory");  // (operands come no earlier: the kernel before is not charged to the wait)
       for (int t = work0; t < total_tiles && ok; t += work_step) {
         const ProductTile tc = product_tile(p, t, part);
         int i = 0;
