@@ -304,6 +304,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
     bool ok = true;
     int i = 0;
     [[maybe_unused]] int tile_left = kb1 - kb0;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // (operands come no earlier: the kernel before is not charged to the wait)
     while (i < n_units && ok) {
       const int piece_units = kPieces ? min(tile_left, p.piece_kb) : kb1 - kb0;  // ... or one tile
       if (!__all_sync(kAll, mbar_wait_bounded(acc_empty_bar(buf), acc_ph ^ 1u, abort_flag, budget_ns))) {

@@ -665,6 +665,7 @@ __global__ void __launch_bounds__(kGemmThreadsWide + (kRaw ? 32 * kScaleWriterWa
       int s = 0, buf = 0;
       uint32_t ph = 0, acc_ph = 0, peek = 0;
       uint32_t a_lo = a_lo0, b_lo = b_lo0, full_addr = full0, empty_addr = empty0, sf_lo = sf_lo0;
+      asm volatile("griddepcontrol.wait;" ::: "memory");  // (operands come no earlier: the kernel before is not charged to the wait)
       for (int t = work0; t < total_tiles && ok; t += work_step) {
         const TileCoord tc = decode_tile(p, t, work_step);
         if (p.narrow_last) set_idesc_width(tc.bn);

@@ -63,3 +63,30 @@ def test_a_16_bit_product(gpu, lib, m, n, k, slices, pair, d):
         op.held = (a, b)
         return op, desc, D, float(k)
     behind_a_long_call(lib, make)
+
+
+@pytest.mark.parametrize("m,n,k,pair", [(300, 256, 1024, False), (300, 256, 1024, True)])
+def test_an_int8_product(gpu, lib, m, n, k, pair):
+    def make(place):
+        a, b = torch.ones((m, k), dtype=torch.uint8, device="cuda"), torch.ones((k, n), dtype=torch.int8, device="cuda")
+        D = torch.zeros((m, n), dtype=torch.int32, device="cuda")
+        op = c.GemmU8S8S32(c.RowMajor, c.RowMajor, c.RowMajor, pair=pair, **place)
+        desc = op.describe(op.Arguments(c.GemmCoord(m, n, k), c.TensorRef(a, k), c.TensorRef(b, n), c.TensorRef(D, n), c.TensorRef(D, n),
+                                        c.LinearCombination(1, 0)))
+        op.held = (a, b)
+        return op, desc, D, k
+    behind_a_long_call(lib, make)
+
+
+@pytest.mark.parametrize("m,n,k,pair", [(300, 256, 1024, False), (300, 256, 1024, True), (8, 512, 2048, None)])
+def test_an_mx_product(gpu, lib, m, n, k, pair):
+    def make(place):
+        a, b = (torch.full(s, 0x38, dtype=torch.uint8, device="cuda") for s in ((m, k), (n, k)))   # e4m3's 1
+        sa, sb = (torch.full((rows, k // 32), 127, dtype=torch.uint8, device="cuda") for rows in (m, n))
+        D = torch.zeros((m, n), device="cuda")
+        op = c.GemmMxE4M3(c.RowMajor, pair=pair, **place)
+        desc = op.describe(op.Arguments(c.GemmCoord(m, n, k), c.MxTensorRef(a, sa, k, k // 32), c.MxTensorRef(b, sb, k, k // 32),
+                                        c.TensorRef(D, n), c.TensorRef(D, n), c.LinearCombination(1.0, 0.0)))
+        op.held = (a, b, sa, sb)
+        return op, desc, D, float(k)
+    behind_a_long_call(lib, make)
