@@ -78,12 +78,12 @@ int product_clusters(DeviceState& st, int form, int size) {
 struct ProductChoice {
   int form = kProductTiles, BN = 128, parts = 1, stages = 0, epi_warps = kProductEpiWarps, ring_bytes = 0, ring_depth = 1;
   int tile_rows = 128;
-  bool swapped = false;
+  bool swapped = false, pieces = false;
 };
 
 // Shared memory of a choice: stages, epilogue warps and their buffers.  `chunks`: bytes of one chunk each of C, D and
 // Z (0: not by TMA); `rows`: an epilogue warp's otherwise.  False: it does not fit.
-bool fit_product(ProductChoice& c, int smem_optin, int chunks, int rows, int k_blocks, bool pieces) {
+bool fit_product(ProductChoice& c, int smem_optin, int chunks, int rows, int k_blocks) {
   const int room = smem_optin - 1024 - kProductBarrierBytes - 4 * kProductBiasFloats;
   const int stage = (kTileM + c.BN / (c.form == kProductPairs ? 2 : 1)) * 128;
   if (c.form == kProductParts) {
@@ -94,7 +94,7 @@ bool fit_product(ProductChoice& c, int smem_optin, int chunks, int rows, int k_b
     // Eight epilogue warps with two buffers for each matrix, unless that leaves the ring of stages short: then one
     // buffer, or four warps (which do not have the registers for the pieces' sums).
     for (int attempt = 0; attempt < 3; ++attempt) {
-      c.epi_warps = attempt < 2 || pieces ? 8 : 4;
+      c.epi_warps = attempt < 2 || c.pieces ? 8 : 4;
       c.ring_depth = attempt == 0 ? 2 : 1;
       c.ring_bytes = chunks ? c.ring_depth * chunks : rows;
       c.stages = (room - c.epi_warps * c.ring_bytes) / stage;
@@ -111,7 +111,7 @@ bool fit_product(ProductChoice& c, int smem_optin, int chunks, int rows, int k_b
 //   256 x 4096 x 4096: tiles of 64 16.6 / 16.3, pairs of 128 20.7 / 18.1, two parts of 128 19.1 / 20.4
 //   4096 x 4096 x 4096: pairs of 256 100 / 94, of 192 102 / 95, of 128 106 / 100, tiles of 128 125 / 115
 // chunk_us: an epilogue warp's time for 32 x 32 elements; hbm_us: the bytes that the call cannot do without.
-double product_us(const ProductChoice& c, const DeviceState& st, int Mk, int Nk, int k_blocks, bool pieces, double chunk_us, double hbm_us) {
+double product_us(const ProductChoice& c, const DeviceState& st, int Mk, int Nk, int k_blocks, int piece_blocks, double chunk_us, double hbm_us) {
   const bool pair = c.form == kProductPairs;
   const int tile_m = pair ? 256 : c.tile_rows;
   const int64_t tiles = static_cast<int64_t>((Mk + tile_m - 1) / tile_m) * ((Nk + c.BN - 1) / c.BN);
@@ -119,7 +119,7 @@ double product_us(const ProductChoice& c, const DeviceState& st, int Mk, int Nk,
   const double rounds = static_cast<double>((tiles + slots - 1) / slots);
   double block = pair ? (c.BN == 128 ? 0.215 : c.BN == 192 ? 0.285 : 0.345)
                       : (c.BN <= 16 ? 0.13 : c.BN == 32 ? 0.145 : c.BN == 64 ? 0.185 : c.BN == 128 ? 0.26 : 0.45);
-  if (pieces) block += 0.05;
+  if (c.pieces) block += 0.4 / piece_blocks;
   const double kb = static_cast<double>((k_blocks + c.parts - 1) / c.parts);
   // (a short loop does not reach the memory's rate from its first load on)
   auto together = [&](double us) { return std::max(hbm_us, us) + 0.25 * std::min(hbm_us, us); };
@@ -229,7 +229,13 @@ int gemm16_call(const cpuops_b200_gemm16_desc* d) {
   const bool by_tma = tma_rows(d->d, d->ldd, d->d_type) && (!use_c || tma_rows(d->c, d->ldc, d->c_type)) &&
                       (!d->z || tma_rows(d->z, d->ldz, d->d_type));
   const int chunks = by_tma ? chunk_bytes(d->d_type) * (d->z ? 2 : 1) + (use_c ? chunk_bytes(d->c_type) : 0) : 0;
-  const bool pieces = d->d_type == kF32 && k_blocks > kProductPieceBlocks;
+  // Pieces of k: an f32 D shows what the tensor cores drop of a running sum from k = 512 on; a 16-bit one where it comes
+  // near half of the rounding's half step (product_kernel.cuh), which sums of 16384 (f16) or 131072 elements (bf16) stay
+  // below.  Their pieces are longer, so that they cost little: 256 x 256 x 65536 f16 by tiles of 128 in one running sum 205 us
+  // (4.3e-4 of the result dropped), in pieces of 8192 215 (4.9e-5), an f32 D's of 512 240.
+  const bool f32_d = d->d_type == kF32;
+  const int piece_blocks = f32_d ? kProductPieceBlocks : kProductPieceBlocks16;
+  const int running = d->type == kF16 ? kProductRunningBlocksF16 : kProductRunningBlocksBf16;
 
   // The choice of form and tile.
   const double c_size = use_c ? type_bytes(d->c_type) : 0, d_size = type_bytes(d->d_type) * (d->z ? 2 : 1);
@@ -244,6 +250,7 @@ int gemm16_call(const cpuops_b200_gemm16_desc* d) {
     c.BN = BN;
     c.parts = parts;
     c.swapped = swapped;
+    c.pieces = f32_d ? k_blocks > piece_blocks : (k_blocks + parts - 1) / parts > running;
     const int b_mn = swapped ? a.mn : b.mn, rows = BN / (form == kProductPairs ? 2 : 1);
     if (b_mn && rows % 64 != 0) return;  // (boxes of 64)
     if (parts > k_blocks) return;
@@ -252,7 +259,7 @@ int gemm16_call(const cpuops_b200_gemm16_desc* d) {
     if ((d->flags & CPUOPS_B200_FLAG_PAIR_ON) && form != kProductPairs) return;
     if ((d->flags & CPUOPS_B200_FLAG_PAIR_OFF) && form == kProductPairs) return;
     if (form != kProductTiles && product_clusters(st, form, form == kProductPairs ? 2 : parts) < 1) return;
-    if (!fit_product(c, st.smem_optin, chunks, use_c && d->c_type == kF32 ? 2 * 4096 : 4096, k_blocks, pieces)) return;
+    if (!fit_product(c, st.smem_optin, chunks, use_c && d->c_type == kF32 ? 2 * 4096 : 4096, k_blocks)) return;
     const int Mk = swapped ? d->n : d->m, Nk = swapped ? d->m : d->n;
     if (form == kProductParts && !(swapped ? b.mn : a.mn)) {
       // Tiles of fewer rows where that gives every cluster one (a tile's other rows are neither loaded nor used):
@@ -266,7 +273,7 @@ int gemm16_call(const cpuops_b200_gemm16_desc* d) {
     if (form == kProductParts && st.sms() < st.sm_count &&
         static_cast<int64_t>((Mk + c.tile_rows - 1) / c.tile_rows) * ((Nk + BN - 1) / BN) * parts > st.sms())
       return;
-    const double us = product_us(c, st, Mk, Nk, k_blocks, pieces, chunk_us, hbm_us);
+    const double us = product_us(c, st, Mk, Nk, k_blocks, piece_blocks, chunk_us, hbm_us);
     if (!found || us < least) {
       best = c;
       least = us;
@@ -332,6 +339,7 @@ int gemm16_call(const cpuops_b200_gemm16_desc* d) {
   p.stages = c.stages;
   p.nacc = 2;
   p.parts = c.parts;
+  p.piece_blocks = piece_blocks;
   p.a_mn = ka.mn;
   p.b_mn = kb.mn;
   p.epi_warps = c.epi_warps;
@@ -389,7 +397,7 @@ int gemm16_call(const cpuops_b200_gemm16_desc* d) {
   g_last_plan.grid = static_cast<int32_t>(grid);
   g_last_plan.c_ring = by_tma && use_c && c.form != kProductParts ? 1 : 0;
   g_last_plan.epilogue_warps = c.epi_warps;
-  CUDA_TRY(cudaLaunchKernelEx(&cfg, product_kernel_of(c.form, pieces, by_tma), tmA, tmB, tmC, tmD, tmZ, p));
+  CUDA_TRY(cudaLaunchKernelEx(&cfg, product_kernel_of(c.form, c.pieces, by_tma), tmA, tmB, tmC, tmD, tmZ, p));
   g_launches.fetch_add(1);
   return call.finish();
 }

@@ -21,7 +21,9 @@ constexpr int kProductMaxStages = 12;
 constexpr int kProductMaxParts = 8;
 constexpr int kProductBarrierBytes = 512;
 constexpr int kProductBiasFloats = 1024;  // 128 for each of eight epilogue warps, 256 for each of four; behind the barriers
-constexpr int kProductPieceBlocks = 8;   // k-blocks of a piece of k (kPieces)
+// kPieces: k-blocks of a piece of k where D is f32; where D has 16 bits, and the longest running sum of such a D, by type.
+constexpr int kProductPieceBlocks = 8, kProductPieceBlocks16 = 128;
+constexpr int kProductRunningBlocksF16 = 256, kProductRunningBlocksBf16 = 2048;
 
 struct ProductParams {
   // Kernel view: Dk (Mk x Nk) = Ak Bk, Ak on the MMA's M side.  `swapped`: the caller's B is Ak, so that
@@ -29,6 +31,7 @@ struct ProductParams {
   int32_t Mk, Nk, K;
   int32_t m_tiles, n_tiles, k_blocks;   // tiles of 128 (pairs: 256) x BN; k-blocks of 64
   int32_t BN, stages, nacc, raster_m, parts;
+  int32_t piece_blocks;                 // kPieces: k-blocks of a piece of k
   int32_t tile_rows;                    // kProductParts: rows of Ak per tile, at most 128 (others: 128)
   int32_t a_mn, b_mn;                   // 1: the m (n) direction is contiguous in memory
   int32_t swapped;

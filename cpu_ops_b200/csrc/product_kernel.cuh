@@ -462,9 +462,13 @@ __device__ __forceinline__ void finish_parts(const ProductParams& p, uint32_t ba
 // them in the order of k.  No workspace, no second launch, and the same result on every run.  (Stored element by element
 // into the owner's memory, a warp's store took some 65 cycles: 256 x 4096 x 4096 in two parts 35 us.)
 //
-// kPieces (D is f32): the accumulator is taken down every kProductPieceBlocks k-blocks and the pieces added in
-// f32 registers.  The tensor cores drop the low bits of a running sum: against float64 it is off by 1e-9 of the result per
-// element of k (2.1e-6 at k = 2048), by 5e-7 at any k in pieces of 512.  A 16-bit D does not show it.
+// kPieces: the accumulator is taken down every p.piece_blocks k-blocks and the pieces added in f32 registers.  The tensor cores
+// drop the low bits of a running sum, towards zero.  Against float64, with operands of both signs, it is off by 1e-9 of the
+// result's norm per element of k (2.1e-6 at k = 2048); where all products have one sign by 6.5e-9 of the result (5.4e-5 at 8192,
+// 4.3e-4 at 65536: what an instruction drops, of 16 elements, goes with the sum so far, at most 2^-22 of it).  An f32 D is
+// summed in pieces of 512: 7e-7 of the norm up to k = 65536 and 1.0e-6 at 2^20, 2.8e-6 of one sign.  A 16-bit D's running sums end
+// where the loss reaches half of the least half step of its rounding (2^-12 of the value for f16, 2^-9 for bf16): after 16384
+// elements, 131072 of bf16; longer ones are summed in pieces of 8192, which drop 6e-5 at most.
 //
 // kTma: C, D and Z pass through shared memory by TMA.  Instances of their own, because next to the pieces' 128 sums either
 // path's registers are at the other's expense (680 bytes of spills with both, 200 with TMA alone).  (kProductParts: true.)
@@ -641,7 +645,7 @@ __global__ void __launch_bounds__(kForm == kProductParts ? 224 : kProductThreads
           tc_fence_after_sync();
           const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(buf * p.BN);
           uint32_t accumulate = 0;
-          const int piece_end = kPieces ? min(i + kProductPieceBlocks, tc.nkb) : tc.nkb;
+          const int piece_end = kPieces ? min(i + p.piece_blocks, tc.nkb) : tc.nkb;
           for (; i < piece_end; ++i) {
             if (!peek && !__all_sync(kAll, mbar_wait_bounded(full_addr, ph, abort_flag, budget_ns))) {
               if (el) product_error(p, abort_flag, kErrMmaWaitFull);
@@ -846,7 +850,7 @@ __global__ void __launch_bounds__(kForm == kProductParts ? 224 : kProductThreads
       if constexpr (kPieces) {
         constexpr int kMine = 4;  // chunks of a warp, of eight warps' 256 columns
         uint32_t sum[kMine][32];
-        for (int i = 0; i < tc.nkb && alive; i += kProductPieceBlocks) {
+        for (int i = 0; i < tc.nkb && alive; i += p.piece_blocks) {
           if (!accumulator(taddr, buf)) {
             alive = false;
             break;
@@ -915,7 +919,7 @@ __global__ void __launch_bounds__(kForm == kProductParts ? 224 : kProductThreads
     [[maybe_unused]] uint32_t sum[kGroups][16];
     const int nkb = product_tile(p, work0, part).nkb;
     bool alive = true;
-    for (int i = 0, it = 0; i < nkb && alive; i += kPieces ? kProductPieceBlocks : nkb, ++it) {
+    for (int i = 0, it = 0; i < nkb && alive; i += kPieces ? p.piece_blocks : nkb, ++it) {
       const int buf = it % nacc;
       const bool ready = mbar_wait_bounded(acc_full_bar(buf), static_cast<uint32_t>(it / nacc) & 1u, abort_flag, budget_ns);
       if (!__all_sync(0xffffffffu, ready)) {
