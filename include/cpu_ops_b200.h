@@ -429,7 +429,10 @@ CPUOPS_B200_API int cpuops_b200_adapters(const cpuops_b200_adapters_desc* desc);
  * device memory only, and `stream`, `flags`, `device`, `memory_space`, locking, stream capture and the
  * stream's workspace mean the same (comments say which calls use the workspace).  Matrices are rows of
  * contiguous elements, ld elements apart; types are CPUOPS_B200_TYPE_*.  Sums are f32 throughout and
- * every stored 16-bit value is rounded once.  Results are bit-identical from run to run, for one setting of
+ * every stored 16-bit value is rounded once.  Exponentials are exp2 instructions on f32: GELU and SiLU here are within 3e-7 of
+ * |z| (in the quantised products' chain they are near their last bit; of z = -inf both give NaN here and there), their slopes
+ * within 8e-7 of |dY|, and the balance loss's scores, before they are normalised, within 3e-7 + 8e-8 times the logit's distance
+ * from its token's largest (sigmoid: |logit|) of themselves.  Results are bit-identical from run to run, for one setting of
  * cpuops_b200_set_sm_limit (on which the parts that are summed depend).  Outputs must not overlap inputs or
  * one another, except where a comment allows it. */
 
@@ -472,7 +475,7 @@ typedef struct cpuops_b200_gemm16_desc {
 CPUOPS_B200_API int cpuops_b200_gemm16(const cpuops_b200_gemm16_desc* desc);
 
 /* The gradient of that epilogue: dZ = dY * act'(Z), dbias[j] = the sum over i of dZ[i][j] before its rounding.
- * dY, Z and dZ are m x n of one type.  (dC of the residual is beta * dY itself; the products' gradients are
+ * dY, Z and dZ are m x n of one type: of an f32 residual stream's gradient the caller makes a 16-bit copy.  (dC of the residual is beta * dY itself; the products' gradients are
  * calls of cpuops_b200_gemm16 on dZ.)  Without an activation Z is not read, and dZ may be NULL.  relu'(z) is 0
  * for z <= 0; where z is infinite gelu' and silu' are their limits, 0 and 1.
  * dZ may be dY or Z.  dbias may be NULL.  Uses the stream's workspace for dbias. */
@@ -550,6 +553,8 @@ CPUOPS_B200_API int cpuops_b200_layer_norm_grad(const cpuops_b200_layer_norm_gra
  * and dlogits = upstream * d loss / d logits, of the logits' type (counts have no gradient).  Tokens without an id
  * (padding, ids of -1) count nowhere and have a gradient of zero; without any such token the loss is 0.
  * An expert whose logit is NaN or -inf is out of its token's sum; +inf counts as the largest number.
+ * dlogits of an even load are about coefficient / (tokens * experts): f16, whose numbers end at 6e-8, needs a loss scale in
+ * upstream (or f32 logits).
  * upstream: the loss's own gradient, one float on the device (NULL: 1).  counts, loss and dlogits may each be NULL;
  * dlogits may be logits (same ld).  Uses the stream's workspace beyond 32 tokens. */
 typedef struct cpuops_b200_balance_loss_desc {
