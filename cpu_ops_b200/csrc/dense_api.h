@@ -14,6 +14,9 @@ constexpr int kDenseMost = 1 << 30;  // of m, n, k: sums of an extent and a tile
 bool activation_ok(int act) {
   return act == 0 || act == CPUOPS_B200_OP_RELU || act == CPUOPS_B200_OP_GELU || act == CPUOPS_B200_OP_SILU;
 }
+int kernel_activation(int act) {
+  return act == CPUOPS_B200_OP_RELU ? kOpRelu : act == CPUOPS_B200_OP_GELU ? kOpGelu : act == CPUOPS_B200_OP_SILU ? kOpSilu : 0;
+}
 bool rows_aligned(const void* base, int64_t ld, int type) {
   return ((reinterpret_cast<uintptr_t>(base) | static_cast<uint64_t>(ld * type_bytes(type))) & 15u) == 0;
 }
@@ -189,9 +192,7 @@ int gemm16_call(const cpuops_b200_gemm16_desc* d) {
 
   ProductParams p;
   memset(&p, 0, sizeof(p));
-  p.K = d->k;
-  p.act = d->activation == CPUOPS_B200_OP_RELU ? kOpRelu : d->activation == CPUOPS_B200_OP_GELU ? kOpGelu
-        : d->activation == CPUOPS_B200_OP_SILU ? kOpSilu : 0;
+  p.act = kernel_activation(d->activation);
   p.alpha = d->alpha;
   p.beta = d->beta;
   p.bias = d->bias;
@@ -444,9 +445,6 @@ int epilogue_grad_call(const cpuops_b200_epilogue_grad_desc* d) {
   p.lddz = d->lddz;
   p.m = d->m;
   p.n = d->n;
-  p.type = d->type;
-  p.act = d->activation == CPUOPS_B200_OP_RELU ? kOpRelu : d->activation == CPUOPS_B200_OP_GELU ? kOpGelu
-        : d->activation == CPUOPS_B200_OP_SILU ? kOpSilu : 0;
   const bool wide = rows_aligned(d->dy, d->lddy, d->type) && (!act || rows_aligned(d->z, d->ldz, d->type)) &&
                     (!d->dz || rows_aligned(d->dz, d->lddz, d->type));
   // 16-bit rows on odd elements: every second one begins in the middle of a word, and a block takes those or the others.
@@ -465,7 +463,7 @@ int epilogue_grad_call(const cpuops_b200_epilogue_grad_desc* d) {
     parts = reinterpret_cast<float*>(ws);
   }
   p.sums = d->dbias ? (parts ? parts : d->dbias) : nullptr;
-  if (int rc = launch_after(epilogue_grad_of(d->type, p.act, wide), dim3(static_cast<unsigned>(strips), static_cast<unsigned>(blocks)), 256, 0,
+  if (int rc = launch_after(epilogue_grad_of(d->type, kernel_activation(d->activation), wide), dim3(static_cast<unsigned>(strips), static_cast<unsigned>(blocks)), 256, 0,
                             call.stream, p))
     return rc;
   if (parts)
@@ -640,7 +638,6 @@ int balance_loss_call(const cpuops_b200_balance_loss_desc* d) {
   p.upstream = d->upstream;
   p.ld = d->ld_logits;
   p.ldg = d->ld_dlogits;
-  p.type = d->logits_type;
   p.tokens = d->tokens;
   p.experts = d->experts;
   p.top_k = d->top_k;

@@ -111,7 +111,7 @@ NormChoice norm_choice_for(int n, bool wide, bool many, bool dr) {
     const bool two = n > 8 * kNormMaxThreads;
     const int per = two ? 16 : 8;
     c.threads = ((n + per - 1) / per + 31) / 32 * 32;
-    c.kernel = two ? norm_kernel<X, Y, true, 2> : norm_kernel<X, Y, true, 1>;
+    c.kernel = two ? norm_kernel<X, Y, 2> : norm_kernel<X, Y, 1>;
   }
   return c;
 }

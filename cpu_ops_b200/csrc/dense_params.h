@@ -28,7 +28,7 @@ constexpr int kProductRunningBlocksF16 = 256, kProductRunningBlocksBf16 = 2048;
 struct ProductParams {
   // Kernel view: Dk (Mk x Nk) = Ak Bk, Ak on the MMA's M side.  `swapped`: the caller's B is Ak, so that
   // kernel rows are the caller's columns.
-  int32_t Mk, Nk, K;
+  int32_t Mk, Nk;
   int32_t m_tiles, n_tiles, k_blocks;   // tiles of 128 (pairs: 256) x BN; k-blocks of 64
   int32_t BN, stages, nacc, raster_m, parts;
   int32_t piece_blocks;                 // kPieces: k-blocks of a piece of k
@@ -61,7 +61,7 @@ struct EpilogueGradParams {
   void* dz;           // may be null without an activation
   float* sums;        // one row of n per block of rows, or the result itself where there is one block; or null
   int64_t lddy, ldz, lddz;
-  int32_t m, n, act, type;
+  int32_t m, n;
   int32_t block_rows;
   int32_t every;      // rows that are not 16-byte aligned: a block takes every row, or every second one
 };
@@ -109,7 +109,7 @@ struct BalanceParams {
   float* part_scores;      // per main block: experts sums of scores
   int32_t* ticket;
   int64_t ld, ldg;
-  int32_t type, tokens, experts, top_k, sigmoid;
+  int32_t tokens, experts, top_k, sigmoid;
   int32_t count_blocks;
   float coefficient;
 };

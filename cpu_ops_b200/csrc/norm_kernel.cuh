@@ -11,13 +11,9 @@
 #pragma once
 
 #include "dense_params.h"
+#include "dense_types.cuh"
 #include "gemm_params.h"
 #include "ptx_sm100.cuh"
-
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
-#include <type_traits>
 
 namespace b200 {
 
@@ -28,20 +24,6 @@ constexpr int kNormWarps = 8;                       // rows that a CTA of norm_r
 constexpr int kNormMaxRing = 4;                     // rows on their way of norm_grad_ring_kernel
 constexpr int kNormLongThreads = 1024;
 constexpr int kNormStrip = 256;      // columns of a CTA of the column kernels
-
-__device__ __forceinline__ float to_f32(float v) { return v; }
-__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T>
-__device__ __forceinline__ T from_f32(float v) {  // (rounded to nearest even)
-  if constexpr (sizeof(T) == 4) {
-    return v;
-  } else if constexpr (std::is_same<T, __half>::value) {
-    return __float2half_rn(v);
-  } else {
-    return __float2bfloat16_rn(v);
-  }
-}
 
 // Eight elements of a row in flight.  kWide: rows are 16-byte aligned; thread t of T holds the elements
 // 8 (t + T j) .. + 7; otherwise t + T i.  `left`: elements of the row from `p` on.
@@ -85,7 +67,7 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
-template <typename T, bool kWide>
+template <bool kWide>
 __device__ __forceinline__ int element_of(int t, int threads, int j, int i) {
   return kWide ? 8 * (t + threads * j) + i : t + threads * (8 * j + i);
 }
@@ -111,7 +93,7 @@ __device__ __forceinline__ Eight<T> load_eight(const T* row, int n, int t, int t
   const Word* words = reinterpret_cast<const Word*>(row);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int c = element_of<T, kWide>(t, threads, j, i);
+    const int c = element_of<kWide>(t, threads, j, i);
     const uint32_t v = c < n ? static_cast<uint32_t>(words[c]) : 0u;
     if constexpr (sizeof(T) == 4) {
       e.w[i] = v;
@@ -147,7 +129,7 @@ __device__ __forceinline__ void store_eight(T* row, int n, int t, int threads, i
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int c = element_of<T, kWide>(t, threads, j, i);
+    const int c = element_of<kWide>(t, threads, j, i);
     if (c < n) row[c] = from_f32<T>(v[i]);
   }
 }
@@ -156,7 +138,7 @@ template <bool kWide>
 __device__ __forceinline__ void load_vector(const float* vec, int n, int t, int threads, int j, float otherwise, float (&v)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int c = element_of<float, kWide>(t, threads, j, i);
+    const int c = element_of<kWide>(t, threads, j, i);
     v[i] = vec != nullptr && c < n ? __ldg(vec + c) : otherwise;
   }
 }
@@ -177,7 +159,7 @@ __device__ __forceinline__ float block_sum(float v, float* slot) {
 }
 
 // Subtracts the mean from eight elements (those beyond the row stay zero) and adds their squares up.
-template <typename X, bool kWide>
+template <bool kWide>
 __device__ __forceinline__ float centred_squares(float (&v)[8], float mean, int n, int t, int threads, int j, float square) {
   if (kWide && 8 * (t + threads * j) + 8 <= n) {
 #pragma unroll
@@ -188,15 +170,15 @@ __device__ __forceinline__ float centred_squares(float (&v)[8], float mean, int 
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      v[i] = element_of<X, kWide>(t, threads, j, i) < n ? v[i] - mean : 0.0f;
+      v[i] = element_of<kWide>(t, threads, j, i) < n ? v[i] - mean : 0.0f;
       square = __fmaf_rn(v[i], v[i], square);
     }
   }
   return square;
 }
 
-// One row per CTA at a time: few rows, or rows longer than a warp holds.
-template <typename X, typename Y, bool kWide, int kV>
+// One row per CTA at a time (of 16-byte aligned rows): few rows, or rows longer than a warp holds.
+template <typename X, typename Y, int kV>
 __global__ void __launch_bounds__(kNormMaxThreads) norm_kernel(const NormParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ float slots[4][32];
@@ -207,11 +189,11 @@ __global__ void __launch_bounds__(kNormMaxThreads) norm_kernel(const NormParams 
   Eight<X> next[kV];
   const X* x = static_cast<const X*>(p.x);
 #pragma unroll
-  for (int j = 0; j < kV; ++j) next[j] = load_eight<X, kWide>(x + blockIdx.x * p.ldx, p.n, t, threads, j);
+  for (int j = 0; j < kV; ++j) next[j] = load_eight<X, true>(x + blockIdx.x * p.ldx, p.n, t, threads, j);
 #pragma unroll
   for (int j = 0; j < kV; ++j) {
-    load_vector<kWide>(p.gamma, p.n, t, threads, j, 1.0f, gamma[j]);
-    load_vector<kWide>(p.beta, p.n, t, threads, j, 0.0f, beta[j]);
+    load_vector<true>(p.gamma, p.n, t, threads, j, 1.0f, gamma[j]);
+    load_vector<true>(p.beta, p.n, t, threads, j, 0.0f, beta[j]);
   }
   int turn = 0;
   for (int64_t row = blockIdx.x; row < p.m; row += gridDim.x, turn ^= 2) {
@@ -225,11 +207,11 @@ __global__ void __launch_bounds__(kNormMaxThreads) norm_kernel(const NormParams 
       }
     if (row + gridDim.x < p.m) {
 #pragma unroll
-      for (int j = 0; j < kV; ++j) next[j] = load_eight<X, kWide>(x + (row + gridDim.x) * p.ldx, p.n, t, threads, j);
+      for (int j = 0; j < kV; ++j) next[j] = load_eight<X, true>(x + (row + gridDim.x) * p.ldx, p.n, t, threads, j);
     }
     const float mean = block_sum(sum, slots[turn]) * inverse;
 #pragma unroll
-    for (int j = 0; j < kV; ++j) square = centred_squares<X, kWide>(v[j], mean, p.n, t, threads, j, square);
+    for (int j = 0; j < kV; ++j) square = centred_squares<true>(v[j], mean, p.n, t, threads, j, square);
     const float rstd = 1.0f / sqrtf(block_sum(square, slots[turn + 1]) * inverse + p.eps);
     if (t == 0) {
       if (p.mean) p.mean[row] = mean;
@@ -241,7 +223,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) norm_kernel(const NormParams 
       float r[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) r[i] = __fmaf_rn(v[j][i] * rstd, gamma[j][i], beta[j][i]);
-      store_eight<Y, kWide>(y, p.n, t, threads, j, r);
+      store_eight<Y, true>(y, p.n, t, threads, j, r);
     }
   }
 }
@@ -289,7 +271,7 @@ __global__ void __launch_bounds__(32 * kNormWarps, sizeof(X) == 2 || kV < 16 ? 2
       float v[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = raw[j][i];
-      square += centred_squares<X, kWide>(v, mean, p.n, lane, 32, j, 0.0f);
+      square += centred_squares<kWide>(v, mean, p.n, lane, 32, j, 0.0f);
     }
     const float rstd = 1.0f / sqrtf(warp_sum(square) * inverse + p.eps);
     if (lane == 0) {
@@ -319,7 +301,7 @@ __global__ void __launch_bounds__(32 * kNormWarps, sizeof(X) == 2 || kV < 16 ? 2
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int c = min(element_of<X, kWide>(lane, 32, j, i), p.n - 1);
+          const int c = min(element_of<kWide>(lane, 32, j, i), p.n - 1);
           r[i] = __fmaf_rn((raw[j][i] - mean) * rstd, weights[c], weights[room + c]);
         }
         store_eight<Y, kWide>(y, p.n, lane, 32, j, r);
@@ -328,9 +310,10 @@ __global__ void __launch_bounds__(32 * kNormWarps, sizeof(X) == 2 || kV < 16 ? 2
   }
 }
 
-// The same with a warp's rows on their way by bulk copies, two rows ahead of the one that is worked on: the loads
-// do not wait for the arithmetic (8192 x 4096 bf16 44 us without, 31 in this form; 12 warps with two rows each, or 16 with
-// one, 31 and 36).  Rows are whole vectors of eight, 16-byte aligned.  Shared memory: gamma and beta, kSlots rows per warp.
+// The same with a warp's next kSlots rows (two of a 16-bit type, one of f32) on their way by bulk copies: the loads do not wait
+// for the arithmetic (8192 x 4096 bf16 44 us without, 25 in this form; 31 before gamma and beta lay without bank conflicts, when
+// 12 warps with two rows each, or 16 with one, took 31 and 36).  Rows are whole vectors of eight, 16-byte aligned.  Shared
+// memory: gamma and beta, kSlots rows per warp.
 template <typename X, typename Y, int kV, int kWarps, int kSlots>
 __global__ void __launch_bounds__(32 * kWarps, 1) norm_ring_kernel(const NormParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -779,7 +762,7 @@ __global__ void __launch_bounds__(kWarp ? 128 : kNormMaxThreads) norm_grad_kerne
 #pragma unroll
       for (int j = 0; j < kV; ++j)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) join[warp][element_of<X, kWide>(t, 32, j, i)] = which ? dbeta[j][i] : dgamma[j][i];
+        for (int i = 0; i < 8; ++i) join[warp][element_of<kWide>(t, 32, j, i)] = which ? dbeta[j][i] : dgamma[j][i];
       __syncthreads();
       for (int c = threadIdx.x; c < p.n; c += 128)
         out[c + which * other] = ((join[0][c] + join[1][c]) + join[2][c]) + join[3][c];
@@ -789,7 +772,7 @@ __global__ void __launch_bounds__(kWarp ? 128 : kNormMaxThreads) norm_grad_kerne
     for (int j = 0; j < kV; ++j) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int c = element_of<X, kWide>(t, threads, j, i);
+        const int c = element_of<kWide>(t, threads, j, i);
         if (c < p.n) {
           out[c] = dgamma[j][i];
           out[c + other] = dbeta[j][i];
@@ -1088,7 +1071,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 && kWide ? 4 : 3) epilogue
   }
   if (p.sums == nullptr) return;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) join[warp][element_of<T, kWide>(lane, 32, 0, i)] = i % 2 ? sums[i / 2].y : sums[i / 2].x;
+  for (int i = 0; i < 8; ++i) join[warp][element_of<kWide>(lane, 32, 0, i)] = i % 2 ? sums[i / 2].y : sums[i / 2].x;
   __syncthreads();
   const int c = threadIdx.x;
   if (c < n) {

@@ -12,6 +12,7 @@
 #pragma once
 
 #include "dense_params.h"
+#include "dense_types.cuh"
 #include "exchange.h"
 #include "gemm_params.h"
 #include "ptx_sm100.cuh"
@@ -90,19 +91,6 @@ __device__ __forceinline__ ProductTile product_tile(const ProductParams& p, int 
   return c;
 }
 
-__device__ __forceinline__ float to_float(float v) { return v; }
-__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T>
-__device__ __forceinline__ T from_float(float v) {
-  if constexpr (std::is_same<T, float>::value) {
-    return v;
-  } else if constexpr (std::is_same<T, __half>::value) {
-    return __float2half_rn(v);
-  } else {
-    return __float2bfloat16_rn(v);
-  }
-}
 __device__ __forceinline__ float load_as_f32(const void* base, int64_t i, int type) {
   if (type == kF32) return static_cast<const float*>(base)[i];
   if (type == kF16) return __half2float(static_cast<const __half*>(base)[i]);
@@ -255,7 +243,7 @@ __device__ __forceinline__ void load_c_rows(const ProductParams& p, int row0, in
   auto rows = [&](auto* base) {
     base += at;
 #pragma unroll
-    for (int r = 0; r < kRows; ++r, base += p.ldc) c[r] = r < nrows ? to_float(*base) : 0.0f;
+    for (int r = 0; r < kRows; ++r, base += p.ldc) c[r] = r < nrows ? to_f32(*base) : 0.0f;
   };
   if (p.c_type == kF32) {
     rows(static_cast<const float*>(p.C));
@@ -306,7 +294,7 @@ __device__ __forceinline__ void write_chunk_rows(const ProductParams& p, uint32_
           if (c_buf) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(c_buf + static_cast<uint32_t>((r0 + i0 + i) * 128 + lane * 4)));
           v[i] = __fmaf_rn(p.beta, x, v[i]);
         }
-        if (i0 + i < nrows) *base = from_float<T>(v[i]);
+        if (i0 + i < nrows) *base = from_f32<T>(v[i]);
       }
     }
   };
@@ -340,7 +328,7 @@ __device__ __forceinline__ void finish_columns(const ProductParams& p, uint32_t 
     const TC* from = static_cast<const TC*>(p.C) + (i * p.ldc + j);
     const int64_t step = p.swapped ? p.ldc : 1;
 #pragma unroll
-    for (int u = 0; u < kCols; ++u) c[u] = u < ncols ? to_float(from[u * step]) : 0.0f;
+    for (int u = 0; u < kCols; ++u) c[u] = u < ncols ? to_f32(from[u * step]) : 0.0f;
   }
   const uint32_t at = base + static_cast<uint32_t>((col * kTileM + row) * 4);
 #pragma unroll
@@ -378,7 +366,7 @@ __device__ __forceinline__ void finish_columns(const ProductParams& p, uint32_t 
     const int64_t step = p.swapped ? ld : 1;
 #pragma unroll
     for (int u = 0; u < kCols; ++u)
-      if (u < ncols) to[u * step] = from_float<T>(v[u]);
+      if (u < ncols) to[u * step] = from_f32<T>(v[u]);
   };
   if (p.Z) store(p.Z, p.ldz);
   if (p.act == kOpRelu) {
@@ -471,7 +459,8 @@ __device__ __forceinline__ void finish_parts(const ProductParams& p, uint32_t ba
 // elements, 131072 of bf16; longer ones are summed in pieces of 8192, which drop 6e-5 at most.
 //
 // kTma: C, D and Z pass through shared memory by TMA.  Instances of their own, because next to the pieces' 128 sums either
-// path's registers are at the other's expense (680 bytes of spills with both, 200 with TMA alone).  (kProductParts: true.)
+// path's registers are at the other's expense (bytes of spill stores of a thread: 680 with both, 204 with TMA alone, 556 without
+// TMA).  (kProductParts: true.)
 template <int kForm, bool kPieces, bool kTma>
 __global__ void __launch_bounds__(kForm == kProductParts ? 224 : kProductThreads, 1)
     product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,

@@ -553,7 +553,7 @@ CPUOPS_B200_API int cpuops_b200_layer_norm_grad(const cpuops_b200_layer_norm_gra
  * and dlogits = upstream * d loss / d logits, of the logits' type (counts have no gradient).  Tokens without an id
  * (padding, ids of -1) count nowhere and have a gradient of zero; without any such token the loss is 0.
  * An expert whose logit is NaN or -inf is out of its token's sum; +inf counts as the largest number.
- * dlogits of an even load are about coefficient / (tokens * experts): f16, whose numbers end at 6e-8, needs a loss scale in
+ * dlogits are of the order of coefficient / (tokens * experts) and less: f16, whose numbers end at 6e-8, needs a loss scale in
  * upstream (or f32 logits).
  * upstream: the loss's own gradient, one float on the device (NULL: 1).  counts, loss and dlogits may each be NULL;
  * dlogits may be logits (same ld).  Uses the stream's workspace beyond 32 tokens. */
