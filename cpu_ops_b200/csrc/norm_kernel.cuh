@@ -310,6 +310,18 @@ __global__ void __launch_bounds__(32 * kNormWarps, sizeof(X) == 2 || kV < 16 ? 2
   }
 }
 
+// Waits for the bulk copies of rows that are on their way, `row` the first of up to `ring` of them, before the CTA or warp that
+// gave up ends.  (Not inlined: its loop beside the rows' cost the gradient's registers, 8192 x 4096 with dr 55 us, 51 in this form.)
+__device__ __noinline__ void drain_rows(uint32_t bar, int ring, uint32_t slot, uint32_t phase, int64_t row, int64_t step, int64_t m) {
+  for (int i = 0; i < ring && row < m; ++i, row += step) {
+    mbar_drain(bar + 8u * slot, phase);
+    if (++slot == static_cast<uint32_t>(ring)) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
+}
+
 // The same with a warp's next kSlots rows (two of a 16-bit type, one of f32) on their way by bulk copies: the loads do not wait
 // for the arithmetic (8192 x 4096 bf16 44 us without, 25 in this form; 31 before gamma and beta lay without bank conflicts, when
 // 12 warps with two rows each, or 16 with one, took 31 and 36).  Rows are whole vectors of eight, 16-byte aligned.  Shared
@@ -350,14 +362,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1) norm_ring_kernel(const NormPar
     if (!__all_sync(0xffffffffu, mbar_wait_bounded(bar + 8u * slot, phase, &abort_flag, budget_ns))) {
       if (lane == 0) {
         leave_error(p.error, kErrProducerWait);
-        // copies that are on their way (this row's, and the next ones') land before the CTA ends
-        for (int64_t r = row; r < p.m && r < row + kSlots * step; r += step) {
-          mbar_drain(bar + 8u * slot, phase);
-          if (++slot == kSlots) {
-            slot = 0;
-            phase ^= 1u;
-          }
-        }
+        drain_rows(bar, kSlots, slot, phase, row, step, p.m);
       }
       break;
     }
@@ -791,13 +796,13 @@ __global__ void __launch_bounds__(kMaxThreads, kMaxThreads == 256 && sizeof(X) =
   extern __shared__ __align__(16) uint8_t rows[];
   __shared__ float2 slots[2][32];
   __shared__ __align__(8) uint64_t barriers[kNormMaxRing];
-  __shared__ int abort_flag, failed[2];  // (failed: by turns, so that no thread sets what another has still to read)
+  __shared__ int abort_flag;
   const int t = threadIdx.x, threads = blockDim.x, n = p.n, lane = t & 31, warp = t >> 5, warps = threads >> 5;
   const float inverse = 1.0f / static_cast<float>(n);
   const uint32_t x_bytes = static_cast<uint32_t>(n) * sizeof(X), dy_bytes = static_cast<uint32_t>(n) * sizeof(Y);
   const uint32_t slot_bytes = (p.dr ? 2u : 1u) * x_bytes + dy_bytes, bar = smem_u32(barriers), ring0 = smem_u32(rows);
   if (t == 0) {
-    abort_flag = failed[0] = failed[1] = 0;
+    abort_flag = 0;
     for (int i = 0; i < p.ring; ++i) mbar_init(bar + 8u * i, 1);
     fence_mbar_init();
   }
@@ -835,7 +840,7 @@ __global__ void __launch_bounds__(kMaxThreads, kMaxThreads == 256 && sizeof(X) =
       next_mean = __ldg(p.mean_in + row + step);
       next_rstd = __ldg(p.rstd_in + row + step);
     }
-    if (!mbar_wait_bounded(bar + 8u * slot, phase, &abort_flag, budget_ns)) failed[turn] = 1;
+    const bool ran_out = !mbar_wait_bounded(bar + 8u * slot, phase, &abort_flag, budget_ns);
     const uint32_t from = ring0 + slot * slot_bytes;
     Eight<X> xs[kV], drs[kV];
     Eight<Y> dys[kV];
@@ -874,8 +879,7 @@ __global__ void __launch_bounds__(kMaxThreads, kMaxThreads == 256 && sizeof(X) =
     float s1 = warp_sum(sum.x + sum.y), s2 = warp_sum(along.x + along.y);
     if (lane == 0) slots[turn][warp] = make_float2(s1, s2);
     fence_proxy_async_shared_cta();  // the slot has been read: before it is filled again
-    __syncthreads();
-    if (failed[turn]) break;
+    if (__syncthreads_or(ran_out)) break;
     if (t == 0) request(row + p.ring * step, slot);
     if (++slot == static_cast<uint32_t>(p.ring)) {
       slot = 0;
@@ -903,14 +907,7 @@ __global__ void __launch_bounds__(kMaxThreads, kMaxThreads == 256 && sizeof(X) =
   if (row < p.m) {  // (a wait ran out)
     if (t == 0) {
       leave_error(p.error, kErrProducerWait);
-      // copies that are on their way (this row's, and the next ones') land before the CTA ends
-      for (int64_t r = row; r < p.m && r < row + p.ring * step; r += step) {
-        mbar_drain(bar + 8u * slot, phase);
-        if (++slot == static_cast<uint32_t>(p.ring)) {
-          slot = 0;
-          phase ^= 1u;
-        }
-      }
+      drain_rows(bar, p.ring, slot, phase, row, step, p.m);
     }
     __syncthreads();
     return;
