@@ -9,7 +9,8 @@
 // A kernel counts, block by block; the other needs all counts (its CTAs add the blocks' up), takes a token
 // per warp, logits read once, and keeps sums of p in registers; its last CTA adds those up.  Bound by latencies: two
 // launches, two hand-overs through L2, a token's three sums across a warp.  8192 tokens of 256 experts, f32: 16 us of a
-// replayed graph (17 MB, 2.6 us at HBM's rate); 1537 of 60, bf16: 8.5; 32 of 64 in one launch: 4.6.
+// replayed graph (17 MB, 2.6 us at HBM's rate); 1537 of 60, bf16: 8.5; 32 of 64 in one launch: 4.6.  Beyond 512 experts a thread's
+// scores, the next token's and its sums do not all fit 128 registers (208 bytes spilled): 8192 of 1024 48 us.
 #pragma once
 
 #include "dense_params.h"
