@@ -21,8 +21,8 @@ def calls(text, name):
 
 def test_waits_for_copies_under_way_do_not_go_by_the_callers_budget():
     """A CTA that gives up waits for what it has issued before it leaves.  With the budget that a caller may set to a
-    microsecond that wait would end before a copy lands; such waits are mbar_drain's.  What is left goes by the budget and ends
-    with its CTA's abort flag too."""
+    microsecond that wait would end before a copy lands; such waits are mbar_drain's.  All others end
+    with their CTA's abort flag too."""
     seen, drains = 0, 0
     for path in sorted(CSRC.glob("*")):
         text = path.read_text()
